@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define M2_B200_ABI_VERSION 6
+#define M2_B200_ABI_VERSION 7
 
 typedef enum { M2_F32 = 0, M2_BF16 = 1, M2_F16 = 2 /* only where an entry point says so */ } m2_dtype;
 
@@ -44,7 +44,7 @@ typedef enum {
 #define M2_DEV_TIMEOUT_MMA   2   /* a wait for tensor-core work or a free accumulator ran out */
 #define M2_DEV_TIMEOUT_EPI   4   /* an epilogue's wait for an accumulator ran out */
 #define M2_DEV_TIMEOUT_EMPTY 8   /* a producer's wait for a free shared-memory stage ran out */
-#define M2_DEV_BAD_INDEX     16  /* m2_embed_layernorm_fwd met an id outside its table (clamped) */
+#define M2_DEV_BAD_INDEX     16  /* m2_embed_layernorm_fwd met an id outside its table (clamped), or m2_token_logprobs_fwd a target outside the vocabulary */
 
 /* ABI version of the loaded library (== M2_B200_ABI_VERSION it was built with). */
 int m2_version(void);
@@ -426,6 +426,143 @@ typedef struct {
 long long m2_encoder_workspace(int batch, int pitch, int d_model, int inter);
 long long m2_encoder_workspace_f32(int batch, int seq_len, int d_model, int inter, int nblocks);
 int m2_encoder_fwd(const m2_encoder_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head: a causal sequence mixer whose state has a fixed size.
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,     o_t = scale * q_t^T S_t
+ * No counterpart in the reference, whose mixer is the long convolution of m2_longconv_fwd
+ * (bert/src/mm/monarch_mixer_sequence_mixer.py:100-154).
+ *   q (batch, seq_len, heads, dk), k (batch, seq_len, kv_heads, dk), v (batch, seq_len, kv_heads, dv): `dtype` (M2_F32 or
+ *   M2_BF16), strides in elements, contiguous channels; head h reads key head h / (heads / kv_heads).  dk, dv <= 128.
+ *   o (batch, seq_len, heads, dv): packed, `dtype`.
+ *   log_decay : float32 (heads), <= 0 (-inf: no memory).
+ *   lengths   : NULL or int64 (batch): tokens of every sequence (clamped to 0 .. seq_len).  What lies behind them is not read,
+ *               rows of o (and gradients) behind them are zero, and the state is that behind the last token.
+ *   state_in  : NULL (zero) or float32 (batch, heads, dk, dv), packed; state_out: NULL or the same.  They may be the same memory.
+ *   workspace : m2_linear_attention_workspace() bytes on a 16-byte boundary (0: NULL).
+ * bf16: float32 sums and state; the weights (q_i . k_j) decay^(i-j) and the state's copy that q meets are rounded to bf16, as
+ * tensor-core operands.  float32: products and sums in float32 throughout.
+ * Gradients (m2_linear_attention_bwd): of q, k, v (packed, `dtype`) and of state_in (d_state_in: NULL or float32), from d_o
+ * (`dtype`, strides, contiguous channels) and d_state_out (NULL: zero).  The decay has none.  Gradients of shared key heads are
+ * float32 sums over their heads.  No atomics: two runs give the same bits.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  int batch, seq_len, heads, kv_heads, dk, dv;
+  m2_dtype dtype;
+  float scale;             /* not 0 */
+  const void* q; long long q_sb, q_st, q_sh;
+  const void* k; long long k_sb, k_st, k_sh;
+  const void* v; long long v_sb, v_st, v_sh;
+  const float* log_decay;
+  const void* lengths;     /* int64 */
+  const float* state_in;
+  void* o;
+  float* state_out;
+  float* workspace;
+} m2_linear_attention_args;
+
+typedef struct {
+  const void* d_o; long long o_sb, o_st, o_sh;
+  const float* d_state_out;
+  void *d_q, *d_k, *d_v;
+  float* d_state_in;
+} m2_linear_attention_grads;
+
+long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, int backward);
+int m2_linear_attention_fwd(const m2_linear_attention_args* args, void* stream);
+int m2_linear_attention_bwd(const m2_linear_attention_args* args, const m2_linear_attention_grads* grads, void* stream);
+
+/* One token of every sequence: q (batch, heads, dk), k, v (batch, kv_heads, ...) with contiguous channels, o packed.  `state`
+ * float32, (b, h) at state[b*s_b + h*s_h] with packed (dk, dv), is read and replaced. */
+typedef struct {
+  int batch, heads, kv_heads, dk, dv;
+  m2_dtype dtype;
+  float scale;
+  const void* q; long long q_sb, q_sh;
+  const void* k; long long k_sb, k_sh;
+  const void* v; long long v_sb, v_sh;
+  const float* log_decay;
+  float* state; long long s_b, s_h;
+  void* o;
+} m2_linear_attention_step_args;
+
+int m2_linear_attention_step(const m2_linear_attention_step_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Norms after and before a block with the block's gate and the residual's scale:
+ *   r = scale * x + gate * N_after(y),      h = N_before(r)
+ * N: LayerNorm or (rms != 0) RMS norm over the n <= 8192 columns, each optional (norm_after, norm_before; without norm_after
+ * N_after(y) = y, without norm_before there is no h).  m2_add_layernorm_fwd (bert/src/bert_layers.py:506) is the case of a
+ * post-norm without gate, scale and norm of y.
+ *   x (rows, n) and r of x_dtype: the residual stream; y (rows, n) and h of y_dtype; row strides ldx, ldy; r, h packed.
+ *   gate_kind 0: none; 1: (n), a channel; 2: (rows / seq_len, n), a sequence of seq_len rows, row stride ldg; 3: (rows, n).
+ *   scale_channel: float32 (n), or NULL: `scale` for all.  Weights and biases float32 (n) or NULL (1 and 0).
+ *   stats : NULL, or (rows, 4) float32 on a 16-byte boundary, for the gradient.
+ * Statistics and everything up to the one rounding of each output are float32; h is of the unrounded r.
+ * Gradients (m2_residual_norm_bwd): from d_r (x_dtype) and d_h (y_dtype), packed, NULL = zero; every output may be NULL.
+ * d_gate has the gate's type and is packed; parameters' gradients are float32 sums in a fixed order.
+ *   workspace: m2_residual_norm_workspace() bytes on a 16-byte boundary.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  long long rows, seq_len;  /* seq_len divides rows; read for gate_kind 2 alone */
+  int n;
+  m2_dtype x_dtype, y_dtype, gate_dtype;
+  int gate_kind, rms, norm_after, norm_before;
+  float eps, scale;
+  const void* x; long long ldx;
+  const void* y; long long ldy;
+  const void* gate; long long ldg;
+  const float* scale_channel;
+  const float *after_weight, *after_bias, *before_weight, *before_bias;
+  void* r; void* h;
+  float* stats;
+} m2_residual_norm_args;
+
+typedef struct {
+  const void *d_r, *d_h;
+  void *d_x, *d_y, *d_gate;
+  float *d_scale, *d_after_weight, *d_after_bias, *d_before_weight, *d_before_bias;
+  float* workspace;
+} m2_residual_norm_grads;
+
+int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* stream);
+long long m2_residual_norm_workspace(long long rows, long long seq_len, int n, int gate_kind);
+int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_residual_norm_grads* grads, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Log probabilities of given tokens, entropy and the best alternatives of rows of logits: behind the decoder of the reference's
+ * masked-LM head (bert/src/bert_layers.py, BertForMaskedLM: cross entropy over the masked positions).
+ *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), row stride ld; targets int64 (rows).
+ *   logprob, entropy float32 (rows); top_logprob float32 and top_id int64 (rows, top), best first, equal values by ascending
+ *   id, NaN before all (top <= 32 and <= vocab).  stats float32 (rows, 2): maximum and log of the sum, for the gradient.
+ * A row whose target is ignore_index is not read: zeros, ids -1.  A target outside the vocabulary: logprob is NaN and
+ * M2_DEV_BAD_INDEX is set.  Logits of -inf have probability 0; where all are, log probabilities are -inf, the entropy 0 and the
+ * gradient 0.  NaN or +inf among the logits make the row's probabilities NaN.  Everything is summed in float32.
+ * Gradient (m2_token_logprobs_bwd): d_logits (rows, vocab) of `dtype`, row stride ldd, from the gradients of logprob, entropy
+ * and top_logprob (each NULL or float32, packed); zero in ignored rows.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  long long rows; int vocab, top;
+  m2_dtype dtype;
+  const void* logits; long long ld;
+  const void* targets; long long ignore_index;
+  float *logprob, *entropy, *stats, *top_logprob;
+  void* top_id;
+} m2_token_logprobs_args;
+
+typedef struct {
+  long long rows; int vocab, top;
+  m2_dtype dtype;
+  const void* logits; long long ld;
+  const void* targets; long long ignore_index;
+  const float *stats, *entropy;
+  const void* top_id;
+  const float *d_logprob, *d_entropy, *d_top_logprob;
+  void* d_logits; long long ldd;
+} m2_token_logprobs_bwd_args;
+
+int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* stream);
+int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, void* stream);
 
 #ifdef __cplusplus
 }

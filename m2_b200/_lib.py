@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm2b200.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 M2_F32, M2_BF16, M2_F16 = 0, 1, 2
 
@@ -150,6 +150,75 @@ class EncoderArgs(C.Structure):
     ]
 
 
+class LinearAttentionArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("seq_len", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("dk", C.c_int), ("dv", C.c_int),
+        ("dtype", C.c_int), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_sb", C.c_longlong), ("q_st", C.c_longlong), ("q_sh", C.c_longlong),
+        ("k", C.c_void_p), ("k_sb", C.c_longlong), ("k_st", C.c_longlong), ("k_sh", C.c_longlong),
+        ("v", C.c_void_p), ("v_sb", C.c_longlong), ("v_st", C.c_longlong), ("v_sh", C.c_longlong),
+        ("log_decay", C.c_void_p), ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("o", C.c_void_p),
+        ("state_out", C.c_void_p), ("workspace", C.c_void_p),
+    ]
+
+
+class LinearAttentionGrads(C.Structure):
+    _fields_ = [
+        ("d_o", C.c_void_p), ("o_sb", C.c_longlong), ("o_st", C.c_longlong), ("o_sh", C.c_longlong),
+        ("d_state_out", C.c_void_p), ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_state_in", C.c_void_p),
+    ]
+
+
+class LinearAttentionStepArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("dk", C.c_int), ("dv", C.c_int),
+        ("dtype", C.c_int), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_sb", C.c_longlong), ("q_sh", C.c_longlong),
+        ("k", C.c_void_p), ("k_sb", C.c_longlong), ("k_sh", C.c_longlong),
+        ("v", C.c_void_p), ("v_sb", C.c_longlong), ("v_sh", C.c_longlong),
+        ("log_decay", C.c_void_p), ("state", C.c_void_p), ("s_b", C.c_longlong), ("s_h", C.c_longlong), ("o", C.c_void_p),
+    ]
+
+
+class ResidualNormArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_longlong), ("seq_len", C.c_longlong), ("n", C.c_int),
+        ("x_dtype", C.c_int), ("y_dtype", C.c_int), ("gate_dtype", C.c_int),
+        ("gate_kind", C.c_int), ("rms", C.c_int), ("norm_after", C.c_int), ("norm_before", C.c_int),
+        ("eps", C.c_float), ("scale", C.c_float),
+        ("x", C.c_void_p), ("ldx", C.c_longlong), ("y", C.c_void_p), ("ldy", C.c_longlong), ("gate", C.c_void_p), ("ldg", C.c_longlong),
+        ("scale_channel", C.c_void_p),
+        ("after_weight", C.c_void_p), ("after_bias", C.c_void_p), ("before_weight", C.c_void_p), ("before_bias", C.c_void_p),
+        ("r", C.c_void_p), ("h", C.c_void_p), ("stats", C.c_void_p),
+    ]
+
+
+class ResidualNormGrads(C.Structure):
+    _fields_ = [
+        ("d_r", C.c_void_p), ("d_h", C.c_void_p), ("d_x", C.c_void_p), ("d_y", C.c_void_p), ("d_gate", C.c_void_p),
+        ("d_scale", C.c_void_p), ("d_after_weight", C.c_void_p), ("d_after_bias", C.c_void_p),
+        ("d_before_weight", C.c_void_p), ("d_before_bias", C.c_void_p), ("workspace", C.c_void_p),
+    ]
+
+
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_longlong), ("vocab", C.c_int), ("top", C.c_int), ("dtype", C.c_int),
+        ("logits", C.c_void_p), ("ld", C.c_longlong), ("targets", C.c_void_p), ("ignore_index", C.c_longlong),
+        ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p), ("top_logprob", C.c_void_p), ("top_id", C.c_void_p),
+    ]
+
+
+class TokenLogprobsBwdArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_longlong), ("vocab", C.c_int), ("top", C.c_int), ("dtype", C.c_int),
+        ("logits", C.c_void_p), ("ld", C.c_longlong), ("targets", C.c_void_p), ("ignore_index", C.c_longlong),
+        ("stats", C.c_void_p), ("entropy", C.c_void_p), ("top_id", C.c_void_p),
+        ("d_logprob", C.c_void_p), ("d_entropy", C.c_void_p), ("d_top_logprob", C.c_void_p),
+        ("d_logits", C.c_void_p), ("ldd", C.c_longlong),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/m2_b200.h declares
 SYMBOLS = {
     "m2_version": (C.c_int, []),
@@ -182,6 +251,15 @@ SYMBOLS = {
     "m2_mixer_split_bytes": (C.c_longlong, [C.c_int]),
     "m2_mlp_split_bytes": (C.c_longlong, [C.c_int, C.c_int, C.c_int]),
     "m2_encoder_fwd": (C.c_int, [C.POINTER(EncoderArgs), C.c_void_p]),
+    "m2_linear_attention_workspace": (C.c_longlong, [C.c_int] * 7),
+    "m2_linear_attention_fwd": (C.c_int, [C.POINTER(LinearAttentionArgs), C.c_void_p]),
+    "m2_linear_attention_bwd": (C.c_int, [C.POINTER(LinearAttentionArgs), C.POINTER(LinearAttentionGrads), C.c_void_p]),
+    "m2_linear_attention_step": (C.c_int, [C.POINTER(LinearAttentionStepArgs), C.c_void_p]),
+    "m2_residual_norm_fwd": (C.c_int, [C.POINTER(ResidualNormArgs), C.c_void_p]),
+    "m2_residual_norm_workspace": (C.c_longlong, [C.c_longlong, C.c_longlong, C.c_int, C.c_int]),
+    "m2_residual_norm_bwd": (C.c_int, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), C.c_void_p]),
+    "m2_token_logprobs_fwd": (C.c_int, [C.POINTER(TokenLogprobsArgs), C.c_void_p]),
+    "m2_token_logprobs_bwd": (C.c_int, [C.POINTER(TokenLogprobsBwdArgs), C.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,489 @@
+// Log probabilities of given tokens, entropy and the best alternatives of every row of logits, and the gradient with respect to
+// the logits: what the loss of the reference's masked-LM head computes behind its decoder (bert/src/bert_layers.py,
+// BertForMaskedLM.forward: CrossEntropyLoss over the masked positions), for any given token.
+//
+// With m = max x, s = sum exp(x_j - m), t = sum (x_j - m) exp(x_j - m):
+//     log p_j = (x_j - m) - log s,      H = -sum p log p = log s - t / s
+//     dx_j = sum_i g_i (1[j = id_i] - p_j) - g_H p_j (log p_j + H)     over the given token and the alternatives.
+//
+// Bound: one read of the logits (gradient: one read, one write).  Forward: every thread streams 16-byte pieces and keeps its own
+// (m, s, t) in float32, rescaled when a piece raises m; one exp a value.  The alternatives are found without sorting: the k-th
+// largest of 64 thread groups' maxima is a lower bound of the row's k-th largest value, so the few values not below it are
+// collected in a second look at the row (L2 or shared memory) and ranked among one another.  Rows with so many equal values that
+// the list overflows are searched k times instead.
+#include "common.cuh"
+
+namespace m2 {
+namespace lp {
+
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int GROUPS = 64;               // of 4 lanes each
+constexpr int MAX_TOP = 32;              // <= GROUPS
+constexpr int CAND = 1024;               // candidates kept per block
+constexpr int MAX_SPLIT = 8;             // blocks of a cluster that share a row
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
+constexpr float LOWEST = -3.402823466e38f;
+constexpr int ST_BAD_TARGET = 16;        // M2_DEV_BAD_INDEX
+
+struct Args {
+  const void* x; long long ld;
+  const long long* target;
+  long long n; int vocab, top, split;
+  long long ignore;
+  float *logprob, *entropy, *stats, *top_lp;
+  long long* top_id;
+};
+
+struct BwdArgs {
+  const void* x; long long ld;
+  const long long* target;
+  long long n; int vocab, top;
+  long long ignore;
+  const float *stats, *entropy;
+  const long long* top_id;
+  const float *g_lp, *g_h, *g_top;
+  void* dx; long long ldd;
+};
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <typename T> struct Piece;      // 16 bytes of a row
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  __device__ static void get(const uint4& u, float (&f)[4]) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+  __device__ static uint4 put(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <> struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static void get(const uint4& u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  __device__ static uint4 put(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// Order of the alternatives: larger value first, NaN before all, equal values (both zeros among them) by ascending id.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long rank_key(float v, int id) {      // larger is better
+  return ((unsigned long long)order_key(v) << 32) | (uint32_t)~id;
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  if (u == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int key_id(unsigned long long k) { return (int)~(uint32_t)k; }
+
+// Running (m, s, t) of exp(x - m); m starts at the lowest finite value, so that x - m is never inf - inf for -inf entries.  Distances are cut at -1e4, far beyond
+// where exp is 0, so that no 0 * inf arises.
+struct Stats { float m, s, t; };
+__device__ __forceinline__ void rebase(Stats& a, float m) {         // to the maximum m >= a.m
+  const float d = a.m - m, f = ex2(d * LOG2E);
+  a.t = f * fmaf(fmaxf(d, -1e4f), a.s, a.t);
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Stats join(Stats a, Stats b) {
+  const float m = fmaxf(a.m, b.m);
+  rebase(a, m);
+  rebase(b, m);
+  return {m, a.s + b.s, a.t + b.t};
+}
+template <int N> __device__ __forceinline__ void add_values(Stats& a, const float (&f)[N]) {
+  float m = f[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, f[i]);
+  if (m > a.m) rebase(a, m);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = f[i] - a.m, e = ex2(d * LOG2E);                 // -inf: d = -inf, e = 0; NaN stays NaN in s
+    a.s += e;
+    a.t = fmaf(fmaxf(d, -1e4f), e, a.t);
+  }
+}
+
+// Elements [lo, hi) of a row as scalar ends and 16-byte pieces.
+template <typename T> struct Span {
+  const T* p;
+  int lo, hi, head, pieces;              // [lo, lo + head) scalar, then pieces of N, then scalars up to hi
+  __device__ Span(const T* row, int lo_, int hi_) : p(row), lo(lo_), hi(hi_) {
+    constexpr int N = Piece<T>::N;
+    head = (int)((16 - (reinterpret_cast<uintptr_t>(row + lo) & 15)) & 15) / (int)sizeof(T);
+    if (head > hi - lo) head = hi - lo;
+    pieces = (hi - lo - head) / N;
+  }
+  __device__ int body() const { return lo + head; }
+  __device__ int tail() const { return lo + head + pieces * Piece<T>::N; }
+  // f(value, id) for the scalar ends, one a thread
+  template <typename F> __device__ void ends(F&& f) const {
+    const int t = threadIdx.x;
+    if (t < head) f(load1(p + lo + t), lo + t);
+    const int i = tail() + t;
+    if (i < hi) f(load1(p + i), i);
+  }
+};
+
+__device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <typename V> __device__ __forceinline__ const V* in_cta(const V* p, uint32_t rank) {     // the same variable in another block
+  uint64_t r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(p), "r"(rank));
+  return reinterpret_cast<const V*>(r);
+}
+
+struct Shared {
+  Stats warp[WARPS];
+  Stats mine;                            // this block's slice
+  uint32_t group[GROUPS];
+  float bound;
+  int count;
+  unsigned long long best[MAX_TOP];      // this block's k best, best first; 0 where there are fewer
+  unsigned long long cand[CAND];
+  unsigned long long found[WARPS];
+};
+
+// The k best of [lo, hi) into sh.best.  Called by all threads; vmax: the largest value that this thread saw (LOWEST if none).
+template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, int k, float vmax) {
+  constexpr int N = Piece<T>::N;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float g = fmaxf(vmax, __shfl_xor_sync(~0u, vmax, 1));
+  g = fmaxf(g, __shfl_xor_sync(~0u, g, 2));
+  if ((tid & 3) == 0) sh.group[tid >> 2] = order_key(g);
+  if (tid < MAX_TOP) sh.best[tid] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  if (tid < GROUPS) {
+    const uint32_t mine = sh.group[tid];
+    int above = 0;                       // how many groups come before this one
+    for (int i = 0; i < GROUPS; ++i) {
+      const uint32_t o = sh.group[i];
+      above += o > mine || (o == mine && i < tid);
+    }
+    if (above == k - 1) sh.bound = key_value((unsigned long long)mine << 32);
+  }
+  __syncthreads();
+  // a group without values, or with -inf alone, says LOWEST: then everything is a candidate
+  const float bound = sh.bound <= LOWEST ? -__int_as_float(0x7f800000) : sh.bound;
+  auto offer = [&](float v, int id) {
+    if (!(v < bound)) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < CAND) sh.cand[at] = rank_key(v, id);
+    }
+  };
+  sp.ends(offer);
+  const uint4* body = reinterpret_cast<const uint4*>(sp.p + sp.body());
+  for (int i = tid; i < sp.pieces; i += THREADS) {
+    float f[N];
+    Piece<T>::get(body[i], f);
+    float m = f[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = max_nan(m, f[j]);
+    if (!(m < bound)) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) offer(f[j], sp.body() + i * N + j);
+    }
+  }
+  __syncthreads();
+  const int count = sh.count;
+  if (count <= CAND) {
+    for (int c = tid; c < count; c += THREADS) {
+      const unsigned long long mine = sh.cand[c];
+      int above = 0;
+      for (int i = 0; i < count; ++i) above += sh.cand[i] > mine;          // ids differ: no two are equal
+      if (above < k) sh.best[above] = mine;
+    }
+    __syncthreads();
+    return;
+  }
+  unsigned long long last = ~0ull;                                         // too many equal values: the next best, k times
+  for (int r = 0; r < k; ++r) {
+    unsigned long long top = 0;
+    auto look = [&](float v, int id) {
+      const unsigned long long q = rank_key(v, id);
+      if (q < last && q > top) top = q;
+    };
+    sp.ends(look);
+    for (int i = tid; i < sp.pieces; i += THREADS) {
+      float f[N];
+      Piece<T>::get(body[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) look(f[j], sp.body() + i * N + j);
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long q = __shfl_xor_sync(~0u, top, o);
+      top = q > top ? q : top;
+    }
+    if (lane == 0) sh.found[warp] = top;
+    __syncthreads();
+    top = 0;
+    for (int w = 0; w < WARPS; ++w) top = sh.found[w] > top ? sh.found[w] : top;
+    if (tid == 0) sh.best[r] = top;
+    last = top;
+    __syncthreads();
+  }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS)
+forward_kernel(const Args a) {
+  constexpr int N = Piece<T>::N;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = a.split;
+  const long long row = blockIdx.x / split;
+  const uint32_t part = split > 1 ? cta_rank() : 0;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const long long target = a.target[row];
+  if (target == a.ignore) {                                                // the whole cluster leaves
+    if (part == 0) {
+      if (tid == 0) {
+        a.logprob[row] = 0.f;
+        a.entropy[row] = 0.f;
+        a.stats[2 * row] = 0.f;
+        a.stats[2 * row + 1] = 0.f;
+      }
+      if (tid < a.top) { a.top_lp[row * a.top + tid] = 0.f; a.top_id[row * a.top + tid] = -1; }
+    }
+    return;
+  }
+  // slices of whole 128-byte lines' worth of ids
+  const int per = ((a.vocab + split - 1) / split + 63) / 64 * 64;
+  const int lo = min((int)part * per, a.vocab), hi = min(lo + per, a.vocab);
+  const Span<T> sp(x, lo, hi);
+  Stats st = {LOWEST, 0.f, 0.f};
+  sp.ends([&](float v, int) { const float f[1] = {v}; add_values<1>(st, f); });
+  const uint4* body = reinterpret_cast<const uint4*>(x + sp.body());
+  constexpr int U = 4;
+  int i = tid;
+  for (; i + (U - 1) * THREADS < sp.pieces; i += U * THREADS) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = __ldg(body + i + j * THREADS);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float f[N];
+      Piece<T>::get(u[j], f);
+      add_values<N>(st, f);
+    }
+  }
+  for (; i < sp.pieces; i += THREADS) {
+    float f[N];
+    Piece<T>::get(__ldg(body + i), f);
+    add_values<N>(st, f);
+  }
+  const float vmax = st.m;
+  for (int o = 16; o > 0; o >>= 1) {
+    const Stats b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o), __shfl_xor_sync(~0u, st.t, o)};
+    st = join(st, b);
+  }
+  if (lane == 0) sh.warp[warp] = st;
+  __syncthreads();
+  if (tid == 0) {
+    st = sh.warp[0];
+    for (int w = 1; w < WARPS; ++w) st = join(st, sh.warp[w]);
+    sh.mine = st;
+  }
+  if constexpr (TOP) select_top<T>(sh, sp, a.top, vmax);
+  if (split > 1) cluster_barrier(); else __syncthreads();
+  if (part == 0) {
+    st = sh.mine;
+    for (int r = 1; r < split; ++r) st = join(st, *in_cta(&sh.mine, r));
+    const float log_s = logf(st.s);
+    const bool none = st.s == 0.f;                                         // every logit is -inf
+    const float minus_inf = -__int_as_float(0x7f800000);
+    auto logp = [&](float v) { return none ? minus_inf : (v - st.m) - log_s; };
+    if (tid == 0) {
+      const bool good = target >= 0 && target < a.vocab;
+      if (!good) atomicOr(&m2_dev_status_word, ST_BAD_TARGET);
+      a.logprob[row] = good ? logp(load1(x + target)) : __int_as_float(0x7fffffff);
+      a.entropy[row] = none ? 0.f : log_s - st.t / st.s;
+      a.stats[2 * row] = st.m;
+      a.stats[2 * row + 1] = none ? -minus_inf : log_s;                    // +inf: every probability is 0
+    }
+    if constexpr (TOP) {
+      if (split == 1) {
+        if (tid < a.top) {
+          const unsigned long long q = sh.best[tid];
+          a.top_lp[row * a.top + tid] = logp(key_value(q));
+          a.top_id[row * a.top + tid] = key_id(q);
+        }
+      } else {                                                             // k best of `split` sorted lists
+        const int n = split * a.top;
+        for (int c = tid; c < n; c += THREADS) sh.cand[c] = in_cta(sh.best, c / a.top)[c % a.top];
+        __syncthreads();
+        for (int c = tid; c < n; c += THREADS) {
+          const unsigned long long q = sh.cand[c];
+          int above = 0;
+          for (int o = 0; o < n; ++o) above += sh.cand[o] > q;
+          if (q != 0 && above < a.top) {
+            a.top_lp[row * a.top + above] = logp(key_value(q));
+            a.top_id[row * a.top + above] = key_id(q);
+          }
+        }
+      }
+    }
+  }
+  if (split > 1) cluster_barrier();                                        // the other blocks' memory was read
+}
+
+constexpr int BWD_PIECES = 8;            // a thread's pieces
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+backward_kernel(const BwdArgs a, int slices) {
+  constexpr int N = Piece<T>::N;
+  const long long row = blockIdx.x / slices;
+  const int slice = (int)(blockIdx.x % slices);
+  constexpr int per = THREADS * BWD_PIECES * N;
+  const int lo = slice * per, hi = min(lo + per, a.vocab);
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  T* dx = static_cast<T*>(a.dx) + row * a.ldd;
+  const int tid = threadIdx.x;
+  const long long target = a.target[row];
+  const bool used = target != a.ignore, good = used && target >= 0 && target < a.vocab;
+  const float m = a.stats[2 * row], log_s = a.stats[2 * row + 1];
+  const float g_h = used && a.g_h ? a.g_h[row] : 0.f, h = a.entropy[row];
+  const float g_lp = good && a.g_lp ? a.g_lp[row] : 0.f;
+  float g = g_lp;
+  if (used && a.g_top) for (int i = 0; i < a.top; ++i) g += a.g_top[row * a.top + i];
+  auto grad = [&](float v) {
+    const float l = (v - m) - log_s, p = ex2(l * LOG2E);
+    return used ? -p * fmaf(g_h, fmaxf(l, -1e4f) + h, g) : 0.f;
+  };
+  const Span<T> sp(x, lo, hi);
+  sp.ends([&](float v, int id) { st_from_float(dx + id, grad(v)); });
+  const uint4* body = reinterpret_cast<const uint4*>(x + sp.body());
+  T* out = dx + sp.body();
+  const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll 4
+  for (int i = tid; i < sp.pieces; i += THREADS) {
+    float f[N];
+    Piece<T>::get(__ldg(body + i), f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = grad(f[j]);
+    if (wide) {
+      reinterpret_cast<uint4*>(out)[i] = Piece<T>::put(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) st_from_float(out + i * N + j, f[j]);
+    }
+  }
+  if (!used) return;
+  __syncthreads();
+  // the ids that get a share of their own, written once more with everything in it
+  if (tid <= a.top) {
+    auto id_of = [&](int i) { return i == a.top ? (good ? target : -1ll) : a.top_id[row * a.top + i]; };
+    auto g_of = [&](int i) { return i == a.top ? g_lp : (a.g_top ? a.g_top[row * a.top + i] : 0.f); };
+    const long long id = id_of(tid);
+    bool first = id >= lo && id < hi;
+    for (int i = 0; first && i < tid; ++i) first = id_of(i) != id;
+    if (first) {
+      float own = 0.f;
+      for (int i = tid; i <= a.top; ++i) own += id_of(i) == id ? g_of(i) : 0.f;
+      const float v = load1(x + id);
+      const bool none = log_s == __int_as_float(0x7f800000);
+      st_from_float(dx + id, none ? 0.f : grad(v) + own);
+    }
+  }
+}
+
+template <typename T> static int launch_forward(const Args& a, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.n * a.split));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = a.split;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  const cudaError_t e = a.top ? cudaLaunchKernelEx(&cfg, forward_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, forward_kernel<T, false>, a);
+  if (e != cudaSuccess) return m2_set_error(M2_ERR_CUDA, "launch of m2_token_logprobs_fwd failed: %s", cudaGetErrorString(e));
+  return M2_OK;
+}
+
+static int check(const char* name, const void* x, long long ld, const void* target, long long n, int vocab, int top, int dtype) {
+  M2_REQUIRE(n >= 0 && vocab >= 1 && (ld >= vocab || ld == 0 || n <= 1), M2_ERR_ARG, "%s: %lld rows of %d logits, %lld apart", name, n, vocab, ld);
+  M2_REQUIRE(top >= 0 && top <= MAX_TOP && top <= vocab, M2_ERR_ARG, "%s: %d alternatives (0 .. %d, at most the %d logits)", name, top, MAX_TOP, vocab);
+  M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: logits are float32 or bf16", name);
+  M2_REQUIRE(vocab <= 1 << 28 && n <= 1 << 27, M2_ERR_UNSUPPORTED, "%s: %lld rows of %d logits are more than the grid takes", name, n, vocab);
+  M2_REQUIRE(n == 0 || (x && target), M2_ERR_ARG, "%s: logits or targets are NULL", name);
+  M2_REQUIRE(m2_aligned(x, dtype == M2_F32 ? 4 : 2) && m2_aligned(target, 8), M2_ERR_ALIGN, "%s: logits or targets are not aligned to their type", name);
+  return M2_OK;
+}
+
+}  // namespace lp
+}  // namespace m2
+
+extern "C" int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* stream) {
+  using namespace m2::lp;
+  M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_fwd: args is NULL");
+  const m2_token_logprobs_args& g = *args;
+  if (int rc = check("m2_token_logprobs_fwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
+  if (g.rows == 0) return M2_OK;
+  M2_REQUIRE(g.logprob && g.entropy && g.stats && (g.top == 0 || (g.top_logprob && g.top_id)), M2_ERR_ARG, "m2_token_logprobs_fwd: an output is NULL");
+  Args a;
+  a.x = g.logits; a.ld = g.ld; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
+  a.logprob = g.logprob; a.entropy = g.entropy; a.stats = g.stats; a.top_lp = g.top_logprob; a.top_id = (long long*)g.top_id;
+  // a row is shared by the blocks of a cluster where the rows alone do not fill the GPU, each block with 4096 logits at least
+  a.split = 1;
+  while (a.split < MAX_SPLIT && g.rows * a.split < 2LL * m2_sm_count() && g.vocab / (a.split * 2) >= 4096) a.split *= 2;
+  const cudaStream_t st = (cudaStream_t)stream;
+  return g.dtype == M2_F32 ? launch_forward<float>(a, st) : launch_forward<__nv_bfloat16>(a, st);
+}
+
+extern "C" int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, void* stream) {
+  using namespace m2::lp;
+  M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_bwd: args is NULL");
+  const m2_token_logprobs_bwd_args& g = *args;
+  if (int rc = check("m2_token_logprobs_bwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
+  if (g.rows == 0) return M2_OK;
+  M2_REQUIRE(g.stats && g.entropy && g.d_logits && (g.top == 0 || g.top_id), M2_ERR_ARG, "m2_token_logprobs_bwd: a result of the forward pass or d_logits is NULL");
+  M2_REQUIRE((g.ldd >= g.vocab || g.rows == 1) && m2_aligned(g.d_logits, g.dtype == M2_F32 ? 4 : 2), M2_ERR_ARG,
+             "m2_token_logprobs_bwd: rows of d_logits overlap or are not aligned to their type");
+  BwdArgs a;
+  a.x = g.logits; a.ld = g.ld; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
+  a.stats = g.stats; a.entropy = g.entropy; a.top_id = (const long long*)g.top_id; a.g_lp = g.d_logprob; a.g_h = g.d_entropy;
+  a.g_top = g.top ? g.d_top_logprob : nullptr; a.dx = g.d_logits; a.ldd = g.ldd;
+  const int per = THREADS * BWD_PIECES * (g.dtype == M2_F32 ? 4 : 8);
+  const int slices = (g.vocab + per - 1) / per;
+  M2_REQUIRE(g.rows * slices <= 0x7fffffffLL, M2_ERR_UNSUPPORTED, "m2_token_logprobs_bwd: %lld rows of %d logits are more than the grid takes", g.rows, g.vocab);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (g.dtype == M2_F32) backward_kernel<float><<<(unsigned)(g.rows * slices), THREADS, 0, st>>>(a, slices);
+  else backward_kernel<__nv_bfloat16><<<(unsigned)(g.rows * slices), THREADS, 0, st>>>(a, slices);
+  M2_LAUNCH_CHECK("m2_token_logprobs_bwd");
+  return M2_OK;
+}

@@ -1,0 +1,181 @@
+"""Linear attention with a decay for each head: a causal sequence mixer whose state has a fixed size, beside the long
+convolutions of MonarchMixerSequenceMixing (the reference's only mixer, bert/src/mm/monarch_mixer_sequence_mixer.py:100-154).
+
+    S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,        o_t = scale q_t^T S_t
+
+linear_attention() takes whole sequences (prompts, training: it has gradients), linear_attention_step() one token of each.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+
+
+def _check(name, q, k, v, log_decay, dims):
+    """(B, H, kv heads, dk, dv, scale's default) of q (B, [L,] H, dk), k and v."""
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ValueError(f"{name}: q, k and v have {dims} dimensions, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    B, (H, dk), (K, dv) = q.shape[0], q.shape[-2:], v.shape[-2:]
+    if k.shape != (*q.shape[:-2], K, dk) or v.shape[:-2] != q.shape[:-2] or K == 0 or H % max(K, 1):
+        raise ValueError(f"{name}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} of q, k and v do not belong together")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{name}: q, k and v are all float32 or all bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if log_decay.shape != (H,):
+        raise ValueError(f"{name}: log_decay has one value for each of the {H} heads, got shape {tuple(log_decay.shape)}")
+    dev = q.device
+    if not q.is_cuda or k.device != dev or v.device != dev or log_decay.device != dev:
+        raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: the decay is a constant of the head and has no gradient; pass log_decay.detach()")
+    return B, H, K, dk, dv
+
+
+def _state(name, s, what, shape, dev):
+    if s.shape != shape or s.dtype != torch.float32 or s.device != dev:
+        raise ValueError(f"{name}: {what} is a float32 tensor {tuple(shape)} on {dev}, got {s.dtype} {tuple(s.shape)} on {s.device}")
+
+
+def _packed(t):
+    """t with contiguous channels."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay(log_decay):
+    return log_decay if log_decay.dtype == torch.float32 and log_decay.is_contiguous() else ops._f32c(log_decay)
+
+
+def _args(q, k, v, log_decay, scale, initial, lengths):
+    B, L, H, dk = q.shape
+    K, dv = v.shape[2:]
+    a = _lib.LinearAttentionArgs()
+    a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv = B, L, H, K, dk, dv
+    a.dtype, a.scale = ops._dt(q), scale
+    a.q, (a.q_sb, a.q_st, a.q_sh, _) = q.data_ptr(), q.stride()
+    a.k, (a.k_sb, a.k_st, a.k_sh, _) = k.data_ptr(), k.stride()
+    a.v, (a.v_sb, a.v_st, a.v_sh, _) = v.data_ptr(), v.stride()
+    a.log_decay = log_decay.data_ptr()
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
+    if initial is not None:
+        a.state_in = initial.data_ptr()
+    return a
+
+
+def _workspace(a, dev, backward):
+    n = _lib.lib().m2_linear_attention_workspace(a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv, backward)
+    w = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
+    if w is not None:
+        a.workspace = w.data_ptr()
+    return w
+
+
+def _forward(q, k, v, log_decay, scale, initial, lengths, want_state):
+    B, L, H, dk = q.shape
+    dv = v.shape[3]
+    o = torch.empty((B, L, H, dv), dtype=q.dtype, device=q.device)
+    state = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
+    a = _args(q, k, v, log_decay, scale, initial, lengths)
+    a.o = o.data_ptr()
+    if want_state:
+        a.state_out = state.data_ptr()
+    work = _workspace(a, q.device, 0)  # noqa: F841  (alive until the launch)
+    ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a))
+    return o, state
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, initial, lengths, want_state):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, initial, lengths)
+        ctx.scale = scale
+        return _forward(q, k, v, log_decay, scale, initial, lengths, want_state)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_o, d_state):
+        q, k, v, log_decay, initial, lengths = ctx.saved_tensors
+        B, L, H, dk = q.shape
+        if d_o is None and d_state is None:
+            return (None,) * 8
+        d_o = torch.zeros((B, L, H, v.shape[3]), dtype=q.dtype, device=q.device) if d_o is None else _packed(d_o)
+        a = _args(q, k, v, log_decay, ctx.scale, initial, lengths)
+        g = _lib.LinearAttentionGrads()
+        g.d_o, (g.o_sb, g.o_st, g.o_sh, _) = d_o.data_ptr(), d_o.stride()
+        if d_state is not None:
+            d_state = d_state.contiguous()
+            g.d_state_out = d_state.data_ptr()
+        dq, dk_, dv_ = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        g.d_q, g.d_k, g.d_v = dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr()
+        d_initial = torch.empty_like(initial) if initial is not None else None
+        if d_initial is not None:
+            g.d_state_in = d_initial.data_ptr()
+        work = _workspace(a, q.device, 1)  # noqa: F841
+        ops._launch("m2_linear_attention_bwd", q, _lib.lib().m2_linear_attention_bwd, C.byref(a), C.byref(g), launches=3)
+        return dq, dk_, dv_, None, None, d_initial, None, None
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
+    """o (B, L, H, dv) for q (B, L, H, dk), k (B, L, K, dk), v (B, L, K, dv), all float32 or all bfloat16, any strides
+    (contiguous channels are read in place); K divides H, head h reads key head h // (H // K); dk, dv <= 128.
+
+    log_decay      (H,) float: log of the factor by which a head's state fades with every token, <= 0; a constant, not trained
+    scale          default dk ** -0.5
+    initial_state  None (zero) or (B, H, dk, dv) float32: what earlier calls left
+    lengths        None or (B,) integers: tokens of every sequence.  What lies behind them is not read; rows of o behind them
+                   are zero and the state is that behind the last token
+    return_state   also return the state behind the last token, (B, H, dk, dv) float32
+
+    Differentiable in q, k, v and initial_state."""
+    name = "linear_attention"
+    B, H, K, dk, dv = _check(name, q, k, v, log_decay, 4)
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale == 0 or not math.isfinite(scale):
+        raise ValueError(f"{name}: scale {scale}")
+    if initial_state is not None:
+        _state(name, initial_state, "initial_state", (B, H, dk, dv), q.device)
+        initial_state = initial_state.contiguous()
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != q.device:
+            raise ValueError(f"{name}: lengths are ({B},) integers on {q.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
+        lengths = lengths.to(torch.long).contiguous()
+    q, k, v = _packed(q), _packed(k), _packed(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (initial_state is not None and initial_state.requires_grad)):
+        o, state = _LinearAttention.apply(q, k, v, _decay(log_decay), scale, initial_state, lengths, return_state)
+    else:
+        o, state = _forward(q, k, v, _decay(log_decay), scale, initial_state, lengths, return_state)
+    return (o, state) if return_state else o
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
+    """One token of each sequence: q (B, H, dk), k (B, K, dk), v (B, K, dv) -> o (B, H, dv).  `state` (B, H, dk, dv) float32,
+    its last two dimensions packed, is updated in place.  It has no gradient: linear_attention(initial_state=...) has."""
+    name = "linear_attention_step"
+    B, H, K, dk, dv = _check(name, q, k, v, log_decay, 3)
+    _state(name, state, "state", (B, H, dk, dv), q.device)
+    s_b, s_h, s_i, s_j = state.stride()
+    size = dk * dv
+    if (s_j != 1 and dv > 1) or (s_i != dv and dk > 1) or (H > 1 and s_h < size) or (B > 1 and s_b < size) or \
+            (B > 1 and H > 1 and s_b < H * s_h and s_h < B * s_b):
+        raise ValueError(f"{name}: state is updated in place: its last two dimensions are packed and no two heads overlap, got strides {state.stride()}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or linear_attention with initial_state")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    q, k, v, ld = _packed(q), _packed(k), _packed(v), _decay(log_decay)
+    o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
+    a = _lib.LinearAttentionStepArgs()
+    a.batch, a.heads, a.kv_heads, a.dk, a.dv = B, H, K, dk, dv
+    a.dtype, a.scale = ops._dt(q), scale
+    a.q, (a.q_sb, a.q_sh, _) = q.data_ptr(), q.stride()
+    a.k, (a.k_sb, a.k_sh, _) = k.data_ptr(), k.stride()
+    a.v, (a.v_sb, a.v_sh, _) = v.data_ptr(), v.stride()
+    a.log_decay, a.state, a.s_b, a.s_h, a.o = ld.data_ptr(), state.data_ptr(), s_b, s_h, o.data_ptr()
+    ops._launch("m2_linear_attention_step", q, _lib.lib().m2_linear_attention_step, C.byref(a))
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+    return o
