@@ -32,7 +32,7 @@ struct Scan {
   float* segments;                       // (batch * heads, n_seg, dk, dv): every segment's own sum, where n_seg > 1
   int n_seg, seg_chunks;
   int sums_only;                         // first of the two launches over segments
-  int wide;                              // rows of q, k, v start on 16-byte boundaries and are whole 16-byte pieces
+  int wide, o_wide;                      // rows of q, k and v (of o) start on 16-byte boundaries and are whole 16-byte pieces
 };
 
 __device__ __forceinline__ float power(float ld, int n) { return n == 0 ? 1.f : expf(ld * n); }
@@ -59,7 +59,6 @@ __device__ __forceinline__ void mac(float (&acc)[4][4], const float4& a, const f
 }
 __device__ __forceinline__ float4 f4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-template <typename T>
 __global__ void __launch_bounds__(256)
 scan_f32_kernel(const Scan a) {
   extern __shared__ float sm[];
@@ -76,9 +75,9 @@ scan_f32_kernel(const Scan a) {
   const int cols = min(DVT, a.dv - col0);
   const int n = seq_length(a, b);
   const float ld = a.log_decay[h];
-  const T* q = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)(h / a.q.div) * a.q.sh;
-  const T* k = static_cast<const T*>(a.k.p) + b * a.k.sb + (long long)(h / a.k.div) * a.k.sh;
-  const T* v = static_cast<const T*>(a.v.p) + b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + col0;
+  const float* q = static_cast<const float*>(a.q.p) + b * a.q.sb + (long long)(h / a.q.div) * a.q.sh;
+  const float* k = static_cast<const float*>(a.k.p) + b * a.k.sb + (long long)(h / a.k.div) * a.k.sh;
+  const float* v = static_cast<const float*>(a.v.p) + b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + col0;
   const int seg_len = a.seg_chunks * C;
   const int at0 = min(seg * seg_len, a.len), at1 = min(at0 + seg_len, a.len);       // places of this segment, in scan order
   const bool last = n <= at1 && (n > at0 || (n == 0 && seg == 0));                  // holds the last token
@@ -111,8 +110,8 @@ scan_f32_kernel(const Scan a) {
       float x = 0.f, y = 0.f;
       if (t < m && i < a.dk) {
         const long long tok = a.reverse ? n - 1 - at - t : at + t;
-        y = ld_as_float(k + tok * a.k.st + i);
-        if (!a.sums_only) x = ld_as_float(q + tok * a.q.st + i);
+        y = __ldg(k + tok * a.k.st + i);
+        if (!a.sums_only) x = __ldg(q + tok * a.q.st + i);
       }
       qt[i * LD + t] = x;
       kt[i * LD + t] = y;
@@ -120,7 +119,7 @@ scan_f32_kernel(const Scan a) {
     for (int e = tid; e < C * DVT; e += 256) {
       const int t = e / DVT, j = e - t * DVT;
       const long long tok = a.reverse ? n - 1 - at - t : at + t;
-      vs[t * LD + j] = t < m && j < cols ? ld_as_float(v + tok * a.v.st + j) : 0.f;
+      vs[t * LD + j] = t < m && j < cols ? __ldg(v + tok * a.v.st + j) : 0.f;
     }
     __syncthreads();
     if (!a.sums_only) {
@@ -153,8 +152,7 @@ scan_f32_kernel(const Scan a) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           if (tx * 4 + y >= cols) continue;
-          if (a.o_f32) static_cast<float*>(a.o)[to + y] = a.scale * o[x][y];
-          else st_from_float(static_cast<T*>(a.o) + to + y, a.scale * o[x][y]);
+          static_cast<float*>(a.o)[to + y] = a.scale * o[x][y];
         }
       }
       __syncthreads();                                                              // st is read by all
@@ -190,8 +188,318 @@ scan_f32_kernel(const Scan a) {
   // rows behind the last token are zero
   const int dead0 = max(at0, n);
   for (long long e = tid; e < (long long)(at1 - dead0) * cols; e += 256) {
+    static_cast<float*>(a.o)[b * a.o_sb + (dead0 + e / cols) * a.o_st + h * a.o_sh + col0 + e % cols] = 0.f;
+  }
+}
+
+// ---- bf16: products on the tensor cores ------------------------------------------------------------------------------------------------
+// A block of 4 warps keeps the columns [col0, col0 + 64) of one (sequence, head) and walks over the chunks; warp w has rows
+// 16 w .. 16 w + 15 of a chunk and rows w DK / 4 .. of the state, whose float32 values stay in its registers.  q, k and v tiles
+// arrive by cp.async one chunk ahead.  A chunk's weights P = (q k^T) decay never leave the registers: the accumulators of q k^T are
+// the operand of P v.  Every warp needs the whole state as an operand: it goes through shared memory as bf16, into the other one of
+// two buffers, so that a chunk has a single block barrier.
+//
+// Why mma.sync: the scan is bound by its bytes.  A token and head of 64 + 64 channels moves 512 bytes, 11.6 ns of an SM's share of
+// 6.5 TB/s, and takes 26 kFLOP (mean), 7 ns at the 555 TFLOP/s that mma.sync reaches on a B200; tiles of 64 tokens whose products
+// feed each other through registers fit it, where tcgen05 would take every product through tensor and shared memory.
+//
+// The state is a sum over thousands of tokens, so nothing of it is rounded to bf16: l^(C-1-j) k_j goes into its product as two or
+// (where the state is returned) three bf16 parts, 16 or 24 bits, and every chunk's sum starts from zero and is added in float32, as
+// tensor cores cut their sums instead of rounding them.
+constexpr int QK_LD(int dk) { return dk * 2; }             // bytes of a tile's row
+
+__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ float lo_of(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float hi_of(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Byte of (row, 16-byte piece) of a tile: pieces are permuted inside 128 bytes, so that 8 rows of one piece lie in different banks.
+template <int LDB> __device__ __forceinline__ int at_piece(int row, int piece) { return row * LDB + ((piece ^ (row & 7)) << 4); }
+
+// C rows of up to LDB / 2 channels; rows from m on and channels from d on are zero.  Row r is token t0 + r dir.
+template <int LDB> __device__ __forceinline__ void load_tile(char* tile, const __nv_bfloat16* p, long long st, long long t0, int dir, int m, int d, bool wide) {
+  constexpr int PIECES = LDB / 16;
+  for (int e = threadIdx.x; e < C * PIECES; e += 128) {
+    const int r = e / PIECES, c = e - r * PIECES;
+    const bool on = r < m && c * 8 < d;
+    const __nv_bfloat16* src = p + (t0 + (long long)(on ? r : 0) * dir) * st + (on ? c * 8 : 0);
+    char* dst = tile + at_piece<LDB>(r, c);
+    if (wide) {
+      cp16(saddr(dst), src, on);
+    } else {
+      uint32_t w[4] = {};
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c * 8 + i < d) w[i >> 1] |= (uint32_t)__bfloat16_as_ushort(src[i]) << (16 * (i & 1));
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <int DK> struct MmaSmem {
+  static constexpr int TILE = C * DK * 2, VT = C * DVT * 2, STAGE = 2 * TILE + VT, STATE = DK * DVT * 2;
+  static constexpr int BYTES = 2 * STAGE + 2 * STATE + (C + 8) * 4;
+};
+
+template <int DK, int PARTS>
+__global__ void __launch_bounds__(128)
+scan_mma_kernel(const Scan a) {
+  extern __shared__ __align__(128) char smem[];
+  typedef MmaSmem<DK> L;
+  constexpr int LK = DK * 2, LV = DVT * 2, MT = DK / 64, KS = DK / 16, NT = DVT / 8;
+  float* pw = reinterpret_cast<float*>(smem + 2 * L::STAGE + 2 * L::STATE);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int bh = blockIdx.z, b = bh / a.heads, h = bh - b * a.heads;
+  const int seg = blockIdx.y, col0 = blockIdx.x * DVT;
+  const int cols = min(DVT, a.dv - col0);
+  const int n = seq_length(a, b);
+  const float ld = a.log_decay[h];
+  typedef __nv_bfloat16 T;
+  const T* q = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)(h / a.q.div) * a.q.sh;
+  const T* k = static_cast<const T*>(a.k.p) + b * a.k.sb + (long long)(h / a.k.div) * a.k.sh;
+  const T* v = static_cast<const T*>(a.v.p) + b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + col0;
+  const int seg_len = a.seg_chunks * C;
+  const int at0 = min(seg * seg_len, a.len), at1 = min(at0 + seg_len, a.len);       // places of this segment, in scan order
+  const bool last = n <= at1 && (n > at0 || (n == 0 && seg == 0));                  // holds the last token
+  if (a.sums_only && (n <= at1 || seg == a.n_seg - 1)) return;                      // nobody reads the last segment's sum
+  const int first = a.reverse && a.init ? 1 : 0;                                    // the given state is one step younger
+  const int end = min(at1, n), dir = a.reverse ? -1 : 1;
+  auto token = [&](int at) { return (long long)(a.reverse ? n - 1 - at : at); };
+  auto fetch = [&](int at, int stage) {
+    char* s = smem + stage * L::STAGE;
+    const int m = min(C, end - at);
+    if (!a.sums_only) load_tile<LK>(s, q, a.q.st, token(at), dir, m, a.dk, a.wide);
+    load_tile<LK>(s + L::TILE, k, a.k.st, token(at), dir, m, a.dk, a.wide);
+    load_tile<LV>(s + 2 * L::TILE, v, a.v.st, token(at), dir, m, cols, a.wide);
+    cp_commit();
+  };
+  if (at0 < end) fetch(at0, 0);
+  for (int i = tid; i <= C; i += 128) pw[i] = power(ld, i);
+  // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1)
+  float s[MT][NT][4];
+  {
+    const float carry = power_m1(ld, seg_len), carry0 = power_m1(ld, seg_len - first);
+    const bool any = !a.sums_only && (n > at0 || last);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = (w * MT + mt) * 16 + g + 8 * (e >> 1), j = nt * 8 + 2 * t4 + (e & 1);
+          float x = 0.f;
+          if (any && i < a.dk && j < cols) {
+            if (a.init) x = a.init_scale * a.init[b * a.s_b + h * a.s_h + i * a.s_i + (col0 + j) * a.s_j];
+            const float* p = a.segments + ((long long)bh * a.n_seg * a.dk + i) * a.dv + col0 + j;
+            for (int r = 0; r < seg; ++r) x = fmaf(x, r ? carry : carry0, x) + p[(long long)r * a.dk * a.dv];
+          }
+          s[mt][nt][e] = x;
+        }
+  }
+  char* state = smem + 2 * L::STAGE;
+  auto write_state = [&](char* to) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = (w * MT + mt) * 16 + g + 8 * e;
+          *reinterpret_cast<uint32_t*>(to + at_piece<LV>(i, nt) + 4 * t4) = pack2(s[mt][nt][2 * e], s[mt][nt][2 * e + 1]);
+        }
+  };
+  if (!a.sums_only) write_state(state);
+  __syncthreads();                                                                  // pw
+  // decays of this thread's weights: inside the diagonal 16 x 16 block, and l^(i-j+15) for the blocks before it
+  float near[2][4], far[2][4];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int gap = g + 8 * (e >> 1) - (x * 8 + 2 * t4 + (e & 1));
+      near[x][e] = gap >= 0 ? pw[gap] : 0.f;
+      far[x][e] = pw[gap + 15];
+    }
+  int stage = 0;
+  for (int at = at0; at < end; at += C, stage ^= 1) {
+    const int m = min(C, end - at);
+    const int young = at == 0 ? first : 0;
+    cp_wait0();
+    __syncthreads();
+    if (at + C < end) fetch(at + C, stage ^ 1);
+    char* qs = smem + stage * L::STAGE;
+    const uint32_t q_at = saddr(qs), k_at = saddr(qs + L::TILE), v_at = saddr(qs + 2 * L::TILE), s_at = saddr(state + stage * L::STATE);
+    const int r8 = lane & 7, half = (lane >> 3) & 1, quad = lane >> 4;
+    if (!a.sums_only) {
+      uint32_t qf[KS][4];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) ldsm(qf[ks], q_at + at_piece<LK>(w * 16 + (lane & 15), ks * 2 + quad));
+      float o[NT][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          uint32_t f[4];
+          ldsm_t(f, s_at + at_piece<LV>(ks * 16 + r8 + 8 * half, np * 2 + quad));
+          mma(o[2 * np], qf[ks], f[0], f[1]);
+          mma(o[2 * np + 1], qf[ks], f[2], f[3]);
+        }
+      const float d0 = pw[w * 16 + g + 1 - young], d1 = pw[w * 16 + g + 9 - young];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) { o[nt][0] *= d0; o[nt][1] *= d0; o[nt][2] *= d1; o[nt][3] *= d1; }
+      for (int jb = 0; jb <= w; ++jb) {                                             // 16 tokens of k and v at a time
+        float p[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t f[4];
+          ldsm(f, k_at + at_piece<LK>(jb * 16 + r8 + 8 * quad, ks * 2 + half));
+          mma(p[0], qf[ks], f[0], f[1]);
+          mma(p[1], qf[ks], f[2], f[3]);
+        }
+        if (jb == w) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[x][e] = near[x][e] == 0.f ? 0.f : p[x][e] * near[x][e];
+        } else {
+          const float f = pw[16 * (w - jb) - 15];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[x][e] *= f * far[x][e];
+        }
+        const uint32_t pf[4] = {pack2(p[0][0], p[0][1]), pack2(p[0][2], p[0][3]), pack2(p[1][0], p[1][1]), pack2(p[1][2], p[1][3])};
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          uint32_t f[4];
+          ldsm_t(f, v_at + at_piece<LV>(jb * 16 + r8 + 8 * half, np * 2 + quad));
+          mma(o[2 * np], pf, f[0], f[1]);
+          mma(o[2 * np + 1], pf, f[2], f[3]);
+        }
+      }
+      if (a.o_f32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = w * 16 + g + 8 * (e >> 1);
+          if (r >= m) continue;
+          float* to = static_cast<float*>(a.o) + b * a.o_sb + token(at + r) * a.o_st + h * a.o_sh + col0;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int j = nt * 8 + 2 * t4 + (e & 1);
+            if (j < cols) to[j] = a.scale * o[nt][e];
+          }
+        }
+      } else {                                                                      // through this warp's own rows of the q tile
+        __syncwarp();
+        const float c = a.scale;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          *reinterpret_cast<uint32_t*>(qs + at_piece<LK>(w * 16 + g, nt) + 4 * t4) = pack2(c * o[nt][0], c * o[nt][1]);
+          *reinterpret_cast<uint32_t*>(qs + at_piece<LK>(w * 16 + g + 8, nt) + 4 * t4) = pack2(c * o[nt][2], c * o[nt][3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = w * 16 + x * 4 + (lane >> 3), c8 = lane & 7;
+          if (r >= m || c8 * 8 >= cols) continue;
+          const uint4 u = *reinterpret_cast<const uint4*>(qs + at_piece<LK>(r, c8));
+          T* to = static_cast<T*>(a.o) + b * a.o_sb + token(at + r) * a.o_st + h * a.o_sh + col0 + c8 * 8;
+          if (a.o_wide) {
+            *reinterpret_cast<uint4*>(to) = u;
+          } else {
+            const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c8 * 8 + i < cols) to[i] = __ushort_as_bfloat16((unsigned short)(ww[i >> 1] >> (16 * (i & 1))));
+          }
+        }
+      }
+    }
+    // state: k^T (v weighted by age), the weight on k's fragment
+    float acc[MT][NT][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < C / 16; ++ks) {
+      uint32_t kf[MT][PARTS][4];
+      float wt[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) wt[x] = pw[max(0, m - 1 - (ks * 16 + 2 * t4 + (x & 1) + 8 * (x >> 1)))];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t f[4];
+        ldsm_t(f, k_at + at_piece<LK>(ks * 16 + r8 + 8 * quad, (w * MT + mt) * 2 + half));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float lo = lo_of(f[x]) * wt[2 * (x >> 1)], hi = hi_of(f[x]) * wt[2 * (x >> 1) + 1];
+#pragma unroll
+          for (int y = 0; y < PARTS; ++y) {
+            const uint32_t u = pack2(lo, hi);
+            kf[mt][y][x] = u;
+            lo -= lo_of(u);
+            hi -= hi_of(u);
+          }
+        }
+      }
+#pragma unroll
+      for (int np = 0; np < NT / 2; ++np) {
+        uint32_t f[4];
+        ldsm_t(f, v_at + at_piece<LV>(ks * 16 + r8 + 8 * half, np * 2 + quad));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int y = PARTS - 1; y >= 0; --y) {
+            mma(acc[mt][2 * np], kf[mt][y], f[0], f[1]);
+            mma(acc[mt][2 * np + 1], kf[mt][y], f[2], f[3]);
+          }
+      }
+    }
+    const float keep = power_m1(ld, m - young);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] = fmaf(s[mt][nt][e], keep, s[mt][nt][e]) + acc[mt][nt][e];
+    if (!a.sums_only && at + C < end) write_state(state + (stage ^ 1) * L::STATE);
+  }
+  const float f = a.sums_only ? 1.f : a.final_scale * (a.reverse ? power(ld, n == 0 && a.init ? 0 : 1) : 1.f);
+  float* to = a.sums_only ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.final && last ? a.final + b * a.s_b + h * a.s_h : nullptr;
+  const long long s_i = a.sums_only ? a.dv : a.s_i, s_j = a.sums_only ? 1 : a.s_j;
+  if (to) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = (w * MT + mt) * 16 + g + 8 * (e >> 1), j = nt * 8 + 2 * t4 + (e & 1);
+          if (i < a.dk && j < cols) to[i * s_i + (col0 + j) * s_j] = f * s[mt][nt][e];
+        }
+  }
+  if (a.sums_only) return;
+  const int dead0 = max(at0, n);                                                    // rows behind the last token are zero
+  for (long long e = tid; e < (long long)(at1 - dead0) * cols; e += 128) {
     const long long to = b * a.o_sb + (dead0 + e / cols) * a.o_st + h * a.o_sh + col0 + e % cols;
-    if (a.o_f32) static_cast<float*>(a.o)[to] = 0.f; else st_from_float(static_cast<T*>(a.o) + to, 0.f);
+    if (a.o_f32) static_cast<float*>(a.o)[to] = 0.f; else static_cast<T*>(a.o)[to] = __float2bfloat16_rn(0.f);
   }
 }
 
@@ -282,20 +590,40 @@ static long long segment_floats(int batch, int heads, int dk, int dv, int len) {
   return n > 1 ? (long long)batch * heads * n * dk * dv : 0;
 }
 
+// Rows in 16-byte pieces: cp.async copies them, and reads no more than them.
+static bool in_pieces(const void* p, long long sb, long long st, long long sh, int d) {
+  return m2_aligned(p, 16) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && d % 8 == 0;
+}
+
+template <int DK, int PARTS> static int launch_mma(const char* name, const Scan& a, dim3 grid, cudaStream_t st) {
+  M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS>), MmaSmem<DK>::BYTES);
+  scan_mma_kernel<DK, PARTS><<<grid, 128, MmaSmem<DK>::BYTES, st>>>(a);
+  M2_LAUNCH_CHECK(name);
+  return M2_OK;
+}
+
 static int run_scan(const char* name, Scan a, int dtype, float* segments, cudaStream_t st) {
   segments_of(a.batch, a.heads, a.dv, a.len, &a.n_seg, &a.seg_chunks);
   a.segments = a.n_seg > 1 ? segments : nullptr;
+  const dim3 grid((a.dv + DVT - 1) / DVT, a.n_seg, a.batch * a.heads);
+  a.wide = in_pieces(a.q.p, a.q.sb, a.q.st, a.q.sh, a.dk) && in_pieces(a.k.p, a.k.sb, a.k.st, a.k.sh, a.dk) && in_pieces(a.v.p, a.v.sb, a.v.st, a.v.sh, a.dv);
+  a.o_wide = in_pieces(a.o, a.o_sb, a.o_st, a.o_sh, a.dv);
+  if (dtype == M2_BF16) {
+    for (a.sums_only = a.n_seg > 1; a.sums_only >= 0; --a.sums_only) {
+      const int rc = a.dk <= 64 ? (a.final ? launch_mma<64, 3>(name, a, grid, st) : launch_mma<64, 2>(name, a, grid, st))
+                                : (a.final ? launch_mma<128, 3>(name, a, grid, st) : launch_mma<128, 2>(name, a, grid, st));
+      if (rc) return rc;
+    }
+    return M2_OK;
+  }
   const int dkp = (a.dk + 15) / 16 * 16;
   const size_t smem = ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float);
-  const dim3 grid((a.dv + DVT - 1) / DVT, a.n_seg, a.batch * a.heads);
   constexpr size_t most = ((size_t)(3 * MAX_D + 2 * C) * LD + C + 4) * sizeof(float);
-  M2_SMEM_ONCE(scan_f32_kernel<float>, most);
-  M2_SMEM_ONCE(scan_f32_kernel<__nv_bfloat16>, most);
+  M2_SMEM_ONCE(scan_f32_kernel, most);
   for (a.sums_only = a.n_seg > 1; a.sums_only >= 0; --a.sums_only) {
-    if (dtype == M2_F32) scan_f32_kernel<float><<<grid, 256, smem, st>>>(a);
-    else scan_f32_kernel<__nv_bfloat16><<<grid, 256, smem, st>>>(a);
+    scan_f32_kernel<<<grid, 256, smem, st>>>(a);
+    M2_LAUNCH_CHECK(name);
   }
-  M2_LAUNCH_CHECK(name);
   return M2_OK;
 }
 
