@@ -534,7 +534,7 @@ int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_residual_no
  * masked-LM head (bert/src/bert_layers.py, BertForMaskedLM: cross entropy over the masked positions).
  *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), row stride ld; targets int64 (rows).
  *   logprob, entropy float32 (rows); top_logprob float32 and top_id int64 (rows, top), best first, equal values by ascending
- *   id, NaN before all (top <= 32 and <= vocab).  stats float32 (rows, 2): maximum and log of the sum, for the gradient.
+ *   id, NaN before all (top <= 32 and <= vocab).  stats NULL, or float32 (rows, 2): maximum and log of the sum, for the gradient.
  * A row whose target is ignore_index is not read: zeros, ids -1.  A target outside the vocabulary: logprob is NaN and
  * M2_DEV_BAD_INDEX is set.  Logits of -inf have probability 0; where all are, log probabilities are -inf, the entropy 0 and the
  * gradient 0.  NaN or +inf among the logits make the row's probabilities NaN.  Everything is summed in float32.

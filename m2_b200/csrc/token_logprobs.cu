@@ -271,8 +271,7 @@ forward_kernel(const Args a) {
       if (tid == 0) {
         a.logprob[row] = 0.f;
         a.entropy[row] = 0.f;
-        a.stats[2 * row] = 0.f;
-        a.stats[2 * row + 1] = 0.f;
+        if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.f;
       }
       if (tid < a.top) { a.top_lp[row * a.top + tid] = 0.f; a.top_id[row * a.top + tid] = -1; }
     }
@@ -329,8 +328,10 @@ forward_kernel(const Args a) {
       if (!good) atomicOr(&m2_dev_status_word, ST_BAD_TARGET);
       a.logprob[row] = good ? logp(load1(x + target)) : __int_as_float(0x7fffffff);
       a.entropy[row] = none ? 0.f : log_s - st.t / st.s;
-      a.stats[2 * row] = st.m;
-      a.stats[2 * row + 1] = none ? -minus_inf : log_s;                    // +inf: every probability is 0
+      if (a.stats) {
+        a.stats[2 * row] = st.m;
+        a.stats[2 * row + 1] = none ? -minus_inf : log_s;                  // +inf: every probability is 0
+      }
     }
     if constexpr (TOP) {
       if (split == 1) {
@@ -454,7 +455,7 @@ extern "C" int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* s
   const m2_token_logprobs_args& g = *args;
   if (int rc = check("m2_token_logprobs_fwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
   if (g.rows == 0) return M2_OK;
-  M2_REQUIRE(g.logprob && g.entropy && g.stats && (g.top == 0 || (g.top_logprob && g.top_id)), M2_ERR_ARG, "m2_token_logprobs_fwd: an output is NULL");
+  M2_REQUIRE(g.logprob && g.entropy && (g.top == 0 || (g.top_logprob && g.top_id)), M2_ERR_ARG, "m2_token_logprobs_fwd: an output is NULL");
   Args a;
   a.x = g.logits; a.ld = g.ld; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
   a.logprob = g.logprob; a.entropy = g.entropy; a.stats = g.stats; a.top_lp = g.top_logprob; a.top_id = (long long*)g.top_id;

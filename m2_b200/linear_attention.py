@@ -16,19 +16,23 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 
 
+_TYPES = {torch.float32: _lib.M2_F32, torch.bfloat16: _lib.M2_BF16}
+
+
 def _check(name, q, k, v, log_decay, dims):
-    """(B, H, kv heads, dk, dv, scale's default) of q (B, [L,] H, dk), k and v."""
-    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
-        raise ValueError(f"{name}: q, k and v have {dims} dimensions, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    B, (H, dk), (K, dv) = q.shape[0], q.shape[-2:], v.shape[-2:]
-    if k.shape != (*q.shape[:-2], K, dk) or v.shape[:-2] != q.shape[:-2] or K == 0 or H % max(K, 1):
-        raise ValueError(f"{name}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} of q, k and v do not belong together")
-    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    """(B, H, kv heads, dk, dv) of q (B, [L,] H, dk), k and v."""
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
+        raise ValueError(f"{name}: q, k and v have {dims} dimensions, got {tuple(qs)}, {tuple(ks)} and {tuple(vs)}")
+    B, (H, dk), (K, dv) = qs[0], qs[-2:], vs[-2:]
+    if ks[:-2] != qs[:-2] or ks[-2] != K or ks[-1] != dk or vs[:-2] != qs[:-2] or K == 0 or H % K:
+        raise ValueError(f"{name}: shapes {tuple(qs)}, {tuple(ks)} and {tuple(vs)} of q, k and v do not belong together")
+    if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"{name}: q, k and v are all float32 or all bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
     if log_decay.shape != (H,):
         raise ValueError(f"{name}: log_decay has one value for each of the {H} heads, got shape {tuple(log_decay.shape)}")
-    dev = q.device
-    if not q.is_cuda or k.device != dev or v.device != dev or log_decay.device != dev:
+    dev = q.get_device()
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or log_decay.get_device() != dev:
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name}: the decay is a constant of the head and has no gradient; pass log_decay.detach()")
@@ -36,8 +40,8 @@ def _check(name, q, k, v, log_decay, dims):
 
 
 def _state(name, s, what, shape, dev):
-    if s.shape != shape or s.dtype != torch.float32 or s.device != dev:
-        raise ValueError(f"{name}: {what} is a float32 tensor {tuple(shape)} on {dev}, got {s.dtype} {tuple(s.shape)} on {s.device}")
+    if s.shape != shape or s.dtype != torch.float32 or s.get_device() != dev:
+        raise ValueError(f"{name}: {what} is a float32 tensor {tuple(shape)} on device {dev}, got {s.dtype} {tuple(s.shape)} on {s.device}")
 
 
 def _packed(t):
@@ -49,21 +53,13 @@ def _decay(log_decay):
     return log_decay if log_decay.dtype == torch.float32 and log_decay.is_contiguous() else ops._f32c(log_decay)
 
 
-def _args(q, k, v, log_decay, scale, initial, lengths):
+def _args(q, k, v, log_decay, scale, initial, lengths, o=None, state=None):
     B, L, H, dk = q.shape
     K, dv = v.shape[2:]
-    a = _lib.LinearAttentionArgs()
-    a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv = B, L, H, K, dk, dv
-    a.dtype, a.scale = ops._dt(q), scale
-    a.q, (a.q_sb, a.q_st, a.q_sh, _) = q.data_ptr(), q.stride()
-    a.k, (a.k_sb, a.k_st, a.k_sh, _) = k.data_ptr(), k.stride()
-    a.v, (a.v_sb, a.v_st, a.v_sh, _) = v.data_ptr(), v.stride()
-    a.log_decay = log_decay.data_ptr()
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    if initial is not None:
-        a.state_in = initial.data_ptr()
-    return a
+    return _lib.LinearAttentionArgs(
+        B, L, H, K, dk, dv, _TYPES[q.dtype], scale, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+        log_decay.data_ptr(), lengths.data_ptr() if lengths is not None else None, initial.data_ptr() if initial is not None else None,
+        o.data_ptr() if o is not None else None, state.data_ptr() if state is not None else None)
 
 
 def _workspace(a, dev, backward):
@@ -77,12 +73,9 @@ def _workspace(a, dev, backward):
 def _forward(q, k, v, log_decay, scale, initial, lengths, want_state):
     B, L, H, dk = q.shape
     dv = v.shape[3]
-    o = torch.empty((B, L, H, dv), dtype=q.dtype, device=q.device)
+    o = q.new_empty((B, L, H, dv))
     state = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
-    a = _args(q, k, v, log_decay, scale, initial, lengths)
-    a.o = o.data_ptr()
-    if want_state:
-        a.state_out = state.data_ptr()
+    a = _args(q, k, v, log_decay, scale, initial, lengths, o, state)
     work = _workspace(a, q.device, 0)  # noqa: F841  (alive until the launch)
     ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a))
     return o, state
@@ -138,7 +131,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
     if scale == 0 or not math.isfinite(scale):
         raise ValueError(f"{name}: scale {scale}")
     if initial_state is not None:
-        _state(name, initial_state, "initial_state", (B, H, dk, dv), q.device)
+        _state(name, initial_state, "initial_state", (B, H, dk, dv), q.get_device())
         initial_state = initial_state.contiguous()
     if lengths is not None:
         if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != q.device:
@@ -157,7 +150,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
     its last two dimensions packed, is updated in place.  It has no gradient: linear_attention(initial_state=...) has."""
     name = "linear_attention_step"
     B, H, K, dk, dv = _check(name, q, k, v, log_decay, 3)
-    _state(name, state, "state", (B, H, dk, dv), q.device)
+    _state(name, state, "state", (B, H, dk, dv), q.get_device())
     s_b, s_h, s_i, s_j = state.stride()
     size = dk * dv
     if (s_j != 1 and dv > 1) or (s_i != dv and dk > 1) or (H > 1 and s_h < size) or (B > 1 and s_b < size) or \
@@ -167,14 +160,10 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or linear_attention with initial_state")
     scale = dk ** -0.5 if scale is None else float(scale)
     q, k, v, ld = _packed(q), _packed(k), _packed(v), _decay(log_decay)
-    o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
-    a = _lib.LinearAttentionStepArgs()
-    a.batch, a.heads, a.kv_heads, a.dk, a.dv = B, H, K, dk, dv
-    a.dtype, a.scale = ops._dt(q), scale
-    a.q, (a.q_sb, a.q_sh, _) = q.data_ptr(), q.stride()
-    a.k, (a.k_sb, a.k_sh, _) = k.data_ptr(), k.stride()
-    a.v, (a.v_sb, a.v_sh, _) = v.data_ptr(), v.stride()
-    a.log_decay, a.state, a.s_b, a.s_h, a.o = ld.data_ptr(), state.data_ptr(), s_b, s_h, o.data_ptr()
+    o = q.new_empty((B, H, dv))
+    a = _lib.LinearAttentionStepArgs(
+        B, H, K, dk, dv, _TYPES[q.dtype], scale, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
+        ld.data_ptr(), state.data_ptr(), s_b, s_h, o.data_ptr())
     ops._launch("m2_linear_attention_step", q, _lib.lib().m2_linear_attention_step, C.byref(a))
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)

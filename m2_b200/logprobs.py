@@ -22,21 +22,30 @@ class TokenLogprobs(NamedTuple):
     top_id: torch.Tensor
 
 
+_TYPES = {torch.float32: _lib.M2_F32, torch.bfloat16: _lib.M2_BF16}
+
+
 def _rows(logits):
-    t = logits.reshape(-1, logits.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    """logits, or a copy, whose rows lie a fixed distance apart, and that distance."""
+    V = logits.shape[-1]
+    if logits.is_contiguous():
+        return logits, V
+    t = logits.reshape(-1, V)
+    t = t if t.stride(1) == 1 or V == 1 else t.contiguous()
+    return t, t.stride(0)
 
 
-def _forward(x, targets, top, ignore_index, shape):
-    n, dev = x.shape[0], x.device
-    logprob, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
-    best = torch.empty((*shape, top), dtype=torch.float32, device=dev)
-    ids = torch.empty((*shape, top), dtype=torch.long, device=dev)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
-    a = _lib.TokenLogprobsArgs()
-    a.rows, a.vocab, a.top, a.dtype = n, x.shape[1], top, ops._dt(x)
-    a.logits, a.ld, a.targets, a.ignore_index = x.data_ptr(), x.stride(0), targets.data_ptr(), ignore_index
-    a.logprob, a.entropy, a.stats, a.top_logprob, a.top_id = logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), best.data_ptr(), ids.data_ptr()
+def _forward(logits, targets, top, ignore_index, want_stats):
+    """The results and, where they are wanted, what the gradient needs besides."""
+    x, ld = _rows(logits)
+    shape, V = targets.shape, logits.shape[-1]
+    n = targets.numel()
+    logprob = torch.empty(shape, dtype=torch.float32, device=x.device)
+    entropy = torch.empty_like(logprob)
+    best, ids = logprob.new_empty((*shape, top)), targets.new_empty((*shape, top))
+    stats = logprob.new_empty((n, 2)) if want_stats else None
+    a = _lib.TokenLogprobsArgs(n, V, top, _TYPES[x.dtype], x.data_ptr(), ld, targets.data_ptr(), ignore_index, logprob.data_ptr(), entropy.data_ptr(),
+                               stats.data_ptr() if want_stats else None, best.data_ptr(), ids.data_ptr())
     ops._launch("m2_token_logprobs_fwd", x, _lib.lib().m2_token_logprobs_fwd, C.byref(a))
     return TokenLogprobs(logprob, entropy, best, ids), stats
 
@@ -44,8 +53,7 @@ def _forward(x, targets, top, ignore_index, shape):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, ignore_index):
-        x = _rows(logits)
-        out, stats = _forward(x, targets, top, ignore_index, logits.shape[:-1])
+        out, stats = _forward(logits, targets, top, ignore_index, True)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(out.top_id)
         ctx.save_for_backward(logits, targets, stats, out.entropy, out.top_id)
@@ -56,15 +64,13 @@ class _TokenLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_logprob, d_entropy, d_top, _):
         logits, targets, stats, entropy, ids = ctx.saved_tensors
-        x = _rows(logits)
+        x, ld = _rows(logits)
         keep = [t.contiguous() if t is not None else None for t in (d_logprob, d_entropy, d_top)]
         d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a = _lib.TokenLogprobsBwdArgs()
-        a.rows, a.vocab, a.top, a.dtype = x.shape[0], x.shape[1], ids.shape[-1], ops._dt(x)
-        a.logits, a.ld, a.targets, a.ignore_index = x.data_ptr(), x.stride(0), targets.data_ptr(), ctx.ignore_index
-        a.stats, a.entropy, a.top_id = stats.data_ptr(), entropy.data_ptr(), ids.data_ptr()
-        a.d_logprob, a.d_entropy, a.d_top_logprob = (t.data_ptr() if t is not None else None for t in keep)
-        a.d_logits, a.ldd = d.data_ptr(), x.shape[1]
+        V = logits.shape[-1]
+        a = _lib.TokenLogprobsBwdArgs(targets.numel(), V, ids.shape[-1], _TYPES[x.dtype], x.data_ptr(), ld, targets.data_ptr(), ctx.ignore_index,
+                                      stats.data_ptr(), entropy.data_ptr(), ids.data_ptr(), *(t.data_ptr() if t is not None else None for t in keep),
+                                      d.data_ptr(), V)
         ops._launch("m2_token_logprobs_bwd", x, _lib.lib().m2_token_logprobs_bwd, C.byref(a))
         return d, None, None, None
 
@@ -81,16 +87,17 @@ def token_logprobs(logits, targets, *, top=0, ignore_index=-100):
     if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"{name}: one target for each row of logits, got {tuple(targets.shape)} and {tuple(logits.shape)}")
     V = logits.shape[-1]
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype not in _TYPES:
         raise TypeError(f"{name}: logits are float32 or bfloat16, got {logits.dtype}")
-    if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+    if targets.dtype != torch.long and (targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool):
         raise TypeError(f"{name}: targets are integers, got {targets.dtype}")
-    if not logits.is_cuda or targets.device != logits.device:
+    if not logits.is_cuda or targets.get_device() != logits.get_device():
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
     top = int(top)
     if V == 0 or not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"{name}: {top} alternatives of {V} logits (0 to {MAX_TOP}, no more than there are)")
-    targets = targets.to(torch.long).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if targets.dtype != torch.long or not targets.is_contiguous():
+        targets = targets.to(torch.long).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, top, int(ignore_index)))
-    return _forward(_rows(logits), targets, top, int(ignore_index), logits.shape[:-1])[0]
+    return _forward(logits, targets, top, int(ignore_index), False)[0]

@@ -38,10 +38,21 @@ class LaunchProfile:
 def _launch(name, tensor, fn, *args, launches=1):
     """Call one launching C-ABI entry point on torch's current stream of tensor's device."""
     global LAUNCHES
-    index = tensor.device.index
-    if index != torch.cuda.current_device():
+    index = tensor.get_device()
+    if index != torch._C._cuda_getDevice():
+        _need_cuda(tensor)
         with torch.cuda.device(index):
             return _launch(name, tensor, fn, *args, launches=launches)
+    if PROFILE is None and not NVTX:               # the stream's handle without a Stream object around it: 2 us a call
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        rc = _observed_launch(name, index, fn, args)
+    if rc:
+        _lib.check(rc, name)
+    LAUNCHES += launches
+
+
+def _observed_launch(name, index, fn, args):
     st = torch.cuda.current_stream(index)
     prof = PROFILE
     if prof is not None:
@@ -55,9 +66,7 @@ def _launch(name, tensor, fn, *args, launches=1):
     if prof is not None:
         e.record(st)
         prof.events.setdefault(name, []).append((s, e))
-    if rc:
-        _lib.check(rc, name)
-    LAUNCHES += launches
+    return rc
 
 
 def observed():

@@ -16,42 +16,37 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 
 _NONE, _CHANNEL, _SEQUENCE, _TOKEN = 0, 1, 2, 3
-_PARAMS = ("after_weight", "after_bias", "before_weight", "before_bias")
+_VECTORS = ("residual_scale", "after_weight", "after_bias", "before_weight", "before_bias")
+_TYPES = {torch.float32: _lib.M2_F32, torch.bfloat16: _lib.M2_BF16}
 
 
 def _rows(t, n):
-    """t as rows of n contiguous columns, read in place where its strides allow it."""
+    """t, or a copy, whose rows of n contiguous columns lie a fixed distance apart, and that distance."""
+    if t.is_contiguous():
+        return t, n
     t = t.reshape(-1, n)
-    return t if t.stride(1) == 1 or n == 1 else t.contiguous()
+    t = t if t.stride(1) == 1 or n == 1 else t.contiguous()
+    return t, t.stride(0)
 
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _args(x, y, gate, kind, seq_len, scale, params, eps, rms):
+def _args(x, y, gate, kind, seq_len, scale, number, params, eps, rms):
+    """The arguments, and the tensors that they point to."""
     n = x.shape[-1]
-    a = _lib.ResidualNormArgs()
-    a.rows, a.n = x.shape[0], n
-    a.seq_len = seq_len
-    a.x_dtype, a.y_dtype = ops._dt(x), ops._dt(y)
-    a.gate_kind, a.rms, a.eps = kind, rms, eps
-    a.x, a.ldx, a.y, a.ldy = x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0)
-    if kind:
-        a.gate, a.gate_dtype = gate.data_ptr(), ops._dt(gate)
-        a.ldg = gate.stride(0)
-    if isinstance(scale, torch.Tensor):
-        a.scale_channel = scale.data_ptr()
-    else:
-        a.scale = scale
-    a.after_weight, a.after_bias, a.before_weight, a.before_bias = (_ptr(p) for p in params)
-    a.norm_after, a.norm_before = params[0] is not None, params[2] is not None
-    return a
+    (x, ldx), (y, ldy), (gate, ldg) = _rows(x, n), _rows(y, n), _rows(gate, n) if kind else (None, 0)
+    w1, b1, w2, b2 = params
+    a = _lib.ResidualNormArgs(
+        x.numel() // n, seq_len, n, _TYPES[x.dtype], _TYPES[y.dtype], _TYPES[gate.dtype] if kind else 0, kind, rms, w1 is not None, w2 is not None,
+        eps, number, x.data_ptr(), ldx, y.data_ptr(), ldy, gate.data_ptr() if kind else None, ldg, _ptr(scale), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2))
+    return a, (x, y, gate)
 
 
-def _forward(a, x, y, shape, stats):
-    r = torch.empty(shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(shape, dtype=y.dtype, device=x.device) if a.norm_before else None
+def _forward(a, x, y, stats):
+    r = x.new_empty(x.shape)
+    h = y.new_empty(x.shape) if a.norm_before else None
     a.r, a.h, a.stats = r.data_ptr(), _ptr(h), _ptr(stats)
     ops._launch("m2_residual_norm_fwd", x, _lib.lib().m2_residual_norm_fwd, C.byref(a))
     return r, h
@@ -62,13 +57,10 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, after_weight, after_bias, before_weight, before_bias, number, kind, seq_len, eps, rms):
-        n = x.shape[-1]
         params = (after_weight, after_bias, before_weight, before_bias)
-        x2, y2 = _rows(x, n), _rows(y, n)
-        g2 = _rows(gate, n) if kind else None
-        a = _args(x2, y2, g2, kind, seq_len, scale if scale is not None else number, params, eps, rms)
+        a, keep = _args(x, y, gate, kind, seq_len, scale, number, params, eps, rms)  # noqa: F841
         stats = torch.empty((a.rows, 4), dtype=torch.float32, device=x.device)
-        out = _forward(a, x2, y2, x.shape, stats)
+        out = _forward(a, x, y, stats)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, gate, scale, *params, stats)
         ctx.plain = (number, kind, seq_len, eps, rms)
@@ -82,9 +74,7 @@ class _ResidualNorm(torch.autograd.Function):
         if d_r is None and d_h is None:
             return (None,) * 13
         n, dev = x.shape[-1], x.device
-        x2, y2 = _rows(x, n), _rows(y, n)
-        g2 = _rows(gate, n) if kind else None
-        a = _args(x2, y2, g2, kind, seq_len, scale if scale is not None else number, params, eps, rms)
+        a, keep = _args(x, y, gate, kind, seq_len, scale, number, params, eps, rms)  # noqa: F841
         a.stats = stats.data_ptr()
         d_r = d_r.contiguous() if d_r is not None else None
         d_h = d_h.contiguous() if d_h is not None else None
@@ -103,13 +93,11 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def _vector(name, what, t, n, dev):
-    if t is None:
-        return None
-    if t.shape != (n,) or t.device != dev or not t.is_floating_point():
-        raise ValueError(f"{name}: {what} has {n} values on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.shape != (n,) or t.get_device() != dev or not t.is_floating_point():
+        raise ValueError(f"{name}: {what} has {n} values on device {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if t.dtype != torch.float32:
         t = t.float()
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=None, after_bias=None, before_weight=None, before_bias=None,
@@ -127,20 +115,19 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=Non
     name = "gated_residual_norm"
     if x.dim() < 1 or x.shape != y.shape:
         raise ValueError(f"{name}: x and y have one shape, got {tuple(x.shape)} and {tuple(y.shape)}")
-    n, dev = x.shape[-1], x.device
-    if not x.is_cuda or y.device != dev or (gate is not None and gate.device != dev):
+    n, dev = x.shape[-1], x.get_device()
+    if dev < 0 or y.get_device() != dev or (gate is not None and gate.get_device() != dev):
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
-    for t in (x, y, gate):
-        if t is not None and t.dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError(f"{name}: tensors are float32 or bfloat16, got {t.dtype}")
+    if x.dtype not in _TYPES or y.dtype not in _TYPES or (gate is not None and gate.dtype not in _TYPES):
+        raise TypeError(f"{name}: tensors are float32 or bfloat16, got {x.dtype}, {y.dtype}{'' if gate is None else f' and {gate.dtype}'}")
     if n == 0:
         raise ValueError(f"{name}: rows without columns")
     if (after_bias is not None and after_weight is None) or (before_bias is not None and before_weight is None):
         raise ValueError(f"{name}: a norm's bias needs its weight")
+    eps = float(eps)
     if not eps >= 0:
         raise ValueError(f"{name}: eps {eps}")
-    rows = x.numel() // n
-    kind, seq_len = _NONE, max(rows, 1)
+    kind, seq_len = _NONE, 1
     if gate is not None:
         if gate.shape == (n,):
             kind, gate = _CHANNEL, gate.contiguous()
@@ -150,14 +137,14 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=Non
             kind, seq_len = _SEQUENCE, max(x.shape[1], 1)
         else:
             raise ValueError(f"{name}: a gate is ({n},), (B, 1, {n}) or {tuple(x.shape)}, got {tuple(gate.shape)}")
-    params = [_vector(name, what, t, n, dev) for what, t in zip(_PARAMS, (after_weight, after_bias, before_weight, before_bias))]
-    scale, number = None, 1.0
-    if isinstance(residual_scale, torch.Tensor):
-        scale = _vector(name, "residual_scale", residual_scale, n, dev)
-    else:
-        number = float(residual_scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, gate, scale, *params)):
-        return _ResidualNorm.apply(x, y, gate, scale, *params, number, kind, seq_len, float(eps), bool(rms))
-    x2, y2 = _rows(x, n), _rows(y, n)
-    a = _args(x2, y2, _rows(gate, n) if kind else None, kind, seq_len, scale if scale is not None else number, params, float(eps), bool(rms))
-    return _forward(a, x2, y2, x.shape, None)
+    tensors = [x, y, gate, residual_scale if isinstance(residual_scale, torch.Tensor) else None, after_weight, after_bias, before_weight, before_bias]
+    for i in range(3, 8):
+        if tensors[i] is not None:
+            tensors[i] = _vector(name, _VECTORS[i - 3], tensors[i], n, dev)
+    number = float(residual_scale) if tensors[3] is None else 1.0
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return _ResidualNorm.apply(*tensors, number, kind, seq_len, eps, bool(rms))
+    a, keep = _args(x, y, gate, kind, seq_len, tensors[3], number, tensors[4:], eps, bool(rms))  # noqa: F841
+    return _forward(a, x, y, None)
