@@ -38,68 +38,117 @@ struct Args {
   int splits;                            // units per sequence
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+// 8 columns as 4 packed pairs (two float32 operations an instruction)
+struct V8 {
+  f32x2 p[4];
+  __device__ __forceinline__ float2 pair(int i) const { float2 f; f2_unpack(p[i], f.x, f.y); return f; }
+};
+__device__ __forceinline__ V8 splat8(float v) { return {{f2_splat(v), f2_splat(v), f2_splat(v), f2_splat(v)}}; }
+__device__ __forceinline__ V8 fma8(const V8& a, const V8& b, const V8& c) { return {{f2_fma(a.p[0], b.p[0], c.p[0]), f2_fma(a.p[1], b.p[1], c.p[1]), f2_fma(a.p[2], b.p[2], c.p[2]), f2_fma(a.p[3], b.p[3], c.p[3])}}; }
+__device__ __forceinline__ V8 mul8(const V8& a, const V8& b) { return {{f2_mul(a.p[0], b.p[0]), f2_mul(a.p[1], b.p[1]), f2_mul(a.p[2], b.p[2]), f2_mul(a.p[3], b.p[3])}}; }
+__device__ __forceinline__ V8 add8(const V8& a, const V8& b) { return {{f2_add(a.p[0], b.p[0]), f2_add(a.p[1], b.p[1]), f2_add(a.p[2], b.p[2]), f2_add(a.p[3], b.p[3])}}; }
+__device__ __forceinline__ float sum8(const V8& a) {
+  const f32x2 s = f2_add(f2_add(a.p[0], a.p[1]), f2_add(a.p[2], a.p[3]));
+  float x, y;
+  f2_unpack(s, x, y);
+  return x + y;
 }
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
+__device__ __forceinline__ V8 first8(const V8& a, int m) {           // zero from column m on
+  V8 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 4; ++i) { const float2 f = a.pair(i); r.p[i] = f2_pack(2 * i < m ? f.x : 0.f, 2 * i + 1 < m ? f.y : 0.f); }
+  return r;
 }
 
-// 8 columns of a row as they lie in memory, so that the next row costs few registers
-template <typename T, bool WIDE> struct Cols;
-template <> struct Cols<__nv_bfloat16, true> {
-  uint4 u;
-  __device__ void load(const __nv_bfloat16* p, int) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ void get(float (&f)[8]) const { unpack8(u, f); }
-  __device__ static void store(__nv_bfloat16* p, const float (&f)[8], int) { *reinterpret_cast<uint4*>(p) = pack8(f); }
-};
-template <> struct Cols<float, true> {
-  float4 u, v;
-  __device__ void load(const float* p, int) { u = reinterpret_cast<const float4*>(p)[0]; v = reinterpret_cast<const float4*>(p)[1]; }
-  __device__ void get(float (&f)[8]) const { f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w; }
-  __device__ static void store(float* p, const float (&f)[8], int) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  }
-};
-template <typename T> struct Cols<T, false> {      // any alignment and any number of columns
-  float e[8];
-  __device__ void load(const T* p, int m) {
+// How rows are read.  FULL: 16-byte pieces, n a multiple of 256, so that every thread has 8 columns; WIDE: 16-byte pieces, threads
+// with 8 columns or none; PLAIN: any alignment, any n.
+enum { PLAIN = 0, WIDE = 1, FULL = 2 };
+
+__device__ __forceinline__ V8 from_bf16(const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  V8 v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < m ? (float)p[i] : 0.f;
-  }
-  __device__ void get(float (&f)[8]) const {
+  for (int i = 0; i < 4; ++i) v.p[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  return v;
+}
+__device__ __forceinline__ V8 from_f32(const uint4& u, const uint4& w) {
+  return {{f2_pack(__uint_as_float(u.x), __uint_as_float(u.y)), f2_pack(__uint_as_float(u.z), __uint_as_float(u.w)),
+           f2_pack(__uint_as_float(w.x), __uint_as_float(w.y)), f2_pack(__uint_as_float(w.z), __uint_as_float(w.w))}};
+}
+template <typename T> __device__ __forceinline__ V8 load_plain(const T* p, int m) {
+  V8 v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = e[i];
-  }
-  __device__ static void store(T* p, const float (&f)[8], int m) {
+  for (int i = 0; i < 4; ++i) v.p[i] = f2_pack(2 * i < m ? (float)p[2 * i] : 0.f, 2 * i + 1 < m ? (float)p[2 * i + 1] : 0.f);
+  return v;
+}
+template <int MODE> __device__ __forceinline__ void store8(__nv_bfloat16* p, const V8& v, int m) {
+  if constexpr (MODE == PLAIN) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < m) st_from_float(p + i, f[i]);
+    for (int i = 0; i < 8; ++i) if (i < m) p[i] = __float2bfloat16_rn(i & 1 ? v.pair(i / 2).y : v.pair(i / 2).x);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __float22bfloat162_rn(v.pair(i));
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-};
-// a gate of either type
-template <bool WIDE> struct GateCols {
-  Cols<float, WIDE> f;
-  Cols<__nv_bfloat16, WIDE> b;
-  __device__ void load(const void* p, long long at, bool f32, int m) {
-    if (f32) f.load(static_cast<const float*>(p) + at, m); else b.load(static_cast<const __nv_bfloat16*>(p) + at, m);
+}
+template <int MODE> __device__ __forceinline__ void store8(float* p, const V8& v, int m) {
+  if constexpr (MODE == PLAIN) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < m) p[i] = i & 1 ? v.pair(i / 2).y : v.pair(i / 2).x;
+  } else {
+    const float2 a = v.pair(0), b = v.pair(1), c = v.pair(2), d = v.pair(3);
+    reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
   }
-  __device__ void get(float (&v)[8], bool f32) const { if (f32) f.get(v); else b.get(v); }
+}
+
+// Rows ahead of their use: every thread copies the 16-byte pieces of its own columns into its own places of shared memory, so that
+// no barrier is needed and no register is held.
+template <int STAGES> struct Ring {
+  uint32_t base, piece, stage;           // shared address of this thread's first place; distances of pieces and of stages
+  uint32_t in, out;                      // the stages to be filled and to be read, as distances
+  __device__ __forceinline__ Ring(void* mem, int pieces) {
+    base = (uint32_t)__cvta_generic_to_shared(mem) + threadIdx.x * 16;
+    piece = blockDim.x * 16;
+    stage = pieces * piece;
+    in = out = 0;
+  }
+  __device__ __forceinline__ void next(uint32_t& at) const { at = at + stage == STAGES * stage ? 0 : at + stage; }
+  // 8 columns of either type; the place behind them
+  __device__ __forceinline__ uint32_t put(uint32_t to, const char* src, bool f32) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + to), "l"(src) : "memory");
+    if (f32) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + to + piece), "l"(src + 16) : "memory");
+    return to + (f32 ? 2 * piece : piece);
+  }
+  __device__ __forceinline__ uint4 piece_at(uint32_t at) const {
+    uint4 u;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(base + at) : "memory");
+    return u;
+  }
+  __device__ __forceinline__ V8 get(uint32_t at, bool f32) const { return f32 ? from_f32(piece_at(at), piece_at(at + piece)) : from_bf16(piece_at(at)); }
+  __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
 };
+// A tensor's rows one after the other, from this thread's columns on
+struct Walk {
+  const char* p; long long step;
+  __device__ __forceinline__ Walk(const void* base, long long ld, long long row, int c0, int size, long long rows_a_step)
+      : p(static_cast<const char*>(base) + (row * ld + c0) * size), step(rows_a_step * ld * size) {}
+  __device__ __forceinline__ const char* go() { const char* q = p; p += step; return q; }
+};
+template <typename T> constexpr bool is_f32 = sizeof(T) == 4;
+template <int MAXT> constexpr int stages = MAXT == 192 ? 3 : 2;      // as many as shared memory has room for
 
 // Sums over the block of two values at once.  Two buffers by turns: one barrier a call.
-struct Reduce {
+template <int MAXT> struct Reduce {
+  static constexpr int CAP = MAXT == 192 ? 6 : 32;     // warps at most: few of them are added without a loop
   float2 (*buf)[32];
   int turn;
-  __device__ float2 operator()(float a, float b) {
+  __device__ __forceinline__ float2 operator()(float a, float b) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(~0u, a, o);
@@ -110,215 +159,272 @@ struct Reduce {
     if ((threadIdx.x & 31) == 0) buf[turn][threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
     float2 s = buf[turn][0];
-    for (int w = 1; w < nw; ++w) { const float2 q = buf[turn][w]; s.x += q.x; s.y += q.y; }
+#pragma unroll(CAP <= 6 ? CAP - 1 : 1)
+    for (int w = 1; w < CAP; ++w) {
+      if (w >= nw) break;
+      const float2 q = buf[turn][w];
+      s.x += q.x;
+      s.y += q.y;
+    }
     turn ^= 1;
     return s;
+  }
+  // mean and sum of squared distances to it over blocks of 256 columns a warp, in one pass: halves of equal size are joined,
+  //   mean = (a + b) / 2,   M = Ma + Mb + (a - b)^2 size / 2,
+  // which loses nothing where the mean is far from zero (sums of squares would)
+  __device__ __forceinline__ float2 moments(const V8& v) {
+    float mean = sum8(v) * 0.125f;
+    const V8 d = add8(v, splat8(-mean));
+    float m2 = sum8(mul8(d, d));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float b = __shfl_xor_sync(~0u, mean, o), q = __shfl_xor_sync(~0u, m2, o), e = b - mean;
+      mean = fmaf(0.5f, e, mean);
+      m2 = fmaf(e * e, 4.f * o, m2 + q);
+    }
+    const int nw = blockDim.x >> 5;
+    if (nw == 1) return make_float2(mean, m2);
+    if ((threadIdx.x & 31) == 0) buf[turn][threadIdx.x >> 5] = make_float2(mean, m2);
+    __syncthreads();
+    // all warps' means against the first one's: distances are as small as the row's spread
+    const float2 f = buf[turn][0];
+    float d1 = 0.f, d2 = 0.f;
+    m2 = f.y;
+#pragma unroll(CAP <= 6 ? CAP - 1 : 1)
+    for (int w = 1; w < CAP; ++w) {
+      if (w >= nw) break;
+      const float2 q = buf[turn][w];
+      const float e = q.x - f.x;
+      d1 += e;
+      d2 = fmaf(e, e, d2);
+      m2 += q.y;
+    }
+    d1 /= nw;
+    mean = f.x + d1;
+    m2 += 256.f * fmaf(-nw * d1, d1, d2);
+    turn ^= 1;
+    return make_float2(mean, m2);
   }
 };
 
 // mean and 1 / deviation of a row whose columns beyond n (m of this thread's 8 are inside) hold 0
-__device__ __forceinline__ float2 row_stats(Reduce& red, const float (&v)[8], int m, float inv_n, float eps, bool rms) {
-  float mean = 0.f, s = 0.f;
-  if (!rms) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += v[i];
-    mean = red(s, 0.f).x * inv_n;
+template <int MODE, int MAXT> __device__ __forceinline__ float2 row_stats(Reduce<MAXT>& red, const V8& v, int m, float inv_n, float eps, bool rms) {
+  if (rms) return make_float2(0.f, rsqrtf(fmaf(red(sum8(mul8(v, v)), 0.f).x, inv_n, eps)));
+  if constexpr (MODE == FULL) {
+    const float2 s = red.moments(v);
+    return make_float2(s.x, rsqrtf(fmaf(s.y, inv_n, eps)));
   }
-  s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { const float d = i < m ? v[i] - mean : 0.f; s = fmaf(d, d, s); }
-  return make_float2(mean, rsqrtf(fmaf(red(s, 0.f).x, inv_n, eps)));
+  const float mean = red(sum8(v), 0.f).x * inv_n;
+  const V8 d = first8(add8(v, splat8(-mean)), m);
+  return make_float2(mean, rsqrtf(fmaf(red(sum8(mul8(d, d)), 0.f).x, inv_n, eps)));
 }
+__device__ __forceinline__ V8 normal(const V8& v, float mean, float rstd) { return mul8(add8(v, splat8(-mean)), splat8(rstd)); }
 
-__device__ __forceinline__ void param(float (&f)[8], const float* p, int c0, int m, float otherwise) {
+__device__ __forceinline__ V8 param(const float* p, int c0, int m, float otherwise) {
+  float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = p && i < m ? __ldg(p + c0 + i) : otherwise;
+  return {{f2_pack(f[0], f[1]), f2_pack(f[2], f[3]), f2_pack(f[4], f[5]), f2_pack(f[6], f[7])}};
+}
+__device__ __forceinline__ V8 channel_gate(const Args& a, int c0, int m) {
+  if (a.gate != G_CHANNEL || m == 0) return splat8(1.f);
+  return a.g_f32 ? load_plain(static_cast<const float*>(a.g) + c0, m) : load_plain(static_cast<const __nv_bfloat16*>(a.g) + c0, m);
+}
+__device__ __forceinline__ V8 gate_plain(const Args& a, long long at, int m) {
+  return a.g_f32 ? load_plain(static_cast<const float*>(a.g) + at, m) : load_plain(static_cast<const __nv_bfloat16*>(a.g) + at, m);
 }
 
-template <typename TX, typename TY, bool WIDE, int MAXT>
-__global__ void __launch_bounds__(MAXT)
+template <typename TX, typename TY, int MODE, int MAXT>
+__global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 3 : 1))
 forward_kernel(const Args a) {
+  extern __shared__ uint4 ring_mem[];
   __shared__ float2 buf[2][32];
-  Reduce red = {buf, 0};
+  Reduce<MAXT> red = {buf, 0};
   const int c0 = threadIdx.x * VEC;
-  const int m = max(0, min(VEC, a.n - c0));                             // this thread's columns
-  const bool live = m > 0;
+  const int m = MODE == FULL ? VEC : max(0, min(VEC, a.n - c0));        // this thread's columns
+  const bool live = MODE == FULL || m > 0;
   const float inv_n = 1.f / a.n;
-  float w1[8], b1[8], w2[8], b2[8], sc[8], gc[8];
-  param(w1, a.w1, c0, m, 1.f); param(b1, a.b1, c0, m, 0.f);
-  param(w2, a.w2, c0, m, 1.f); param(b2, a.b2, c0, m, 0.f);
-  param(sc, a.a, c0, m, a.scale);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) gc[i] = 1.f;
-  if (a.gate == G_CHANNEL && live) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < m) gc[i] = a.g_f32 ? static_cast<const float*>(a.g)[c0 + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(a.g)[c0 + i]);
-  }
+  const V8 w1 = param(a.w1, c0, m, 1.f), b1 = param(a.b1, c0, m, 0.f), w2 = param(a.w2, c0, m, 1.f), b2 = param(a.b2, c0, m, 0.f);
+  const V8 sc = param(a.a, c0, m, a.scale);
   const bool by_row = a.gate >= G_SEQUENCE;
-  Cols<TX, WIDE> cx;
-  Cols<TY, WIDE> cy;
-  GateCols<WIDE> cg;
-  auto fetch = [&](long long row) {
-    if (!live) return;
-    cx.load(static_cast<const TX*>(a.x) + row * a.ldx + c0, m);
-    cy.load(static_cast<const TY*>(a.y) + row * a.ldy + c0, m);
-    if (by_row) cg.load(a.g, (a.gate == G_TOKEN ? row : row / a.seq_len) * a.ldg + c0, a.g_f32, m);
-  };
-  if ((long long)blockIdx.x < a.rows) fetch(blockIdx.x);
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float x[8] = {}, v[8] = {}, g[8];
-    if (live) { cx.get(x); cy.get(v); }
-    if (by_row && live) {
-      cg.get(g, a.g_f32);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = gc[i];
+  V8 gc = channel_gate(a, c0, m);
+  constexpr int STAGES = stages<MAXT>;
+  constexpr int PX = is_f32<TX> ? 2 : 1, PY = is_f32<TY> ? 2 : 1;
+  Ring<STAGES> ring(ring_mem, PX + PY + (by_row ? (a.g_f32 ? 2 : 1) : 0));
+  Walk wx(a.x, a.ldx, blockIdx.x, c0, sizeof(TX), gridDim.x), wy(a.y, a.ldy, blockIdx.x, c0, sizeof(TY), gridDim.x);
+  Walk wr(a.r, a.n, blockIdx.x, c0, sizeof(TX), gridDim.x), wh(a.h, a.n, blockIdx.x, c0, sizeof(TY), gridDim.x);
+  auto gate_at = [&](long long row) { return ((a.gate == G_TOKEN ? row : row / a.seq_len) * a.ldg + c0); };
+  long long ahead = blockIdx.x;          // the next row to be copied
+  auto fetch = [&]() {
+    if (MODE == PLAIN) return;
+    if (live && ahead < a.rows) {
+      uint32_t to = ring.put(ring.in, wx.go(), is_f32<TX>);
+      to = ring.put(to, wy.go(), is_f32<TY>);
+      if (by_row) ring.put(to, static_cast<const char*>(a.g) + (gate_at(ahead) << (a.g_f32 ? 2 : 1)), a.g_f32);
     }
-    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    ahead += gridDim.x;
+    ring.next(ring.in);
+    ring.commit();
+  };
+  for (int s = 0; s < STAGES - 1; ++s) fetch();
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    V8 x = splat8(0.f), v = x, g = gc;
+    if constexpr (MODE == PLAIN) {
+      if (live) {
+        x = load_plain(reinterpret_cast<const TX*>(wx.go()), m);
+        v = load_plain(reinterpret_cast<const TY*>(wy.go()), m);
+        if (by_row) g = gate_plain(a, gate_at(row), m);
+      }
+    } else {
+      ring.wait();
+      if (live) {
+        x = ring.get(ring.out, is_f32<TX>);
+        v = ring.get(ring.out + PX * ring.piece, is_f32<TY>);
+        if (by_row) g = ring.get(ring.out + (PX + PY) * ring.piece, a.g_f32);
+      }
+      ring.next(ring.out);
+      fetch();
+    }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
     if (a.norm1) {
-      s1 = row_stats(red, v, m, inv_n, a.eps, a.rms);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - s1.x) * s1.y, w1[i], b1[i]);
+      s1 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.eps, a.rms);
+      v = fma8(normal(v, s1.x, s1.y), w1, b1);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < m ? fmaf(g[i], v[i], sc[i] * x[i]) : 0.f;
-    if (live) Cols<TX, WIDE>::store(static_cast<TX*>(a.r) + row * a.n + c0, v, m);
+    v = fma8(g, v, mul8(sc, x));
+    if (MODE != FULL) v = first8(v, m);
+    TX* to = reinterpret_cast<TX*>(const_cast<char*>(wr.go()));
+    if (live) store8<MODE>(to, v, m);
     if (a.norm2) {
-      s2 = row_stats(red, v, m, inv_n, a.eps, a.rms);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - s2.x) * s2.y, w2[i], b2[i]);
-      if (live) Cols<TY, WIDE>::store(static_cast<TY*>(a.h) + row * a.n + c0, v, m);
+      s2 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.eps, a.rms);
+      v = fma8(normal(v, s2.x, s2.y), w2, b2);
+      TY* to = reinterpret_cast<TY*>(const_cast<char*>(wh.go()));
+      if (live) store8<MODE>(to, v, m);
     }
     if (a.stats && threadIdx.x == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(s1.x, s1.y, s2.x, s2.y);
   }
 }
 
-template <typename TX, typename TY, bool WIDE, int MAXT>
-__global__ void __launch_bounds__(MAXT)
+template <typename TX, typename TY, int MODE, int MAXT>
+__global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 2 : 1))
 backward_kernel(const Args a) {
+  extern __shared__ uint4 ring_mem[];
   __shared__ float2 buf[2][32];
-  Reduce red = {buf, 0};
+  Reduce<MAXT> red = {buf, 0};
   const int c0 = threadIdx.x * VEC;
-  const int m = max(0, min(VEC, a.n - c0));
-  const bool live = m > 0;
+  const int m = MODE == FULL ? VEC : max(0, min(VEC, a.n - c0));
+  const bool live = MODE == FULL || m > 0;
   const float inv_n = 1.f / a.n;
-  float w1[8], b1[8], w2[8], sc[8], gc[8];
-  param(w1, a.w1, c0, m, 1.f); param(b1, a.b1, c0, m, 0.f);
-  param(w2, a.w2, c0, m, 1.f);
-  param(sc, a.a, c0, m, a.scale);
+  const V8 w1 = param(a.w1, c0, m, 1.f), b1 = param(a.b1, c0, m, 0.f), w2 = param(a.w2, c0, m, 1.f), sc = param(a.a, c0, m, a.scale);
+  V8 gc = channel_gate(a, c0, m);
+  V8 sum[S_COUNT];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) gc[i] = 1.f;
-  if (a.gate == G_CHANNEL && live) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < m) gc[i] = a.g_f32 ? static_cast<const float*>(a.g)[c0 + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(a.g)[c0 + i]);
-  }
-  float sum[S_COUNT][8] = {};
-  const bool by_row = a.gate >= G_SEQUENCE;
+  for (int k = 0; k < S_COUNT; ++k) sum[k] = splat8(0.f);
+  const bool by_row = a.gate >= G_SEQUENCE, has_r = a.dr != nullptr, has_h = a.dh != nullptr;
+  constexpr int PX = is_f32<TX> ? 2 : 1, PY = is_f32<TY> ? 2 : 1, STAGES = stages<MAXT>;
   const long long per = (a.seq_len + a.splits - 1) / a.splits;            // rows of a unit
   const long long units = a.rows / a.seq_len * a.splits;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const long long seq = unit / a.splits, first = seq * a.seq_len;
     const long long row0 = first + min(a.seq_len, (unit - seq * a.splits) * per), row1 = min(first + a.seq_len, row0 + per);
-    Cols<TX, WIDE> cx, cdr;
-    Cols<TY, WIDE> cy, cdh;
-    GateCols<WIDE> cg;
-    float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
-    auto fetch = [&](long long row) {
-      st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
-      if (!live) return;
-      cx.load(static_cast<const TX*>(a.x) + row * a.ldx + c0, m);
-      cy.load(static_cast<const TY*>(a.y) + row * a.ldy + c0, m);
-      if (by_row) cg.load(a.g, (a.gate == G_TOKEN ? row : seq) * a.ldg + c0, a.g_f32, m);
-      if (a.dr) cdr.load(static_cast<const TX*>(a.dr) + row * a.n + c0, m);
-      if (a.dh) cdh.load(static_cast<const TY*>(a.dh) + row * a.n + c0, m);
+    Ring<STAGES> ring(ring_mem, 2 * PX + 2 * PY + (by_row ? (a.g_f32 ? 2 : 1) : 0));
+    Walk wx(a.x, a.ldx, row0, c0, sizeof(TX), 1), wy(a.y, a.ldy, row0, c0, sizeof(TY), 1), wdr(a.dr, a.n, row0, c0, sizeof(TX), 1);
+    Walk wdh(a.dh, a.n, row0, c0, sizeof(TY), 1), wg(a.g, a.gate == G_TOKEN ? a.ldg : 0, row0, c0, a.g_f32 ? 4 : 2, 1);
+    if (a.gate == G_SEQUENCE) wg.p += (seq * a.ldg) << (a.g_f32 ? 2 : 1);
+    Walk wdx(a.dx, a.n, row0, c0, sizeof(TX), 1), wdy(a.dy, a.n, row0, c0, sizeof(TY), 1), wdg(a.dg, a.n, row0, c0, a.g_f32 ? 4 : 2, 1);
+    long long ahead = row0;
+    auto fetch = [&]() {
+      if (MODE == PLAIN) return;
+      if (live && ahead < row1) {
+        uint32_t to = ring.put(ring.in, wx.go(), is_f32<TX>);
+        to = ring.put(to, wy.go(), is_f32<TY>);
+        if (has_r) ring.put(to, wdr.go(), is_f32<TX>);
+        to += PX * ring.piece;
+        if (has_h) ring.put(to, wdh.go(), is_f32<TY>);
+        to += PY * ring.piece;
+        if (by_row) ring.put(to, wg.go(), a.g_f32);
+      }
+      ++ahead;
+      ring.next(ring.in);
+      ring.commit();
     };
-    if (row0 < row1) fetch(row0);
+    auto stats_of = [&](long long row) { return *reinterpret_cast<const float4*>(a.stats + 4 * row); };
+    for (int s = 0; s < STAGES - 1; ++s) fetch();
+    float4 next = row0 < row1 ? stats_of(row0) : make_float4(0.f, 1.f, 0.f, 1.f);
     for (long long row = row0; row < row1; ++row) {
-      float x[8] = {}, yh[8] = {}, g[8], u[8] = {}, dh[8] = {};
-      const float4 s = st;
-      if (live) {
-        cx.get(x);
-        cy.get(yh);
-        if (a.dr) cdr.get(u);
-        if (a.dh) cdh.get(dh);
-      }
-      if (by_row && live) {
-        cg.get(g, a.g_f32);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = gc[i];
-      }
-      if (row + 1 < row1) fetch(row + 1);
-      float n1[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (a.norm1) yh[i] = (yh[i] - s.x) * s.y;
-        n1[i] = a.norm1 ? fmaf(yh[i], w1[i], b1[i]) : yh[i];
-      }
-      if (a.norm2 && a.dh) {
-        float rh[8], p = 0.f, q = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          rh[i] = i < m ? (fmaf(g[i], n1[i], sc[i] * x[i]) - s.z) * s.w : 0.f;
-          const float d = dh[i] * w2[i];
-          sum[S_W2][i] = fmaf(dh[i], rh[i], sum[S_W2][i]);
-          sum[S_B2][i] += dh[i];
-          p += d;
-          q = fmaf(d, rh[i], q);
+      V8 x = splat8(0.f), yh = x, g = gc, u = x, dh = x;
+      const float4 s = next;
+      if (row + 1 < row1) next = stats_of(row + 1);
+      if constexpr (MODE == PLAIN) {
+        if (live) {
+          x = load_plain(reinterpret_cast<const TX*>(wx.go()), m);
+          yh = load_plain(reinterpret_cast<const TY*>(wy.go()), m);
+          if (has_r) u = load_plain(reinterpret_cast<const TX*>(wdr.go()), m);
+          if (has_h) dh = load_plain(reinterpret_cast<const TY*>(wdh.go()), m);
+          if (by_row) g = gate_plain(a, (a.gate == G_TOKEN ? row : seq) * a.ldg + c0, m);
         }
-        const float2 t = red(p, q);
-        const float mp = a.rms ? 0.f : t.x * inv_n, mq = t.y * inv_n;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = i < m ? fmaf(s.w, fmaf(-rh[i], mq, fmaf(dh[i], w2[i], -mp)), u[i]) : 0.f;
+      } else {
+        ring.wait();
+        if (live) {
+          x = ring.get(ring.out, is_f32<TX>);
+          yh = ring.get(ring.out + PX * ring.piece, is_f32<TY>);
+          if (has_r) u = ring.get(ring.out + (PX + PY) * ring.piece, is_f32<TX>);
+          if (has_h) dh = ring.get(ring.out + (2 * PX + PY) * ring.piece, is_f32<TY>);
+          if (by_row) g = ring.get(ring.out + (2 * PX + 2 * PY) * ring.piece, a.g_f32);
+        }
+        ring.next(ring.out);
+        fetch();
       }
-      float d[8], dg[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum[S_SCALE][i] = fmaf(x[i], u[i], sum[S_SCALE][i]);
-        dg[i] = u[i] * n1[i];
-        if (a.gate != G_TOKEN) sum[S_GATE][i] += dg[i];
-        d[i] = g[i] * u[i];
-        x[i] = sc[i] * u[i];
+      V8 n1 = yh;
+      if (a.norm1) {
+        yh = normal(yh, s.x, s.y);
+        n1 = fma8(yh, w1, b1);
       }
-      if (live && a.dx) Cols<TX, WIDE>::store(static_cast<TX*>(a.dx) + row * a.n + c0, x, m);
+      if (has_h) {
+        V8 rh = normal(fma8(g, n1, mul8(sc, x)), s.z, s.w);
+        if (MODE != FULL) rh = first8(rh, m);
+        const V8 d = mul8(dh, w2);
+        sum[S_W2] = fma8(dh, rh, sum[S_W2]);
+        sum[S_B2] = add8(sum[S_B2], dh);
+        const float2 t = red(sum8(d), sum8(mul8(d, rh)));
+        // u += rstd (d - mean(d) - r^ mean(d r^))
+        u = fma8(splat8(s.w), fma8(rh, splat8(-t.y * inv_n), add8(d, splat8(a.rms ? 0.f : -t.x * inv_n))), u);
+        if (MODE != FULL) u = first8(u, m);
+      }
+      sum[S_SCALE] = fma8(x, u, sum[S_SCALE]);
+      const V8 dg = mul8(u, n1);
+      if (a.gate != G_TOKEN) sum[S_GATE] = add8(sum[S_GATE], dg);
+      V8 d = mul8(g, u);
+      char* to = const_cast<char*>(wdx.go());
+      if (live && a.dx) store8<MODE>(reinterpret_cast<TX*>(to), mul8(sc, u), m);
       if (live && a.gate == G_TOKEN && a.dg) {
-        if (a.g_f32) Cols<float, WIDE>::store(static_cast<float*>(a.dg) + row * a.n + c0, dg, m);
-        else Cols<__nv_bfloat16, WIDE>::store(static_cast<__nv_bfloat16*>(a.dg) + row * a.n + c0, dg, m);
+        to = const_cast<char*>(wdg.go());
+        if (a.g_f32) store8<MODE>(reinterpret_cast<float*>(to), dg, m);
+        else store8<MODE>(reinterpret_cast<__nv_bfloat16*>(to), dg, m);
       }
       if (a.norm1) {
-        float p = 0.f, q = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sum[S_W1][i] = fmaf(d[i], yh[i], sum[S_W1][i]);
-          sum[S_B1][i] += d[i];
-          d[i] *= w1[i];
-          p += i < m ? d[i] : 0.f;
-          q = i < m ? fmaf(d[i], yh[i], q) : q;
-        }
-        const float2 t = red(p, q);
-        const float mp = a.rms ? 0.f : t.x * inv_n, mq = t.y * inv_n;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = s.y * fmaf(-yh[i], mq, d[i] - mp);
+        sum[S_W1] = fma8(d, yh, sum[S_W1]);
+        sum[S_B1] = add8(sum[S_B1], d);
+        d = mul8(d, w1);
+        V8 q = mul8(d, yh);
+        if (MODE != FULL) q = first8(q, m);
+        const float2 t = red(sum8(d), sum8(q));                             // d is 0 in dead columns, as u is
+        d = mul8(splat8(s.y), fma8(yh, splat8(-t.y * inv_n), add8(d, splat8(a.rms ? 0.f : -t.x * inv_n))));
       }
-      if (live && a.dy) Cols<TY, WIDE>::store(static_cast<TY*>(a.dy) + row * a.n + c0, d, m);
+      to = const_cast<char*>(wdy.go());
+      if (live && a.dy) store8<MODE>(reinterpret_cast<TY*>(to), d, m);
     }
     if (a.gate == G_SEQUENCE && a.dg) {                                   // this unit's share of the sequence's gate
       if (live) {
-        if (a.gate_sums) Cols<float, false>::store(a.gate_sums + unit * a.n + c0, sum[S_GATE], m);
-        else if (a.g_f32) Cols<float, false>::store(static_cast<float*>(a.dg) + seq * a.n + c0, sum[S_GATE], m);
-        else Cols<__nv_bfloat16, false>::store(static_cast<__nv_bfloat16*>(a.dg) + seq * a.n + c0, sum[S_GATE], m);
+        if (a.gate_sums) store8<PLAIN>(a.gate_sums + unit * a.n + c0, sum[S_GATE], m);
+        else if (a.g_f32) store8<PLAIN>(static_cast<float*>(a.dg) + seq * a.n + c0, sum[S_GATE], m);
+        else store8<PLAIN>(static_cast<__nv_bfloat16*>(a.dg) + seq * a.n + c0, sum[S_GATE], m);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum[S_GATE][i] = 0.f;
+      sum[S_GATE] = splat8(0.f);
     }
   }
   if (live && a.sums) {
 #pragma unroll
-    for (int k = 0; k < S_COUNT; ++k)
-      Cols<float, false>::store(a.sums + ((long long)blockIdx.x * S_COUNT + k) * a.n + c0, sum[k], m);
+    for (int k = 0; k < S_COUNT; ++k) store8<PLAIN>(a.sums + ((long long)blockIdx.x * S_COUNT + k) * a.n + c0, sum[k], m);
   }
 }
 
@@ -356,12 +462,12 @@ join_kernel(const JoinArgs j) {
 }
 
 struct Plan { int threads, blocks, splits; long long units; };
-// blocks: as many as the SMs hold at once (about 120 registers a thread), no more than there are units.  Sequences are cut into
-// units where there are fewer of them than blocks; without a gate per sequence all rows are one sequence.
+// blocks: as many as the SMs hold at once by their registers (96 and 168 a thread), no more than there are units.  Sequences are cut
+// into units where there are fewer of them than blocks; without a gate per sequence all rows are one sequence.
 static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   Plan p;
   p.threads = ((n + VEC - 1) / VEC + 31) / 32 * 32;
-  const int per_sm = p.threads > 512 ? 1 : max(1, min(16, (backward ? 384 : 512) / p.threads));
+  const int per_sm = p.threads > 512 ? 1 : max(1, min(16, (backward ? 384 : 640) / p.threads));
   const long long most = (long long)m2_sm_count() * per_sm;
   const long long seqs = rows / seq_len;
   long long splits = (most + seqs - 1) / seqs;
@@ -372,24 +478,32 @@ static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   return p;
 }
 
-template <typename TX, typename TY, bool WIDE> static void launch_t(const Args& a, bool backward, int blocks, int threads, cudaStream_t st) {
-  if (threads <= 256) {
-    if (backward) backward_kernel<TX, TY, WIDE, 256><<<blocks, threads, 0, st>>>(a);
-    else forward_kernel<TX, TY, WIDE, 256><<<blocks, threads, 0, st>>>(a);
+template <typename TX, typename TY, int MODE, int MAXT> static int launch_t(const Args& a, bool backward, int blocks, int threads, cudaStream_t st) {
+  const int gate = a.gate >= G_SEQUENCE ? (a.g_f32 ? 2 : 1) : 0;
+  const int pieces = ((is_f32<TX> ? 2 : 1) + (is_f32<TY> ? 2 : 1)) * (backward ? 2 : 1) + gate;
+  const int smem = MODE == PLAIN ? 0 : stages<MAXT> * pieces * threads * 16;
+  constexpr int most = MODE == PLAIN ? 0 : stages<MAXT> * (((is_f32<TX> ? 2 : 1) + (is_f32<TY> ? 2 : 1)) * 2 + 2) * MAXT * 16;
+  static_assert(most <= 227 * 1024 - 1024, "ring");
+  if (backward) {
+    if (MODE != PLAIN) M2_SMEM_ONCE((backward_kernel<TX, TY, MODE, MAXT>), most);
+    backward_kernel<TX, TY, MODE, MAXT><<<blocks, threads, smem, st>>>(a);
   } else {
-    if (backward) backward_kernel<TX, TY, WIDE, 1024><<<blocks, threads, 0, st>>>(a);
-    else forward_kernel<TX, TY, WIDE, 1024><<<blocks, threads, 0, st>>>(a);
+    if (MODE != PLAIN) M2_SMEM_ONCE((forward_kernel<TX, TY, MODE, MAXT>), most);
+    forward_kernel<TX, TY, MODE, MAXT><<<blocks, threads, smem, st>>>(a);
   }
+  return M2_OK;
 }
-static void launch(const Args& a, int xt, int yt, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
+// wide rows of up to 4096 columns go through the ring: longer ones would not fit into shared memory
+template <typename TX, typename TY> static int launch_n(const Args& a, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
+  if (threads > 512) return launch_t<TX, TY, PLAIN, 1024>(a, backward, blocks, threads, st);
+  if (!wide) return launch_t<TX, TY, PLAIN, 512>(a, backward, blocks, threads, st);
+  if (a.n % 256) return launch_t<TX, TY, WIDE, 512>(a, backward, blocks, threads, st);
+  return threads <= 192 ? launch_t<TX, TY, FULL, 192>(a, backward, blocks, threads, st) : launch_t<TX, TY, FULL, 512>(a, backward, blocks, threads, st);
+}
+static int launch(const Args& a, int xt, int yt, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
   typedef __nv_bfloat16 B;
-  if (wide) {
-    if (xt == M2_F32) yt == M2_F32 ? launch_t<float, float, true>(a, backward, blocks, threads, st) : launch_t<float, B, true>(a, backward, blocks, threads, st);
-    else yt == M2_F32 ? launch_t<B, float, true>(a, backward, blocks, threads, st) : launch_t<B, B, true>(a, backward, blocks, threads, st);
-  } else {
-    if (xt == M2_F32) yt == M2_F32 ? launch_t<float, float, false>(a, backward, blocks, threads, st) : launch_t<float, B, false>(a, backward, blocks, threads, st);
-    else yt == M2_F32 ? launch_t<B, float, false>(a, backward, blocks, threads, st) : launch_t<B, B, false>(a, backward, blocks, threads, st);
-  }
+  if (xt == M2_F32) return yt == M2_F32 ? launch_n<float, float>(a, wide, backward, blocks, threads, st) : launch_n<float, B>(a, wide, backward, blocks, threads, st);
+  return yt == M2_F32 ? launch_n<B, float>(a, wide, backward, blocks, threads, st) : launch_n<B, B>(a, wide, backward, blocks, threads, st);
 }
 
 static int fill(const char* name, Args& a, const m2_residual_norm_args& g) {
@@ -432,7 +546,8 @@ extern "C" int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* str
   M2_REQUIRE(m2_aligned(g.stats, 16), M2_ERR_ALIGN, "m2_residual_norm_fwd: stats is not on a 16-byte boundary");
   a.r = g.r; a.h = g.h; a.stats = g.stats;
   const Plan p = plan_of(g.rows, g.rows, g.n, false);
-  launch(a, g.x_dtype, g.y_dtype, wide_rows(g) && m2_aligned(g.r, 16) && m2_aligned(g.h, 16), false, p.blocks, p.threads, (cudaStream_t)stream);
+  if (int rc = launch(a, g.x_dtype, g.y_dtype, wide_rows(g) && m2_aligned(g.r, 16) && m2_aligned(g.h, 16), false, p.blocks, p.threads, (cudaStream_t)stream))
+    return rc;
   M2_LAUNCH_CHECK("m2_residual_norm_fwd");
   return M2_OK;
 }
@@ -462,7 +577,7 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   a.gate_sums = a.gate == G_SEQUENCE && p.splits > 1 ? d.workspace + (long long)p.blocks * S_COUNT * a.n : nullptr;
   const bool wide = wide_rows(g) && m2_aligned(d.d_r, 16) && m2_aligned(d.d_h, 16) && m2_aligned(d.d_x, 16) && m2_aligned(d.d_y, 16) && m2_aligned(d.d_gate, 16);
   const cudaStream_t st = (cudaStream_t)stream;
-  launch(a, g.x_dtype, g.y_dtype, wide, true, p.blocks, p.threads, st);
+  if (int rc = launch(a, g.x_dtype, g.y_dtype, wide, true, p.blocks, p.threads, st)) return rc;
   M2_LAUNCH_CHECK("m2_residual_norm_bwd");
   JoinArgs j = {};
   j.sums = a.sums; j.blocks = p.blocks; j.n = a.n;
