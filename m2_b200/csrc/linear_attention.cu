@@ -35,6 +35,16 @@ struct Scan {
   int wide, o_wide;                      // rows of q, k and v (of o) start on 16-byte boundaries and are whole 16-byte pieces
 };
 
+// Scans that run side by side in one launch (the three of a gradient): blockIdx.x counts the 64-column tiles of all of them
+struct Scans { Scan s[3]; int tiles[3]; };
+template <bool MANY> __device__ __forceinline__ const Scan& pick_scan(const Scans& p, int& tile) {
+  tile = blockIdx.x;
+  int r = 0;
+  if (MANY)
+    while (r < 2 && tile >= p.tiles[r]) tile -= p.tiles[r++];
+  return p.s[MANY ? r : 0];
+}
+
 __device__ __forceinline__ float power(float ld, int n) { return n == 0 ? 1.f : expf(ld * n); }
 // l^n - 1: a state is carried as T + (l^n - 1) T, so that the factor's own rounding does not add up over the chunks of a long memory
 __device__ __forceinline__ float power_m1(float ld, int n) { return n == 0 ? 0.f : expm1f(ld * n); }
@@ -59,9 +69,12 @@ __device__ __forceinline__ void mac(float (&acc)[4][4], const float4& a, const f
 }
 __device__ __forceinline__ float4 f4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
+template <bool MANY>
 __global__ void __launch_bounds__(256)
-scan_f32_kernel(const Scan a) {
+scan_f32_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ float sm[];
+  int tile;
+  const Scan& a = pick_scan<MANY>(scans, tile);
   const int dkp = (a.dk + 15) / 16 * 16;
   float* qt = sm;                        // [dkp][LD]  (k index, token)
   float* kt = qt + dkp * LD;             // [dkp][LD]
@@ -71,7 +84,7 @@ scan_f32_kernel(const Scan a) {
   float* pw = st + dkp * LD;             // [C + 1]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int bh = blockIdx.z, b = bh / a.heads, h = bh - b * a.heads;
-  const int seg = blockIdx.y, col0 = blockIdx.x * DVT;
+  const int seg = blockIdx.y, col0 = tile * DVT;
   const int cols = min(DVT, a.dv - col0);
   const int n = seq_length(a, b);
   const float ld = a.log_decay[h];
@@ -197,17 +210,16 @@ scan_f32_kernel(const Scan a) {
 // 16 w .. 16 w + 15 of a chunk and rows w DK / 4 .. of the state, whose float32 values stay in its registers.  q, k and v tiles
 // arrive by cp.async one chunk ahead.  A chunk's weights P = (q k^T) decay never leave the registers: the accumulators of q k^T are
 // the operand of P v.  Every warp needs the whole state as an operand: it goes through shared memory as bf16, into the other one of
-// two buffers, so that a chunk has a single block barrier.
-//
-// Why mma.sync: the scan is bound by its bytes.  A token and head of 64 + 64 channels moves 512 bytes, 11.6 ns of an SM's share of
-// 6.5 TB/s, and takes 26 kFLOP (mean), 7 ns at the 555 TFLOP/s that mma.sync reaches on a B200; tiles of 64 tokens whose products
-// feed each other through registers fit it, where tcgen05 would take every product through tensor and shared memory.
+// two buffers, so that a chunk has a single block barrier and the warps of the SM's blocks drift apart and fill each other's waits.
 //
 // The state is a sum over thousands of tokens, so nothing of it is rounded to bf16: l^(C-1-j) k_j goes into its product as two or
-// (where the state is returned) three bf16 parts, 16 or 24 bits, and every chunk's sum starts from zero and is added in float32, as
+// (where the state is returned) three bf16 parts of 8 bits, and every chunk's sum starts from zero and is added in float32, as
 // tensor cores cut their sums instead of rounding them.
-constexpr int QK_LD(int dk) { return dk * 2; }             // bytes of a tile's row
-
+//
+// Bound: a token and head of 64 + 64 channels moves 512 bytes, 64 of them 0.74 us of an SM's share of 6.5 TB/s; the products take
+// 0.55 us (two parts) at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
+// unrolled (2.2 k instructions a warp) does not fit the SM's instruction cache and waited for it more than for anything else.  The
+// same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took as long.
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -215,8 +227,11 @@ __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+__device__ __forceinline__ void stsm(uint32_t a, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -225,76 +240,113 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 __device__ __forceinline__ float lo_of(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_of(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+// The upper 8 bits of two values, as bf16, and what is left of them
+__device__ __forceinline__ uint32_t cut_off(f32x2& z) {
+  float l, g;
+  f2_unpack(z, l, g);
+  const uint32_t u = __float_as_uint(l), w = __float_as_uint(g);
+  z = f2_fma(f2_pack(__uint_as_float(u & 0xffff0000u), __uint_as_float(w & 0xffff0000u)), f2_splat(-1.f), z);
+  return __byte_perm(u, w, 0x7632);
+}
+__device__ __forceinline__ uint32_t pack_up(f32x2 z) {
+  float l, g;
+  f2_unpack(z, l, g);
+  return pack2(l, g);
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait0() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Byte of (row, 16-byte piece) of a tile: pieces are permuted inside 128 bytes, so that 8 rows of one piece lie in different banks.
-template <int LDB> __device__ __forceinline__ int at_piece(int row, int piece) { return row * LDB + ((piece ^ (row & 7)) << 4); }
+// Tiles are rows of 64 channels, 128 bytes, in 16-byte pieces; pieces are permuted so that 8 rows of one piece lie in different
+// banks.  128 channels are two tiles.
+constexpr int SUB = C * 128;
+__device__ __forceinline__ uint32_t at_piece(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
-// C rows of up to LDB / 2 channels; rows from m on and channels from d on are zero.  Row r is token t0 + r dir.
-template <int LDB> __device__ __forceinline__ void load_tile(char* tile, const __nv_bfloat16* p, long long st, long long t0, int dir, int m, int d, bool wide) {
-  constexpr int PIECES = LDB / 16;
-  for (int e = threadIdx.x; e < C * PIECES; e += 128) {
-    const int r = e / PIECES, c = e - r * PIECES;
-    const bool on = r < m && c * 8 < d;
-    const __nv_bfloat16* src = p + (t0 + (long long)(on ? r : 0) * dir) * st + (on ? c * 8 : 0);
-    char* dst = tile + at_piece<LDB>(r, c);
-    if (wide) {
-      cp16(saddr(dst), src, on);
-    } else {
-      uint32_t w[4] = {};
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c * 8 + i < d) w[i >> 1] |= (uint32_t)__bfloat16_as_ushort(src[i]) << (16 * (i & 1));
-      }
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+// What a thread copies of one operand: piece c of rows r0, r0 + 16, r0 + 32, r0 + 48 of every chunk
+struct Copy {
+  const __nv_bfloat16* p;                // of row r0 of the chunk at hand
+  long long row16;                       // elements from one of its rows to the next; 4 of them from chunk to chunk
+  int d;                                 // channels of the operand from this piece on
+  __device__ __forceinline__ Copy(const void* base, long long at, long long st, int dir, int channels) {
+    const int c = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+    p = static_cast<const __nv_bfloat16*>(base) + at + (long long)r0 * dir * st + c * 8;
+    row16 = 16 * dir * st;
+    d = channels - c * 8;
   }
-}
-
-template <int DK> struct MmaSmem {
-  static constexpr int TILE = C * DK * 2, VT = C * DVT * 2, STAGE = 2 * TILE + VT, STATE = DK * DVT * 2;
-  static constexpr int BYTES = 2 * STAGE + 2 * STATE + (C + 8) * 4;
+  // into the tile(s) at `tile`; rows from m on and channels beyond the operand's become zero
+  template <int SUBS> __device__ __forceinline__ void load(uint32_t tile, int m, bool wide) {
+    const int c = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+    const uint32_t dst = tile + at_piece(r0, c);
+    const __nv_bfloat16* src = p;
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + s * SUB + i * 2048), "l"(src + s * 64),
+                       "r"(r0 + 16 * i < m && s * 64 < d ? 16 : 0) : "memory");
+        src += row16;
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll 1
+        for (int s = 0; s < SUBS; ++s) {
+          uint32_t w[4] = {};
+          if (r0 + 16 * i < m) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (s * 64 + x < d) w[x >> 1] |= (uint32_t)__bfloat16_as_ushort(src[s * 64 + x]) << (16 * (x & 1));
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + s * SUB + i * 2048), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        src += row16;
+      }
+    }
+    p += 4 * row16;
+  }
 };
 
-template <int DK, int PARTS>
-__global__ void __launch_bounds__(128)
-scan_mma_kernel(const Scan a) {
+template <int DK> struct MmaSmem {
+  static constexpr int TILE = DK / 64 * SUB, STAGE = 2 * TILE + SUB, STATE = DK * 128;
+  static constexpr int OFF_S = 2 * STAGE, OFF_T = OFF_S + 2 * STATE, BYTES = OFF_T + 256 * 4;
+};
+
+template <int DK, int PARTS, bool MANY>
+__global__ void __launch_bounds__(128, (DK == 64 ? 3 : 2))
+scan_mma_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ __align__(128) char smem[];
+  int tile;
+  const Scan& a = pick_scan<MANY>(scans, tile);
   typedef MmaSmem<DK> L;
-  constexpr int LK = DK * 2, LV = DVT * 2, MT = DK / 64, KS = DK / 16, NT = DVT / 8;
-  float* pw = reinterpret_cast<float*>(smem + 2 * L::STAGE + 2 * L::STATE);
+  typedef __nv_bfloat16 T;
+  constexpr int MT = DK / 64, NT = DVT / 8;
+  float* pz = reinterpret_cast<float*>(smem + L::OFF_T) + 64;                       // pz[n] = scale l^n for n = 0 .. 63, 0 below
+  float* pr = pz + 64;                                                              // pr[x] = l^(63-x), 0 beyond (and behind it for 64 more)
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int bh = blockIdx.z, b = bh / a.heads, h = bh - b * a.heads;
-  const int seg = blockIdx.y, col0 = blockIdx.x * DVT;
+  const int seg = blockIdx.y, col0 = tile * DVT;
   const int cols = min(DVT, a.dv - col0);
   const int n = seq_length(a, b);
   const float ld = a.log_decay[h];
-  typedef __nv_bfloat16 T;
-  const T* q = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)(h / a.q.div) * a.q.sh;
-  const T* k = static_cast<const T*>(a.k.p) + b * a.k.sb + (long long)(h / a.k.div) * a.k.sh;
-  const T* v = static_cast<const T*>(a.v.p) + b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + col0;
   const int seg_len = a.seg_chunks * C;
   const int at0 = min(seg * seg_len, a.len), at1 = min(at0 + seg_len, a.len);       // places of this segment, in scan order
   const bool last = n <= at1 && (n > at0 || (n == 0 && seg == 0));                  // holds the last token
   if (a.sums_only && (n <= at1 || seg == a.n_seg - 1)) return;                      // nobody reads the last segment's sum
   const int first = a.reverse && a.init ? 1 : 0;                                    // the given state is one step younger
   const int end = min(at1, n), dir = a.reverse ? -1 : 1;
-  auto token = [&](int at) { return (long long)(a.reverse ? n - 1 - at : at); };
-  auto fetch = [&](int at, int stage) {
-    char* s = smem + stage * L::STAGE;
-    const int m = min(C, end - at);
-    if (!a.sums_only) load_tile<LK>(s, q, a.q.st, token(at), dir, m, a.dk, a.wide);
-    load_tile<LK>(s + L::TILE, k, a.k.st, token(at), dir, m, a.dk, a.wide);
-    load_tile<LV>(s + 2 * L::TILE, v, a.v.st, token(at), dir, m, cols, a.wide);
+  const long long tok0 = a.reverse ? n - 1 - at0 : at0;                             // token at place at0
+  Copy cq(a.q.p, b * a.q.sb + (long long)(h / a.q.div) * a.q.sh + tok0 * a.q.st, a.q.st, dir, a.dk);
+  Copy ck(a.k.p, b * a.k.sb + (long long)(h / a.k.div) * a.k.sh + tok0 * a.k.st, a.k.st, dir, a.dk);
+  Copy cv(a.v.p, b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + tok0 * a.v.st + col0, a.v.st, dir, cols);
+  const uint32_t base = saddr(smem);
+  auto fetch = [&](uint32_t to, int m) {
+    if (!a.sums_only) cq.load<DK / 64>(to, m, a.wide);
+    ck.load<DK / 64>(to + L::TILE, m, a.wide);
+    cv.load<1>(to + 2 * L::TILE, m, a.wide);
     cp_commit();
   };
-  if (at0 < end) fetch(at0, 0);
-  for (int i = tid; i <= C; i += 128) pw[i] = power(ld, i);
+  if (at0 < end) fetch(base, end - at0);
+  for (int i = tid; i < 256; i += 128) pz[i - 64] = i < 64 ? 0.f : i < 128 ? a.scale * power(ld, i - 64) : i < 192 ? power(ld, 191 - i) : 0.f;
   // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1)
   float s[MT][NT][4];
   {
@@ -316,170 +368,177 @@ scan_mma_kernel(const Scan a) {
           s[mt][nt][e] = x;
         }
   }
-  char* state = smem + 2 * L::STAGE;
-  auto write_state = [&](char* to) {
+  // offsets of this lane's rows for ldmatrix and stmatrix; a step of 16 channels is an exclusive or with 32
+  const int r8 = lane & 7, half = (lane >> 3) & 1, quad = lane >> 4;
+  const uint32_t off_a = (r8 + 8 * half) * 128 + ((quad ^ r8) << 4);                // 16 rows, two pieces: A, and B from rows of k
+  const uint32_t off_b = (r8 + 8 * quad) * 128 + ((half ^ r8) << 4);                // the other order
+  auto write_state = [&](uint32_t to) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = (w * MT + mt) * 16 + g + 8 * e;
-          *reinterpret_cast<uint32_t*>(to + at_piece<LV>(i, nt) + 4 * t4) = pack2(s[mt][nt][2 * e], s[mt][nt][2 * e + 1]);
-        }
+      for (int np = 0; np < NT / 2; ++np) {
+        const float (&x)[4] = s[mt][2 * np], (&y)[4] = s[mt][2 * np + 1];
+        stsm(to + (w * MT + mt) * 2048 + (off_a ^ (np << 5)), pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3]));
+      }
   };
-  if (!a.sums_only) write_state(state);
-  __syncthreads();                                                                  // pw
-  // decays of this thread's weights: inside the diagonal 16 x 16 block, and l^(i-j+15) for the blocks before it
-  float near[2][4], far[2][4];
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int gap = g + 8 * (e >> 1) - (x * 8 + 2 * t4 + (e & 1));
-      near[x][e] = gap >= 0 ? pw[gap] : 0.f;
-      far[x][e] = pw[gap + 15];
-    }
-  int stage = 0;
-  for (int at = at0; at < end; at += C, stage ^= 1) {
+  if (!a.sums_only) write_state(base + L::OFF_S);
+  uint32_t stage = 0, sbuf = 0;          // bytes to the buffers at hand
+  // o: rows 4 x + lane / 8 of this warp's 16, 16-byte piece lane & 7
+  const int o_row = w * 16 + (lane >> 3), o_c = lane & 7;
+  T* o_at = static_cast<T*>(a.o) + b * a.o_sb + (tok0 + (long long)o_row * dir) * a.o_st + h * a.o_sh + col0 + o_c * 8;
+  const long long o_step = 4LL * dir * a.o_st;
+  for (int at = at0; at < end; at += C) {
     const int m = min(C, end - at);
     const int young = at == 0 ? first : 0;
     cp_wait0();
     __syncthreads();
-    if (at + C < end) fetch(at + C, stage ^ 1);
-    char* qs = smem + stage * L::STAGE;
-    const uint32_t q_at = saddr(qs), k_at = saddr(qs + L::TILE), v_at = saddr(qs + 2 * L::TILE), s_at = saddr(state + stage * L::STATE);
-    const int r8 = lane & 7, half = (lane >> 3) & 1, quad = lane >> 4;
+    if (at + C < end) fetch(base + (L::STAGE - stage), end - at - C);
+    const uint32_t qs = base + stage, ks_ = qs + L::TILE, vs = ks_ + L::TILE, ss = base + L::OFF_S + sbuf;
     if (!a.sums_only) {
-      uint32_t qf[KS][4];
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) ldsm(qf[ks], q_at + at_piece<LK>(w * 16 + (lane & 15), ks * 2 + quad));
+      uint32_t qf[MT][4][4];
       float o[NT][4] = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int x = 0; x < MT; ++x) {
 #pragma unroll
-        for (int np = 0; np < NT / 2; ++np) {
-          uint32_t f[4];
-          ldsm_t(f, s_at + at_piece<LV>(ks * 16 + r8 + 8 * half, np * 2 + quad));
-          mma(o[2 * np], qf[ks], f[0], f[1]);
-          mma(o[2 * np + 1], qf[ks], f[2], f[3]);
-        }
-      const float d0 = pw[w * 16 + g + 1 - young], d1 = pw[w * 16 + g + 9 - young];
+        for (int ks = 0; ks < 4; ++ks) ldsm(qf[x][ks], qs + x * SUB + w * 2048 + (off_a ^ (ks << 5)));
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) { o[nt][0] *= d0; o[nt][1] *= d0; o[nt][2] *= d1; o[nt][3] *= d1; }
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int np = 0; np < NT / 2; ++np) {
+            uint32_t f[4];
+            ldsm_t(f, ss + (x * 4 + ks) * 2048 + (off_a ^ (np << 5)));
+            mma(o[2 * np], qf[x][ks], f[0], f[1]);
+            mma(o[2 * np + 1], qf[x][ks], f[2], f[3]);
+          }
+      }
+      const float d0 = a.scale * power(ld, w * 16 + g + 1 - young), d1 = a.scale * power(ld, w * 16 + g + 9 - young);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        f2_unpack(f2_mul(f2_pack(o[nt][0], o[nt][1]), f2_splat(d0)), o[nt][0], o[nt][1]);
+        f2_unpack(f2_mul(f2_pack(o[nt][2], o[nt][3]), f2_splat(d1)), o[nt][2], o[nt][3]);
+      }
+#pragma unroll 1
       for (int jb = 0; jb <= w; ++jb) {                                             // 16 tokens of k and v at a time
-        float p[2][4] = {};
+        float p[2][4] = {}, p2[2][4] = {};                                          // two chains of half the length
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t f[4];
-          ldsm(f, k_at + at_piece<LK>(jb * 16 + r8 + 8 * quad, ks * 2 + half));
-          mma(p[0], qf[ks], f[0], f[1]);
-          mma(p[1], qf[ks], f[2], f[3]);
-        }
-        if (jb == w) {
+        for (int x = 0; x < MT; ++x)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int ks = 0; ks < 4; ++ks) {
+            uint32_t f[4];
+            ldsm(f, ks_ + x * SUB + jb * 2048 + (off_b ^ (ks << 5)));
+            mma(ks & 1 ? p2[0] : p[0], qf[x][ks], f[0], f[1]);
+            mma(ks & 1 ? p2[1] : p[1], qf[x][ks], f[2], f[3]);
+          }
+        const float* f = pz + (16 * (w - jb) + g - 2 * t4);                         // l^(i - j): 0 above the diagonal
+        const int gap = 16 * (w - jb) + g - 2 * t4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[x][e] = near[x][e] == 0.f ? 0.f : p[x][e] * near[x][e];
-        } else {
-          const float f = pw[16 * (w - jb) - 15];
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[x][e] *= f * far[x][e];
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int off = 8 * (e >> 1) - 8 * x - (e & 1);
+            p[x][e] = gap + off >= 0 ? (p[x][e] + p2[x][e]) * f[off] : 0.f;
+          }
         const uint32_t pf[4] = {pack2(p[0][0], p[0][1]), pack2(p[0][2], p[0][3]), pack2(p[1][0], p[1][1]), pack2(p[1][2], p[1][3])};
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
-          uint32_t f[4];
-          ldsm_t(f, v_at + at_piece<LV>(jb * 16 + r8 + 8 * half, np * 2 + quad));
-          mma(o[2 * np], pf, f[0], f[1]);
-          mma(o[2 * np + 1], pf, f[2], f[3]);
+          uint32_t v[4];
+          ldsm_t(v, vs + jb * 2048 + (off_a ^ (np << 5)));
+          mma(o[2 * np], pf, v[0], v[1]);
+          mma(o[2 * np + 1], pf, v[2], v[3]);
         }
       }
       if (a.o_f32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = w * 16 + g + 8 * (e >> 1);
+        for (int e = 0; e < 2; ++e) {
+          const int r = w * 16 + g + 8 * e;
           if (r >= m) continue;
-          float* to = static_cast<float*>(a.o) + b * a.o_sb + token(at + r) * a.o_st + h * a.o_sh + col0;
+          float* to = static_cast<float*>(a.o) + b * a.o_sb + (tok0 + (long long)(at - at0 + r) * dir) * a.o_st + h * a.o_sh + col0 + 2 * t4;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const int j = nt * 8 + 2 * t4 + (e & 1);
-            if (j < cols) to[j] = a.scale * o[nt][e];
+            if (a.o_wide) {
+              if (nt * 8 < cols) *reinterpret_cast<float2*>(to + nt * 8) = make_float2(o[nt][2 * e], o[nt][2 * e + 1]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if (nt * 8 + 2 * t4 + x < cols) to[nt * 8 + x] = o[nt][2 * e + x];
+            }
           }
         }
       } else {                                                                      // through this warp's own rows of the q tile
         __syncwarp();
-        const float c = a.scale;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          *reinterpret_cast<uint32_t*>(qs + at_piece<LK>(w * 16 + g, nt) + 4 * t4) = pack2(c * o[nt][0], c * o[nt][1]);
-          *reinterpret_cast<uint32_t*>(qs + at_piece<LK>(w * 16 + g + 8, nt) + 4 * t4) = pack2(c * o[nt][2], c * o[nt][3]);
-        }
+        for (int np = 0; np < NT / 2; ++np)
+          stsm(qs + w * 2048 + (off_a ^ (np << 5)), pack2(o[2 * np][0], o[2 * np][1]), pack2(o[2 * np][2], o[2 * np][3]),
+               pack2(o[2 * np + 1][0], o[2 * np + 1][1]), pack2(o[2 * np + 1][2], o[2 * np + 1][3]));
         __syncwarp();
+        T* to = o_at;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int r = w * 16 + x * 4 + (lane >> 3), c8 = lane & 7;
-          if (r >= m || c8 * 8 >= cols) continue;
-          const uint4 u = *reinterpret_cast<const uint4*>(qs + at_piece<LK>(r, c8));
-          T* to = static_cast<T*>(a.o) + b * a.o_sb + token(at + r) * a.o_st + h * a.o_sh + col0 + c8 * 8;
-          if (a.o_wide) {
-            *reinterpret_cast<uint4*>(to) = u;
-          } else {
-            const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+          const int r = o_row + 4 * x;
+          uint4 u;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(qs + at_piece(r, o_c)) : "memory");
+          if (r < m && o_c * 8 < cols) {
+            if (a.o_wide) {
+              *reinterpret_cast<uint4*>(to) = u;
+            } else {
+              const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c8 * 8 + i < cols) to[i] = __ushort_as_bfloat16((unsigned short)(ww[i >> 1] >> (16 * (i & 1))));
+              for (int i = 0; i < 8; ++i)
+                if (o_c * 8 + i < cols) to[i] = __ushort_as_bfloat16((unsigned short)(ww[i >> 1] >> (16 * (i & 1))));
+            }
           }
+          to += o_step;
         }
+        o_at += 16 * o_step;
       }
     }
     // state: k^T (v weighted by age), the weight on k's fragment
     float acc[MT][NT][4] = {};
-#pragma unroll
+    const float* wt = pr + (C - m) + 2 * t4;
+#pragma unroll 1
     for (int ks = 0; ks < C / 16; ++ks) {
       uint32_t kf[MT][PARTS][4];
-      float wt[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) wt[x] = pw[max(0, m - 1 - (ks * 16 + 2 * t4 + (x & 1) + 8 * (x >> 1)))];
+      const f32x2 w0 = f2_pack(wt[0], wt[1]), w1 = f2_pack(wt[8], wt[9]);
+      wt += 16;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t f[4];
-        ldsm_t(f, k_at + at_piece<LK>(ks * 16 + r8 + 8 * quad, (w * MT + mt) * 2 + half));
+        const int c16 = w * MT + mt;                                                // channels 16 c16 ..
+        ldsm_t(f, ks_ + (c16 >> 2) * SUB + ks * 2048 + (off_b ^ ((c16 & 3) << 5)));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          float lo = lo_of(f[x]) * wt[2 * (x >> 1)], hi = hi_of(f[x]) * wt[2 * (x >> 1) + 1];
+          f32x2 z = f2_mul(f2_pack(lo_of(f[x]), hi_of(f[x])), x < 2 ? w0 : w1);
 #pragma unroll
-          for (int y = 0; y < PARTS; ++y) {
-            const uint32_t u = pack2(lo, hi);
-            kf[mt][y][x] = u;
-            lo -= lo_of(u);
-            hi -= hi_of(u);
-          }
+          for (int y = 0; y < PARTS - 1; ++y) kf[mt][y][x] = cut_off(z);
+          kf[mt][PARTS - 1][x] = pack_up(z);
         }
       }
 #pragma unroll
       for (int np = 0; np < NT / 2; ++np) {
         uint32_t f[4];
-        ldsm_t(f, v_at + at_piece<LV>(ks * 16 + r8 + 8 * half, np * 2 + quad));
+        ldsm_t(f, vs + ks * 2048 + (off_a ^ (np << 5)));
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int y = PARTS - 1; y >= 0; --y)
 #pragma unroll
-          for (int y = PARTS - 1; y >= 0; --y) {
+          for (int mt = 0; mt < MT; ++mt) {
             mma(acc[mt][2 * np], kf[mt][y], f[0], f[1]);
             mma(acc[mt][2 * np + 1], kf[mt][y], f[2], f[3]);
           }
       }
     }
-    const float keep = power_m1(ld, m - young);
+    const f32x2 keep = f2_splat(power_m1(ld, m - young));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][nt][e] = fmaf(s[mt][nt][e], keep, s[mt][nt][e]) + acc[mt][nt][e];
-    if (!a.sums_only && at + C < end) write_state(state + (stage ^ 1) * L::STATE);
+        for (int e = 0; e < 4; e += 2) {
+          const f32x2 z = f2_pack(s[mt][nt][e], s[mt][nt][e + 1]);
+          f2_unpack(f2_add(f2_fma(z, keep, z), f2_pack(acc[mt][nt][e], acc[mt][nt][e + 1])), s[mt][nt][e], s[mt][nt][e + 1]);
+        }
+    stage = L::STAGE - stage;
+    sbuf = L::STATE - sbuf;
+    if (!a.sums_only && at + C < end) write_state(base + L::OFF_S + sbuf);
   }
   const float f = a.sums_only ? 1.f : a.final_scale * (a.reverse ? power(ld, n == 0 && a.init ? 0 : 1) : 1.f);
   float* to = a.sums_only ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.final && last ? a.final + b * a.s_b + h * a.s_h : nullptr;
@@ -573,10 +632,10 @@ step_kernel(const m2_linear_attention_step_args a) {
   }
 }
 
-// Segments: where the blocks of all (sequence, head) pairs do not fill the GPU, a long axis is cut; every segment's own sum is made
-// first (reading k and v once more) and the segments then run side by side.
-static void segments_of(int batch, int heads, int dv, int len, int* n_seg, int* seg_chunks) {
-  const long long blocks = (long long)batch * heads * ((dv + DVT - 1) / DVT), want = 2LL * m2_sm_count();
+// Segments: where the blocks of all (sequence, head) pairs and 64-column tiles do not fill the GPU, a long axis is cut; every
+// segment's own sum is made first (reading k and v once more) and the segments then run side by side.
+static void segments_of(int batch, int heads, int tiles, int len, int* n_seg, int* seg_chunks) {
+  const long long blocks = (long long)batch * heads * tiles, want = 2LL * m2_sm_count();
   const int chunks = (len + C - 1) / C;
   long long seg = (want + blocks - 1) / blocks;
   if (seg > chunks / 4) seg = chunks / 4;               // four chunks at least
@@ -584,10 +643,12 @@ static void segments_of(int batch, int heads, int dv, int len, int* n_seg, int* 
   *seg_chunks = chunks ? (int)((chunks + seg - 1) / seg) : 1;
   *n_seg = chunks ? (chunks + *seg_chunks - 1) / *seg_chunks : 1;
 }
-static long long segment_floats(int batch, int heads, int dk, int dv, int len) {
+static int tiles_of(int dv) { return (dv + DVT - 1) / DVT; }
+// of `scans` scans side by side, each with a state of dk x dv or dv x dk
+static long long segment_floats(int batch, int heads, int dk, int dv, int tiles, int scans, int len) {
   int n, c;
-  segments_of(batch, heads, dv, len, &n, &c);
-  return n > 1 ? (long long)batch * heads * n * dk * dv : 0;
+  segments_of(batch, heads, tiles, len, &n, &c);
+  return n > 1 ? (long long)scans * batch * heads * n * dk * dv : 0;
 }
 
 // Rows in 16-byte pieces: cp.async copies them, and reads no more than them.
@@ -595,34 +656,61 @@ static bool in_pieces(const void* p, long long sb, long long st, long long sh, i
   return m2_aligned(p, 16) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && d % 8 == 0;
 }
 
-template <int DK, int PARTS> static int launch_mma(const char* name, const Scan& a, dim3 grid, cudaStream_t st) {
-  M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS>), MmaSmem<DK>::BYTES);
-  scan_mma_kernel<DK, PARTS><<<grid, 128, MmaSmem<DK>::BYTES, st>>>(a);
+template <int DK, int PARTS, bool MANY> static int launch_mma(const char* name, const Scans& p, dim3 grid, cudaStream_t st) {
+  M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS, MANY>), MmaSmem<DK>::BYTES);
+  scan_mma_kernel<DK, PARTS, MANY><<<grid, 128, MmaSmem<DK>::BYTES, st>>>(p);
+  M2_LAUNCH_CHECK(name);
+  return M2_OK;
+}
+template <int DK> static int launch_mma_of(const char* name, const Scans& p, bool many, bool parts3, dim3 grid, cudaStream_t st) {
+  if (many) return parts3 ? launch_mma<DK, 3, true>(name, p, grid, st) : launch_mma<DK, 2, true>(name, p, grid, st);
+  return parts3 ? launch_mma<DK, 3, false>(name, p, grid, st) : launch_mma<DK, 2, false>(name, p, grid, st);
+}
+template <bool MANY> static int launch_f32(const char* name, const Scans& p, int dk, dim3 grid, cudaStream_t st) {
+  const int dkp = (dk + 15) / 16 * 16;
+  constexpr size_t most = ((size_t)(3 * MAX_D + 2 * C) * LD + C + 4) * sizeof(float);
+  M2_SMEM_ONCE(scan_f32_kernel<MANY>, most);
+  scan_f32_kernel<MANY><<<grid, 256, ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float), st>>>(p);
   M2_LAUNCH_CHECK(name);
   return M2_OK;
 }
 
-static int run_scan(const char* name, Scan a, int dtype, float* segments, cudaStream_t st) {
-  segments_of(a.batch, a.heads, a.dv, a.len, &a.n_seg, &a.seg_chunks);
-  a.segments = a.n_seg > 1 ? segments : nullptr;
-  const dim3 grid((a.dv + DVT - 1) / DVT, a.n_seg, a.batch * a.heads);
-  a.wide = in_pieces(a.q.p, a.q.sb, a.q.st, a.q.sh, a.dk) && in_pieces(a.k.p, a.k.sb, a.k.st, a.k.sh, a.dk) && in_pieces(a.v.p, a.v.sb, a.v.st, a.v.sh, a.dv);
-  a.o_wide = in_pieces(a.o, a.o_sb, a.o_st, a.o_sh, a.dv);
-  if (dtype == M2_BF16) {
-    for (a.sums_only = a.n_seg > 1; a.sums_only >= 0; --a.sums_only) {
-      const int rc = a.dk <= 64 ? (a.final ? launch_mma<64, 3>(name, a, grid, st) : launch_mma<64, 2>(name, a, grid, st))
-                                : (a.final ? launch_mma<128, 3>(name, a, grid, st) : launch_mma<128, 2>(name, a, grid, st));
+// `count` scans over the same (sequence, head) pairs: one launch for those whose keys have up to 64 channels and one for the others
+// (float32: one for all), each behind one of the segments' sums where the axis is cut.
+static int run_scans(const char* name, Scan* list, int count, int dtype, float* segments, cudaStream_t st) {
+  int tiles = 0, n_seg, seg_chunks;
+  for (int i = 0; i < count; ++i) tiles += tiles_of(list[i].dv);
+  segments_of(list[0].batch, list[0].heads, tiles, list[0].len, &n_seg, &seg_chunks);
+  for (int i = 0; i < count; ++i) {
+    Scan& a = list[i];
+    a.n_seg = n_seg;
+    a.seg_chunks = seg_chunks;
+    a.segments = n_seg > 1 ? segments + (long long)i * a.batch * a.heads * n_seg * a.dk * a.dv : nullptr;
+    a.wide = in_pieces(a.q.p, a.q.sb, a.q.st, a.q.sh, a.dk) && in_pieces(a.k.p, a.k.sb, a.k.st, a.k.sh, a.dk) && in_pieces(a.v.p, a.v.sb, a.v.st, a.v.sh, a.dv);
+    a.o_wide = in_pieces(a.o, a.o_sb, a.o_st, a.o_sh, a.dv);
+  }
+  for (int large = 0; large < 2; ++large) {
+    Scans p = {};
+    int n = 0, dk = 0;
+    unsigned x = 0;
+    bool parts3 = false;
+    for (int i = 0; i < count; ++i) {
+      if (dtype == M2_BF16 ? (list[i].dk > 64) != (large == 1) : large == 1) continue;
+      p.s[n] = list[i];
+      p.tiles[n] = tiles_of(list[i].dv);
+      x += p.tiles[n++];
+      dk = list[i].dk > dk ? list[i].dk : dk;
+      parts3 |= list[i].final != nullptr;
+    }
+    if (n == 0) continue;
+    const dim3 grid(x, n_seg, list[0].batch * list[0].heads);
+    for (int sums = n_seg > 1; sums >= 0; --sums) {
+      for (int i = 0; i < n; ++i) p.s[i].sums_only = sums;
+      const int rc = dtype != M2_BF16 ? (n > 1 ? launch_f32<true>(name, p, dk, grid, st) : launch_f32<false>(name, p, dk, grid, st))
+                     : large          ? launch_mma_of<128>(name, p, n > 1, parts3, grid, st)
+                                      : launch_mma_of<64>(name, p, n > 1, parts3, grid, st);
       if (rc) return rc;
     }
-    return M2_OK;
-  }
-  const int dkp = (a.dk + 15) / 16 * 16;
-  const size_t smem = ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float);
-  constexpr size_t most = ((size_t)(3 * MAX_D + 2 * C) * LD + C + 4) * sizeof(float);
-  M2_SMEM_ONCE(scan_f32_kernel, most);
-  for (a.sums_only = a.n_seg > 1; a.sums_only >= 0; --a.sums_only) {
-    scan_f32_kernel<<<grid, 256, smem, st>>>(a);
-    M2_LAUNCH_CHECK(name);
   }
   return M2_OK;
 }
@@ -659,10 +747,9 @@ static Scan base_of(const m2_linear_attention_args& g) {
 extern "C" long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, int backward) {
   using namespace m2::la;
   if (batch < 1 || seq_len < 1 || heads < 1 || kv_heads < 1 || dk < 1 || dv < 1) return 0;
-  long long floats = segment_floats(batch, heads, dk, dv, seq_len);
+  long long floats = segment_floats(batch, heads, dk, dv, tiles_of(dv), 1, seq_len);
   if (backward) {
-    const long long other = segment_floats(batch, heads, dv, dk, seq_len);
-    floats = floats > other ? floats : other;
+    floats = segment_floats(batch, heads, dk, dv, 2 * tiles_of(dk) + tiles_of(dv), 3, seq_len);
     if (heads != kv_heads) floats += (long long)batch * seq_len * heads * (dk + dv);
   }
   return floats * (long long)sizeof(float);
@@ -688,7 +775,7 @@ extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, voi
   s.dk = g.dk; s.dv = g.dv; s.scale = g.scale;
   s.init = g.state_in; s.init_scale = 1.f; s.final = g.state_out; s.final_scale = 1.f;
   s.s_j = 1; s.s_i = g.dv; s.s_h = (long long)g.dk * g.dv; s.s_b = s.s_h * g.heads;
-  return run_scan("m2_linear_attention_fwd", s, g.dtype, g.workspace, (cudaStream_t)stream);
+  return run_scans("m2_linear_attention_fwd", &s, 1, g.dtype, g.workspace, (cudaStream_t)stream);
 }
 
 extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, const m2_linear_attention_grads* grads, void* stream) {
@@ -718,27 +805,26 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
   const Operand u = {d.d_o, d.o_sb, d.o_st, d.o_sh, 1};
   const long long s_h = (long long)g.dk * g.dv, s_b = s_h * g.heads;
   const long long row_k = (long long)g.heads * g.dk, row_v = (long long)g.heads * g.dv;
-  Scan s = base_of(g);                   // dq = scan(do, v, k) from the transposed initial state
-  s.q = u; s.k = v; s.v = k;
-  s.o = d.d_q; s.o_sb = row_k * g.seq_len; s.o_st = row_k; s.o_sh = g.dk;
-  s.dk = g.dv; s.dv = g.dk; s.scale = g.scale;
-  s.init = g.state_in; s.init_scale = 1.f;
-  s.s_b = s_b; s.s_h = s_h; s.s_i = 1; s.s_j = g.dv;
-  if (int rc = run_scan("m2_linear_attention_bwd (d_q)", s, g.dtype, segments, st)) return rc;
-  s = base_of(g);                        // dk = reversed scan(v, do, q)
-  s.q = v; s.k = u; s.v = q; s.reverse = 1;
-  s.o = group > 1 ? (void*)part_k : d.d_k; s.o_f32 = group > 1; s.o_sb = row_k * g.seq_len; s.o_st = row_k; s.o_sh = g.dk;
-  s.dk = g.dv; s.dv = g.dk; s.scale = g.scale;
-  s.init = d.d_state_out; s.init_scale = 1.f / g.scale;
-  s.s_b = s_b; s.s_h = s_h; s.s_i = 1; s.s_j = g.dv;
-  if (int rc = run_scan("m2_linear_attention_bwd (d_k)", s, g.dtype, segments, st)) return rc;
-  s = base_of(g);                        // dv = reversed scan(k, q, do), and what is left of the state is the initial state's gradient
-  s.q = k; s.k = q; s.v = u; s.reverse = 1;
-  s.o = group > 1 ? (void*)part_v : d.d_v; s.o_f32 = group > 1; s.o_sb = row_v * g.seq_len; s.o_st = row_v; s.o_sh = g.dv;
-  s.dk = g.dk; s.dv = g.dv; s.scale = g.scale;
-  s.init = d.d_state_out; s.init_scale = 1.f / g.scale; s.final = d.d_state_in; s.final_scale = g.scale;
-  s.s_b = s_b; s.s_h = s_h; s.s_i = g.dv; s.s_j = 1;
-  if (int rc = run_scan("m2_linear_attention_bwd (d_v)", s, g.dtype, segments, st)) return rc;
+  Scan list[3];
+  Scan& x = list[0] = base_of(g);        // dq = scan(do, v, k) from the transposed initial state
+  x.q = u; x.k = v; x.v = k;
+  x.o = d.d_q; x.o_sb = row_k * g.seq_len; x.o_st = row_k; x.o_sh = g.dk;
+  x.dk = g.dv; x.dv = g.dk; x.scale = g.scale;
+  x.init = g.state_in; x.init_scale = 1.f;
+  x.s_b = s_b; x.s_h = s_h; x.s_i = 1; x.s_j = g.dv;
+  Scan& y = list[1] = base_of(g);        // dk = reversed scan(v, do, q)
+  y.q = v; y.k = u; y.v = q; y.reverse = 1;
+  y.o = group > 1 ? (void*)part_k : d.d_k; y.o_f32 = group > 1; y.o_sb = row_k * g.seq_len; y.o_st = row_k; y.o_sh = g.dk;
+  y.dk = g.dv; y.dv = g.dk; y.scale = g.scale;
+  y.init = d.d_state_out; y.init_scale = 1.f / g.scale;
+  y.s_b = s_b; y.s_h = s_h; y.s_i = 1; y.s_j = g.dv;
+  Scan& z = list[2] = base_of(g);        // dv = reversed scan(k, q, do), and what is left of the state is the initial state's gradient
+  z.q = k; z.k = q; z.v = u; z.reverse = 1;
+  z.o = group > 1 ? (void*)part_v : d.d_v; z.o_f32 = group > 1; z.o_sb = row_v * g.seq_len; z.o_st = row_v; z.o_sh = g.dv;
+  z.dk = g.dk; z.dv = g.dv; z.scale = g.scale;
+  z.init = d.d_state_out; z.init_scale = 1.f / g.scale; z.final = d.d_state_in; z.final_scale = g.scale;
+  z.s_b = s_b; z.s_h = s_h; z.s_i = g.dv; z.s_j = 1;
+  if (int rc = run_scans("m2_linear_attention_bwd", list, 3, g.dtype, segments, st)) return rc;
   if (group > 1 && tokens > 0) {
     for (int w = 0; w < 2; ++w) {
       const float* part = w ? part_v : part_k;
