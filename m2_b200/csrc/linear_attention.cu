@@ -99,20 +99,21 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
   const int first = a.reverse && a.init ? 1 : 0;                                    // the given state is one step younger
   float* own = a.segments ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : nullptr;
   // the state in front of this segment
-  if (!a.sums_only) {
-    const float carry = power_m1(ld, seg_len), carry0 = power_m1(ld, seg_len - first);
-    for (int e = tid; e < dkp * DVT; e += 256) {
-      const int i = e / DVT, j = e - i * DVT;
-      float s = 0.f;
-      if (i < a.dk && j < cols && (n > at0 || last)) {
-        if (a.init) s = a.init_scale * a.init[b * a.s_b + h * a.s_h + i * a.s_i + (col0 + j) * a.s_j];
-        const float* p = a.segments + ((long long)bh * a.n_seg * a.dk + i) * a.dv + col0 + j;
-        for (int r = 0; r < seg; ++r) s = fmaf(s, r ? carry : carry0, s) + p[(long long)r * a.dk * a.dv];
+  for (int e = tid; e < dkp * DVT; e += 256) {
+    const int i = e / DVT, j = e - i * DVT;
+    float s = 0.f;
+    if (!a.sums_only && i < a.dk && j < cols && (n > at0 || last)) {
+      if (a.init) s = a.init_scale * a.init[b * a.s_b + h * a.s_h + i * a.s_i + (col0 + j) * a.s_j];
+      const float* p = a.segments + ((long long)bh * a.n_seg * a.dk + i) * a.dv + col0 + j;
+      const float later = power_m1(ld, seg_len);
+      float carry = power_m1(ld, seg_len - first);
+#pragma unroll 8
+      for (int r = 0; r < seg; ++r) {
+        s = fmaf(s, carry, s) + p[(long long)r * a.dk * a.dv];
+        carry = later;
       }
-      st[i * LD + j] = s;
     }
-  } else {
-    for (int e = tid; e < dkp * DVT; e += 256) st[e / DVT * LD + e % DVT] = 0.f;
+    st[i * LD + j] = s;
   }
   for (int at = at0; at < min(at1, n); at += C) {
     const int m = min(C, n - at);                                                   // tokens of this chunk
@@ -347,11 +348,10 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   };
   if (at0 < end) fetch(base, end - at0);
   for (int i = tid; i < 256; i += 128) pz[i - 64] = i < 64 ? 0.f : i < 128 ? a.scale * power(ld, i - 64) : i < 192 ? power(ld, 191 - i) : 0.f;
-  // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1)
-  float s[MT][NT][4];
-  {
-    const float carry = power_m1(ld, seg_len), carry0 = power_m1(ld, seg_len - first);
-    const bool any = !a.sums_only && (n > at0 || last);
+  // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1).  All
+  // elements of one segment's sum are asked for at once
+  float s[MT][NT][4] = {};
+  auto each = [&](auto&& f) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -359,16 +359,24 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = (w * MT + mt) * 16 + g + 8 * (e >> 1), j = nt * 8 + 2 * t4 + (e & 1);
-          float x = 0.f;
-          if (any && i < a.dk && j < cols) {
-            if (a.init) x = a.init_scale * a.init[b * a.s_b + h * a.s_h + i * a.s_i + (col0 + j) * a.s_j];
-            const float* p = a.segments + ((long long)bh * a.n_seg * a.dk + i) * a.dv + col0 + j;
-            for (int r = 0; r < seg; ++r) x = fmaf(x, r ? carry : carry0, x) + p[(long long)r * a.dk * a.dv];
-          }
-          s[mt][nt][e] = x;
+          if (i < a.dk && j < cols) f(s[mt][nt][e], i, j);
         }
+  };
+  if (!a.sums_only && (n > at0 || last)) {
+    if (a.init) {
+      const float* p = a.init + b * a.s_b + h * a.s_h + col0 * a.s_j;
+      each([&](float& x, int i, int j) { x = a.init_scale * p[i * a.s_i + j * a.s_j]; });
+    }
+    float carry = power_m1(ld, seg_len - first);
+    const float* p = a.segments + (long long)bh * a.n_seg * a.dk * a.dv + col0;
+#pragma unroll 1
+    for (int r = 0; r < seg; ++r, p += a.dk * a.dv) {
+      each([&](float& x, int i, int j) { x = fmaf(x, carry, x) + p[i * a.dv + j]; });
+      carry = power_m1(ld, seg_len);
+    }
   }
-  // offsets of this lane's rows for ldmatrix and stmatrix; a step of 16 channels is an exclusive or with 32
+  // offsets of this lane's rows for ldmatrix and stmatrix; a step of 16 channels is an exclusive or with 32 (tiles start on
+  // 128-byte boundaries, so that it is one of the whole address too)
   const int r8 = lane & 7, half = (lane >> 3) & 1, quad = lane >> 4;
   const uint32_t off_a = (r8 + 8 * half) * 128 + ((quad ^ r8) << 4);                // 16 rows, two pieces: A, and B from rows of k
   const uint32_t off_b = (r8 + 8 * quad) * 128 + ((half ^ r8) << 4);                // the other order
@@ -378,7 +386,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
 #pragma unroll
       for (int np = 0; np < NT / 2; ++np) {
         const float (&x)[4] = s[mt][2 * np], (&y)[4] = s[mt][2 * np + 1];
-        stsm(to + (w * MT + mt) * 2048 + (off_a ^ (np << 5)), pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3]));
+        stsm((to + off_a + (w * MT + mt) * 2048) ^ (np << 5), pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3]));
       }
   };
   if (!a.sums_only) write_state(base + L::OFF_S);
@@ -395,18 +403,19 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
     if (at + C < end) fetch(base + (L::STAGE - stage), end - at - C);
     const uint32_t qs = base + stage, ks_ = qs + L::TILE, vs = ks_ + L::TILE, ss = base + L::OFF_S + sbuf;
     if (!a.sums_only) {
+      const uint32_t q_a = qs + w * 2048 + off_a;
       uint32_t qf[MT][4][4];
       float o[NT][4] = {};
 #pragma unroll
       for (int x = 0; x < MT; ++x) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) ldsm(qf[x][ks], qs + x * SUB + w * 2048 + (off_a ^ (ks << 5)));
+        for (int ks = 0; ks < 4; ++ks) ldsm(qf[x][ks], (q_a + x * SUB) ^ (ks << 5));
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
             uint32_t f[4];
-            ldsm_t(f, ss + (x * 4 + ks) * 2048 + (off_a ^ (np << 5)));
+            ldsm_t(f, (ss + off_a + (x * 4 + ks) * 2048) ^ (np << 5));
             mma(o[2 * np], qf[x][ks], f[0], f[1]);
             mma(o[2 * np + 1], qf[x][ks], f[2], f[3]);
           }
@@ -419,13 +428,14 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
       }
 #pragma unroll 1
       for (int jb = 0; jb <= w; ++jb) {                                             // 16 tokens of k and v at a time
+        const uint32_t k_b = ks_ + off_b + jb * 2048, v_a = vs + off_a + jb * 2048;
         float p[2][4] = {}, p2[2][4] = {};                                          // two chains of half the length
 #pragma unroll
         for (int x = 0; x < MT; ++x)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             uint32_t f[4];
-            ldsm(f, ks_ + x * SUB + jb * 2048 + (off_b ^ (ks << 5)));
+            ldsm(f, (k_b + x * SUB) ^ (ks << 5));
             mma(ks & 1 ? p2[0] : p[0], qf[x][ks], f[0], f[1]);
             mma(ks & 1 ? p2[1] : p[1], qf[x][ks], f[2], f[3]);
           }
@@ -442,7 +452,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
           uint32_t v[4];
-          ldsm_t(v, vs + jb * 2048 + (off_a ^ (np << 5)));
+          ldsm_t(v, v_a ^ (np << 5));
           mma(o[2 * np], pf, v[0], v[1]);
           mma(o[2 * np + 1], pf, v[2], v[3]);
         }
@@ -468,7 +478,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
         __syncwarp();
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np)
-          stsm(qs + w * 2048 + (off_a ^ (np << 5)), pack2(o[2 * np][0], o[2 * np][1]), pack2(o[2 * np][2], o[2 * np][3]),
+          stsm(q_a ^ (np << 5), pack2(o[2 * np][0], o[2 * np][1]), pack2(o[2 * np][2], o[2 * np][3]),
                pack2(o[2 * np + 1][0], o[2 * np + 1][1]), pack2(o[2 * np + 1][2], o[2 * np + 1][3]));
         __syncwarp();
         T* to = o_at;
@@ -495,16 +505,16 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
     // state: k^T (v weighted by age), the weight on k's fragment
     float acc[MT][NT][4] = {};
     const float* wt = pr + (C - m) + 2 * t4;
+    uint32_t k_b = ks_ + off_b, v_a = vs + off_a;
 #pragma unroll 1
     for (int ks = 0; ks < C / 16; ++ks) {
       uint32_t kf[MT][PARTS][4];
       const f32x2 w0 = f2_pack(wt[0], wt[1]), w1 = f2_pack(wt[8], wt[9]);
-      wt += 16;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t f[4];
         const int c16 = w * MT + mt;                                                // channels 16 c16 ..
-        ldsm_t(f, ks_ + (c16 >> 2) * SUB + ks * 2048 + (off_b ^ ((c16 & 3) << 5)));
+        ldsm_t(f, (k_b + (c16 >> 2) * SUB) ^ ((c16 & 3) << 5));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           f32x2 z = f2_mul(f2_pack(lo_of(f[x]), hi_of(f[x])), x < 2 ? w0 : w1);
@@ -516,7 +526,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
 #pragma unroll
       for (int np = 0; np < NT / 2; ++np) {
         uint32_t f[4];
-        ldsm_t(f, vs + ks * 2048 + (off_a ^ (np << 5)));
+        ldsm_t(f, v_a ^ (np << 5));
 #pragma unroll
         for (int y = PARTS - 1; y >= 0; --y)
 #pragma unroll
@@ -525,6 +535,9 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
             mma(acc[mt][2 * np + 1], kf[mt][y], f[2], f[3]);
           }
       }
+      wt += 16;
+      k_b += 2048;
+      v_a += 2048;
     }
     const f32x2 keep = f2_splat(power_m1(ld, m - young));
 #pragma unroll
@@ -638,7 +651,7 @@ static void segments_of(int batch, int heads, int tiles, int len, int* n_seg, in
   const long long blocks = (long long)batch * heads * tiles, want = 2LL * m2_sm_count();
   const int chunks = (len + C - 1) / C;
   long long seg = (want + blocks - 1) / blocks;
-  if (seg > chunks / 4) seg = chunks / 4;               // four chunks at least
+  if (seg > chunks / 2) seg = chunks / 2;               // two chunks at least
   if (seg < 1) seg = 1;
   *seg_chunks = chunks ? (int)((chunks + seg - 1) / seg) : 1;
   *n_seg = chunks ? (chunks + *seg_chunks - 1) / *seg_chunks : 1;
