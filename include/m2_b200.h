@@ -468,7 +468,7 @@ typedef struct {
   float* d_state_in;
 } m2_linear_attention_grads;
 
-long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, int backward);
+long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, m2_dtype dtype, int backward);
 int m2_linear_attention_fwd(const m2_linear_attention_args* args, void* stream);
 int m2_linear_attention_bwd(const m2_linear_attention_args* args, const m2_linear_attention_grads* grads, void* stream);
 

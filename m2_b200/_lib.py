@@ -251,7 +251,7 @@ SYMBOLS = {
     "m2_mixer_split_bytes": (C.c_longlong, [C.c_int]),
     "m2_mlp_split_bytes": (C.c_longlong, [C.c_int, C.c_int, C.c_int]),
     "m2_encoder_fwd": (C.c_int, [C.POINTER(EncoderArgs), C.c_void_p]),
-    "m2_linear_attention_workspace": (C.c_longlong, [C.c_int] * 7),
+    "m2_linear_attention_workspace": (C.c_longlong, [C.c_int] * 8),
     "m2_linear_attention_fwd": (C.c_int, [C.POINTER(LinearAttentionArgs), C.c_void_p]),
     "m2_linear_attention_bwd": (C.c_int, [C.POINTER(LinearAttentionArgs), C.POINTER(LinearAttentionGrads), C.c_void_p]),
     "m2_linear_attention_step": (C.c_int, [C.POINTER(LinearAttentionStepArgs), C.c_void_p]),

@@ -49,6 +49,20 @@ __device__ __forceinline__ float power(float ld, int n) { return n == 0 ? 1.f : 
 // l^n - 1: a state is carried as T + (l^n - 1) T, so that the factor's own rounding does not add up over the chunks of a long memory
 __device__ __forceinline__ float power_m1(float ld, int n) { return n == 0 ? 0.f : expm1f(ld * n); }
 
+// Where the state in front of a segment lies: the given state for the first one, else what join_segments left; NULL: zero
+struct Front {
+  const float* p; long long s_i, s_j; float f;
+  __device__ __forceinline__ Front(const Scan& a, int bh, int b, int h, int seg, int col0) {
+    const bool given = seg == 0 || !a.segments;
+    p = a.sums_only ? nullptr : given ? a.init : a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv;
+    s_i = given ? a.s_i : a.dv;
+    s_j = given ? a.s_j : 1;
+    f = given ? a.init_scale : 1.f;
+    if (p) p += (given ? b * a.s_b + h * a.s_h : 0) + col0 * s_j;
+  }
+  __device__ __forceinline__ float operator()(int i, int j) const { return f * p[i * s_i + j * s_j]; }
+};
+
 __device__ __forceinline__ int seq_length(const Scan& a, int b) {
   if (!a.lengths) return a.len;
   const long long n = a.lengths[b];
@@ -75,6 +89,7 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ float sm[];
   int tile;
   const Scan& a = pick_scan<MANY>(scans, tile);
+  pdl_wait();
   const int dkp = (a.dk + 15) / 16 * 16;
   float* qt = sm;                        // [dkp][LD]  (k index, token)
   float* kt = qt + dkp * LD;             // [dkp][LD]
@@ -99,21 +114,10 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
   const int first = a.reverse && a.init ? 1 : 0;                                    // the given state is one step younger
   float* own = a.segments ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : nullptr;
   // the state in front of this segment
+  const Front front(a, bh, b, h, seg, col0);
   for (int e = tid; e < dkp * DVT; e += 256) {
     const int i = e / DVT, j = e - i * DVT;
-    float s = 0.f;
-    if (!a.sums_only && i < a.dk && j < cols && (n > at0 || last)) {
-      if (a.init) s = a.init_scale * a.init[b * a.s_b + h * a.s_h + i * a.s_i + (col0 + j) * a.s_j];
-      const float* p = a.segments + ((long long)bh * a.n_seg * a.dk + i) * a.dv + col0 + j;
-      const float later = power_m1(ld, seg_len);
-      float carry = power_m1(ld, seg_len - first);
-#pragma unroll 8
-      for (int r = 0; r < seg; ++r) {
-        s = fmaf(s, carry, s) + p[(long long)r * a.dk * a.dv];
-        carry = later;
-      }
-    }
-    st[i * LD + j] = s;
+    st[i * LD + j] = front.p && i < a.dk && j < cols && (n > at0 || last) ? front(i, j) : 0.f;
   }
   for (int at = at0; at < min(at1, n); at += C) {
     const int m = min(C, n - at);                                                   // tokens of this chunk
@@ -318,6 +322,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ __align__(128) char smem[];
   int tile;
   const Scan& a = pick_scan<MANY>(scans, tile);
+  pdl_wait();
   typedef MmaSmem<DK> L;
   typedef __nv_bfloat16 T;
   constexpr int MT = DK / 64, NT = DVT / 8;
@@ -348,10 +353,10 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   };
   if (at0 < end) fetch(base, end - at0);
   for (int i = tid; i < 256; i += 128) pz[i - 64] = i < 64 ? 0.f : i < 128 ? a.scale * power(ld, i - 64) : i < 192 ? power(ld, 191 - i) : 0.f;
-  // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1).  All
-  // elements of one segment's sum are asked for at once
+  // the state in front of this segment: (mt, nt, e) is row (w MT + mt) 16 + g + 8 (e >> 1), column nt 8 + 2 t4 + (e & 1)
   float s[MT][NT][4] = {};
-  auto each = [&](auto&& f) {
+  const Front front(a, bh, b, h, seg, col0);
+  if (front.p && (n > at0 || last)) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -359,21 +364,10 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = (w * MT + mt) * 16 + g + 8 * (e >> 1), j = nt * 8 + 2 * t4 + (e & 1);
-          if (i < a.dk && j < cols) f(s[mt][nt][e], i, j);
+          const bool in = i < a.dk && j < cols;
+          const float x = front(in ? i : 0, in ? j : 0);          // no branch around the load: all are under way at once
+          s[mt][nt][e] = in ? x : 0.f;
         }
-  };
-  if (!a.sums_only && (n > at0 || last)) {
-    if (a.init) {
-      const float* p = a.init + b * a.s_b + h * a.s_h + col0 * a.s_j;
-      each([&](float& x, int i, int j) { x = a.init_scale * p[i * a.s_i + j * a.s_j]; });
-    }
-    float carry = power_m1(ld, seg_len - first);
-    const float* p = a.segments + (long long)bh * a.n_seg * a.dk * a.dv + col0;
-#pragma unroll 1
-    for (int r = 0; r < seg; ++r, p += a.dk * a.dv) {
-      each([&](float& x, int i, int j) { x = fmaf(x, carry, x) + p[i * a.dv + j]; });
-      carry = power_m1(ld, seg_len);
-    }
   }
   // offsets of this lane's rows for ldmatrix and stmatrix; a step of 16 channels is an exclusive or with 32 (tiles start on
   // 128-byte boundaries, so that it is one of the whole address too)
@@ -575,6 +569,32 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   }
 }
 
+// The segments' own sums become the states in front of them, in place: a thread walks over the segments of one element.  (Sums of
+// segments that reach beyond the last token were not written; they reach only segments that have no tokens.)
+__global__ void __launch_bounds__(256)
+join_segments(const __grid_constant__ Scans scans) {
+  const Scan& a = scans.s[blockIdx.z];
+  pdl_wait();
+  const int bh = blockIdx.y, b = bh / a.heads, h = bh - b * a.heads, e = blockIdx.x * 256 + threadIdx.x, size = a.dk * a.dv;
+  if (e >= size) return;
+  float* p = a.segments + (long long)bh * a.n_seg * size + e;
+  const float ld = a.log_decay[h], later = power_m1(ld, a.seg_chunks * C);
+  float carry = power_m1(ld, a.seg_chunks * C - (a.reverse && a.init ? 1 : 0));
+  float x = a.init ? a.init_scale * a.init[b * a.s_b + h * a.s_h + e / a.dv * a.s_i + e % a.dv * a.s_j] : 0.f;
+  for (int r0 = 0; r0 < a.n_seg; r0 += 8) {
+    float y[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) y[r] = r0 + r < a.n_seg - 1 ? p[(long long)(r0 + r) * size] : 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r0 + r >= a.n_seg) break;
+      p[(long long)(r0 + r) * size] = x;
+      x = fmaf(x, carry, x) + y[r];
+      carry = later;
+    }
+  }
+}
+
 // Gradients of shared heads: out[b, t, h, i] = sum over the group's heads, in their order.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -597,6 +617,7 @@ __global__ void __launch_bounds__(256)
 step_kernel(const m2_linear_attention_step_args a) {
   __shared__ float red[16][DVT + 4];
   __shared__ float qs[MAX_D], ks[MAX_D];
+  pdl_wait();
   const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads, col0 = blockIdx.y * DVT;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int cols = min(DVT, a.dv - col0), kvh = h / (a.heads / a.kv_heads);
@@ -647,10 +668,12 @@ step_kernel(const m2_linear_attention_step_args a) {
 
 // Segments: where the blocks of all (sequence, head) pairs and 64-column tiles do not fill the GPU, a long axis is cut; every
 // segment's own sum is made first (reading k and v once more) and the segments then run side by side.
-static void segments_of(int batch, int heads, int tiles, int len, int* n_seg, int* seg_chunks) {
-  const long long blocks = (long long)batch * heads * tiles, want = 2LL * m2_sm_count();
+// A cut costs half as much again, so there is one only where all blocks still run at once: an SM holds three of them, two with
+// 128 channels or float32.
+static void segments_of(int batch, int heads, int tiles, int len, bool small, int* n_seg, int* seg_chunks) {
+  const long long blocks = (long long)batch * heads * tiles;
   const int chunks = (len + C - 1) / C;
-  long long seg = (want + blocks - 1) / blocks;
+  long long seg = (small ? 3LL : 2LL) * m2_sm_count() / blocks;
   if (seg > chunks / 2) seg = chunks / 2;               // two chunks at least
   if (seg < 1) seg = 1;
   *seg_chunks = chunks ? (int)((chunks + seg - 1) / seg) : 1;
@@ -658,9 +681,9 @@ static void segments_of(int batch, int heads, int tiles, int len, int* n_seg, in
 }
 static int tiles_of(int dv) { return (dv + DVT - 1) / DVT; }
 // of `scans` scans side by side, each with a state of dk x dv or dv x dk
-static long long segment_floats(int batch, int heads, int dk, int dv, int tiles, int scans, int len) {
+static long long segment_floats(int batch, int heads, int dk, int dv, int tiles, int scans, int len, int dtype) {
   int n, c;
-  segments_of(batch, heads, tiles, len, &n, &c);
+  segments_of(batch, heads, tiles, len, dtype == M2_BF16 && dk <= 64 && (scans == 1 || dv <= 64), &n, &c);
   return n > 1 ? (long long)scans * batch * heads * n * dk * dv : 0;
 }
 
@@ -669,11 +692,11 @@ static bool in_pieces(const void* p, long long sb, long long st, long long sh, i
   return m2_aligned(p, 16) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && d % 8 == 0;
 }
 
+static long long elements(const Scans& p) { return (long long)p.s[0].batch * p.s[0].len * p.s[0].heads * (p.s[0].dk > p.s[0].dv ? p.s[0].dk : p.s[0].dv); }
+
 template <int DK, int PARTS, bool MANY> static int launch_mma(const char* name, const Scans& p, dim3 grid, cudaStream_t st) {
   M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS, MANY>), MmaSmem<DK>::BYTES);
-  scan_mma_kernel<DK, PARTS, MANY><<<grid, 128, MmaSmem<DK>::BYTES, st>>>(p);
-  M2_LAUNCH_CHECK(name);
-  return M2_OK;
+  return m2_launch(name, elements(p), scan_mma_kernel<DK, PARTS, MANY>, grid, 128, MmaSmem<DK>::BYTES, st, p);
 }
 template <int DK> static int launch_mma_of(const char* name, const Scans& p, bool many, bool parts3, dim3 grid, cudaStream_t st) {
   if (many) return parts3 ? launch_mma<DK, 3, true>(name, p, grid, st) : launch_mma<DK, 2, true>(name, p, grid, st);
@@ -683,17 +706,19 @@ template <bool MANY> static int launch_f32(const char* name, const Scans& p, int
   const int dkp = (dk + 15) / 16 * 16;
   constexpr size_t most = ((size_t)(3 * MAX_D + 2 * C) * LD + C + 4) * sizeof(float);
   M2_SMEM_ONCE(scan_f32_kernel<MANY>, most);
-  scan_f32_kernel<MANY><<<grid, 256, ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float), st>>>(p);
-  M2_LAUNCH_CHECK(name);
-  return M2_OK;
+  return m2_launch(name, elements(p), scan_f32_kernel<MANY>, grid, 256, ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float), st, p);
 }
 
 // `count` scans over the same (sequence, head) pairs: one launch for those whose keys have up to 64 channels and one for the others
 // (float32: one for all), each behind one of the segments' sums where the axis is cut.
 static int run_scans(const char* name, Scan* list, int count, int dtype, float* segments, cudaStream_t st) {
   int tiles = 0, n_seg, seg_chunks;
-  for (int i = 0; i < count; ++i) tiles += tiles_of(list[i].dv);
-  segments_of(list[0].batch, list[0].heads, tiles, list[0].len, &n_seg, &seg_chunks);
+  bool small = dtype == M2_BF16;
+  for (int i = 0; i < count; ++i) {
+    tiles += tiles_of(list[i].dv);
+    small = small && list[i].dk <= 64;
+  }
+  segments_of(list[0].batch, list[0].heads, tiles, list[0].len, small, &n_seg, &seg_chunks);
   for (int i = 0; i < count; ++i) {
     Scan& a = list[i];
     a.n_seg = n_seg;
@@ -723,6 +748,9 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
                      : large          ? launch_mma_of<128>(name, p, n > 1, parts3, grid, st)
                                       : launch_mma_of<64>(name, p, n > 1, parts3, grid, st);
       if (rc) return rc;
+      if (sums) {
+        if (int e = m2_launch(name, elements(p), join_segments, dim3((p.s[0].dk * p.s[0].dv + 255) / 256, grid.z, n), 256, 0, st, p)) return e;
+      }
     }
   }
   return M2_OK;
@@ -757,12 +785,12 @@ static Scan base_of(const m2_linear_attention_args& g) {
 }  // namespace la
 }  // namespace m2
 
-extern "C" long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, int backward) {
+extern "C" long long m2_linear_attention_workspace(int batch, int seq_len, int heads, int kv_heads, int dk, int dv, m2_dtype dtype, int backward) {
   using namespace m2::la;
   if (batch < 1 || seq_len < 1 || heads < 1 || kv_heads < 1 || dk < 1 || dv < 1) return 0;
-  long long floats = segment_floats(batch, heads, dk, dv, tiles_of(dv), 1, seq_len);
+  long long floats = segment_floats(batch, heads, dk, dv, tiles_of(dv), 1, seq_len, dtype);
   if (backward) {
-    floats = segment_floats(batch, heads, dk, dv, 2 * tiles_of(dk) + tiles_of(dv), 3, seq_len);
+    floats = segment_floats(batch, heads, dk, dv, 2 * tiles_of(dk) + tiles_of(dv), 3, seq_len, dtype);
     if (heads != kv_heads) floats += (long long)batch * seq_len * heads * (dk + dv);
   }
   return floats * (long long)sizeof(float);
@@ -776,7 +804,7 @@ extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, voi
   if (g.batch == 0) return M2_OK;
   if (int rc = check_operands("m2_linear_attention_fwd", g)) return rc;
   M2_REQUIRE(g.o || g.seq_len == 0, M2_ERR_ARG, "m2_linear_attention_fwd: o is NULL");
-  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, 0) == 0, M2_ERR_ARG,
+  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, 0) == 0, M2_ERR_ARG,
              "m2_linear_attention_fwd: this shape needs a workspace");
   const int group = g.heads / g.kv_heads;
   const long long row = (long long)g.heads * g.dv;
@@ -801,7 +829,7 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
   if (int rc = check_operands("m2_linear_attention_bwd", g)) return rc;
   M2_REQUIRE(g.seq_len == 0 || (d.d_o && d.d_q && d.d_k && d.d_v), M2_ERR_ARG, "m2_linear_attention_bwd: d_o, d_q, d_k or d_v is NULL");
   M2_REQUIRE(m2_aligned(d.d_o, g.dtype == M2_F32 ? 4 : 2), M2_ERR_ALIGN, "m2_linear_attention_bwd: d_o is not aligned to its type");
-  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, 1) == 0, M2_ERR_ARG,
+  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, 1) == 0, M2_ERR_ARG,
              "m2_linear_attention_bwd: this shape needs a workspace");
   const int group = g.heads / g.kv_heads;
   const cudaStream_t st = (cudaStream_t)stream;
@@ -865,8 +893,7 @@ extern "C" int m2_linear_attention_step(const m2_linear_attention_step_args* arg
              "m2_linear_attention_step: a tensor is not aligned to its type");
   const dim3 grid(g.batch * g.heads, (g.dv + DVT - 1) / DVT);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (g.dtype == M2_F32) step_kernel<float><<<grid, 256, 0, st>>>(g);
-  else step_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g);
-  M2_LAUNCH_CHECK("m2_linear_attention_step");
-  return M2_OK;
+  const long long states = (long long)g.batch * g.heads * g.dk * g.dv;
+  return g.dtype == M2_F32 ? m2_launch("m2_linear_attention_step", states, step_kernel<float>, grid, 256, 0, st, g)
+                           : m2_launch("m2_linear_attention_step", states, step_kernel<__nv_bfloat16>, grid, 256, 0, st, g);
 }

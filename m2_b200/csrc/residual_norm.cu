@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 3 : 1))
 forward_kernel(const Args a) {
   extern __shared__ uint4 ring_mem[];
   __shared__ float2 buf[2][32];
+  pdl_wait();
   Reduce<MAXT> red = {buf, 0};
   const int c0 = threadIdx.x * VEC;
   const int m = MODE == FULL ? VEC : max(0, min(VEC, a.n - c0));        // this thread's columns
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 2 : 1))
 backward_kernel(const Args a) {
   extern __shared__ uint4 ring_mem[];
   __shared__ float2 buf[2][32];
+  pdl_wait();
   Reduce<MAXT> red = {buf, 0};
   const int c0 = threadIdx.x * VEC;
   const int m = MODE == FULL ? VEC : max(0, min(VEC, a.n - c0));
@@ -439,6 +441,7 @@ struct JoinArgs {
 __global__ void __launch_bounds__(512)
 join_kernel(const JoinArgs j) {
   __shared__ float part[16][33];
+  pdl_wait();
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const long long what = blockIdx.y;      // a column sum, or S_COUNT + a sequence
@@ -486,12 +489,11 @@ template <typename TX, typename TY, int MODE, int MAXT> static int launch_t(cons
   static_assert(most <= 227 * 1024 - 1024, "ring");
   if (backward) {
     if (MODE != PLAIN) M2_SMEM_ONCE((backward_kernel<TX, TY, MODE, MAXT>), most);
-    backward_kernel<TX, TY, MODE, MAXT><<<blocks, threads, smem, st>>>(a);
+    return m2_launch("m2_residual_norm_bwd", a.rows * a.n, backward_kernel<TX, TY, MODE, MAXT>, dim3(blocks), threads, smem, st, a);
   } else {
     if (MODE != PLAIN) M2_SMEM_ONCE((forward_kernel<TX, TY, MODE, MAXT>), most);
-    forward_kernel<TX, TY, MODE, MAXT><<<blocks, threads, smem, st>>>(a);
+    return m2_launch("m2_residual_norm_fwd", a.rows * a.n, forward_kernel<TX, TY, MODE, MAXT>, dim3(blocks), threads, smem, st, a);
   }
-  return M2_OK;
 }
 // wide rows of up to 4096 columns go through the ring: longer ones would not fit into shared memory
 template <typename TX, typename TY> static int launch_n(const Args& a, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
@@ -548,7 +550,6 @@ extern "C" int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* str
   const Plan p = plan_of(g.rows, g.rows, g.n, false);
   if (int rc = launch(a, g.x_dtype, g.y_dtype, wide_rows(g) && m2_aligned(g.r, 16) && m2_aligned(g.h, 16), false, p.blocks, p.threads, (cudaStream_t)stream))
     return rc;
-  M2_LAUNCH_CHECK("m2_residual_norm_fwd");
   return M2_OK;
 }
 
@@ -578,7 +579,6 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   const bool wide = wide_rows(g) && m2_aligned(d.d_r, 16) && m2_aligned(d.d_h, 16) && m2_aligned(d.d_x, 16) && m2_aligned(d.d_y, 16) && m2_aligned(d.d_gate, 16);
   const cudaStream_t st = (cudaStream_t)stream;
   if (int rc = launch(a, g.x_dtype, g.y_dtype, wide, true, p.blocks, p.threads, st)) return rc;
-  M2_LAUNCH_CHECK("m2_residual_norm_bwd");
   JoinArgs j = {};
   j.sums = a.sums; j.blocks = p.blocks; j.n = a.n;
   j.out[S_W1] = d.d_after_weight; j.out[S_B1] = d.d_after_bias; j.out[S_W2] = d.d_before_weight; j.out[S_B2] = d.d_before_bias; j.out[S_SCALE] = d.d_scale;
@@ -588,8 +588,7 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   if (seq) { j.gate_sums = a.gate_sums; j.splits = p.splits; j.seqs = a.rows / a.seq_len; j.dg = a.dg; }
   if (seq || j.channel_dg || d.d_after_weight || d.d_after_bias || d.d_before_weight || d.d_before_bias || d.d_scale) {
     const long long ys = S_COUNT + (seq ? j.seqs : 0);
-    join_kernel<<<dim3((a.n + 31) / 32, (unsigned)ys), 512, 0, st>>>(j);
-    M2_LAUNCH_CHECK("m2_residual_norm_bwd (sums)");
+    return m2_launch("m2_residual_norm_bwd (sums)", a.rows * a.n, join_kernel, dim3((a.n + 31) / 32, (unsigned)ys), 512, 0, st, j);
   }
   return M2_OK;
 }

@@ -262,6 +262,7 @@ forward_kernel(const Args a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int split = a.split;
+  pdl_wait();
   const long long row = blockIdx.x / split;
   const uint32_t part = split > 1 ? cta_rank() : 0;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
@@ -425,12 +426,14 @@ template <typename T> static int launch_forward(const Args& a, cudaStream_t st) 
   cfg.gridDim = dim3((unsigned)(a.n * a.split));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = a.split;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = a.n * a.vocab <= M2_OVERLAP_ELEMENTS;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = a.split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.split > 1 ? 2 : 1;
   const cudaError_t e = a.top ? cudaLaunchKernelEx(&cfg, forward_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, forward_kernel<T, false>, a);
   if (e != cudaSuccess) return m2_set_error(M2_ERR_CUDA, "launch of m2_token_logprobs_fwd failed: %s", cudaGetErrorString(e));
   return M2_OK;

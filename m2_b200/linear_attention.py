@@ -63,7 +63,7 @@ def _args(q, k, v, log_decay, scale, initial, lengths, o=None, state=None):
 
 
 def _workspace(a, dev, backward):
-    n = _lib.lib().m2_linear_attention_workspace(a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv, backward)
+    n = _lib.lib().m2_linear_attention_workspace(a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv, a.dtype, backward)
     w = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
     if w is not None:
         a.workspace = w.data_ptr()

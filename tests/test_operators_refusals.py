@@ -110,8 +110,8 @@ def test_c_entries_refuse_before_any_launch():
 
 def test_workspaces():
     lib = _lib.lib()
-    assert lib.m2_linear_attention_workspace(1, 64, 4, 4, 64, 64, 0) == 0                 # a short text needs none
-    assert lib.m2_linear_attention_workspace(2, 10, 4, 2, 8, 6, 1) == 2 * 10 * 4 * 14 * 4  # gradients of shared heads
-    assert lib.m2_linear_attention_workspace(0, 64, 4, 4, 64, 64, 0) == 0
+    assert lib.m2_linear_attention_workspace(1, 64, 4, 4, 64, 64, 1, 0) == 0                 # a short text needs none
+    assert lib.m2_linear_attention_workspace(2, 10, 4, 2, 8, 6, 1, 1) == 2 * 10 * 4 * 14 * 4  # gradients of shared heads
+    assert lib.m2_linear_attention_workspace(0, 64, 4, 4, 64, 64, 1, 0) == 0
     assert lib.m2_residual_norm_workspace(0, 1, 8, 0) == 0
     assert lib.m2_residual_norm_workspace(1, 1, 8, 0) == 6 * 8 * 4
