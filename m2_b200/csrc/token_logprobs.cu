@@ -8,17 +8,18 @@
 //
 // Bound: one read of the logits (gradient: one read, one write).  Forward: every thread streams 16-byte pieces and keeps its own
 // (m, s, t) in float32, rescaled when a piece raises m; one exp a value.  The alternatives are found without sorting: the k-th
-// largest of 64 thread groups' maxima is a lower bound of the row's k-th largest value, so the few values not below it are
-// collected in a second look at the row (L2 or shared memory) and ranked among one another.  Rows with so many equal values that
-// the list overflows are searched k times instead.
+// largest of 64 thread groups' maxima is a lower bound of the row's k-th largest value, so the few threads whose own maximum is not
+// below it look at their values once more, collect what is not below it, and these are ranked among one another.  Rows with so many
+// equal values that the list overflows are searched k times instead.
 #include "common.cuh"
 
 namespace m2 {
 namespace lp {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
-constexpr int GROUPS = 64;               // of 4 lanes each
+constexpr int GROUPS = 64;
+constexpr int SHARE = THREADS / GROUPS;   // threads of a group: 2 or 4
 constexpr int MAX_TOP = 32;              // <= GROUPS
 constexpr int CAND = 1024;               // candidates kept per block
 constexpr int MAX_SPLIT = 8;             // blocks of a cluster that share a row
@@ -118,17 +119,39 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
   rebase(b, m);
   return {m, a.s + b.s, a.t + b.t};
 }
-template <int N> __device__ __forceinline__ void add_values(Stats& a, const float (&f)[N]) {
-  float m = f[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, f[i]);
+__device__ __forceinline__ void add_value(Stats& a, float f) {
+  if (f > a.m) rebase(a, f);
+  const float d = f - a.m, e = ex2(d * LOG2E);                      // -inf: d = -inf, e = 0; NaN stays NaN in s
+  a.s += e;
+  a.t = fmaf(fmaxf(d, -1e4f), e, a.t);
+}
+__device__ __forceinline__ float largest(const uint4& u, const float (&f)[4]) { return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])); }
+__device__ __forceinline__ float largest(const uint4& u, const float (&f)[8]) {         // pairs of bf16 at once
+  auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+  const __nv_bfloat162 m = __hmax2(__hmax2(pair(u.x), pair(u.y)), __hmax2(pair(u.z), pair(u.w)));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+// the values of a 16-byte piece, two at a time
+template <int N> __device__ __forceinline__ void add_piece(Stats& a, const uint4& u, const float (&f)[N]) {
+  const float m = largest(u, f);
   if (m > a.m) rebase(a, m);
+  const f32x2 back = f2_splat(-a.m);
+  f32x2 s = f2_splat(0.f), t = s;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = f[i] - a.m, e = ex2(d * LOG2E);                 // -inf: d = -inf, e = 0; NaN stays NaN in s
-    a.s += e;
-    a.t = fmaf(fmaxf(d, -1e4f), e, a.t);
+  for (int i = 0; i < N; i += 2) {
+    const f32x2 d = f2_add(f2_pack(f[i], f[i + 1]), back);
+    float d0, d1, x0, x1;
+    f2_unpack(d, d0, d1);
+    f2_unpack(f2_mul(d, f2_splat(LOG2E)), x0, x1);
+    const f32x2 e = f2_pack(ex2(x0), ex2(x1));
+    s = f2_add(s, e);
+    t = f2_fma(f2_pack(fmaxf(d0, -1e4f), fmaxf(d1, -1e4f)), e, t);
   }
+  float x, y;
+  f2_unpack(s, x, y);
+  a.s += x + y;
+  f2_unpack(t, x, y);
+  a.t += x + y;
 }
 
 // Elements [lo, hi) of a row as scalar ends and 16-byte pieces.
@@ -166,7 +189,7 @@ template <typename V> __device__ __forceinline__ const V* in_cta(const V* p, uin
 struct Shared {
   Stats warp[WARPS];
   Stats mine;                            // this block's slice
-  uint32_t group[GROUPS];
+  alignas(16) uint32_t group[GROUPS];
   float bound;
   int count;
   unsigned long long best[MAX_TOP];      // this block's k best, best first; 0 where there are fewer
@@ -174,24 +197,33 @@ struct Shared {
   unsigned long long found[WARPS];
 };
 
-// The k best of [lo, hi) into sh.best.  Called by all threads; vmax: the largest value that this thread saw (LOWEST if none).
-template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, int k, float vmax) {
+// The k best of [lo, hi) into sh.best.  Called by all threads; vmax: the largest value that this thread saw (LOWEST if none), nan:
+// whether it saw a NaN (or an infinity, which makes one in its sum).
+template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, int k, float vmax, bool nan) {
   constexpr int N = Piece<T>::N;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float g = fmaxf(vmax, __shfl_xor_sync(~0u, vmax, 1));
-  g = fmaxf(g, __shfl_xor_sync(~0u, g, 2));
-  if ((tid & 3) == 0) sh.group[tid >> 2] = order_key(g);
+  float g = vmax;
+#pragma unroll
+  for (int o = 1; o < SHARE; o <<= 1) g = fmaxf(g, __shfl_xor_sync(~0u, g, o));
+  if (tid % SHARE == 0) sh.group[tid / SHARE] = order_key(g);
   if (tid < MAX_TOP) sh.best[tid] = 0;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  if (tid < GROUPS) {
-    const uint32_t mine = sh.group[tid];
-    int above = 0;                       // how many groups come before this one
-    for (int i = 0; i < GROUPS; ++i) {
-      const uint32_t o = sh.group[i];
-      above += o > mine || (o == mine && i < tid);
+  {                                      // a group's threads share the others: how many come before it
+    constexpr int PER = GROUPS / SHARE;
+    const int g = tid / SHARE, q = tid % SHARE;
+    const uint32_t mine = sh.group[g];
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(sh.group + q * PER + i);
+      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) above += w[j] + (q * PER + i + j < g ? 1u : 0u) > mine;      // keys of maxima end below 2^32 - 1
     }
-    if (above == k - 1) sh.bound = key_value((unsigned long long)mine << 32);
+#pragma unroll
+    for (int o = 1; o < SHARE; o <<= 1) above += __shfl_xor_sync(~0u, above, o);
+    if (q == 0 && above == k - 1) sh.bound = key_value((unsigned long long)mine << 32);
   }
   __syncthreads();
   // a group without values, or with -inf alone, says LOWEST: then everything is a candidate
@@ -202,17 +234,38 @@ template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, 
       if (at < CAND) sh.cand[at] = rank_key(v, id);
     }
   };
-  sp.ends(offer);
   const uint4* body = reinterpret_cast<const uint4*>(sp.p + sp.body());
-  for (int i = tid; i < sp.pieces; i += THREADS) {
-    float f[N];
-    Piece<T>::get(body[i], f);
-    float m = f[0];
+  // few threads have a candidate among their values; the warp looks at those of such threads together, a piece a lane
+  const bool mine = nan || !(vmax < bound);
+  if (mine) sp.ends(offer);
+  for (unsigned need = __ballot_sync(~0u, mine); need;) {
+    constexpr int B = 4;                 // such threads at once
+    int at[B];
 #pragma unroll
-    for (int j = 1; j < N; ++j) m = max_nan(m, f[j]);
-    if (!(m < bound)) {
+    for (int x = 0; x < B; ++x) {
+      at[x] = need ? warp * 32 + __ffs(need) - 1 + lane * THREADS : sp.pieces;
+      need &= need - 1;
+    }
+    while (__any_sync(~0u, at[0] < sp.pieces)) {       // the first of them has the lowest places
+      uint4 u[B];
 #pragma unroll
-      for (int j = 0; j < N; ++j) offer(f[j], sp.body() + i * N + j);
+      for (int x = 0; x < B; ++x)
+        if (at[x] < sp.pieces) u[x] = __ldg(body + at[x]);
+#pragma unroll
+      for (int x = 0; x < B; ++x) {
+        if (at[x] < sp.pieces) {
+          float f[N];
+          Piece<T>::get(u[x], f);
+          float m = f[0];
+#pragma unroll
+          for (int j = 1; j < N; ++j) m = max_nan(m, f[j]);
+          if (!(m < bound)) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) offer(f[j], sp.body() + at[x] * N + j);
+          }
+        }
+        at[x] += 32 * THREADS;
+      }
     }
   }
   __syncthreads();
@@ -256,7 +309,7 @@ template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, 
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 forward_kernel(const Args a) {
   constexpr int N = Piece<T>::N;
   __shared__ Shared sh;
@@ -283,27 +336,31 @@ forward_kernel(const Args a) {
   const int lo = min((int)part * per, a.vocab), hi = min(lo + per, a.vocab);
   const Span<T> sp(x, lo, hi);
   Stats st = {LOWEST, 0.f, 0.f};
-  sp.ends([&](float v, int) { const float f[1] = {v}; add_values<1>(st, f); });
+  sp.ends([&](float v, int) { add_value(st, v); });
   const uint4* body = reinterpret_cast<const uint4*>(x + sp.body());
+  // the next pieces are under way while these are summed
   constexpr int U = 4;
-  int i = tid;
-  for (; i + (U - 1) * THREADS < sp.pieces; i += U * THREADS) {
-    uint4 u[U];
+  uint4 now[U], next[U];
+  auto fetch = [&](uint4 (&u)[U], int i) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) u[j] = __ldg(body + i + j * THREADS);
+    for (int j = 0; j < U; ++j)
+      if (i + j * THREADS < sp.pieces) u[j] = __ldg(body + i + j * THREADS);
+  };
+  fetch(now, tid);
+  for (int i = tid; i < sp.pieces; i += U * THREADS) {
+    fetch(next, i + U * THREADS);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      float f[N];
-      Piece<T>::get(u[j], f);
-      add_values<N>(st, f);
+      if (i + j * THREADS < sp.pieces) {
+        float f[N];
+        Piece<T>::get(now[j], f);
+        add_piece<N>(st, now[j], f);
+      }
+      now[j] = next[j];
     }
   }
-  for (; i < sp.pieces; i += THREADS) {
-    float f[N];
-    Piece<T>::get(__ldg(body + i), f);
-    add_values<N>(st, f);
-  }
   const float vmax = st.m;
+  const bool nan = st.s != st.s;
   for (int o = 16; o > 0; o >>= 1) {
     const Stats b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o), __shfl_xor_sync(~0u, st.t, o)};
     st = join(st, b);
@@ -315,7 +372,7 @@ forward_kernel(const Args a) {
     for (int w = 1; w < WARPS; ++w) st = join(st, sh.warp[w]);
     sh.mine = st;
   }
-  if constexpr (TOP) select_top<T>(sh, sp, a.top, vmax);
+  if constexpr (TOP) select_top<T>(sh, sp, a.top, vmax, nan);
   if (split > 1) cluster_barrier(); else __syncthreads();
   if (part == 0) {
     st = sh.mine;
@@ -384,6 +441,15 @@ backward_kernel(const BwdArgs a, int slices) {
     const float l = (v - m) - log_s, p = ex2(l * LOG2E);
     return used ? -p * fmaf(g_h, fmaxf(l, -1e4f) + h, g) : 0.f;
   };
+  const float c = -fmaf(g_h, h, g);      // -p (g_H (l + H) + g) as p (c - g_H l)
+  auto grad2 = [&](float& v, float& w) {
+    const f32x2 l = f2_add(f2_add(f2_pack(v, w), f2_splat(-m)), f2_splat(-log_s));
+    float l0, l1, x0, x1;
+    f2_unpack(l, l0, l1);
+    f2_unpack(f2_mul(l, f2_splat(LOG2E)), x0, x1);
+    const f32x2 k = f2_fma(f2_splat(-g_h), f2_pack(fmaxf(l0, -1e4f), fmaxf(l1, -1e4f)), f2_splat(c));
+    f2_unpack(f2_mul(f2_pack(ex2(x0), ex2(x1)), k), v, w);
+  };
   const Span<T> sp(x, lo, hi);
   sp.ends([&](float v, int id) { st_from_float(dx + id, grad(v)); });
   const uint4* body = reinterpret_cast<const uint4*>(x + sp.body());
@@ -394,7 +460,10 @@ backward_kernel(const BwdArgs a, int slices) {
     float f[N];
     Piece<T>::get(__ldg(body + i), f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = grad(f[j]);
+    for (int j = 0; j < N; j += 2) {
+      grad2(f[j], f[j + 1]);
+      if (!used) f[j] = f[j + 1] = 0.f;
+    }
     if (wide) {
       reinterpret_cast<uint4*>(out)[i] = Piece<T>::put(f);
     } else {
