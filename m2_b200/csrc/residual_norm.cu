@@ -444,14 +444,27 @@ join_kernel(const JoinArgs j) {
   pdl_wait();
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
-  const long long what = blockIdx.y;      // a column sum, or S_COUNT + a sequence
+  const long long what = blockIdx.y;      // a column sum, or S_COUNT + a sequence (or 16 of them: few units each)
+  if (what >= S_COUNT && j.splits <= 16) {
+    const long long seq = (what - S_COUNT) * 16 + ty;
+    if (seq >= j.seqs || c >= j.n) return;
+    const float* p = j.gate_sums + seq * j.splits * (long long)j.n + c;
+    float s = 0.f;
+    for (int i = 0; i < j.splits; ++i) s += p[(long long)i * j.n];
+    if (j.g_f32) static_cast<float*>(j.dg)[seq * j.n + c] = s;
+    else st_from_float(static_cast<__nv_bfloat16*>(j.dg) + seq * j.n + c, s);
+    return;
+  }
   const bool seq = what >= S_COUNT;
   if (!seq && !j.out[what] && !(what == S_GATE && j.channel_dg)) return;
   const float* p = seq ? j.gate_sums + (what - S_COUNT) * j.splits * (long long)j.n : j.sums + what * j.n;
   const long long step = seq ? j.n : (long long)S_COUNT * j.n;
   const int count = seq ? j.splits : j.blocks;
   float s = 0.f;
-  if (c < j.n) for (int i = ty; i < count; i += 16) s += p[i * step + c];
+  if (c < j.n) {
+#pragma unroll 4
+    for (int i = ty; i < count; i += 16) s += p[i * step + c];
+  }
   part[ty][lane] = s;
   __syncthreads();
   if (ty == 0 && c < j.n) {
@@ -466,15 +479,20 @@ join_kernel(const JoinArgs j) {
 
 struct Plan { int threads, blocks, splits; long long units; };
 // blocks: as many as the SMs hold at once by their registers (96 and 168 a thread), no more than there are units.  Sequences are cut
-// into units where there are fewer of them than blocks; without a gate per sequence all rows are one sequence.
+// into units where that fills the blocks better; without a gate per sequence all rows are one sequence.
 static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   Plan p;
   p.threads = ((n + VEC - 1) / VEC + 31) / 32 * 32;
   const int per_sm = p.threads > 512 ? 1 : max(1, min(16, (backward ? 384 : 640) / p.threads));
   const long long most = (long long)m2_sm_count() * per_sm;
   const long long seqs = rows / seq_len;
-  long long splits = (most + seqs - 1) / seqs;
-  if (splits > seq_len) splits = seq_len;
+  // the number of units a sequence whose rows, round after round of blocks, take the least time (256 sequences on 592 blocks: 2)
+  long long splits = 1, best = -1;
+  const long long top = seqs < most ? (most / seqs < seq_len ? most / seqs : seq_len) : (seq_len < 4 ? seq_len : 4);
+  for (long long s = seqs < most ? top : 1; s <= top; ++s) {
+    const long long time = (seqs * s + most - 1) / most * ((seq_len + s - 1) / s);
+    if (best < 0 || time < best) { best = time; splits = s; }
+  }
   p.splits = (int)splits;
   p.units = seqs * splits;
   p.blocks = (int)(p.units < most ? p.units : most);
@@ -587,7 +605,7 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   const bool seq = a.gate_sums && a.dg;
   if (seq) { j.gate_sums = a.gate_sums; j.splits = p.splits; j.seqs = a.rows / a.seq_len; j.dg = a.dg; }
   if (seq || j.channel_dg || d.d_after_weight || d.d_after_bias || d.d_before_weight || d.d_before_bias || d.d_scale) {
-    const long long ys = S_COUNT + (seq ? j.seqs : 0);
+    const long long ys = S_COUNT + (!seq ? 0 : j.splits <= 16 ? (j.seqs + 15) / 16 : j.seqs);
     return m2_launch("m2_residual_norm_bwd (sums)", a.rows * a.n, join_kernel, dim3((a.n + 31) / 32, (unsigned)ys), 512, 0, st, j);
   }
   return M2_OK;
