@@ -123,25 +123,51 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
     const int m = min(C, n - at);                                                   // tokens of this chunk
     const int young = at == 0 ? first : 0;
     __syncthreads();
-    for (int e = tid; e < dkp * C; e += 256) {                                      // tokens by the lane: no bank conflicts
-      const int i = e / C, t = e - i * C;
-      float x = 0.f, y = 0.f;
-      if (t < m && i < a.dk) {
-        const long long tok = a.reverse ? n - 1 - at - t : at + t;
-        y = __ldg(k + tok * a.k.st + i);
-        if (!a.sums_only) x = __ldg(q + tok * a.q.st + i);
+    if (a.wide) {                        // 16-byte pieces; a warp takes 8 tokens x 4 pieces, so that few lanes of a store share a bank
+      const int lane = tid & 31;
+#pragma unroll 4
+      for (int e = tid >> 5; e < dkp / 2; e += 8) {
+        const int t = (e & 7) * 8 + (lane & 7), i = (e >> 3) * 16 + (lane >> 3) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (t < m && i < a.dk) {
+          const long long tok = a.reverse ? n - 1 - at - t : at + t;
+          y = __ldg(reinterpret_cast<const float4*>(k + tok * a.k.st + i));
+          if (!a.sums_only) x = __ldg(reinterpret_cast<const float4*>(q + tok * a.q.st + i));
+        }
+        float* xs = qt + i * LD + t;
+        float* ys = kt + i * LD + t;
+        xs[0] = x.x; xs[LD] = x.y; xs[2 * LD] = x.z; xs[3 * LD] = x.w;
+        ys[0] = y.x; ys[LD] = y.y; ys[2 * LD] = y.z; ys[3 * LD] = y.w;
       }
-      qt[i * LD + t] = x;
-      kt[i * LD + t] = y;
-    }
-    for (int e = tid; e < C * DVT; e += 256) {
-      const int t = e / DVT, j = e - t * DVT;
-      const long long tok = a.reverse ? n - 1 - at - t : at + t;
-      vs[t * LD + j] = t < m && j < cols ? __ldg(v + tok * a.v.st + j) : 0.f;
+#pragma unroll
+      for (int e = tid; e < C * DVT / 4; e += 256) {
+        const int t = e / (DVT / 4), j = e % (DVT / 4) * 4;
+        const long long tok = a.reverse ? n - 1 - at - t : at + t;
+        *reinterpret_cast<float4*>(vs + t * LD + j) =
+            t < m && j < cols ? __ldg(reinterpret_cast<const float4*>(v + tok * a.v.st + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    } else {
+      for (int e = tid; e < dkp * C; e += 256) {                                    // tokens by the lane: no bank conflicts
+        const int i = e / C, t = e - i * C;
+        float x = 0.f, y = 0.f;
+        if (t < m && i < a.dk) {
+          const long long tok = a.reverse ? n - 1 - at - t : at + t;
+          y = __ldg(k + tok * a.k.st + i);
+          if (!a.sums_only) x = __ldg(q + tok * a.q.st + i);
+        }
+        qt[i * LD + t] = x;
+        kt[i * LD + t] = y;
+      }
+      for (int e = tid; e < C * DVT; e += 256) {
+        const int t = e / DVT, j = e - t * DVT;
+        const long long tok = a.reverse ? n - 1 - at - t : at + t;
+        vs[t * LD + j] = t < m && j < cols ? __ldg(v + tok * a.v.st + j) : 0.f;
+      }
     }
     __syncthreads();
     if (!a.sums_only) {
       float acc[4][4] = {};
+      #pragma unroll 8
       for (int i = 0; i < dkp; ++i) mac(acc, f4(kt + i * LD + ty * 4), f4(qt + i * LD + tx * 4));
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -152,6 +178,7 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
       }
       __syncthreads();
       float o[4][4] = {};
+      #pragma unroll 8
       for (int i = 0; i < dkp; ++i) mac(o, f4(qt + i * LD + ty * 4), f4(st + i * LD + tx * 4));
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -167,21 +194,31 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
         if (t >= m) continue;
         const long long tok = a.reverse ? n - 1 - at - t : at + t;
         const long long to = b * a.o_sb + tok * a.o_st + h * a.o_sh + col0 + tx * 4;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          if (tx * 4 + y >= cols) continue;
-          static_cast<float*>(a.o)[to + y] = a.scale * o[x][y];
+        float* op = static_cast<float*>(a.o) + to;
+        if (a.o_wide) {
+          if (tx * 4 < cols) *reinterpret_cast<float4*>(op) = make_float4(a.scale * o[x][0], a.scale * o[x][1], a.scale * o[x][2], a.scale * o[x][3]);
+          continue;
         }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (tx * 4 + y < cols) op[y] = a.scale * o[x][y];
       }
       __syncthreads();                                                              // st is read by all
     }
     const float keep = power_m1(ld, m - young);
     for (int i0 = ty * 4; i0 < dkp; i0 += 64) {
       float s[4][4] = {};
-      for (int j = 0; j < m; ++j) {
-        const float f = pw[m - 1 - j];
-        const float4 kk = make_float4(f * kt[i0 * LD + j], f * kt[(i0 + 1) * LD + j], f * kt[(i0 + 2) * LD + j], f * kt[(i0 + 3) * LD + j]);
-        mac(s, kk, f4(vs + j * LD + tx * 4));
+      for (int j = 0; j < m; j += 4) {   // tokens behind the last one are zero in v
+        float4 kk[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) kk[x] = f4(kt + (i0 + x) * LD + j);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float f = pw[max(0, m - 1 - j - y)];
+          const float4 vv = f4(vs + (j + y) * LD + tx * 4);
+          auto of = [&](const float4& u) { return y == 0 ? u.x : y == 1 ? u.y : y == 2 ? u.z : u.w; };
+          mac(s, make_float4(f * of(kk[0]), f * of(kk[1]), f * of(kk[2]), f * of(kk[3])), vv);
+        }
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -687,9 +724,10 @@ static long long segment_floats(int batch, int heads, int dk, int dv, int tiles,
   return n > 1 ? (long long)scans * batch * heads * n * dk * dv : 0;
 }
 
-// Rows in 16-byte pieces: cp.async copies them, and reads no more than them.
-static bool in_pieces(const void* p, long long sb, long long st, long long sh, int d) {
-  return m2_aligned(p, 16) && sb % 8 == 0 && st % 8 == 0 && sh % 8 == 0 && d % 8 == 0;
+// Rows in 16-byte pieces, which are read whole and nothing beside them
+static bool in_pieces(const void* p, long long sb, long long st, long long sh, int d, int dtype) {
+  const int piece = dtype == M2_F32 ? 4 : 8;
+  return m2_aligned(p, 16) && sb % piece == 0 && st % piece == 0 && sh % piece == 0 && d % piece == 0;
 }
 
 static long long elements(const Scans& p) { return (long long)p.s[0].batch * p.s[0].len * p.s[0].heads * (p.s[0].dk > p.s[0].dv ? p.s[0].dk : p.s[0].dv); }
@@ -724,8 +762,8 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
     a.n_seg = n_seg;
     a.seg_chunks = seg_chunks;
     a.segments = n_seg > 1 ? segments + (long long)i * a.batch * a.heads * n_seg * a.dk * a.dv : nullptr;
-    a.wide = in_pieces(a.q.p, a.q.sb, a.q.st, a.q.sh, a.dk) && in_pieces(a.k.p, a.k.sb, a.k.st, a.k.sh, a.dk) && in_pieces(a.v.p, a.v.sb, a.v.st, a.v.sh, a.dv);
-    a.o_wide = in_pieces(a.o, a.o_sb, a.o_st, a.o_sh, a.dv);
+    a.wide = in_pieces(a.q.p, a.q.sb, a.q.st, a.q.sh, a.dk, dtype) && in_pieces(a.k.p, a.k.sb, a.k.st, a.k.sh, a.dk, dtype) && in_pieces(a.v.p, a.v.sb, a.v.st, a.v.sh, a.dv, dtype);
+    a.o_wide = in_pieces(a.o, a.o_sb, a.o_st, a.o_sh, a.dv, M2_BF16);
   }
   for (int large = 0; large < 2; ++large) {
     Scans p = {};
