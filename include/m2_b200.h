@@ -440,6 +440,8 @@ int m2_encoder_fwd(const m2_encoder_args* args, void* stream);
  *               rows of o (and gradients) behind them are zero, and the state is that behind the last token.
  *   state_in  : NULL (zero) or float32 (batch, heads, dk, dv), packed; state_out: NULL or the same.  They may be the same memory.
  *   workspace : m2_linear_attention_workspace() bytes on a 16-byte boundary (0: NULL).
+ * A NaN or an infinity in a token's v reaches, besides the tokens after it, outputs of up to 63 tokens before it (their weight
+ * for it is 0, and 0 times it is NaN).
  * bf16: float32 sums and state; the weights (q_i . k_j) decay^(i-j) and the state's copy that q meets are rounded to bf16, as
  * tensor-core operands.  float32: products and sums in float32 throughout.
  * Gradients (m2_linear_attention_bwd): of q, k, v (packed, `dtype`) and of state_in (d_state_in: NULL or float32), from d_o

@@ -14,7 +14,7 @@ from .hyena_filter import (ExponentialModulation, HyenaFilter, OptimModule,  # n
 from .sequence_mixer import MonarchMixerSequenceMixing  # noqa: F401
 from .glu_mlp import BertGatedLinearUnitMLP  # noqa: F401
 from .graph import GraphedForward  # noqa: F401
-from .linear_attention import linear_attention, linear_attention_step  # noqa: F401
+from .linear_attn import linear_attention, linear_attention_step  # noqa: F401
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from .residual_norm import gated_residual_norm  # noqa: F401
 

@@ -49,16 +49,17 @@ __device__ __forceinline__ float power(float ld, int n) { return n == 0 ? 1.f : 
 // l^n - 1: a state is carried as T + (l^n - 1) T, so that the factor's own rounding does not add up over the chunks of a long memory
 __device__ __forceinline__ float power_m1(float ld, int n) { return n == 0 ? 0.f : expm1f(ld * n); }
 
-// Where the state in front of a segment lies: the given state for the first one, else what join_segments left; NULL: zero
+// Where the state in front of a segment lies: what join_segments left, or (uncut) the given state; NULL: zero.  Behind a cut the given
+// state is read by join_segments alone: it may be the memory that the last segment's state goes to.
 struct Front {
   const float* p; long long s_i, s_j; float f;
   __device__ __forceinline__ Front(const Scan& a, int bh, int b, int h, int seg, int col0) {
-    const bool given = seg == 0 || !a.segments;
-    p = a.sums_only ? nullptr : given ? a.init : a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv;
-    s_i = given ? a.s_i : a.dv;
-    s_j = given ? a.s_j : 1;
-    f = given ? a.init_scale : 1.f;
-    if (p) p += (given ? b * a.s_b + h * a.s_h : 0) + col0 * s_j;
+    const bool cut = a.segments != nullptr;
+    p = a.sums_only ? nullptr : cut ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.init;
+    s_i = cut ? a.dv : a.s_i;
+    s_j = cut ? 1 : a.s_j;
+    f = cut ? 1.f : a.init_scale;
+    if (p) p += (cut ? 0 : b * a.s_b + h * a.s_h) + col0 * s_j;
   }
   __device__ __forceinline__ float operator()(int i, int j) const { return f * p[i * s_i + j * s_j]; }
 };
@@ -801,7 +802,7 @@ static int check(const char* name, int batch, int len, int heads, int kv_heads, 
   M2_REQUIRE((long long)batch * heads <= 65535, M2_ERR_UNSUPPORTED, "%s: batch * heads up to 65535, got %d * %d", name, batch, heads);
   M2_REQUIRE(len <= 1 << 24, M2_ERR_UNSUPPORTED, "%s: up to %d steps, got %d", name, 1 << 24, len);
   M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: q, k and v are float32 or bf16", name);
-  M2_REQUIRE(scale != 0.f && scale - scale == 0.f, M2_ERR_ARG, "%s: scale %g", name, scale);
+  M2_REQUIRE(scale != 0.f && scale - scale == 0.f && 1.f / scale - 1.f / scale == 0.f, M2_ERR_ARG, "%s: scale %g", name, scale);
   return M2_OK;
 }
 

@@ -488,7 +488,7 @@ static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   const long long seqs = rows / seq_len;
   // the number of units a sequence whose rows, round after round of blocks, take the least time (256 sequences on 592 blocks: 2)
   long long splits = 1, best = -1;
-  const long long top = seqs < most ? (most / seqs < seq_len ? most / seqs : seq_len) : (seq_len < 4 ? seq_len : 4);
+  const long long top = seqs < most ? (most / seqs < seq_len ? most / seqs : seq_len) : seqs >= 4 * most ? 1 : (seq_len < 4 ? seq_len : 4);
   for (long long s = seqs < most ? top : 1; s <= top; ++s) {
     const long long time = (seqs * s + most - 1) / most * ((seq_len + s - 1) / s);
     if (best < 0 || time < best) { best = time; splits = s; }

@@ -8,7 +8,6 @@ linear_attention() takes whole sequences (prompts, training: it has gradients), 
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -124,11 +123,12 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
                    are zero and the state is that behind the last token
     return_state   also return the state behind the last token, (B, H, dk, dv) float32
 
+    A NaN or an infinity in v[:, t] reaches, besides the tokens after t, outputs of up to 63 tokens before it.
     Differentiable in q, k, v and initial_state."""
     name = "linear_attention"
     B, H, K, dk, dv = _check(name, q, k, v, log_decay, 4)
     scale = dk ** -0.5 if scale is None else float(scale)
-    if scale == 0 or not math.isfinite(scale):
+    if not 2.0 ** -100 <= abs(scale) <= 2.0 ** 100:
         raise ValueError(f"{name}: scale {scale}")
     if initial_state is not None:
         _state(name, initial_state, "initial_state", (B, H, dk, dv), q.get_device())
@@ -159,6 +159,8 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or linear_attention with initial_state")
     scale = dk ** -0.5 if scale is None else float(scale)
+    if not 2.0 ** -100 <= abs(scale) <= 2.0 ** 100:
+        raise ValueError(f"{name}: scale {scale}")
     q, k, v, ld = _packed(q), _packed(k), _packed(v), _decay(log_decay)
     o = q.new_empty((B, H, dv))
     a = _lib.LinearAttentionStepArgs(

@@ -224,8 +224,11 @@ def test_refusals_on_the_device():
     q, k, v, ld, s0 = make(2, 4, 4, 4, 16, 16, torch.float32)
     with pytest.raises(RuntimeError, match="constant"):
         m2_b200.linear_attention(q, k, v, ld.clone().requires_grad_())
-    with pytest.raises(ValueError, match="scale"):
-        m2_b200.linear_attention(q, k, v, ld, scale=0.0)
+    for scale in (0.0, float("nan"), float("inf"), 1e-45):
+        with pytest.raises(ValueError, match="scale"):
+            m2_b200.linear_attention(q, k, v, ld, scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            m2_b200.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0, scale=scale)
     with pytest.raises(ValueError, match="initial_state"):
         m2_b200.linear_attention(q, k, v, ld, initial_state=s0.bfloat16())
     with pytest.raises(ValueError, match="lengths"):
@@ -295,3 +298,19 @@ def test_same_bits_twice_on_another_stream_and_in_a_graph(dtype):
     graph.replay()
     new = run()
     assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(new, a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_state_in_and_out_in_the_same_memory(dtype):
+    """A caller of the C interface continues a text in place, the axis cut over many blocks."""
+    import ctypes as C
+    from m2_b200 import _lib, linear_attn as la
+    q, k, v, ld, s0 = (t.contiguous() for t in make(2, 3000, 3, 3, 64, 64, dtype))
+    ref = m2_b200.linear_attention(q, k, v, ld, initial_state=s0, return_state=True)
+    for _ in range(5):
+        state, o = s0.clone(), torch.empty_like(v)
+        a = la._args(q, k, v, ld, 64 ** -0.5, state, None, o, state)
+        work = la._workspace(a, q.device, 0)
+        assert work is not None
+        m2_b200.ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a))
+        assert torch.equal(o, ref[0]) and torch.equal(state, ref[1])

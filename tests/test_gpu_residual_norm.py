@@ -63,6 +63,8 @@ CASES = [
     (2, 130, 768, "f", "b", "sequence", "channel", True, True, True, False),
     (40, 3, 768, "b", "b", "sequence", "number", True, True, False, True),
     (700, 4, 64, "f", "f", "sequence", "channel", True, True, True, False),
+    (3000, 5, 16, "f", "b", "sequence", "channel", True, True, True, False),
+    (20000, 2, 8, "f", "b", "sequence", "number", True, True, False, True),
     (1, 3000, 40, "f", "b", "sequence", "channel", True, True, True, False),
     (2, 9, 1536, "b", "f", "token", "channel", False, True, True, True),
     (2, 9, 1536, "f", "b", "none", "number", True, False, True, False),
