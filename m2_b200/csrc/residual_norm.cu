@@ -6,10 +6,13 @@
 // With u = dr + N2'(dh):  dx = a u,  da = sum x u,  dn = g u,  dg = u N1(y),  dy = N1'(dn), and for a norm with normalised values v^
 //     N'(d) = rstd (d w - mean(d w) - v^ mean(d w v^)),      dw = sum d v^,      db = sum d      (no mean(d w) for the RMS norm).
 //
-// Bound: every tensor crosses HBM once in each direction.  A block of ceil(n / 256) warps walks over rows and a thread owns the
-// same 8 columns of each: weights stay in its registers, and so do the column sums of the gradient, which meet in a second, small
-// launch that adds the blocks' sums in a fixed order (no atomics: two runs give the same bits).  The next row is loaded while the
-// present one is reduced.  Everything is float32 until the one rounding of each output.
+// Bound: every tensor crosses HBM once in each direction.  Forward: a warp has a row (forward_warp_kernel), 131072 x 1536 with a
+// float32 stream and a gate per token 555 us, 5.1 TB/s or 0.78 of the measured copy rate.  Gradient, and rows of other lengths: a
+// block of ceil(n / 256) warps walks over rows and a thread owns the same 8 columns of each: weights stay in its registers, and so do
+// the column sums of the gradient, which meet in a second, small launch that adds the blocks' sums in a fixed order (no atomics: two
+// runs give the same bits); 32768 x 768 148 us, 3.1 TB/s: 168 registers a thread admit 12 warps an SM, whose two sums over the row
+// then show (with the parameters in shared memory and 96 registers it spilled, 346 us).  Rows to come are copied ahead (cp.async).
+// Everything is float32 until the one rounding of each output.
 #include "common.cuh"
 
 namespace m2 {
@@ -235,7 +238,7 @@ __device__ __forceinline__ V8 gate_plain(const Args& a, long long at, int m) {
 }
 
 template <typename TX, typename TY, int MODE, int MAXT>
-__global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 3 : 1))
+__global__ void __launch_bounds__(MAXT)
 forward_kernel(const Args a) {
   extern __shared__ uint4 ring_mem[];
   __shared__ float2 buf[2][32];
@@ -302,6 +305,140 @@ forward_kernel(const Args a) {
       if (live) store8<MODE>(to, v, m);
     }
     if (a.stats && threadIdx.x == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(s1.x, s1.y, s2.x, s2.y);
+  }
+}
+
+// Forward of rows of 256 K columns, K <= 8: a warp has a row, 8 columns of each 256 a lane, so that nothing waits for a barrier and
+// the 5 steps of a sum over lanes serve the whole row (with 8 columns a thread and a block per row they were half of the
+// instructions: 598 us at 131072 x 1536).  y goes to registers; x and the gate wait in the lane's own places of shared memory until
+// N_after is done, the parameters lie beside them.
+constexpr int WARP_ROWS = 8;             // warps of a block
+template <typename TX, typename TY, int K>
+__global__ void __launch_bounds__(32 * WARP_ROWS, 2)
+forward_warp_kernel(const Args a) {
+  extern __shared__ uint4 ring_mem[];
+  constexpr int N = 256 * K, PX = is_f32<TX> ? 2 : 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float inv_n = 1.f / N;
+  const bool by_row = a.gate >= G_SEQUENCE, a_channel = a.a != nullptr, g_channel = a.gate == G_CHANNEL;
+  pdl_wait();
+  // parameters: columns 8 l .. 8 l + 3 of every lane, then the others, so that a load meets every bank once
+  float4* par = reinterpret_cast<float4*>(ring_mem);
+  constexpr int PLANE = N / 4;
+  for (int e = threadIdx.x; e < PLANE; e += 32 * WARP_ROWS) {
+    const int half = e / (32 * K), k = e / 32 % K, l = e & 31, c = k * 256 + l * 8 + half * 4;
+    auto get = [&](const float* p, float otherwise) {
+      return p ? make_float4(__ldg(p + c), __ldg(p + c + 1), __ldg(p + c + 2), __ldg(p + c + 3)) : make_float4(otherwise, otherwise, otherwise, otherwise);
+    };
+    par[e] = get(a.w1, 1.f);
+    par[PLANE + e] = get(a.b1, 0.f);
+    par[2 * PLANE + e] = get(a.w2, 1.f);
+    par[3 * PLANE + e] = get(a.b2, 0.f);
+    if (a_channel) par[4 * PLANE + e] = get(a.a, 0.f);
+    if (g_channel) {
+      float4 f;
+      if (a.g_f32) f = get(static_cast<const float*>(a.g), 0.f);
+      else {
+        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.g) + c;
+        f = make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]), __bfloat162float(p[3]));
+      }
+      par[5 * PLANE + e] = f;
+    }
+  }
+  __syncthreads();
+  auto param8 = [&](int i, int k) -> V8 {
+    const float4 f = par[i * PLANE + k * 32 + lane], g = par[i * PLANE + (K + k) * 32 + lane];
+    return {{f2_pack(f.x, f.y), f2_pack(f.z, f.w), f2_pack(g.x, g.y), f2_pack(g.z, g.w)}};
+  };
+  // this lane's pieces of x and the gate: 32 lanes apart
+  const int gp = by_row ? (a.g_f32 ? 2 : 1) : 0;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring_mem) + 6 * N * 4 + (warp * K * (PX + gp) * 32 + lane) * 16;
+  auto copy = [&](int piece, const char* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + piece * 512), "l"(src) : "memory");
+  };
+  auto piece = [&](int i) {
+    uint4 u;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(mine + i * 512) : "memory");
+    return u;
+  };
+  const int c0 = lane * 8;
+  auto stats = [&](const V8 (&v)[K]) -> float2 {
+    if (a.rms) {
+      V8 q = mul8(v[0], v[0]);
+#pragma unroll
+      for (int k = 1; k < K; ++k) q = fma8(v[k], v[k], q);
+      float s = sum8(q);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) s += __shfl_xor_sync(~0u, s, o);
+      return make_float2(0.f, rsqrtf(fmaf(s, inv_n, a.eps)));
+    }
+    V8 t = v[0];
+#pragma unroll
+    for (int k = 1; k < K; ++k) t = add8(t, v[k]);
+    float mean = sum8(t) * (1.f / (8 * K));
+    const V8 back = splat8(-mean);
+    t = splat8(0.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k) { const V8 d = add8(v[k], back); t = fma8(d, d, t); }
+    float m2 = sum8(t);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {   // halves of 8 K o values, as in Reduce::moments
+      const float b = __shfl_xor_sync(~0u, mean, o), q = __shfl_xor_sync(~0u, m2, o), e = b - mean;
+      mean = fmaf(0.5f, e, mean);
+      m2 = fmaf(e * e, 4.f * K * o, m2 + q);
+    }
+    return make_float2(mean, rsqrtf(fmaf(m2, inv_n, a.eps)));
+  };
+  for (long long row = (long long)blockIdx.x * WARP_ROWS + warp; row < a.rows; row += (long long)gridDim.x * WARP_ROWS) {
+    const char* px = static_cast<const char*>(a.x) + (row * a.ldx + c0) * (long long)sizeof(TX);
+    const char* py = static_cast<const char*>(a.y) + (row * a.ldy + c0) * (long long)sizeof(TY);
+    uint4 raw[K][is_f32<TY> ? 2 : 1];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      raw[k][0] = *reinterpret_cast<const uint4*>(py + k * 256 * sizeof(TY));
+      if (is_f32<TY>) raw[k][is_f32<TY> ? 1 : 0] = *reinterpret_cast<const uint4*>(py + k * 256 * sizeof(TY) + 16);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      copy(k * PX, px + k * 256 * sizeof(TX));
+      if (PX == 2) copy(k * PX + 1, px + k * 256 * sizeof(TX) + 16);
+    }
+    if (by_row) {
+      const char* pg = static_cast<const char*>(a.g) + (((a.gate == G_TOKEN ? row : row / a.seq_len) * a.ldg + c0) << (a.g_f32 ? 2 : 1));
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        copy(K * PX + k * gp, pg + (k * 256 << (a.g_f32 ? 2 : 1)));
+        if (a.g_f32) copy(K * PX + k * gp + 1, pg + (k * 256 << 2) + 16);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    V8 v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = is_f32<TY> ? from_f32(raw[k][0], raw[k][is_f32<TY> ? 1 : 0]) : from_bf16(raw[k][0]);
+    float2 s1 = make_float2(0.f, 1.f), s2 = s1;
+    if (a.norm1) {
+      s1 = stats(v);
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = fma8(normal(v[k], s1.x, s1.y), param8(0, k), param8(1, k));
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    TX* pr = static_cast<TX*>(a.r) + row * N + c0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const V8 x = is_f32<TX> ? from_f32(piece(k * PX), piece(k * PX + PX - 1)) : from_bf16(piece(k * PX));
+      V8 g = v[k];
+      if (by_row) g = mul8(g, a.g_f32 ? from_f32(piece(K * PX + 2 * k), piece(K * PX + 2 * k + 1)) : from_bf16(piece(K * PX + k)));
+      else if (g_channel) g = mul8(g, param8(5, k));
+      v[k] = fma8(a_channel ? param8(4, k) : splat8(a.scale), x, g);
+      store8<FULL>(pr + k * 256, v[k], 8);
+    }
+    if (a.norm2) {
+      s2 = stats(v);
+      TY* ph = static_cast<TY*>(a.h) + row * N + c0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) store8<FULL>(ph + k * 256, fma8(normal(v[k], s2.x, s2.y), param8(2, k), param8(3, k)), 8);
+    }
+    if (a.stats && lane == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(s1.x, s1.y, s2.x, s2.y);
   }
 }
 
@@ -478,12 +615,12 @@ join_kernel(const JoinArgs j) {
 }
 
 struct Plan { int threads, blocks, splits; long long units; };
-// blocks: as many as the SMs hold at once by their registers (96 and 168 a thread), no more than there are units.  Sequences are cut
+// blocks: as many as the SMs hold at once by their registers (up to 128 and 168 a thread), no more than there are units.  Sequences are cut
 // into units where that fills the blocks better; without a gate per sequence all rows are one sequence.
 static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   Plan p;
   p.threads = ((n + VEC - 1) / VEC + 31) / 32 * 32;
-  const int per_sm = p.threads > 512 ? 1 : max(1, min(16, (backward ? 384 : 640) / p.threads));
+  const int per_sm = p.threads > 512 ? 1 : max(1, min(16, (backward ? 384 : 512) / p.threads));
   const long long most = (long long)m2_sm_count() * per_sm;
   const long long seqs = rows / seq_len;
   // the number of units a sequence whose rows, round after round of blocks, take the least time (256 sequences on 592 blocks: 2)
@@ -499,33 +636,59 @@ static Plan plan_of(long long rows, long long seq_len, int n, bool backward) {
   return p;
 }
 
-template <typename TX, typename TY, int MODE, int MAXT> static int launch_t(const Args& a, bool backward, int blocks, int threads, cudaStream_t st) {
+constexpr int SMEM_MOST = 226 * 1024;
+template <typename TX, typename TY> static int smem_of(const Args& a, int ring_stages, bool backward, int threads) {
   const int gate = a.gate >= G_SEQUENCE ? (a.g_f32 ? 2 : 1) : 0;
-  const int pieces = ((is_f32<TX> ? 2 : 1) + (is_f32<TY> ? 2 : 1)) * (backward ? 2 : 1) + gate;
-  const int smem = MODE == PLAIN ? 0 : stages<MAXT> * pieces * threads * 16;
-  constexpr int most = MODE == PLAIN ? 0 : stages<MAXT> * (((is_f32<TX> ? 2 : 1) + (is_f32<TY> ? 2 : 1)) * 2 + 2) * MAXT * 16;
-  static_assert(most <= 227 * 1024 - 1024, "ring");
-  if (backward) {
-    if (MODE != PLAIN) M2_SMEM_ONCE((backward_kernel<TX, TY, MODE, MAXT>), most);
+  return ring_stages * (((is_f32<TX> ? 2 : 1) + (is_f32<TY> ? 2 : 1)) * (backward ? 2 : 1) + gate) * threads * 16;
+}
+template <typename TX, typename TY, int MODE, int MAXT, bool BACK> static int launch_t(const Args& a, int blocks, int threads, cudaStream_t st) {
+  const int smem = smem_of<TX, TY>(a, MODE == PLAIN ? 0 : stages<MAXT>, BACK, threads);
+  if constexpr (BACK) {
+    if (MODE != PLAIN) M2_SMEM_ONCE((backward_kernel<TX, TY, MODE, MAXT>), SMEM_MOST);
     return m2_launch("m2_residual_norm_bwd", a.rows * a.n, backward_kernel<TX, TY, MODE, MAXT>, dim3(blocks), threads, smem, st, a);
   } else {
-    if (MODE != PLAIN) M2_SMEM_ONCE((forward_kernel<TX, TY, MODE, MAXT>), most);
+    if (MODE != PLAIN) M2_SMEM_ONCE((forward_kernel<TX, TY, MODE, MAXT>), SMEM_MOST);
     return m2_launch("m2_residual_norm_fwd", a.rows * a.n, forward_kernel<TX, TY, MODE, MAXT>, dim3(blocks), threads, smem, st, a);
   }
 }
-// wide rows of up to 4096 columns go through the ring: longer ones would not fit into shared memory
-template <typename TX, typename TY> static int launch_n(const Args& a, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
-  if (threads > 512) return launch_t<TX, TY, PLAIN, 1024>(a, backward, blocks, threads, st);
-  if (!wide) return launch_t<TX, TY, PLAIN, 512>(a, backward, blocks, threads, st);
-  if (a.n % 256) return launch_t<TX, TY, WIDE, 512>(a, backward, blocks, threads, st);
-  return threads <= 192 ? launch_t<TX, TY, FULL, 192>(a, backward, blocks, threads, st) : launch_t<TX, TY, FULL, 512>(a, backward, blocks, threads, st);
+template <typename TX, typename TY, int K> static int launch_warp_k(const Args& a, cudaStream_t st) {
+  const int gate = a.gate >= G_SEQUENCE ? (a.g_f32 ? 2 : 1) : 0;
+  const int smem = 6 * 256 * K * 4 + WARP_ROWS * K * ((is_f32<TX> ? 2 : 1) + gate) * 512;
+  constexpr int most = 6 * 256 * K * 4 + WARP_ROWS * K * 4 * 512;
+  M2_SMEM_ONCE((forward_warp_kernel<TX, TY, K>), most);
+  const long long blocks = (a.rows + WARP_ROWS - 1) / WARP_ROWS, held = (long long)m2_sm_count() * (K == 1 ? 4 : smem > 112 * 1024 ? 1 : 2);
+  return m2_launch("m2_residual_norm_fwd", a.rows * a.n, forward_warp_kernel<TX, TY, K>, dim3((unsigned)(blocks < held ? blocks : held)), 32 * WARP_ROWS, smem, st, a);
 }
-static int launch(const Args& a, int xt, int yt, bool wide, bool backward, int blocks, int threads, cudaStream_t st) {
+template <typename TX, typename TY> static int launch_warp(const Args& a, cudaStream_t st) {
+  switch (a.n / 256) {
+    case 1: return launch_warp_k<TX, TY, 1>(a, st);
+    case 2: return launch_warp_k<TX, TY, 2>(a, st);
+    case 3: return launch_warp_k<TX, TY, 3>(a, st);
+    case 4: return launch_warp_k<TX, TY, 4>(a, st);
+    case 5: return launch_warp_k<TX, TY, 5>(a, st);
+    case 6: return launch_warp_k<TX, TY, 6>(a, st);
+    case 7: return launch_warp_k<TX, TY, 7>(a, st);
+    default: return launch_warp_k<TX, TY, 8>(a, st);
+  }
+}
+// Rows in 16-byte pieces: forward, a warp a row where a warp's registers hold it; else a block a row through the ring, up to 4096
+// columns (longer rows would not fit into shared memory).
+template <typename TX, typename TY, bool BACK> static int launch_n(const Args& a, bool wide, int blocks, int threads, cudaStream_t st) {
+  if (threads > 512) return launch_t<TX, TY, PLAIN, 1024, BACK>(a, blocks, threads, st);
+  if (!wide) return launch_t<TX, TY, PLAIN, 512, BACK>(a, blocks, threads, st);
+  if (a.n % 256) return launch_t<TX, TY, WIDE, 512, BACK>(a, blocks, threads, st);
+  if constexpr (BACK) {
+    if (threads <= 192) return launch_t<TX, TY, FULL, 192, true>(a, blocks, threads, st);
+  } else {
+    if (a.n <= 2048) return launch_warp<TX, TY>(a, st);
+  }
+  return launch_t<TX, TY, FULL, 512, BACK>(a, blocks, threads, st);
+}
+template <bool BACK> static int launch_types(const Args& a, int xt, int yt, bool wide, int blocks, int threads, cudaStream_t st) {
   typedef __nv_bfloat16 B;
-  if (xt == M2_F32) return yt == M2_F32 ? launch_n<float, float>(a, wide, backward, blocks, threads, st) : launch_n<float, B>(a, wide, backward, blocks, threads, st);
-  return yt == M2_F32 ? launch_n<B, float>(a, wide, backward, blocks, threads, st) : launch_n<B, B>(a, wide, backward, blocks, threads, st);
+  if (xt == M2_F32) return yt == M2_F32 ? launch_n<float, float, BACK>(a, wide, blocks, threads, st) : launch_n<float, B, BACK>(a, wide, blocks, threads, st);
+  return yt == M2_F32 ? launch_n<B, float, BACK>(a, wide, blocks, threads, st) : launch_n<B, B, BACK>(a, wide, blocks, threads, st);
 }
-
 static int fill(const char* name, Args& a, const m2_residual_norm_args& g) {
   M2_REQUIRE(g.n >= 1 && g.rows >= 0 && g.seq_len >= 1 && g.rows % g.seq_len == 0, M2_ERR_ARG, "%s: %lld rows of %d columns in sequences of %lld", name,
              g.rows, g.n, g.seq_len);
@@ -566,7 +729,7 @@ extern "C" int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* str
   M2_REQUIRE(m2_aligned(g.stats, 16), M2_ERR_ALIGN, "m2_residual_norm_fwd: stats is not on a 16-byte boundary");
   a.r = g.r; a.h = g.h; a.stats = g.stats;
   const Plan p = plan_of(g.rows, g.rows, g.n, false);
-  if (int rc = launch(a, g.x_dtype, g.y_dtype, wide_rows(g) && m2_aligned(g.r, 16) && m2_aligned(g.h, 16), false, p.blocks, p.threads, (cudaStream_t)stream))
+  if (int rc = launch_types<false>(a, g.x_dtype, g.y_dtype, wide_rows(g) && m2_aligned(g.r, 16) && m2_aligned(g.h, 16), p.blocks, p.threads, (cudaStream_t)stream))
     return rc;
   return M2_OK;
 }
@@ -596,7 +759,7 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   a.gate_sums = a.gate == G_SEQUENCE && p.splits > 1 ? d.workspace + (long long)p.blocks * S_COUNT * a.n : nullptr;
   const bool wide = wide_rows(g) && m2_aligned(d.d_r, 16) && m2_aligned(d.d_h, 16) && m2_aligned(d.d_x, 16) && m2_aligned(d.d_y, 16) && m2_aligned(d.d_gate, 16);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = launch(a, g.x_dtype, g.y_dtype, wide, true, p.blocks, p.threads, st)) return rc;
+  if (int rc = launch_types<true>(a, g.x_dtype, g.y_dtype, wide, p.blocks, p.threads, st)) return rc;
   JoinArgs j = {};
   j.sums = a.sums; j.blocks = p.blocks; j.n = a.n;
   j.out[S_W1] = d.d_after_weight; j.out[S_B1] = d.d_after_bias; j.out[S_W2] = d.d_before_weight; j.out[S_B2] = d.d_before_bias; j.out[S_SCALE] = d.d_scale;
