@@ -35,10 +35,15 @@ struct Scan {
   int wide, o_wide;                      // rows of q, k and v (of o) start on 16-byte boundaries and are whole 16-byte pieces
 };
 
-// Scans that run side by side in one launch (the three of a gradient): blockIdx.x counts the 64-column tiles of all of them
+// Scans that run side by side in one launch (the three of a gradient): blockIdx.x counts the 64-column tiles of all of them, and those of
+// one (sequence, head) after the other
 struct Scans { Scan s[3]; int tiles[3]; };
-template <bool MANY> __device__ __forceinline__ const Scan& pick_scan(const Scans& p, int& tile) {
-  tile = blockIdx.x;
+template <bool MANY> __device__ __forceinline__ const Scan& pick_scan(const Scans& p, int& tile, int& bh) {
+  const int all = p.tiles[0] + (MANY ? p.tiles[1] + p.tiles[2] : 0);
+  // divisions by constants, which stay in uniform registers as the block index does
+  const unsigned x = blockIdx.x;
+  bh = all == 1 ? x : all == 2 ? x / 2 : all == 3 ? x / 3 : all == 4 ? x / 4 : all == 5 ? x / 5 : x / 6;
+  tile = x - bh * all;
   int r = 0;
   if (MANY)
     while (r < 2 && tile >= p.tiles[r]) tile -= p.tiles[r++];
@@ -72,7 +77,8 @@ __device__ __forceinline__ int seq_length(const Scan& a, int b) {
 
 // ---- float32: products on CUDA cores ---------------------------------------------------------------------------------------------------
 // 256 threads as 16 x 16, each with 4 x 4 outputs of a 64 x 64 product; operands lie in shared memory with the summed index outside
-// (two 16-byte loads for 16 products).
+// (two 16-byte loads for 16 products).  Bound by its instructions: 3.7 k FMAs and 2.3 k others a warp and chunk; 4 x 509 tokens of 12
+// heads of 64, cut into four segments: 72 us.  Tensor cores would take six products of bf16 parts for each of these.
 constexpr int LD = 68;                   // row pitch of the tiles: 16-byte rows, spread over the banks
 
 __device__ __forceinline__ void mac(float (&acc)[4][4], const float4& a, const float4& b) {
@@ -88,8 +94,8 @@ template <bool MANY>
 __global__ void __launch_bounds__(256)
 scan_f32_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ float sm[];
-  int tile;
-  const Scan& a = pick_scan<MANY>(scans, tile);
+  int tile, bh;
+  const Scan& a = pick_scan<MANY>(scans, tile, bh);
   pdl_wait();
   const int dkp = (a.dk + 15) / 16 * 16;
   float* qt = sm;                        // [dkp][LD]  (k index, token)
@@ -99,7 +105,7 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
   float* st = pt + C * LD;               // [dkp][LD]  (k index, column)
   float* pw = st + dkp * LD;             // [C + 1]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int bh = blockIdx.z, b = bh / a.heads, h = bh - b * a.heads;
+  const int b = bh / a.heads, h = bh - b * a.heads;
   const int seg = blockIdx.y, col0 = tile * DVT;
   const int cols = min(DVT, a.dv - col0);
   const int n = seq_length(a, b);
@@ -262,7 +268,10 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
 // Bound: a token and head of 64 + 64 channels moves 512 bytes, 64 of them 0.74 us of an SM's share of 6.5 TB/s; the products take
 // 0.55 us (two parts) at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
 // unrolled (2.2 k instructions a warp) does not fit the SM's instruction cache and waited for it more than for anything else.  The
-// same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took as long.
+// same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took longer.
+// Measured: 32 x 2048 tokens, 12 heads of 64: 148 us, 2.7 TB/s, the tensor pipe 42 % busy, 1.2 k instructions a warp and chunk, which
+// 12 warps an SM issue at 38 % of its rate (registers and shared memory admit no more); 16 x 2048, 12 heads of 128: 267 us, the pipe
+// 55 % busy, and its three scans back 542 us in one launch (741 in three).
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -358,8 +367,8 @@ template <int DK, int PARTS, bool MANY>
 __global__ void __launch_bounds__(128, (DK == 64 ? 3 : 2))
 scan_mma_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ __align__(128) char smem[];
-  int tile;
-  const Scan& a = pick_scan<MANY>(scans, tile);
+  int tile, bh;
+  const Scan& a = pick_scan<MANY>(scans, tile, bh);
   pdl_wait();
   typedef MmaSmem<DK> L;
   typedef __nv_bfloat16 T;
@@ -367,7 +376,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   float* pz = reinterpret_cast<float*>(smem + L::OFF_T) + 64;                       // pz[n] = scale l^n for n = 0 .. 63, 0 below
   float* pr = pz + 64;                                                              // pr[x] = l^(63-x), 0 beyond (and behind it for 64 more)
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int bh = blockIdx.z, b = bh / a.heads, h = bh - b * a.heads;
+  const int b = bh / a.heads, h = bh - b * a.heads;
   const int seg = blockIdx.y, col0 = tile * DVT;
   const int cols = min(DVT, a.dv - col0);
   const int n = seq_length(a, b);
@@ -613,7 +622,8 @@ __global__ void __launch_bounds__(256)
 join_segments(const __grid_constant__ Scans scans) {
   const Scan& a = scans.s[blockIdx.z];
   pdl_wait();
-  const int bh = blockIdx.y, b = bh / a.heads, h = bh - b * a.heads, e = blockIdx.x * 256 + threadIdx.x, size = a.dk * a.dv;
+  const int size = a.dk * a.dv, parts = (size + 255) / 256;
+  const int bh = blockIdx.x / parts, b = bh / a.heads, h = bh - b * a.heads, e = (blockIdx.x - bh * parts) * 256 + threadIdx.x;
   if (e >= size) return;
   float* p = a.segments + (long long)bh * a.n_seg * size + e;
   const float ld = a.log_decay[h], later = power_m1(ld, a.seg_chunks * C);
@@ -649,7 +659,8 @@ group_sum_kernel(const float* part, T* out, long long rows, int kv_heads, int gr
 
 // ---- one token ---------------------------------------------------------------------------------------------------------------------------
 // A block per (sequence, head): 16 column quads x 16 row groups of threads walk over the state once, reading and writing it, while
-// q^T S is summed.  Bound by the state's bytes.
+// q^T S is summed.  Bound by the state's bytes: 256 sequences of 12 heads of 128 x 128 72 us, 5.7 TB/s, 0.87 of the measured copy rate;
+// one sequence 2.6 us, a launch.
 template <typename T>
 __global__ void __launch_bounds__(256)
 step_kernel(const m2_linear_attention_step_args a) {
@@ -780,7 +791,8 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
       parts3 |= list[i].final != nullptr;
     }
     if (n == 0) continue;
-    const dim3 grid(x, n_seg, list[0].batch * list[0].heads);
+    const unsigned pairs = (unsigned)list[0].batch * list[0].heads;
+    const dim3 grid(x * pairs, n_seg);
     for (int sums = n_seg > 1; sums >= 0; --sums) {
       for (int i = 0; i < n; ++i) p.s[i].sums_only = sums;
       const int rc = dtype != M2_BF16 ? (n > 1 ? launch_f32<true>(name, p, dk, grid, st) : launch_f32<false>(name, p, dk, grid, st))
@@ -788,7 +800,7 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
                                       : launch_mma_of<64>(name, p, n > 1, parts3, grid, st);
       if (rc) return rc;
       if (sums) {
-        if (int e = m2_launch(name, elements(p), join_segments, dim3((p.s[0].dk * p.s[0].dv + 255) / 256, grid.z, n), 256, 0, st, p)) return e;
+        if (int e = m2_launch(name, elements(p), join_segments, dim3((p.s[0].dk * p.s[0].dv + 255) / 256 * pairs, 1, n), 256, 0, st, p)) return e;
       }
     }
   }
@@ -799,7 +811,7 @@ static int check(const char* name, int batch, int len, int heads, int kv_heads, 
   M2_REQUIRE(batch >= 0 && len >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, M2_ERR_ARG, "%s: batch %d, %d steps, %d heads on %d key heads", name,
              batch, len, heads, kv_heads);
   M2_REQUIRE(dk >= 1 && dv >= 1 && dk <= MAX_D && dv <= MAX_D, M2_ERR_UNSUPPORTED, "%s: heads of 1 to %d channels, got %d and %d", name, MAX_D, dk, dv);
-  M2_REQUIRE((long long)batch * heads <= 65535, M2_ERR_UNSUPPORTED, "%s: batch * heads up to 65535, got %d * %d", name, batch, heads);
+  M2_REQUIRE((long long)batch * heads <= 1 << 24, M2_ERR_UNSUPPORTED, "%s: batch * heads up to %d, got %d * %d", name, 1 << 24, batch, heads);
   M2_REQUIRE(len <= 1 << 24, M2_ERR_UNSUPPORTED, "%s: up to %d steps, got %d", name, 1 << 24, len);
   M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: q, k and v are float32 or bf16", name);
   M2_REQUIRE(scale != 0.f && scale - scale == 0.f && 1.f / scale - 1.f / scale == 0.f, M2_ERR_ARG, "%s: scale %g", name, scale);

@@ -24,7 +24,7 @@ def _check(name, q, k, v, log_decay, dims):
     if len(qs) != dims or len(ks) != dims or len(vs) != dims:
         raise ValueError(f"{name}: q, k and v have {dims} dimensions, got {tuple(qs)}, {tuple(ks)} and {tuple(vs)}")
     B, (H, dk), (K, dv) = qs[0], qs[-2:], vs[-2:]
-    if ks[:-2] != qs[:-2] or ks[-2] != K or ks[-1] != dk or vs[:-2] != qs[:-2] or K == 0 or H % K:
+    if dk == 0 or dv == 0 or ks[:-2] != qs[:-2] or ks[-2] != K or ks[-1] != dk or vs[:-2] != qs[:-2] or K == 0 or H % K:
         raise ValueError(f"{name}: shapes {tuple(qs)}, {tuple(ks)} and {tuple(vs)} of q, k and v do not belong together")
     if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"{name}: q, k and v are all float32 or all bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")

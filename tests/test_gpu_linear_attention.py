@@ -314,3 +314,21 @@ def test_state_in_and_out_in_the_same_memory(dtype):
         assert work is not None
         m2_b200.ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a))
         assert torch.equal(o, ref[0]) and torch.equal(state, ref[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_sequences_than_a_grid_axis(dtype):
+    q, k, v, ld, s0 = make(70001, 3, 1, 1, 4, 4, dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o, s = m2_b200.linear_attention(*leaves, ld, initial_state=s0, return_state=True)
+    grads = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    tail = [t.detach()[-5:].clone().requires_grad_() for t in leaves]
+    ro, rs = m2_b200.linear_attention(*tail, ld, initial_state=s0[-5:], return_state=True)
+    assert torch.equal(o[-5:], ro) and torch.equal(s[-5:], rs)
+    for a, b in zip(grads, torch.autograd.grad(ro, tail, torch.ones_like(ro))):
+        assert torch.equal(a[-5:], b)
+    state, few = s0.clone(), s0[-5:].clone()
+    with torch.no_grad():
+        o = m2_b200.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
+        ro = m2_b200.linear_attention_step(q[-5:, 0], k[-5:, 0], v[-5:, 0], ld, few)
+    assert torch.equal(o[-5:], ro) and torch.equal(state[-5:], few)
