@@ -436,9 +436,16 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   const int o_row = w * 16 + (lane >> 3), o_c = lane & 7;
   T* o_at = static_cast<T*>(a.o) + b * a.o_sb + (tok0 + (long long)o_row * dir) * a.o_st + h * a.o_sh + col0 + o_c * 8;
   const long long o_step = 4LL * dir * a.o_st;
+  float d0 = 0.f, d1 = 0.f;              // what the state fades by on the way to rows g and g + 8 of this warp's, with the output's scale
+  f32x2 keep = f2_splat(0.f);            // and through a chunk, less 1
   for (int at = at0; at < end; at += C) {
     const int m = min(C, end - at);
-    const int young = at == 0 ? first : 0;
+    if (at == at0 || at == C || m < C) { // else as in the chunk before
+      const int young = at == 0 ? first : 0;
+      d0 = a.scale * power(ld, w * 16 + g + 1 - young);
+      d1 = a.scale * power(ld, w * 16 + g + 9 - young);
+      keep = f2_splat(power_m1(ld, m - young));
+    }
     cp_wait0();
     __syncthreads();
     if (at + C < end) fetch(base + (L::STAGE - stage), end - at - C);
@@ -461,7 +468,6 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
             mma(o[2 * np + 1], qf[x][ks], f[2], f[3]);
           }
       }
-      const float d0 = a.scale * power(ld, w * 16 + g + 1 - young), d1 = a.scale * power(ld, w * 16 + g + 9 - young);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         f2_unpack(f2_mul(f2_pack(o[nt][0], o[nt][1]), f2_splat(d0)), o[nt][0], o[nt][1]);
@@ -580,7 +586,6 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
       k_b += 2048;
       v_a += 2048;
     }
-    const f32x2 keep = f2_splat(power_m1(ld, m - young));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
