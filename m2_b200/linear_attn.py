@@ -97,18 +97,14 @@ class _LinearAttention(torch.autograd.Function):
             return (None,) * 8
         d_o = torch.zeros((B, L, H, v.shape[3]), dtype=q.dtype, device=q.device) if d_o is None else _packed(d_o)
         a = _args(q, k, v, log_decay, ctx.scale, initial, lengths)
-        g = _lib.LinearAttentionGrads()
-        g.d_o, (g.o_sb, g.o_st, g.o_sh, _) = d_o.data_ptr(), d_o.stride()
+        dq, dk_, dv_ = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        d_initial = initial.new_empty(initial.shape) if initial is not None else None
         if d_state is not None:
             d_state = d_state.contiguous()
-            g.d_state_out = d_state.data_ptr()
-        dq, dk_, dv_ = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        g.d_q, g.d_k, g.d_v = dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr()
-        d_initial = torch.empty_like(initial) if initial is not None else None
-        if d_initial is not None:
-            g.d_state_in = d_initial.data_ptr()
+        g = _lib.LinearAttentionGrads(d_o.data_ptr(), *d_o.stride()[:3], d_state.data_ptr() if d_state is not None else None,
+                                      dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), d_initial.data_ptr() if d_initial is not None else None)
         work = _workspace(a, q.device, 1)  # noqa: F841
-        ops._launch("m2_linear_attention_bwd", q, _lib.lib().m2_linear_attention_bwd, C.byref(a), C.byref(g), launches=3)
+        ops._launch("m2_linear_attention_bwd", q, _lib.lib().m2_linear_attention_bwd, C.byref(a), C.byref(g))
         return dq, dk_, dv_, None, None, d_initial, None, None
 
 

@@ -73,21 +73,17 @@ class _ResidualNorm(torch.autograd.Function):
         number, kind, seq_len, eps, rms = ctx.plain
         if d_r is None and d_h is None:
             return (None,) * 13
-        n, dev = x.shape[-1], x.device
+        n = x.shape[-1]
         a, keep = _args(x, y, gate, kind, seq_len, scale, number, params, eps, rms)  # noqa: F841
         a.stats = stats.data_ptr()
         d_r = d_r.contiguous() if d_r is not None else None
         d_h = d_h.contiguous() if d_h is not None else None
         want = ctx.needs_input_grad
-        like = (x, y, gate, scale, *params)
-        out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if w and t is not None else None for t, w in zip(like, want)]
+        out = [t.new_empty(t.shape) if w and t is not None else None for t, w in zip((x, y, gate, scale, *params), want)]
         if a.rows == 0:                                        # nothing to launch: sums over no rows
             return (*[t.zero_() if t is not None else None for t in out], None, None, None, None, None)
-        g = _lib.ResidualNormGrads()
-        g.d_r, g.d_h = _ptr(d_r), _ptr(d_h)
-        g.d_x, g.d_y, g.d_gate, g.d_scale, g.d_after_weight, g.d_after_bias, g.d_before_weight, g.d_before_bias = (_ptr(t) for t in out)
-        work = torch.empty(_lib.lib().m2_residual_norm_workspace(a.rows, seq_len, n, kind) // 4, dtype=torch.float32, device=dev)
-        g.workspace = work.data_ptr()
+        work = stats.new_empty(_lib.lib().m2_residual_norm_workspace(a.rows, seq_len, n, kind) // 4)
+        g = _lib.ResidualNormGrads(_ptr(d_r), _ptr(d_h), *(_ptr(t) for t in out), work.data_ptr())
         ops._launch("m2_residual_norm_bwd", x, _lib.lib().m2_residual_norm_bwd, C.byref(a), C.byref(g), launches=2)
         return (*out, None, None, None, None, None)
 
