@@ -116,6 +116,27 @@ def test_long_axis_in_segments_equals_the_same_in_pieces(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (40, 72)])
+def test_texts_that_end_in_any_segment(dk, dv, dtype):
+    """Texts of very different lengths whose axis is cut: they end in front of, on and behind the cuts, and gradients run back from there."""
+    L, H, K = 650, 2, 1
+    lengths = torch.tensor([0, 1, 127, 128, 129, 400, 512, 650], device="cuda")
+    q, k, v, ld, s0 = make(len(lengths), L, H, K, dk, dv, dtype, seed=11)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, s0)]
+    o, s = m2_b200.linear_attention(*leaves[:3], ld, initial_state=leaves[3], lengths=lengths, return_state=True)
+    do, ds = torch.randn_like(o), torch.randn_like(s)
+    grads = torch.autograd.grad([o, s], leaves, [do, ds])
+    runs = []
+    for sign in (lambda t: t, torch.abs):                   # the definition, and of the absolute values
+        wide = [sign(t.detach().double()).requires_grad_() for t in leaves]
+        out = definition(*wide[:3], ld.double(), dk ** -0.5, wide[3], lengths)
+        runs.append([*out, *torch.autograd.grad(out, wide, [sign(do.double()), sign(ds.double())])])
+    ref, big = runs
+    for name, got, r, M, d in zip(("o", "state", "dq", "dk", "dv", "d initial"), [o, s, *grads], ref, big, (dk, 0, dv, dv + 2, dk + 2, 0)):
+        within(got, r, slack(dtype if d else torch.float32, L, d + 80, M, r), name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_values_behind_a_text_are_not_read(dtype):
     q, k, v, ld, s0 = make(3, 150, 2, 2, 64, 64, dtype)
     n = torch.tensor([0, 97, 150], device="cuda")
