@@ -358,19 +358,20 @@ struct Copy {
   }
 };
 
-template <int DK> struct MmaSmem {
-  static constexpr int TILE = DK / 64 * SUB, STAGE = 2 * TILE + SUB, STATE = DK * 128;
+template <int DK, bool SUMS> struct MmaSmem {
+  static constexpr int TILE = DK / 64 * SUB, K = SUMS ? 0 : TILE, STAGE = K + TILE + SUB, STATE = SUMS ? 0 : DK * 128;      // K: k behind q
   static constexpr int OFF_S = 2 * STAGE, OFF_T = OFF_S + 2 * STATE, BYTES = OFF_T + 256 * 4;
 };
 
-template <int DK, int PARTS, bool MANY>
-__global__ void __launch_bounds__(128, (DK == 64 ? 3 : 2))
+// SUMS: a segment's own sum alone, the first of the launches over segments
+template <int DK, int PARTS, bool MANY, bool SUMS>
+__global__ void __launch_bounds__(128, (DK == 64 ? 3 : 2) + SUMS)
 scan_mma_kernel(const __grid_constant__ Scans scans) {
   extern __shared__ __align__(128) char smem[];
   int tile, bh;
   const Scan& a = pick_scan<MANY>(scans, tile, bh);
   pdl_wait();
-  typedef MmaSmem<DK> L;
+  typedef MmaSmem<DK, SUMS> L;
   typedef __nv_bfloat16 T;
   constexpr int MT = DK / 64, NT = DVT / 8;
   float* pz = reinterpret_cast<float*>(smem + L::OFF_T) + 64;                       // pz[n] = scale l^n for n = 0 .. 63, 0 below
@@ -384,7 +385,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   const int seg_len = a.seg_chunks * C;
   const int at0 = min(seg * seg_len, a.len), at1 = min(at0 + seg_len, a.len);       // places of this segment, in scan order
   const bool last = n <= at1 && (n > at0 || (n == 0 && seg == 0));                  // holds the last token
-  if (a.sums_only && (n <= at1 || seg == a.n_seg - 1)) return;                      // nobody reads the last segment's sum
+  if (SUMS && (n <= at1 || seg == a.n_seg - 1)) return;                      // nobody reads the last segment's sum
   const int first = a.reverse && a.init ? 1 : 0;                                    // the given state is one step younger
   const int end = min(at1, n), dir = a.reverse ? -1 : 1;
   const long long tok0 = a.reverse ? n - 1 - at0 : at0;                             // token at place at0
@@ -393,9 +394,9 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   Copy cv(a.v.p, b * a.v.sb + (long long)(h / a.v.div) * a.v.sh + tok0 * a.v.st + col0, a.v.st, dir, cols);
   const uint32_t base = saddr(smem);
   auto fetch = [&](uint32_t to, int m) {
-    if (!a.sums_only) cq.load<DK / 64>(to, m, a.wide);
-    ck.load<DK / 64>(to + L::TILE, m, a.wide);
-    cv.load<1>(to + 2 * L::TILE, m, a.wide);
+    if (!SUMS) cq.load<DK / 64>(to, m, a.wide);
+    ck.load<DK / 64>(to + L::K, m, a.wide);
+    cv.load<1>(to + L::K + L::TILE, m, a.wide);
     cp_commit();
   };
   if (at0 < end) fetch(base, end - at0);
@@ -430,7 +431,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
         stsm((to + off_a + (w * MT + mt) * 2048) ^ (np << 5), pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3]));
       }
   };
-  if (!a.sums_only) write_state(base + L::OFF_S);
+  if (!SUMS) write_state(base + L::OFF_S);
   uint32_t stage = 0, sbuf = 0;          // bytes to the buffers at hand
   // o: rows 4 x + lane / 8 of this warp's 16, 16-byte piece lane & 7
   const int o_row = w * 16 + (lane >> 3), o_c = lane & 7;
@@ -449,8 +450,8 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
     cp_wait0();
     __syncthreads();
     if (at + C < end) fetch(base + (L::STAGE - stage), end - at - C);
-    const uint32_t qs = base + stage, ks_ = qs + L::TILE, vs = ks_ + L::TILE, ss = base + L::OFF_S + sbuf;
-    if (!a.sums_only) {
+    const uint32_t qs = base + stage, ks_ = qs + L::K, vs = ks_ + L::TILE, ss = base + L::OFF_S + sbuf;
+    if (!SUMS) {
       const uint32_t q_a = qs + w * 2048 + off_a;
       uint32_t qf[MT][4][4];
       float o[NT][4] = {};
@@ -597,11 +598,11 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
         }
     stage = L::STAGE - stage;
     sbuf = L::STATE - sbuf;
-    if (!a.sums_only && at + C < end) write_state(base + L::OFF_S + sbuf);
+    if (!SUMS && at + C < end) write_state(base + L::OFF_S + sbuf);
   }
-  const float f = a.sums_only ? 1.f : a.final_scale * (a.reverse ? power(ld, n == 0 && a.init ? 0 : 1) : 1.f);
-  float* to = a.sums_only ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.final && last ? a.final + b * a.s_b + h * a.s_h : nullptr;
-  const long long s_i = a.sums_only ? a.dv : a.s_i, s_j = a.sums_only ? 1 : a.s_j;
+  const float f = SUMS ? 1.f : a.final_scale * (a.reverse ? power(ld, n == 0 && a.init ? 0 : 1) : 1.f);
+  float* to = SUMS ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.final && last ? a.final + b * a.s_b + h * a.s_h : nullptr;
+  const long long s_i = SUMS ? a.dv : a.s_i, s_j = SUMS ? 1 : a.s_j;
   if (to) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -613,7 +614,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
           if (i < a.dk && j < cols) to[i * s_i + (col0 + j) * s_j] = f * s[mt][nt][e];
         }
   }
-  if (a.sums_only) return;
+  if (SUMS) return;
   const int dead0 = max(at0, n);                                                    // rows behind the last token are zero
   for (long long e = tid; e < (long long)(at1 - dead0) * cols; e += 128) {
     const long long to = b * a.o_sb + (dead0 + e / cols) * a.o_st + h * a.o_sh + col0 + e % cols;
@@ -749,13 +750,14 @@ static bool in_pieces(const void* p, long long sb, long long st, long long sh, i
 
 static long long elements(const Scans& p) { return (long long)p.s[0].batch * p.s[0].len * p.s[0].heads * (p.s[0].dk > p.s[0].dv ? p.s[0].dk : p.s[0].dv); }
 
-template <int DK, int PARTS, bool MANY> static int launch_mma(const char* name, const Scans& p, dim3 grid, cudaStream_t st) {
-  M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS, MANY>), MmaSmem<DK>::BYTES);
-  return m2_launch(name, elements(p), scan_mma_kernel<DK, PARTS, MANY>, grid, 128, MmaSmem<DK>::BYTES, st, p);
+template <int DK, int PARTS, bool MANY, bool SUMS> static int launch_mma(const char* name, const Scans& p, dim3 grid, cudaStream_t st) {
+  constexpr int bytes = MmaSmem<DK, SUMS>::BYTES;
+  M2_SMEM_ONCE((scan_mma_kernel<DK, PARTS, MANY, SUMS>), bytes);
+  return m2_launch(name, elements(p), scan_mma_kernel<DK, PARTS, MANY, SUMS>, grid, 128, bytes, st, p);
 }
-template <int DK> static int launch_mma_of(const char* name, const Scans& p, bool many, bool parts3, dim3 grid, cudaStream_t st) {
-  if (many) return parts3 ? launch_mma<DK, 3, true>(name, p, grid, st) : launch_mma<DK, 2, true>(name, p, grid, st);
-  return parts3 ? launch_mma<DK, 3, false>(name, p, grid, st) : launch_mma<DK, 2, false>(name, p, grid, st);
+template <int DK, int PARTS> static int launch_mma_of(const char* name, const Scans& p, bool many, bool sums, dim3 grid, cudaStream_t st) {
+  if (many) return sums ? launch_mma<DK, PARTS, true, true>(name, p, grid, st) : launch_mma<DK, PARTS, true, false>(name, p, grid, st);
+  return sums ? launch_mma<DK, PARTS, false, true>(name, p, grid, st) : launch_mma<DK, PARTS, false, false>(name, p, grid, st);
 }
 template <bool MANY> static int launch_f32(const char* name, const Scans& p, int dk, dim3 grid, cudaStream_t st) {
   const int dkp = (dk + 15) / 16 * 16;
@@ -801,8 +803,9 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
     for (int sums = n_seg > 1; sums >= 0; --sums) {
       for (int i = 0; i < n; ++i) p.s[i].sums_only = sums;
       const int rc = dtype != M2_BF16 ? (n > 1 ? launch_f32<true>(name, p, dk, grid, st) : launch_f32<false>(name, p, dk, grid, st))
-                     : large          ? launch_mma_of<128>(name, p, n > 1, parts3, grid, st)
-                                      : launch_mma_of<64>(name, p, n > 1, parts3, grid, st);
+                     : large  ? (parts3 ? launch_mma_of<128, 3>(name, p, n > 1, sums, grid, st) : launch_mma_of<128, 2>(name, p, n > 1, sums, grid, st))
+                     : parts3 ? launch_mma_of<64, 3>(name, p, n > 1, sums, grid, st)
+                              : launch_mma_of<64, 2>(name, p, n > 1, sums, grid, st);
       if (rc) return rc;
       if (sums) {
         if (int e = m2_launch(name, elements(p), join_segments, dim3((p.s[0].dk * p.s[0].dv + 255) / 256 * pairs, 1, n), 256, 0, st, p)) return e;
