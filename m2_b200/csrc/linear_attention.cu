@@ -174,7 +174,7 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
     __syncthreads();
     if (!a.sums_only) {
       float acc[4][4] = {};
-      #pragma unroll 8
+#pragma unroll 8
       for (int i = 0; i < dkp; ++i) mac(acc, f4(kt + i * LD + ty * 4), f4(qt + i * LD + tx * 4));
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -185,8 +185,10 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
       }
       __syncthreads();
       float o[4][4] = {};
-      #pragma unroll 8
-      for (int i = 0; i < dkp; ++i) mac(o, f4(qt + i * LD + ty * 4), f4(st + i * LD + tx * 4));
+      if (front.p || at > at0) {         // else the state is zero
+#pragma unroll 8
+        for (int i = 0; i < dkp; ++i) mac(o, f4(qt + i * LD + ty * 4), f4(st + i * LD + tx * 4));
+      }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float f = pw[ty * 4 + x + 1 - young];
@@ -210,8 +212,16 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
         for (int y = 0; y < 4; ++y)
           if (tx * 4 + y < cols) op[y] = a.scale * o[x][y];
       }
-      __syncthreads();                                                              // st is read by all
+      __syncthreads();                                                              // st and vs are read by all
     }
+    for (int e = tid; e < C * DVT / 4; e += 256) {                                  // v by its age, l^(m-1-j)
+      const int t = e / (DVT / 4), j = e % (DVT / 4) * 4;
+      float4* p = reinterpret_cast<float4*>(vs + t * LD + j);
+      const float f = pw[max(0, m - 1 - t)];
+      const float4 u = *p;
+      *p = make_float4(f * u.x, f * u.y, f * u.z, f * u.w);
+    }
+    __syncthreads();
     const float keep = power_m1(ld, m - young);
     for (int i0 = ty * 4; i0 < dkp; i0 += 64) {
       float s[4][4] = {};
@@ -221,10 +231,8 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
         for (int x = 0; x < 4; ++x) kk[x] = f4(kt + (i0 + x) * LD + j);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const float f = pw[max(0, m - 1 - j - y)];
-          const float4 vv = f4(vs + (j + y) * LD + tx * 4);
           auto of = [&](const float4& u) { return y == 0 ? u.x : y == 1 ? u.y : y == 2 ? u.z : u.w; };
-          mac(s, make_float4(f * of(kk[0]), f * of(kk[1]), f * of(kk[2]), f * of(kk[3])), vv);
+          mac(s, make_float4(of(kk[0]), of(kk[1]), of(kk[2]), of(kk[3])), f4(vs + (j + y) * LD + tx * 4));
         }
       }
 #pragma unroll
