@@ -151,3 +151,37 @@ def test_a_prompt_continued_token_by_token():
             got = ref.gather(-1, target[:, None])[:, 0]
             assert (out.logprob.double() - got).abs().max() <= 2.0 ** -14 * ref.abs().max()
             assert (out.top_logprob.double() - ref.topk(5, -1).values).abs().max() <= 2.0 ** -14 * ref.abs().max()
+
+
+def test_calls_on_several_streams_at_once():
+    """Nothing is shared between calls: the same bits on four streams side by side."""
+    q, k, v = (torch.randn(2, 900, 4, 64, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    x, y = torch.randn(64, 40, 768, device="cuda", requires_grad=True), torch.randn(64, 40, 768, device="cuda").bfloat16().requires_grad_()
+    gate, w = torch.randn(64, 1, 768, device="cuda", requires_grad=True), torch.randn(768, device="cuda", requires_grad=True)
+    logits, target = torch.randn(200, 30528, device="cuda").bfloat16().requires_grad_(), torch.randint(0, 30528, (200,), device="cuda")
+    ld = LD.cuda()
+    state = torch.randn(2, 4, 64, 64, device="cuda")
+
+    def run():
+        o, s = m2_b200.linear_attention(q, k, v, ld, return_state=True)
+        outs = [o, s, *torch.autograd.grad([o, s], [q, k, v], [torch.ones_like(o), torch.ones_like(s)])]
+        r, h = m2_b200.gated_residual_norm(x, y, gate=gate, after_weight=w, before_weight=w, eps=EPS)
+        outs += [r, h, *torch.autograd.grad([r, h], [x, y, gate, w], [torch.ones_like(r), torch.ones_like(h)])]
+        t = m2_b200.token_logprobs(logits, target, top=20)
+        outs += [*t, *torch.autograd.grad(t.logprob.sum() + t.entropy.sum(), [logits])]
+        own = state.clone()
+        with torch.no_grad():
+            outs += [m2_b200.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, own), own]
+        return [t.detach() for t in outs]
+
+    ref = run()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(run())
+        torch.cuda.synchronize()
+        for outs in got:
+            assert all(torch.equal(a, b) for a, b in zip(outs, ref))
