@@ -269,9 +269,10 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
 // the operand of P v.  Every warp needs the whole state as an operand: it goes through shared memory as bf16, into the other one of
 // two buffers, so that a chunk has a single block barrier and the warps of the SM's blocks drift apart and fill each other's waits.
 //
-// The state is a sum over thousands of tokens, so nothing of it is rounded to bf16: l^(C-1-j) k_j goes into its product as two or
-// (where the state is returned) three bf16 parts of 8 bits, and every chunk's sum starts from zero and is added in float32, as
-// tensor cores cut their sums instead of rounding them.
+// The state is a sum over thousands of tokens: l^(C-1-j) k_j goes into its product as three bf16 parts of 8 bits, all 24 of it, and
+// every chunk's sum starts from zero and is added in float32, as tensor cores cut their sums instead of rounding them.  A gradient's
+// state that goes nowhere but, rounded to bf16, into products has two parts, 16 bits.  Forward there are always three: o has the same
+// bits whether or not the state is asked for (two parts took 121 us where three take 137, 32 x 2048 tokens, 12 heads of 64).
 //
 // Bound: a token and head of 64 + 64 channels moves 512 bytes, 64 of them 0.74 us of an SM's share of 6.5 TB/s; the products take
 // 0.55 us (two parts) at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
@@ -776,7 +777,8 @@ template <bool MANY> static int launch_f32(const char* name, const Scans& p, int
 
 // `count` scans over the same (sequence, head) pairs: one launch for those whose keys have up to 64 channels and one for the others
 // (float32: one for all), each behind one of the segments' sums where the axis is cut.
-static int run_scans(const char* name, Scan* list, int count, int dtype, float* segments, cudaStream_t st) {
+// `whole`: weighted keys keep all their bits though no state is returned.
+static int run_scans(const char* name, Scan* list, int count, int dtype, float* segments, bool whole, cudaStream_t st) {
   int tiles = 0, n_seg, seg_chunks;
   bool small = dtype == M2_BF16;
   for (int i = 0; i < count; ++i) {
@@ -796,7 +798,7 @@ static int run_scans(const char* name, Scan* list, int count, int dtype, float* 
     Scans p = {};
     int n = 0, dk = 0;
     unsigned x = 0;
-    bool parts3 = false;
+    bool parts3 = whole;
     for (int i = 0; i < count; ++i) {
       if (dtype == M2_BF16 ? (list[i].dk > 64) != (large == 1) : large == 1) continue;
       p.s[n] = list[i];
@@ -883,7 +885,7 @@ extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, voi
   s.dk = g.dk; s.dv = g.dv; s.scale = g.scale;
   s.init = g.state_in; s.init_scale = 1.f; s.final = g.state_out; s.final_scale = 1.f;
   s.s_j = 1; s.s_i = g.dv; s.s_h = (long long)g.dk * g.dv; s.s_b = s.s_h * g.heads;
-  return run_scans("m2_linear_attention_fwd", &s, 1, g.dtype, g.workspace, (cudaStream_t)stream);
+  return run_scans("m2_linear_attention_fwd", &s, 1, g.dtype, g.workspace, true, (cudaStream_t)stream);
 }
 
 extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, const m2_linear_attention_grads* grads, void* stream) {
@@ -932,7 +934,7 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
   z.dk = g.dk; z.dv = g.dv; z.scale = g.scale;
   z.init = d.d_state_out; z.init_scale = 1.f / g.scale; z.final = d.d_state_in; z.final_scale = g.scale;
   z.s_b = s_b; z.s_h = s_h; z.s_i = g.dv; z.s_j = 1;
-  if (int rc = run_scans("m2_linear_attention_bwd", list, 3, g.dtype, segments, st)) return rc;
+  if (int rc = run_scans("m2_linear_attention_bwd", list, 3, g.dtype, segments, false, st)) return rc;
   if (group > 1 && tokens > 0) {
     for (int w = 0; w < 2; ++w) {
       const float* part = w ? part_v : part_k;
