@@ -430,19 +430,28 @@ backward_kernel(const BwdArgs a, int slices) {
   const int slice = (int)(blockIdx.x % slices);
   constexpr int per = THREADS * BWD_PIECES * N;
   const int lo = slice * per, hi = min(lo + per, a.vocab);
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
   T* dx = static_cast<T*>(a.dx) + row * a.ldd;
   const int tid = threadIdx.x;
   const long long target = a.target[row];
-  const bool used = target != a.ignore, good = used && target >= 0 && target < a.vocab;
+  if (target == a.ignore) {              // nothing is read: 8192 x 30528 bf16 with 85 % of the rows ignored 101 us, where reading them took 183
+    const Span<T> z(dx, lo, hi);
+    if (tid < z.head) st_from_float(dx + lo + tid, 0.f);
+    if (z.tail() + tid < hi) st_from_float(dx + z.tail() + tid, 0.f);
+    uint4* out = reinterpret_cast<uint4*>(dx + z.body());
+#pragma unroll 4
+    for (int i = tid; i < z.pieces; i += THREADS) out[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const bool good = target >= 0 && target < a.vocab;
   const float m = a.stats[2 * row], log_s = a.stats[2 * row + 1];
-  const float g_h = used && a.g_h ? a.g_h[row] : 0.f, h = a.entropy[row];
+  const float g_h = a.g_h ? a.g_h[row] : 0.f, h = a.entropy[row];
   const float g_lp = good && a.g_lp ? a.g_lp[row] : 0.f;
   float g = g_lp;
-  if (used && a.g_top) for (int i = 0; i < a.top; ++i) g += a.g_top[row * a.top + i];
+  if (a.g_top) for (int i = 0; i < a.top; ++i) g += a.g_top[row * a.top + i];
   auto grad = [&](float v) {
     const float l = (v - m) - log_s, p = ex2(l * LOG2E);
-    return used ? -p * fmaf(g_h, fmaxf(l, -1e4f) + h, g) : 0.f;
+    return -p * fmaf(g_h, fmaxf(l, -1e4f) + h, g);
   };
   const float c = -fmaf(g_h, h, g);      // -p (g_H (l + H) + g) as p (c - g_H l)
   auto grad2 = [&](float& v, float& w) {
@@ -463,10 +472,7 @@ backward_kernel(const BwdArgs a, int slices) {
     float f[N];
     Piece<T>::get(__ldg(body + i), f);
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      grad2(f[j], f[j + 1]);
-      if (!used) f[j] = f[j + 1] = 0.f;
-    }
+    for (int j = 0; j < N; j += 2) grad2(f[j], f[j + 1]);
     if (wide) {
       reinterpret_cast<uint4*>(out)[i] = Piece<T>::put(f);
     } else {
@@ -474,7 +480,6 @@ backward_kernel(const BwdArgs a, int slices) {
       for (int j = 0; j < N; ++j) st_from_float(out + i * N + j, f[j]);
     }
   }
-  if (!used) return;
   __syncthreads();
   // the ids that get a share of their own, written once more with everything in it
   if (tid <= a.top) {
