@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define M2_B200_ABI_VERSION 7
+#define M2_B200_ABI_VERSION 8
 
 typedef enum { M2_F32 = 0, M2_BF16 = 1, M2_F16 = 2 /* only where an entry point says so */ } m2_dtype;
 
@@ -439,7 +439,8 @@ int m2_encoder_fwd(const m2_encoder_args* args, void* stream);
  *   lengths   : NULL or int64 (batch): tokens of every sequence (clamped to 0 .. seq_len).  What lies behind them is not read,
  *               rows of o (and gradients) behind them are zero, and the state is that behind the last token.
  *   state_in  : NULL (zero) or float32 (batch, heads, dk, dv), packed; state_out: NULL or the same.  They may be the same memory.
- *   workspace : m2_linear_attention_workspace() bytes on a 16-byte boundary (0: NULL).
+ *   workspace : m2_linear_attention_workspace() bytes on a 16-byte boundary (0: NULL).  The size goes by the multiprocessors of the
+ *   current device: ask for it on the device that the call runs on.  workspace_bytes: its size; too small a one is refused.
  * A NaN or an infinity in a token's v reaches, besides the tokens after it, outputs of up to 63 tokens before it (their weight
  * for it is 0, and 0 times it is NaN).
  * bf16: float32 sums and state; the weights (q_i . k_j) decay^(i-j) and the state's copy that q meets are rounded to bf16, as
@@ -460,7 +461,7 @@ typedef struct {
   const float* state_in;
   void* o;
   float* state_out;
-  float* workspace;
+  float* workspace; long long workspace_bytes;
 } m2_linear_attention_args;
 
 typedef struct {
@@ -503,7 +504,8 @@ int m2_linear_attention_step(const m2_linear_attention_step_args* args, void* st
  * Statistics and everything up to the one rounding of each output are float32; h is of the unrounded r.
  * Gradients (m2_residual_norm_bwd): from d_r (x_dtype) and d_h (y_dtype), packed, NULL = zero; every output may be NULL.
  * d_gate has the gate's type and is packed; parameters' gradients are float32 sums in a fixed order.
- *   workspace: m2_residual_norm_workspace() bytes on a 16-byte boundary.
+ *   workspace: m2_residual_norm_workspace() bytes on a 16-byte boundary, asked for on the device that the call runs on, as its size
+ *   goes by the multiprocessors of the current device.  workspace_bytes: its size; too small a one is refused.
  * ------------------------------------------------------------------------------------- */
 typedef struct {
   long long rows, seq_len;  /* seq_len divides rows; read for gate_kind 2 alone */
@@ -524,7 +526,7 @@ typedef struct {
   const void *d_r, *d_h;
   void *d_x, *d_y, *d_gate;
   float *d_scale, *d_after_weight, *d_after_bias, *d_before_weight, *d_before_bias;
-  float* workspace;
+  float* workspace; long long workspace_bytes;
 } m2_residual_norm_grads;
 
 int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* stream);

@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm2b200.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 M2_F32, M2_BF16, M2_F16 = 0, 1, 2
 
@@ -158,7 +158,7 @@ class LinearAttentionArgs(C.Structure):
         ("k", C.c_void_p), ("k_sb", C.c_longlong), ("k_st", C.c_longlong), ("k_sh", C.c_longlong),
         ("v", C.c_void_p), ("v_sb", C.c_longlong), ("v_st", C.c_longlong), ("v_sh", C.c_longlong),
         ("log_decay", C.c_void_p), ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("o", C.c_void_p),
-        ("state_out", C.c_void_p), ("workspace", C.c_void_p),
+        ("state_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
     ]
 
 
@@ -197,7 +197,7 @@ class ResidualNormGrads(C.Structure):
     _fields_ = [
         ("d_r", C.c_void_p), ("d_h", C.c_void_p), ("d_x", C.c_void_p), ("d_y", C.c_void_p), ("d_gate", C.c_void_p),
         ("d_scale", C.c_void_p), ("d_after_weight", C.c_void_p), ("d_after_bias", C.c_void_p),
-        ("d_before_weight", C.c_void_p), ("d_before_bias", C.c_void_p), ("workspace", C.c_void_p),
+        ("d_before_weight", C.c_void_p), ("d_before_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
     ]
 
 

@@ -844,6 +844,15 @@ static int check_operands(const char* name, const m2_linear_attention_args& g) {
   return M2_OK;
 }
 
+// The plan of the launch is made for the current device, as the size is that was asked for: a plan for more multiprocessors than the
+// workspace was made for would write behind it.
+static int check_workspace(const char* name, const m2_linear_attention_args& g, int backward) {
+  const long long need = m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, backward);
+  M2_REQUIRE(need == 0 || (g.workspace && g.workspace_bytes >= need), M2_ERR_ARG, "%s: a workspace of %lld bytes, on this device the shape needs %lld", name,
+             g.workspace ? g.workspace_bytes : 0, need);
+  return M2_OK;
+}
+
 static Scan base_of(const m2_linear_attention_args& g) {
   Scan s = {};
   s.batch = g.batch; s.len = g.seq_len; s.heads = g.heads;
@@ -873,8 +882,7 @@ extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, voi
   if (g.batch == 0) return M2_OK;
   if (int rc = check_operands("m2_linear_attention_fwd", g)) return rc;
   M2_REQUIRE(g.o || g.seq_len == 0, M2_ERR_ARG, "m2_linear_attention_fwd: o is NULL");
-  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, 0) == 0, M2_ERR_ARG,
-             "m2_linear_attention_fwd: this shape needs a workspace");
+  if (int rc = check_workspace("m2_linear_attention_fwd", g, 0)) return rc;
   const int group = g.heads / g.kv_heads;
   const long long row = (long long)g.heads * g.dv;
   Scan s = base_of(g);
@@ -898,8 +906,7 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
   if (int rc = check_operands("m2_linear_attention_bwd", g)) return rc;
   M2_REQUIRE(g.seq_len == 0 || (d.d_o && d.d_q && d.d_k && d.d_v), M2_ERR_ARG, "m2_linear_attention_bwd: d_o, d_q, d_k or d_v is NULL");
   M2_REQUIRE(m2_aligned(d.d_o, g.dtype == M2_F32 ? 4 : 2), M2_ERR_ALIGN, "m2_linear_attention_bwd: d_o is not aligned to its type");
-  M2_REQUIRE(g.workspace || m2_linear_attention_workspace(g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, 1) == 0, M2_ERR_ARG,
-             "m2_linear_attention_bwd: this shape needs a workspace");
+  if (int rc = check_workspace("m2_linear_attention_bwd", g, 1)) return rc;
   const int group = g.heads / g.kv_heads;
   const cudaStream_t st = (cudaStream_t)stream;
   const long long tokens = (long long)g.batch * g.seq_len;

@@ -753,6 +753,8 @@ extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_
   M2_REQUIRE(g.stats && m2_aligned(g.stats, 16), M2_ERR_ARG, "m2_residual_norm_bwd: stats of the forward pass, on a 16-byte boundary, are needed");
   M2_REQUIRE(d.workspace && m2_aligned(d.workspace, 16), M2_ERR_ARG, "m2_residual_norm_bwd: a workspace on a 16-byte boundary is needed");
   a.stats = g.stats; a.dr = d.d_r; a.dh = a.norm2 ? d.d_h : nullptr; a.dx = d.d_x; a.dy = d.d_y; a.dg = d.d_gate;
+  const long long need = m2_residual_norm_workspace(g.rows, g.gate_kind == G_SEQUENCE ? g.seq_len : g.rows, g.n, g.gate_kind);
+  M2_REQUIRE(d.workspace_bytes >= need, M2_ERR_ARG, "m2_residual_norm_bwd: a workspace of %lld bytes, on this device the shape needs %lld", d.workspace_bytes, need);
   const Plan p = plan_of(a.rows, a.seq_len, a.n, true);
   a.splits = p.splits;
   a.sums = d.workspace;

@@ -62,10 +62,10 @@ def _args(q, k, v, log_decay, scale, initial, lengths, o=None, state=None):
 
 
 def _workspace(a, dev, backward):
-    n = _lib.lib().m2_linear_attention_workspace(a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv, a.dtype, backward)
+    n = ops._on_device(dev.index, _lib.lib().m2_linear_attention_workspace, a.batch, a.seq_len, a.heads, a.kv_heads, a.dk, a.dv, a.dtype, backward)
     w = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
     if w is not None:
-        a.workspace = w.data_ptr()
+        a.workspace, a.workspace_bytes = w.data_ptr(), n
     return w
 
 

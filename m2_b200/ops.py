@@ -52,6 +52,14 @@ def _launch(name, tensor, fn, *args, launches=1):
     LAUNCHES += launches
 
 
+def _on_device(index, fn, *args):
+    """fn(*args) with `index` as the current device: workspace sizes go by its multiprocessors, as the launch's plan does."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def _observed_launch(name, index, fn, args):
     st = torch.cuda.current_stream(index)
     prof = PROFILE

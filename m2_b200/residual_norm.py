@@ -82,8 +82,9 @@ class _ResidualNorm(torch.autograd.Function):
         out = [t.new_empty(t.shape) if w and t is not None else None for t, w in zip((x, y, gate, scale, *params), want)]
         if a.rows == 0:                                        # nothing to launch: sums over no rows
             return (*[t.zero_() if t is not None else None for t in out], None, None, None, None, None)
-        work = stats.new_empty(_lib.lib().m2_residual_norm_workspace(a.rows, seq_len, n, kind) // 4)
-        g = _lib.ResidualNormGrads(_ptr(d_r), _ptr(d_h), *(_ptr(t) for t in out), work.data_ptr())
+        size = ops._on_device(x.get_device(), _lib.lib().m2_residual_norm_workspace, a.rows, seq_len, n, kind)
+        work = stats.new_empty(size // 4)
+        g = _lib.ResidualNormGrads(_ptr(d_r), _ptr(d_h), *(_ptr(t) for t in out), work.data_ptr(), size)
         ops._launch("m2_residual_norm_bwd", x, _lib.lib().m2_residual_norm_bwd, C.byref(a), C.byref(g), launches=2)
         return (*out, None, None, None, None, None)
 
