@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define M2_B200_ABI_VERSION 8
+#define M2_B200_ABI_VERSION 9
 
 typedef enum { M2_F32 = 0, M2_BF16 = 1, M2_F16 = 2 /* only where an entry point says so */ } m2_dtype;
 
@@ -426,6 +426,10 @@ typedef struct {
 long long m2_encoder_workspace(int batch, int pitch, int d_model, int inter);
 long long m2_encoder_workspace_f32(int batch, int seq_len, int d_model, int inter, int nblocks);
 int m2_encoder_fwd(const m2_encoder_args* args, void* stream);
+
+/* Kernels that this thread's last call of an m2_linear_attention_*, m2_residual_norm_* or m2_token_logprobs_* entry point launched:
+ * their number goes by the shape (a long axis that is cut, shared heads, the sums of parameters' gradients). */
+int m2_last_launches(void);
 
 /* ---------------------------------------------------------------------------------------
  * Linear attention with a decay for each head: a causal sequence mixer whose state has a fixed size.

@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm2b200.so")
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 M2_F32, M2_BF16, M2_F16 = 0, 1, 2
 
@@ -222,6 +222,7 @@ class TokenLogprobsBwdArgs(C.Structure):
 # name -> (restype, argtypes); every symbol include/m2_b200.h declares
 SYMBOLS = {
     "m2_version": (C.c_int, []),
+    "m2_last_launches": (C.c_int, []),
     "m2_last_error": (C.c_char_p, []),
     "m2_device_status": (C.c_int, [C.POINTER(C.c_int)]),
     "m2_selftest_wait_timeout": (C.c_int, [C.c_ulonglong, C.c_void_p]),

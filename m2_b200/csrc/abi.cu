@@ -12,6 +12,11 @@ int m2_set_error(int code, const char* fmt, ...) {
   return code;
 }
 
+int& m2_launch_count() {
+  static thread_local int n = 0;
+  return n;
+}
+
 int m2_sm_count() {
   static std::atomic<int> cached[64];
   int dev = 0;
@@ -25,6 +30,8 @@ int m2_sm_count() {
 }
 
 extern "C" int m2_version(void) { return M2_B200_ABI_VERSION; }
+
+extern "C" int m2_last_launches(void) { return m2_launch_count(); }
 
 extern "C" const char* m2_last_error(void) { return g_err; }
 

@@ -24,6 +24,9 @@ int m2_set_error(int code, const char* fmt, ...);   // stores a thread-local mes
   do { cudaError_t e_ = cudaGetLastError(); \
        if (e_ != cudaSuccess) return m2_set_error(M2_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e_)); } while (0)
 
+// Kernels that this thread launched with m2_launch (or counted beside it); entry points that report their launches set it to 0.
+int& m2_launch_count();
+
 // Multiprocessors of the current device (asked for once per device).
 int m2_sm_count();
 
@@ -60,6 +63,7 @@ static int m2_launch(const char* name, long long elements, void (*kern)(KArgs...
   cfg.numAttrs = elements <= M2_OVERLAP_ELEMENTS ? 1 : 0;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
   if (e != cudaSuccess) return m2_set_error(M2_ERR_CUDA, "launch of %s failed: %s", name, cudaGetErrorString(e));
+  ++m2_launch_count();
   return M2_OK;
 }
 

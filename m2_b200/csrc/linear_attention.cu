@@ -876,6 +876,7 @@ extern "C" long long m2_linear_attention_workspace(int batch, int seq_len, int h
 
 extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, void* stream) {
   using namespace m2::la;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_linear_attention_fwd: args is NULL");
   const m2_linear_attention_args& g = *args;
   if (int rc = check("m2_linear_attention_fwd", g.batch, g.seq_len, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, g.scale)) return rc;
@@ -898,6 +899,7 @@ extern "C" int m2_linear_attention_fwd(const m2_linear_attention_args* args, voi
 
 extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, const m2_linear_attention_grads* grads, void* stream) {
   using namespace m2::la;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr && grads != nullptr, M2_ERR_ARG, "m2_linear_attention_bwd: args or grads is NULL");
   const m2_linear_attention_args& g = *args;
   const m2_linear_attention_grads& d = *grads;
@@ -951,6 +953,7 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
       const int grid = (int)(blocks < 16LL * m2_sm_count() ? blocks : 16LL * m2_sm_count());
       if (g.dtype == M2_F32) group_sum_kernel<float><<<grid, 256, 0, st>>>(part, static_cast<float*>(out), tokens, g.kv_heads, group, width);
       else group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(part, static_cast<__nv_bfloat16*>(out), tokens, g.kv_heads, group, width);
+      ++m2_launch_count();
     }
     M2_LAUNCH_CHECK("m2_linear_attention_bwd (shared heads)");
   }
@@ -959,6 +962,7 @@ extern "C" int m2_linear_attention_bwd(const m2_linear_attention_args* args, con
 
 extern "C" int m2_linear_attention_step(const m2_linear_attention_step_args* args, void* stream) {
   using namespace m2::la;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_linear_attention_step: args is NULL");
   const m2_linear_attention_step_args& g = *args;
   if (int rc = check("m2_linear_attention_step", g.batch, 1, g.heads, g.kv_heads, g.dk, g.dv, g.dtype, g.scale)) return rc;

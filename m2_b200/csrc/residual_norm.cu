@@ -720,6 +720,7 @@ static bool wide_rows(const m2_residual_norm_args& g) {
 
 extern "C" int m2_residual_norm_fwd(const m2_residual_norm_args* args, void* stream) {
   using namespace m2::rn;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_residual_norm_fwd: args is NULL");
   const m2_residual_norm_args& g = *args;
   Args a;
@@ -744,6 +745,7 @@ extern "C" long long m2_residual_norm_workspace(long long rows, long long seq_le
 
 extern "C" int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_residual_norm_grads* grads, void* stream) {
   using namespace m2::rn;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr && grads != nullptr, M2_ERR_ARG, "m2_residual_norm_bwd: args or grads is NULL");
   const m2_residual_norm_args& g = *args;
   const m2_residual_norm_grads& d = *grads;

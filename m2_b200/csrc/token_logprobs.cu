@@ -513,6 +513,7 @@ template <typename T> static int launch_forward(const Args& a, cudaStream_t st) 
   cfg.numAttrs = a.split > 1 ? 2 : 1;
   const cudaError_t e = a.top ? cudaLaunchKernelEx(&cfg, forward_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, forward_kernel<T, false>, a);
   if (e != cudaSuccess) return m2_set_error(M2_ERR_CUDA, "launch of m2_token_logprobs_fwd failed: %s", cudaGetErrorString(e));
+  ++m2_launch_count();
   return M2_OK;
 }
 
@@ -531,6 +532,7 @@ static int check(const char* name, const void* x, long long ld, const void* targ
 
 extern "C" int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* stream) {
   using namespace m2::lp;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_fwd: args is NULL");
   const m2_token_logprobs_args& g = *args;
   if (int rc = check("m2_token_logprobs_fwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
@@ -548,6 +550,7 @@ extern "C" int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* s
 
 extern "C" int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, void* stream) {
   using namespace m2::lp;
+  m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_bwd: args is NULL");
   const m2_token_logprobs_bwd_args& g = *args;
   if (int rc = check("m2_token_logprobs_bwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
@@ -566,5 +569,6 @@ extern "C" int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, voi
   if (g.dtype == M2_F32) backward_kernel<float><<<(unsigned)(g.rows * slices), THREADS, 0, st>>>(a, slices);
   else backward_kernel<__nv_bfloat16><<<(unsigned)(g.rows * slices), THREADS, 0, st>>>(a, slices);
   M2_LAUNCH_CHECK("m2_token_logprobs_bwd");
+  ++m2_launch_count();
   return M2_OK;
 }

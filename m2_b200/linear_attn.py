@@ -76,7 +76,7 @@ def _forward(q, k, v, log_decay, scale, initial, lengths, want_state):
     state = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device) if want_state else None
     a = _args(q, k, v, log_decay, scale, initial, lengths, o, state)
     work = _workspace(a, q.device, 0)  # noqa: F841  (alive until the launch)
-    ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a))
+    ops._launch("m2_linear_attention_fwd", q, _lib.lib().m2_linear_attention_fwd, C.byref(a), launches=None)
     return o, state
 
 
@@ -104,7 +104,7 @@ class _LinearAttention(torch.autograd.Function):
         g = _lib.LinearAttentionGrads(d_o.data_ptr(), *d_o.stride()[:3], d_state.data_ptr() if d_state is not None else None,
                                       dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), d_initial.data_ptr() if d_initial is not None else None)
         work = _workspace(a, q.device, 1)  # noqa: F841
-        ops._launch("m2_linear_attention_bwd", q, _lib.lib().m2_linear_attention_bwd, C.byref(a), C.byref(g))
+        ops._launch("m2_linear_attention_bwd", q, _lib.lib().m2_linear_attention_bwd, C.byref(a), C.byref(g), launches=None)
         return dq, dk_, dv_, None, None, d_initial, None, None
 
 
@@ -162,7 +162,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
     a = _lib.LinearAttentionStepArgs(
         B, H, K, dk, dv, _TYPES[q.dtype], scale, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
         ld.data_ptr(), state.data_ptr(), s_b, s_h, o.data_ptr())
-    ops._launch("m2_linear_attention_step", q, _lib.lib().m2_linear_attention_step, C.byref(a))
+    ops._launch("m2_linear_attention_step", q, _lib.lib().m2_linear_attention_step, C.byref(a), launches=None)
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)
     return o

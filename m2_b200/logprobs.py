@@ -46,7 +46,7 @@ def _forward(logits, targets, top, ignore_index, want_stats):
     stats = logprob.new_empty((n, 2)) if want_stats else None
     a = _lib.TokenLogprobsArgs(n, V, top, _TYPES[x.dtype], x.data_ptr(), ld, targets.data_ptr(), ignore_index, logprob.data_ptr(), entropy.data_ptr(),
                                stats.data_ptr() if want_stats else None, best.data_ptr(), ids.data_ptr())
-    ops._launch("m2_token_logprobs_fwd", x, _lib.lib().m2_token_logprobs_fwd, C.byref(a))
+    ops._launch("m2_token_logprobs_fwd", x, _lib.lib().m2_token_logprobs_fwd, C.byref(a), launches=None)
     return TokenLogprobs(logprob, entropy, best, ids), stats
 
 
@@ -71,7 +71,7 @@ class _TokenLogprobs(torch.autograd.Function):
         a = _lib.TokenLogprobsBwdArgs(targets.numel(), V, ids.shape[-1], _TYPES[x.dtype], x.data_ptr(), ld, targets.data_ptr(), ctx.ignore_index,
                                       stats.data_ptr(), entropy.data_ptr(), ids.data_ptr(), *(t.data_ptr() if t is not None else None for t in keep),
                                       d.data_ptr(), V)
-        ops._launch("m2_token_logprobs_bwd", x, _lib.lib().m2_token_logprobs_bwd, C.byref(a))
+        ops._launch("m2_token_logprobs_bwd", x, _lib.lib().m2_token_logprobs_bwd, C.byref(a), launches=None)
         return d, None, None, None
 
 

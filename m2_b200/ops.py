@@ -36,7 +36,8 @@ class LaunchProfile:
 
 
 def _launch(name, tensor, fn, *args, launches=1):
-    """Call one launching C-ABI entry point on torch's current stream of tensor's device."""
+    """Call one launching C-ABI entry point on torch's current stream of tensor's device.  launches: the kernels that it launches;
+    None: the library says how many they were."""
     global LAUNCHES
     index = tensor.get_device()
     if index != torch._C._cuda_getDevice():
@@ -49,7 +50,7 @@ def _launch(name, tensor, fn, *args, launches=1):
         rc = _observed_launch(name, index, fn, args)
     if rc:
         _lib.check(rc, name)
-    LAUNCHES += launches
+    LAUNCHES += launches if launches is not None else _lib.lib().m2_last_launches()
 
 
 def _on_device(index, fn, *args):

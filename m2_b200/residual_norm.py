@@ -48,7 +48,7 @@ def _forward(a, x, y, stats):
     r = x.new_empty(x.shape)
     h = y.new_empty(x.shape) if a.norm_before else None
     a.r, a.h, a.stats = r.data_ptr(), _ptr(h), _ptr(stats)
-    ops._launch("m2_residual_norm_fwd", x, _lib.lib().m2_residual_norm_fwd, C.byref(a))
+    ops._launch("m2_residual_norm_fwd", x, _lib.lib().m2_residual_norm_fwd, C.byref(a), launches=None)
     return r, h
 
 
@@ -85,7 +85,7 @@ class _ResidualNorm(torch.autograd.Function):
         size = ops._on_device(x.get_device(), _lib.lib().m2_residual_norm_workspace, a.rows, seq_len, n, kind)
         work = stats.new_empty(size // 4)
         g = _lib.ResidualNormGrads(_ptr(d_r), _ptr(d_h), *(_ptr(t) for t in out), work.data_ptr(), size)
-        ops._launch("m2_residual_norm_bwd", x, _lib.lib().m2_residual_norm_bwd, C.byref(a), C.byref(g), launches=2)
+        ops._launch("m2_residual_norm_bwd", x, _lib.lib().m2_residual_norm_bwd, C.byref(a), C.byref(g), launches=None)
         return (*out, None, None, None, None, None)
 
 

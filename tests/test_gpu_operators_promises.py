@@ -58,3 +58,48 @@ def test_gradient_of_ignored_rows_is_zero_up_to_its_ends(V, dtype):
         ref = -p[row] - p[row] * (p[row].log() + H)
         ref[t[row]] += 1
         assert (d[row].double() - ref).abs().max() <= torch.finfo(dtype).eps / 2 * ref.abs().max() + (V / 256 + 128) * 2.0 ** -24 * 40
+
+
+def launched(fn):
+    """What ops.LAUNCHES counts of a call, and the kernels of a graph that holds the call."""
+    from cuda.bindings import runtime
+    fn()
+    torch.cuda.synchronize()
+    graph, before = torch.cuda.CUDAGraph(keep_graph=True), ops.LAUNCHES
+    with torch.cuda.graph(graph):
+        fn()
+    counted = ops.LAUNCHES - before
+    count = runtime.cudaGraphGetNodes(graph.raw_cuda_graph(), 0)[2]
+    nodes = runtime.cudaGraphGetNodes(graph.raw_cuda_graph(), count)[1]
+    kind = runtime.cudaGraphNodeType.cudaGraphNodeTypeKernel
+    return counted, sum(runtime.cudaGraphNodeGetType(n)[1] == kind for n in nodes)
+
+
+def test_every_kernel_is_counted():
+    ld = torch.linspace(-0.1, -0.01, 4, device="cuda")
+    found = []
+    for L, K, dk, dv, dtype in ((64, 4, 64, 64, torch.bfloat16), (2000, 4, 64, 64, torch.bfloat16), (2000, 2, 64, 128, torch.bfloat16), (64, 2, 64, 128, torch.bfloat16),
+                                (2000, 2, 32, 32, torch.float32), (0, 4, 64, 64, torch.bfloat16)):
+        q, k, v = (torch.randn(1, L, h, d, device="cuda").to(dtype) for h, d in ((4, dk), (K, dk), (K, dv)))
+        found.append(launched(lambda: m2_b200.linear_attention(q, k, v, ld)))
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+
+        def gradients():                                    # one graph: the forward pass and, behind it, its gradients
+            o = m2_b200.linear_attention(q, k, v, ld)
+            torch.autograd.grad(o, [q, k, v], up)
+
+        up = torch.ones(1, L, 4, dv, dtype=dtype, device="cuda")
+        found.append(launched(gradients))
+    q, state = torch.randn(2, 4, 64, device="cuda"), torch.zeros(2, 4, 64, 64, device="cuda")
+    found.append(launched(lambda: m2_b200.linear_attention_step(q, q, q, ld, state)))
+    found.append(launched(lambda: m2_b200.linear_attention_step(q[:0], q[:0], q[:0], ld, state[:0])))
+    x, w = torch.randn(3, 50, 256, device="cuda", requires_grad=True), torch.ones(256, device="cuda", requires_grad=True)
+    gate, up = torch.ones(3, 1, 256, device="cuda", requires_grad=True), torch.ones(3, 50, 256, device="cuda")
+    for wanted in ([x], [x, w], [x, gate]):
+        fixed = [t if any(t is v for v in wanted) else t.detach() for t in (w, gate)]
+        found.append(launched(lambda: torch.autograd.grad(m2_b200.gated_residual_norm(x, x.detach(), gate=fixed[1], after_weight=fixed[0])[0], wanted, up)))
+    t, up = torch.zeros(3, 50, dtype=torch.long, device="cuda"), torch.ones(3, 50, device="cuda")
+    found.append(launched(lambda: m2_b200.token_logprobs(x.detach(), t, top=3)))
+    found.append(launched(lambda: torch.autograd.grad(m2_b200.token_logprobs(x, t)[0], [x], up)))
+    assert all(a == b for a, b in found), found
+    assert found[0] == (1, 1) and found[2] == (3, 3) and found[5][0] > 9, found
