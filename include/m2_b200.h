@@ -501,7 +501,8 @@ int m2_linear_attention_step(const m2_linear_attention_step_args* args, void* st
  * N: LayerNorm or (rms != 0) RMS norm over the n <= 8192 columns, each optional (norm_after, norm_before; without norm_after
  * N_after(y) = y, without norm_before there is no h).  m2_add_layernorm_fwd (bert/src/bert_layers.py:506) is the case of a
  * post-norm without gate, scale and norm of y.
- *   x (rows, n) and r of x_dtype: the residual stream; y (rows, n) and h of y_dtype; row strides ldx, ldy; r, h packed.
+ *   x (rows, n) and r of x_dtype: the residual stream; y (rows, n) and h of y_dtype; row strides ldx, ldy (rows that are read may
+ *   overlap: windows, or 0 for one row); r, h packed.
  *   gate_kind 0: none; 1: (n), a channel; 2: (rows / seq_len, n), a sequence of seq_len rows, row stride ldg; 3: (rows, n).
  *   scale_channel: float32 (n), or NULL: `scale` for all.  Weights and biases float32 (n) or NULL (1 and 0).
  *   stats : NULL, or (rows, 4) float32 on a 16-byte boundary, for the gradient.
@@ -540,7 +541,7 @@ int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_residual_no
 /* ---------------------------------------------------------------------------------------
  * Log probabilities of given tokens, entropy and the best alternatives of rows of logits: behind the decoder of the reference's
  * masked-LM head (bert/src/bert_layers.py, BertForMaskedLM: cross entropy over the masked positions).
- *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), row stride ld; targets int64 (rows).
+ *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), row stride ld (rows may overlap); targets int64 (rows).
  *   logprob, entropy float32 (rows); top_logprob float32 and top_id int64 (rows, top), best first, equal values by ascending
  *   id, NaN before all (top <= 32 and <= vocab).  stats NULL, or float32 (rows, 2): maximum and log of the sum, for the gradient.
  * A row whose target is ignore_index is not read: zeros, ids -1.  A target outside the vocabulary: logprob is NaN and

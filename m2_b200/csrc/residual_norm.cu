@@ -698,7 +698,7 @@ static int fill(const char* name, Args& a, const m2_residual_norm_args& g) {
   M2_REQUIRE(g.gate_kind >= 0 && g.gate_kind <= 3, M2_ERR_ARG, "%s: gate_kind %d", name, g.gate_kind);
   M2_REQUIRE(g.rows == 0 || (g.x && g.y && (g.gate_kind == 0 || g.gate)), M2_ERR_ARG, "%s: x, y or the gate is NULL", name);
   M2_REQUIRE(g.eps >= 0.f, M2_ERR_ARG, "%s: eps %g", name, g.eps);
-  M2_REQUIRE((g.ldx >= g.n || g.ldx == 0 || g.rows <= 1) && (g.ldy >= g.n || g.ldy == 0 || g.rows <= 1), M2_ERR_ARG, "%s: a row stride is smaller than a row", name);
+  M2_REQUIRE(g.rows <= 1 || (g.ldx >= 0 && g.ldy >= 0 && (g.gate_kind < G_SEQUENCE || g.ldg >= 0)), M2_ERR_ARG, "%s: a row stride is negative", name);
   a = Args{};
   a.x = g.x; a.y = g.y; a.g = g.gate; a.ldx = g.ldx; a.ldy = g.ldy; a.ldg = g.ldg;
   a.rows = g.rows;

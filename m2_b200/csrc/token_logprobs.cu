@@ -518,7 +518,7 @@ template <typename T> static int launch_forward(const Args& a, cudaStream_t st) 
 }
 
 static int check(const char* name, const void* x, long long ld, const void* target, long long n, int vocab, int top, int dtype) {
-  M2_REQUIRE(n >= 0 && vocab >= 1 && (ld >= vocab || ld == 0 || n <= 1), M2_ERR_ARG, "%s: %lld rows of %d logits, %lld apart", name, n, vocab, ld);
+  M2_REQUIRE(n >= 0 && vocab >= 1 && (ld >= 0 || n <= 1), M2_ERR_ARG, "%s: %lld rows of %d logits, %lld apart", name, n, vocab, ld);
   M2_REQUIRE(top >= 0 && top <= MAX_TOP && top <= vocab, M2_ERR_ARG, "%s: %d alternatives (0 .. %d, at most the %d logits)", name, top, MAX_TOP, vocab);
   M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: logits are float32 or bf16", name);
   M2_REQUIRE(vocab <= 1 << 28 && n <= 1 << 27, M2_ERR_UNSUPPORTED, "%s: %lld rows of %d logits are more than the grid takes", name, n, vocab);

@@ -103,3 +103,26 @@ def test_every_kernel_is_counted():
     found.append(launched(lambda: torch.autograd.grad(m2_b200.token_logprobs(x, t)[0], [x], up)))
     assert all(a == b for a, b in found), found
     assert found[0] == (1, 1) and found[2] == (3, 3) and found[5][0] > 9, found
+
+
+@pytest.mark.parametrize("step", [8, 1])
+def test_rows_may_overlap(step):
+    """Windows of one tensor, read in place: a row's neighbour begins before it ends."""
+    base = torch.randn(2000, device="cuda")
+    rows, w = base.unfold(0, 768, step), torch.randn(768, device="cuda")
+    apart = rows.contiguous()
+    t = torch.arange(len(rows), device="cuda") % 768
+    got, ref = (m2_b200.token_logprobs(x, t, top=3) for x in (rows, apart))
+    assert torch.equal(got.top_id, ref.top_id)
+    for a, b in zip(got[:3], ref[:3]):                      # where a row begins decides which thread adds which values
+        assert torch.equal(a, b) if step == 8 else (a - b).abs().max() <= (768 / 256 + 64) * 2.0 ** -24 + 16 * 2.0 ** -24 * (b.abs().max() + 40)
+    for gate, after in ((None, w), (rows, w), (rows, None)):
+        got = m2_b200.gated_residual_norm(rows, rows, gate=gate, after_weight=after, before_weight=w, eps=1e-5)
+        ref = m2_b200.gated_residual_norm(apart, apart, gate=gate if gate is None else apart, after_weight=after, before_weight=w, eps=1e-5)
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b) if step == 8 else ((a - b).abs() <= 256 * 2.0 ** -24 * b.abs().amax(-1, keepdim=True)).all()
+    x = base.clone().requires_grad_()                       # the gradient of a value is the sum over the rows that hold it
+    (d,) = torch.autograd.grad(m2_b200.token_logprobs(x.unfold(0, 768, step), t).logprob.sum(), [x])
+    y = base.double().requires_grad_()
+    (e,) = torch.autograd.grad(torch.log_softmax(y.unfold(0, 768, step), -1).gather(-1, t[:, None]).sum(), [y])
+    assert (d.double() - e).abs().max() <= (768 / 256 + 128 + len(rows)) * 2.0 ** -24 * len(rows)
