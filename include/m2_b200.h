@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define M2_B200_ABI_VERSION 9
+#define M2_B200_ABI_VERSION 10
 
 typedef enum { M2_F32 = 0, M2_BF16 = 1, M2_F16 = 2 /* only where an entry point says so */ } m2_dtype;
 
@@ -541,7 +541,9 @@ int m2_residual_norm_bwd(const m2_residual_norm_args* args, const m2_residual_no
 /* ---------------------------------------------------------------------------------------
  * Log probabilities of given tokens, entropy and the best alternatives of rows of logits: behind the decoder of the reference's
  * masked-LM head (bert/src/bert_layers.py, BertForMaskedLM: cross entropy over the masked positions).
- *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), row stride ld (rows may overlap); targets int64 (rows).
+ *   logits (rows, vocab) of `dtype` (M2_F32 or M2_BF16), rows ld apart (they may overlap), or, where group > 0, groups of `group` rows
+ *   ld_group apart: row r begins at (r / group) ld_group + (r % group) ld (the texts of a batch without their last rows, say).
+ *   targets int64 (rows).
  *   logprob, entropy float32 (rows); top_logprob float32 and top_id int64 (rows, top), best first, equal values by ascending
  *   id, NaN before all (top <= 32 and <= vocab).  stats NULL, or float32 (rows, 2): maximum and log of the sum, for the gradient.
  * A row whose target is ignore_index is not read: zeros, ids -1.  A target outside the vocabulary: logprob is NaN and
@@ -557,6 +559,7 @@ typedef struct {
   const void* targets; long long ignore_index;
   float *logprob, *entropy, *stats, *top_logprob;
   void* top_id;
+  long long group, ld_group;
 } m2_token_logprobs_args;
 
 typedef struct {
@@ -568,6 +571,7 @@ typedef struct {
   const void* top_id;
   const float *d_logprob, *d_entropy, *d_top_logprob;
   void* d_logits; long long ldd;
+  long long group, ld_group;   /* of logits */
 } m2_token_logprobs_bwd_args;
 
 int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* stream);

@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm2b200.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 M2_F32, M2_BF16, M2_F16 = 0, 1, 2
 
@@ -206,6 +206,7 @@ class TokenLogprobsArgs(C.Structure):
         ("rows", C.c_longlong), ("vocab", C.c_int), ("top", C.c_int), ("dtype", C.c_int),
         ("logits", C.c_void_p), ("ld", C.c_longlong), ("targets", C.c_void_p), ("ignore_index", C.c_longlong),
         ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p), ("top_logprob", C.c_void_p), ("top_id", C.c_void_p),
+        ("group", C.c_longlong), ("ld_group", C.c_longlong),
     ]
 
 
@@ -215,7 +216,7 @@ class TokenLogprobsBwdArgs(C.Structure):
         ("logits", C.c_void_p), ("ld", C.c_longlong), ("targets", C.c_void_p), ("ignore_index", C.c_longlong),
         ("stats", C.c_void_p), ("entropy", C.c_void_p), ("top_id", C.c_void_p),
         ("d_logprob", C.c_void_p), ("d_entropy", C.c_void_p), ("d_top_logprob", C.c_void_p),
-        ("d_logits", C.c_void_p), ("ldd", C.c_longlong),
+        ("d_logits", C.c_void_p), ("ldd", C.c_longlong), ("group", C.c_longlong), ("ld_group", C.c_longlong),
     ]
 
 

@@ -30,8 +30,21 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr float LOWEST = -3.402823466e38f;
 constexpr int ST_BAD_TARGET = 16;        // M2_DEV_BAD_INDEX
 
+// Rows ld apart, or groups of them (texts of a batch whose last rows are left out, say): up to 2^27 rows, so that 32 bits divide them
+struct Rows {
+  const void* p; long long ld, ld_group; unsigned group;
+  template <typename T> __device__ __forceinline__ const T* at(long long row) const {
+    long long to = row * ld;
+    if (group) {
+      const unsigned g = (unsigned)row / group;
+      to = g * ld_group + ((unsigned)row - g * group) * ld;
+    }
+    return static_cast<const T*>(p) + to;
+  }
+};
+
 struct Args {
-  const void* x; long long ld;
+  Rows x;
   const long long* target;
   long long n; int vocab, top, split;
   long long ignore;
@@ -40,7 +53,7 @@ struct Args {
 };
 
 struct BwdArgs {
-  const void* x; long long ld;
+  Rows x;
   const long long* target;
   long long n; int vocab, top;
   long long ignore;
@@ -321,7 +334,7 @@ forward_kernel(const Args a) {
   pdl_wait();
   const long long row = blockIdx.x / split;
   const uint32_t part = split > 1 ? cta_rank() : 0;
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const T* x = a.x.at<T>(row);
   const long long target = a.target[row];
   if (target == a.ignore) {                                                // the whole cluster leaves
     if (part == 0) {
@@ -442,7 +455,7 @@ backward_kernel(const BwdArgs a, int slices) {
     for (int i = tid; i < z.pieces; i += THREADS) out[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  const T* x = a.x.at<T>(row);
   const bool good = target >= 0 && target < a.vocab;
   const float m = a.stats[2 * row], log_s = a.stats[2 * row + 1];
   const float g_h = a.g_h ? a.g_h[row] : 0.f, h = a.entropy[row];
@@ -517,7 +530,8 @@ template <typename T> static int launch_forward(const Args& a, cudaStream_t st) 
   return M2_OK;
 }
 
-static int check(const char* name, const void* x, long long ld, const void* target, long long n, int vocab, int top, int dtype) {
+static int check(const char* name, const void* x, long long ld, long long group, long long ld_group, const void* target, long long n, int vocab, int top, int dtype) {
+  M2_REQUIRE(group >= 0 && group <= 1 << 27 && ld_group >= 0, M2_ERR_ARG, "%s: groups of %lld rows, %lld apart", name, group, ld_group);
   M2_REQUIRE(n >= 0 && vocab >= 1 && (ld >= 0 || n <= 1), M2_ERR_ARG, "%s: %lld rows of %d logits, %lld apart", name, n, vocab, ld);
   M2_REQUIRE(top >= 0 && top <= MAX_TOP && top <= vocab, M2_ERR_ARG, "%s: %d alternatives (0 .. %d, at most the %d logits)", name, top, MAX_TOP, vocab);
   M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: logits are float32 or bf16", name);
@@ -535,11 +549,11 @@ extern "C" int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* s
   m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_fwd: args is NULL");
   const m2_token_logprobs_args& g = *args;
-  if (int rc = check("m2_token_logprobs_fwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
+  if (int rc = check("m2_token_logprobs_fwd", g.logits, g.ld, g.group, g.ld_group, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
   if (g.rows == 0) return M2_OK;
   M2_REQUIRE(g.logprob && g.entropy && (g.top == 0 || (g.top_logprob && g.top_id)), M2_ERR_ARG, "m2_token_logprobs_fwd: an output is NULL");
   Args a;
-  a.x = g.logits; a.ld = g.ld; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
+  a.x = {g.logits, g.ld, g.ld_group, (unsigned)g.group}; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
   a.logprob = g.logprob; a.entropy = g.entropy; a.stats = g.stats; a.top_lp = g.top_logprob; a.top_id = (long long*)g.top_id;
   // a row is shared by the blocks of a cluster where the rows alone do not fill the GPU, each block with 4096 logits at least
   a.split = 1;
@@ -553,13 +567,13 @@ extern "C" int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, voi
   m2_launch_count() = 0;
   M2_REQUIRE(args != nullptr, M2_ERR_ARG, "m2_token_logprobs_bwd: args is NULL");
   const m2_token_logprobs_bwd_args& g = *args;
-  if (int rc = check("m2_token_logprobs_bwd", g.logits, g.ld, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
+  if (int rc = check("m2_token_logprobs_bwd", g.logits, g.ld, g.group, g.ld_group, g.targets, g.rows, g.vocab, g.top, g.dtype)) return rc;
   if (g.rows == 0) return M2_OK;
   M2_REQUIRE(g.stats && g.entropy && g.d_logits && (g.top == 0 || g.top_id), M2_ERR_ARG, "m2_token_logprobs_bwd: a result of the forward pass or d_logits is NULL");
   M2_REQUIRE((g.ldd >= g.vocab || g.rows == 1) && m2_aligned(g.d_logits, g.dtype == M2_F32 ? 4 : 2), M2_ERR_ARG,
              "m2_token_logprobs_bwd: rows of d_logits overlap or are not aligned to their type");
   BwdArgs a;
-  a.x = g.logits; a.ld = g.ld; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
+  a.x = {g.logits, g.ld, g.ld_group, (unsigned)g.group}; a.target = (const long long*)g.targets; a.n = g.rows; a.vocab = g.vocab; a.top = g.top; a.ignore = g.ignore_index;
   a.stats = g.stats; a.entropy = g.entropy; a.top_id = (const long long*)g.top_id; a.g_lp = g.d_logprob; a.g_h = g.d_entropy;
   a.g_top = g.top ? g.d_top_logprob : nullptr; a.dx = g.d_logits; a.ldd = g.ldd;
   const int per = THREADS * BWD_PIECES * (g.dtype == M2_F32 ? 4 : 8);

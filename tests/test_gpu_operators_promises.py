@@ -1,4 +1,6 @@
 """What the documentation of linear_attention, gated_residual_norm and token_logprobs says beside their formulas."""
+import gc
+
 import pytest
 import torch
 
@@ -126,3 +128,61 @@ def test_rows_may_overlap(step):
     y = base.double().requires_grad_()
     (e,) = torch.autograd.grad(torch.log_softmax(y.unfold(0, 768, step), -1).gather(-1, t[:, None]).sum(), [y])
     assert (d.double() - e).abs().max() <= (768 / 256 + 128 + len(rows)) * 2.0 ** -24 * len(rows)
+
+
+def peak(fn):
+    """Bytes that fn() holds beyond what was held before, at most, and what it returns."""
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = fn()
+    return torch.cuda.max_memory_allocated() - before, out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_of_a_batch_are_read_in_place(dtype):
+    V = 4096
+    x = torch.randn(5, 33, V, device="cuda").to(dtype)
+    t = torch.randint(0, V, (5, 32), device="cuda")
+    t[2, 3:] = -100
+    swapped = torch.randn(32, 5, V, device="cuda").to(dtype).transpose(0, 1)
+    layouts = [x[:, :-1], x[:, 1:], swapped, x[:1, :-1].expand(5, 32, V), x.as_strided((5, 32, V), (V, 8, 1)), x[:, None, :-1].expand(5, 1, 32, V),
+               x[:, None, :-1, :V // 2 * 2]]
+    for y in layouts:
+        u = t.view(y.shape[:-1])
+        apart = y.contiguous()
+        used, got = peak(lambda: m2_b200.token_logprobs(y, u, top=4))
+        ref = m2_b200.token_logprobs(apart, u, top=4)
+        assert used < apart.numel() * apart.element_size() / 4
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+        y, apart = y.detach().requires_grad_(), apart.requires_grad_()
+        ups = [torch.randn_like(a) for a in ref[:3]]
+        outs = m2_b200.token_logprobs(y, u, top=4)
+        used, (d,) = peak(lambda: torch.autograd.grad(outs[:3], [y], ups))
+        (e,) = torch.autograd.grad(m2_b200.token_logprobs(apart, u, top=4)[:3], [apart], ups)
+        assert torch.equal(d, e) and used < 1.25 * apart.numel() * apart.element_size()
+
+
+def test_logits_that_have_to_be_copied_are_copied_once():
+    x = torch.randn(3, 2, 8, 2, 2048, device="cuda").transpose(1, 3).requires_grad_()      # (3, 2, 8, 2, V): no two strides
+    t = torch.randint(0, 2048, x.shape[:-1], device="cuda")
+    out, ref = m2_b200.token_logprobs(x, t, top=2), m2_b200.token_logprobs(x.detach().contiguous(), t, top=2)
+    assert all(torch.equal(a, b) for a, b in zip(out, ref))
+    used, (d,) = peak(lambda: torch.autograd.grad(out.logprob, [x], torch.ones_like(out.logprob)))
+    assert used < 1.5 * x.numel() * 4
+    apart = x.detach().contiguous().requires_grad_()
+    (e,) = torch.autograd.grad(m2_b200.token_logprobs(apart, t).logprob, [apart], torch.ones_like(out.logprob))
+    assert torch.equal(d, e)
+    columns = torch.randn(2048, 6, device="cuda").t()
+    assert torch.equal(m2_b200.token_logprobs(columns, t[0, 0, :6, 0]).logprob, m2_b200.token_logprobs(columns.contiguous(), t[0, 0, :6, 0]).logprob)
+
+
+def test_groups_of_rows_far_apart():
+    far = 2 ** 31 + 64
+    big = torch.empty(far + 3 * 512, dtype=torch.bfloat16, device="cuda")
+    y = big.as_strided((2, 3, 512), (far, 512, 1))
+    near = torch.randn(2, 3, 512, device="cuda").bfloat16()
+    y.copy_(near)
+    t = torch.randint(0, 512, (2, 3), device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(m2_b200.token_logprobs(y, t, top=2), m2_b200.token_logprobs(near, t, top=2)))

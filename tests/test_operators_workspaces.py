@@ -1,4 +1,4 @@
-"""Workspaces of linear_attention and gated_residual_norm, on the host: no GPU is touched."""
+"""Workspaces of linear_attention and gated_residual_norm, and rows of token_logprobs, on the host: no GPU is touched."""
 import ctypes as C
 
 import torch
@@ -65,3 +65,10 @@ def test_the_size_is_asked_for_on_the_tensors_device(monkeypatch):
         assert w.numel() == 100 + index and a.workspace == w.data_ptr() and a.workspace_bytes == 4 * (100 + index)
     assert asked == [0, 1] and now == [0]
     assert ops._on_device(1, lambda x: (x, now[0]), 5) == (5, 1)
+
+
+def test_groups_of_rows_that_make_no_sense_are_refused():
+    for group, ld_group in ((-1, 8), (1, -8), (1 << 28, 8)):
+        t = _lib.TokenLogprobsArgs(rows=2, vocab=8, ld=8, group=group, ld_group=ld_group, logits=SOMEWHERE, targets=SOMEWHERE)
+        rc, msg = refused(_lib.lib().m2_token_logprobs_fwd, t)
+        assert rc == 1 and "groups" in msg
