@@ -21,12 +21,25 @@ _TYPES = {torch.float32: _lib.M2_F32, torch.bfloat16: _lib.M2_BF16}
 
 
 def _rows(t, n):
-    """t, or a copy, whose rows of n contiguous columns lie a fixed distance apart, and that distance."""
+    """The rows of t, which _evenly() gave, and the distance between them."""
     if t.is_contiguous():
         return t, n
-    t = t.reshape(-1, n)
-    t = t if t.stride(1) == 1 or n == 1 else t.contiguous()
+    t = t.view(-1, n)
     return t, t.stride(0)
+
+
+def _evenly(t):
+    """t, or a copy: rows of adjacent columns a fixed distance apart.  Made before the gradient's function takes it, so that there is one copy."""
+    if t.is_contiguous():
+        return t
+    n = t.shape[-1]
+    if t.stride(-1) == 1 or n == 1:
+        try:
+            t.view(-1, n)
+            return t
+        except RuntimeError:
+            pass
+    return t.contiguous()
 
 
 def _ptr(t):
@@ -101,7 +114,8 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=Non
                         eps=1e-12, rms=False):
     """(r, h) with r = residual_scale * x + gate * N_after(y) and h = N_before(r), in one launch.
 
-    x, y            (..., D), float32 or bfloat16 each, D <= 8192; r has x's type, h has y's
+    x, y            (..., D), float32 or bfloat16 each, D <= 8192; r has x's type, h has y's.  Rows a fixed distance apart are
+                    read in place, others (x[:, :-1] of a batch) are copied first
     gate            None, (D,), (B, 1, D) for x (B, L, D), or x's shape; float32 or bfloat16
     residual_scale  a number or a tensor (D,)
     after_weight, after_bias    of N_after, (D,); without a weight N_after(y) = y
@@ -134,6 +148,9 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=Non
             kind, seq_len = _SEQUENCE, max(x.shape[1], 1)
         else:
             raise ValueError(f"{name}: a gate is ({n},), (B, 1, {n}) or {tuple(x.shape)}, got {tuple(gate.shape)}")
+    x, y = _evenly(x), _evenly(y)
+    if kind > _CHANNEL:
+        gate = _evenly(gate)
     tensors = [x, y, gate, residual_scale if isinstance(residual_scale, torch.Tensor) else None, after_weight, after_bias, before_weight, before_bias]
     for i in range(3, 8):
         if tensors[i] is not None:

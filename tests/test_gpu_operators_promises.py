@@ -186,3 +186,20 @@ def test_groups_of_rows_far_apart():
     y.copy_(near)
     t = torch.randint(0, 512, (2, 3), device="cuda")
     assert all(torch.equal(a, b) for a, b in zip(m2_b200.token_logprobs(y, t, top=2), m2_b200.token_logprobs(near, t, top=2)))
+
+
+def test_rows_of_norms_that_have_to_be_copied_are_copied_once():
+    x, y, gate = (torch.randn(8, 513, 1024, device="cuda")[:, :-1].requires_grad_() for _ in range(3))
+    w, size = torch.randn(1024, device="cuda"), 8 * 512 * 1024 * 4
+    up = [torch.randn(8, 512, 1024, device="cuda") for _ in range(2)]
+    outs = m2_b200.gated_residual_norm(x, y, gate=gate, after_weight=w, before_weight=w, eps=1e-5)
+    used, grads = peak(lambda: torch.autograd.grad(outs, [x, y, gate], up))
+    assert used < 4.5 * size                                # three gradients and the blocks' column sums; three copies more are 6.5
+    apart = [t.detach().contiguous().requires_grad_() for t in (x, y, gate)]
+    refs = m2_b200.gated_residual_norm(apart[0], apart[1], gate=apart[2], after_weight=w, before_weight=w, eps=1e-5)
+    assert all(torch.equal(a, b) for a, b in zip(outs, refs))
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(refs, apart, up)))
+    # broadcast over the batch: copied, and the gradient summed
+    row = torch.randn(1, 512, 1024, device="cuda", requires_grad=True)
+    (d,) = torch.autograd.grad(m2_b200.gated_residual_norm(row.expand(8, 512, 1024), apart[1].detach(), residual_scale=2.0)[0], [row], up[0])
+    assert (d - 2 * up[0].sum(0, keepdim=True)).abs().max() <= 8 * 2.0 ** -24 * 2 * up[0].abs().sum(0).max()
