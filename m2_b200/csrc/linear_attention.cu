@@ -733,11 +733,17 @@ step_kernel(const m2_linear_attention_step_args a) {
 // Segments: where the blocks of all (sequence, head) pairs and 64-column tiles do not fill the GPU, a long axis is cut; every
 // segment's own sum is made first (reading k and v once more) and the segments then run side by side.
 // A cut costs half as much again, so there is one only where all blocks still run at once: an SM holds three of them, two with
-// 128 channels or float32.
-static void segments_of(int batch, int heads, int tiles, int len, bool small, int* n_seg, int* seg_chunks) {
+// more than 64 channels, and of float32 two with up to 96 channels and one with more (cut for two of those: 4096 float32 tokens of 4 heads
+// of 128 150 us, gradients 400; for one 144 and 368).
+static size_t f32_smem(int dk) { return ((size_t)(3 * ((dk + 15) / 16 * 16) + 2 * C) * LD + C + 4) * sizeof(float); }
+static int blocks_an_sm(int dtype, int dk) {             // dk: of the launch's widest keys
+  if (dtype == M2_BF16) return dk <= 64 ? 3 : 2;
+  return 2 * (f32_smem(dk) + 1024) <= 228 * 1024 ? 2 : 1;       // a block's own 1 KB beside; registers admit two
+}
+static void segments_of(int batch, int heads, int tiles, int len, int an_sm, int* n_seg, int* seg_chunks) {
   const long long blocks = (long long)batch * heads * tiles;
   const int chunks = (len + C - 1) / C;
-  long long seg = (small ? 3LL : 2LL) * m2_sm_count() / blocks;
+  long long seg = (long long)an_sm * m2_sm_count() / blocks;
   if (seg > chunks / 2) seg = chunks / 2;               // two chunks at least
   if (seg < 1) seg = 1;
   *seg_chunks = chunks ? (int)((chunks + seg - 1) / seg) : 1;
@@ -747,7 +753,7 @@ static int tiles_of(int dv) { return (dv + DVT - 1) / DVT; }
 // of `scans` scans side by side, each with a state of dk x dv or dv x dk
 static long long segment_floats(int batch, int heads, int dk, int dv, int tiles, int scans, int len, int dtype) {
   int n, c;
-  segments_of(batch, heads, tiles, len, dtype == M2_BF16 && dk <= 64 && (scans == 1 || dv <= 64), &n, &c);
+  segments_of(batch, heads, tiles, len, blocks_an_sm(dtype, scans == 1 || dk > dv ? dk : dv), &n, &c);
   return n > 1 ? (long long)scans * batch * heads * n * dk * dv : 0;
 }
 
@@ -769,23 +775,20 @@ template <int DK, int PARTS> static int launch_mma_of(const char* name, const Sc
   return sums ? launch_mma<DK, PARTS, false, true>(name, p, grid, st) : launch_mma<DK, PARTS, false, false>(name, p, grid, st);
 }
 template <bool MANY> static int launch_f32(const char* name, const Scans& p, int dk, dim3 grid, cudaStream_t st) {
-  const int dkp = (dk + 15) / 16 * 16;
-  constexpr size_t most = ((size_t)(3 * MAX_D + 2 * C) * LD + C + 4) * sizeof(float);
-  M2_SMEM_ONCE(scan_f32_kernel<MANY>, most);
-  return m2_launch(name, elements(p), scan_f32_kernel<MANY>, grid, 256, ((size_t)(3 * dkp + 2 * C) * LD + C + 4) * sizeof(float), st, p);
+  M2_SMEM_ONCE(scan_f32_kernel<MANY>, f32_smem(MAX_D));
+  return m2_launch(name, elements(p), scan_f32_kernel<MANY>, grid, 256, f32_smem(dk), st, p);
 }
 
 // `count` scans over the same (sequence, head) pairs: one launch for those whose keys have up to 64 channels and one for the others
 // (float32: one for all), each behind one of the segments' sums where the axis is cut.
 // `whole`: weighted keys keep all their bits though no state is returned.
 static int run_scans(const char* name, Scan* list, int count, int dtype, float* segments, bool whole, cudaStream_t st) {
-  int tiles = 0, n_seg, seg_chunks;
-  bool small = dtype == M2_BF16;
+  int tiles = 0, widest = 0, n_seg, seg_chunks;
   for (int i = 0; i < count; ++i) {
     tiles += tiles_of(list[i].dv);
-    small = small && list[i].dk <= 64;
+    widest = list[i].dk > widest ? list[i].dk : widest;
   }
-  segments_of(list[0].batch, list[0].heads, tiles, list[0].len, small, &n_seg, &seg_chunks);
+  segments_of(list[0].batch, list[0].heads, tiles, list[0].len, blocks_an_sm(dtype, widest), &n_seg, &seg_chunks);
   for (int i = 0; i < count; ++i) {
     Scan& a = list[i];
     a.n_seg = n_seg;

@@ -72,3 +72,17 @@ def test_groups_of_rows_that_make_no_sense_are_refused():
         t = _lib.TokenLogprobsArgs(rows=2, vocab=8, ld=8, group=group, ld_group=ld_group, logits=SOMEWHERE, targets=SOMEWHERE)
         rc, msg = refused(_lib.lib().m2_token_logprobs_fwd, t)
         assert rc == 1 and "groups" in msg
+
+
+def test_a_long_axis_is_cut_into_as_many_pieces_as_run_at_once():
+    """148 multiprocessors, a B200's, which are also assumed where there is no GPU."""
+    lib = _lib.lib()
+
+    def pieces(dk, dv, dtype, backward):
+        size = lib.m2_linear_attention_workspace(1, 1 << 16, 2, 2, dk, dv, dtype, backward)
+        return size // (4 * (3 if backward else 1) * 2 * dk * dv)
+
+    for dk, dv, dtype, an_sm in ((64, 64, 1, 3), (128, 64, 1, 2), (96, 64, 0, 2), (97, 64, 0, 1), (128, 64, 0, 1), (64, 64, 0, 2)):
+        assert pieces(dk, dv, dtype, 0) <= an_sm * 148 // 2 < 1.1 * pieces(dk, dv, dtype, 0)
+        tiles = 2 * ((dk + 63) // 64) + 1                  # of the three gradients
+        assert pieces(dk, dv, dtype, 1) <= an_sm * 148 // (2 * tiles) < 1.1 * pieces(dk, dv, dtype, 1)
