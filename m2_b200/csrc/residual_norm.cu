@@ -210,14 +210,22 @@ template <int MAXT> struct Reduce {
   }
 };
 
+// s / n from inv_n = 1 / n rounded, and one step of Newton's method on what is left: exact where the quotient is a float32 number, so
+// that a row of equal values (whose sum is exact) has exactly their mean.  s * inv_n is one step off for n = 56 or 1000, say, which at
+// eps 1e-12 became values of 0.1.  A division took 3 to 6 % longer, 32768 x 600 88 -> 92 us.
+__device__ __forceinline__ float quotient(float s, float n, float inv_n) {
+  const float q = s * inv_n;
+  return fmaf(fmaf(-q, n, s), inv_n, q);
+}
+
 // mean and 1 / deviation of a row whose columns beyond n (m of this thread's 8 are inside) hold 0
-template <int MODE, int MAXT> __device__ __forceinline__ float2 row_stats(Reduce<MAXT>& red, const V8& v, int m, float inv_n, float eps, bool rms) {
+template <int MODE, int MAXT> __device__ __forceinline__ float2 row_stats(Reduce<MAXT>& red, const V8& v, int m, float inv_n, float n, float eps, bool rms) {
   if (rms) return make_float2(0.f, rsqrtf(fmaf(red(sum8(mul8(v, v)), 0.f).x, inv_n, eps)));
   if constexpr (MODE == FULL) {
     const float2 s = red.moments(v);
     return make_float2(s.x, rsqrtf(fmaf(s.y, inv_n, eps)));
   }
-  const float mean = red(sum8(v), 0.f).x * inv_n;
+  const float mean = quotient(red(sum8(v), 0.f).x, n, inv_n);
   const V8 d = first8(add8(v, splat8(-mean)), m);
   return make_float2(mean, rsqrtf(fmaf(red(sum8(mul8(d, d)), 0.f).x, inv_n, eps)));
 }
@@ -291,7 +299,7 @@ forward_kernel(const Args a) {
     }
     float2 s1 = make_float2(0.f, 1.f), s2 = s1;
     if (a.norm1) {
-      s1 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.eps, a.rms);
+      s1 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.n, a.eps, a.rms);
       v = fma8(normal(v, s1.x, s1.y), w1, b1);
     }
     v = fma8(g, v, mul8(sc, x));
@@ -299,7 +307,7 @@ forward_kernel(const Args a) {
     TX* to = reinterpret_cast<TX*>(const_cast<char*>(wr.go()));
     if (live) store8<MODE>(to, v, m);
     if (a.norm2) {
-      s2 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.eps, a.rms);
+      s2 = row_stats<MODE, MAXT>(red, v, m, inv_n, a.n, a.eps, a.rms);
       v = fma8(normal(v, s2.x, s2.y), w2, b2);
       TY* to = reinterpret_cast<TY*>(const_cast<char*>(wh.go()));
       if (live) store8<MODE>(to, v, m);
@@ -375,7 +383,7 @@ forward_warp_kernel(const Args a) {
     V8 t = v[0];
 #pragma unroll
     for (int k = 1; k < K; ++k) t = add8(t, v[k]);
-    float mean = sum8(t) * (1.f / (8 * K));
+    float mean = quotient(sum8(t), 8.f * K, 1.f / (8 * K));
     const V8 back = splat8(-mean);
     t = splat8(0.f);
 #pragma unroll

@@ -203,3 +203,18 @@ def test_rows_of_norms_that_have_to_be_copied_are_copied_once():
     row = torch.randn(1, 512, 1024, device="cuda", requires_grad=True)
     (d,) = torch.autograd.grad(m2_b200.gated_residual_norm(row.expand(8, 512, 1024), apart[1].detach(), residual_scale=2.0)[0], [row], up[0])
     assert (d - 2 * up[0].sum(0, keepdim=True)).abs().max() <= 8 * 2.0 ** -24 * 2 * up[0].abs().sum(0).max()
+
+
+@pytest.mark.parametrize("D", [31, 96, 257, 600, 768, 1000, 1280, 1536, 1792, 2056, 4096, 8000])
+def test_rows_of_equal_values_are_normalised_to_zero(D):
+    """A sum of D values of 8 bits is exact in float32, so their mean is too; at the default eps a mean that is off by a step of
+    float32 makes a value of about 0.1 of nothing."""
+    c = torch.cat([torch.arange(128, 256, device="cuda") / 128, torch.arange(-255, -127, device="cuda") * 3.0])[:, None]
+    c = c.bfloat16().float()
+    y = c.expand(-1, D).contiguous()
+    w, b = torch.rand(D, device="cuda") + 0.5, torch.randn(D, device="cuda")
+    for x in (y, y.bfloat16()):
+        r, h = m2_b200.gated_residual_norm(x, torch.zeros_like(x), before_weight=w, before_bias=b)
+        assert torch.equal(r, x) and torch.equal(h, b.to(x.dtype).expand_as(h))
+        r, h = m2_b200.gated_residual_norm(torch.zeros_like(x), x, after_weight=w, after_bias=b, before_weight=w)
+        assert torch.equal(r, b.to(x.dtype).expand_as(r))
