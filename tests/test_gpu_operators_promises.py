@@ -218,3 +218,23 @@ def test_rows_of_equal_values_are_normalised_to_zero(D):
         assert torch.equal(r, x) and torch.equal(h, b.to(x.dtype).expand_as(h))
         r, h = m2_b200.gated_residual_norm(torch.zeros_like(x), x, after_weight=w, after_bias=b, before_weight=w)
         assert torch.equal(r, b.to(x.dtype).expand_as(r))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L", [150, 2000])
+def test_an_infinity_stays_in_its_channels_and_behind_its_token(L, dtype):
+    q, k, v = (torch.randn(1, L, 2, 64, device="cuda").to(dtype) for _ in range(3))
+    ld = torch.tensor([-0.01, -0.02], device="cuda")
+    o, s = m2_b200.linear_attention(q, k, v, ld, return_state=True)
+    bad = k.clone()
+    bad[0, 100, 0, 3] = float("inf")
+    p, t = m2_b200.linear_attention(q, bad, v, ld, return_state=True)
+    assert torch.equal(p[:, :, 1], o[:, :, 1]) and torch.equal(p[:, :100], o[:, :100]) and not torch.isfinite(p[0, 100:, 0]).any()
+    assert not torch.isfinite(t[0, 0, 3]).any() and torch.equal(t[0, 1], s[0, 1])
+    assert torch.equal(t[0, 0, :3], s[0, 0, :3]) and torch.equal(t[0, 0, 4:], s[0, 0, 4:])
+    bad = v.clone()
+    bad[0, 100, 0, 3] = float("inf")
+    p, t = m2_b200.linear_attention(q, k, bad, ld, return_state=True)
+    assert torch.equal(p[:, :, 1], o[:, :, 1]) and torch.equal(p[:, :37], o[:, :37]) and not torch.isfinite(p[0, 100:, 0, 3]).any()
+    assert torch.equal(p[..., :3], o[..., :3]) and torch.equal(p[..., 4:], o[..., 4:])
+    assert not torch.isfinite(t[0, 0, :, 3]).any() and torch.equal(t[..., :3], s[..., :3]) and torch.equal(t[..., 4:], s[..., 4:])
