@@ -77,8 +77,8 @@ __device__ __forceinline__ int seq_length(const Scan& a, int b) {
 
 // ---- float32: products on CUDA cores ---------------------------------------------------------------------------------------------------
 // 256 threads as 16 x 16, each with 4 x 4 outputs of a 64 x 64 product; operands lie in shared memory with the summed index outside
-// (two 16-byte loads for 16 products).  Bound by its instructions: 3.7 k FMAs and 2.3 k others a warp and chunk; 4 x 509 tokens of 12
-// heads of 64, cut into four segments: 72 us.  Tensor cores would take six products of bf16 parts for each of these.
+// (two 16-byte loads for 16 products).  Bound by its instructions: 3.6 k FMAs and 1.9 k others a warp and chunk; 4 x 509 tokens of 12
+// heads of 64, cut into four segments: 67 us (sums 23, scan 47 under a profiler).  Tensor cores would take six products of bf16 parts for each of these.
 constexpr int LD = 68;                   // row pitch of the tiles: 16-byte rows, spread over the banks
 
 __device__ __forceinline__ void mac(float (&acc)[4][4], const float4& a, const float4& b) {
@@ -275,12 +275,13 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
 // bits whether or not the state is asked for (two parts took 121 us where three take 137, 32 x 2048 tokens, 12 heads of 64).
 //
 // Bound: a token and head of 64 + 64 channels moves 512 bytes, 64 of them 0.74 us of an SM's share of 6.5 TB/s; the products take
-// 0.55 us (two parts) at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
+// 0.55 us with two parts and 0.69 with three at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
 // unrolled (2.2 k instructions a warp) does not fit the SM's instruction cache and waited for it more than for anything else.  The
 // same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took longer.
-// Measured: 32 x 2048 tokens, 12 heads of 64: 148 us, 2.7 TB/s, the tensor pipe 42 % busy, 1.2 k instructions a warp and chunk, which
-// 12 warps an SM issue at 38 % of its rate (registers and shared memory admit no more); 16 x 2048, 12 heads of 128: 267 us, the pipe
-// 55 % busy, and its three scans back 542 us in one launch (741 in three).
+// Measured: 32 x 2048 tokens, 12 heads of 64: 137 to 145 us, 2.8 TB/s, the tensor pipe 42 % busy, 1.2 k instructions a warp and chunk,
+// which 12 warps an SM issue at 38 % of its rate (registers and shared memory admit no more); 16 x 2048, 12 heads of 128: 255 to 266 us,
+// the pipe 55 % busy, and its three scans back 535 us in one launch (741 in three).  Heads of 65 to 127 channels do the work of 128:
+// 96 take 268 us, 80 take 307 (their tiles are loaded as 128 channels with zeros behind).
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");

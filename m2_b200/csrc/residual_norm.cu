@@ -7,11 +7,12 @@
 //     N'(d) = rstd (d w - mean(d w) - v^ mean(d w v^)),      dw = sum d v^,      db = sum d      (no mean(d w) for the RMS norm).
 //
 // Bound: every tensor crosses HBM once in each direction.  Forward: a warp has a row (forward_warp_kernel), 131072 x 1536 with a
-// float32 stream and a gate per token 555 us, 5.1 TB/s or 0.78 of the measured copy rate.  Gradient, and rows of other lengths: a
+// float32 stream and a gate per token 500 to 550 us, 5.1 to 5.6 TB/s or 0.78 to 0.86 of the measured copy rate.  Gradient, and rows of other lengths: a
 // block of ceil(n / 256) warps walks over rows and a thread owns the same 8 columns of each: weights stay in its registers, and so do
 // the column sums of the gradient, which meet in a second, small launch that adds the blocks' sums in a fixed order (no atomics: two
-// runs give the same bits); 32768 x 768 148 us, 3.1 TB/s: 168 registers a thread admit 12 warps an SM, whose two sums over the row
+// runs give the same bits); 32768 x 768 144 to 150 us, 3.1 TB/s: 168 registers a thread admit 12 warps an SM, whose two sums over the row
 // then show (with the parameters in shared memory and 96 registers it spilled, 346 us).  Rows to come are copied ahead (cp.async).
+// Of those registers 48 are the six column sums, which are kept whether or not they are asked for.
 // Everything is float32 until the one rounding of each output.
 #include "common.cuh"
 
@@ -450,6 +451,9 @@ forward_warp_kernel(const Args a) {
   }
 }
 
+// MAXT: 192 threads, up to 1536 columns, are the most of which two blocks an SM have 168 registers a thread (65,536 / 384); that form
+// spills 24 bytes.  512 threads have 128 and spill 400 to 480 bytes, 1024 have 64 and spill 1272; neither has been made to fit.  As rows
+// get wider than the first form, 32768 x 1536 267 us becomes 757 at 2048 columns; 8192 x 8192 takes 1328 (floors 139, 185 and 185).
 template <typename TX, typename TY, int MODE, int MAXT>
 __global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 2 : 1))
 backward_kernel(const Args a) {
@@ -680,7 +684,10 @@ template <typename TX, typename TY> static int launch_warp(const Args& a, cudaSt
   }
 }
 // Rows in 16-byte pieces: forward, a warp a row where a warp's registers hold it; else a block a row through the ring, up to 4096
-// columns (longer rows would not fit into shared memory).
+// columns.  Longer rows, and rows in no pieces, are loaded value by value: 8192 x 8192 with a float32 stream takes 833 us, 16384 x 4096
+// through the ring 283.  (Two stages of 8192 columns would fit into shared memory forward, and backward where the types and the gate
+// leave 226 KB; there is no such form.)  Widths that are no multiple of 256 take the gradient's form of 512 threads even where 192
+// would do: 32768 x 96 81 us, x 1000 319.
 template <typename TX, typename TY, bool BACK> static int launch_n(const Args& a, bool wide, int blocks, int threads, cudaStream_t st) {
   if (threads > 512) return launch_t<TX, TY, PLAIN, 1024, BACK>(a, blocks, threads, st);
   if (!wide) return launch_t<TX, TY, PLAIN, 512, BACK>(a, blocks, threads, st);

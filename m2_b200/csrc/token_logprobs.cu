@@ -11,8 +11,8 @@
 // largest of 64 thread groups' maxima is a lower bound of the row's k-th largest value, so the few threads whose own maximum is not
 // below it look at their values once more, collect what is not below it, and these are ranked among one another.  Rows with so many
 // equal values that the list overflows are searched k times instead.
-// Measured: 8192 x 30528 bf16 106 us (4.7 TB/s, one exp a value keeps the SFUs 60 % busy), its gradient 184 us (5.4 TB/s); 4096 x
-// 30528 float32 89 us (5.6 TB/s), with 5 alternatives 101 us; one row of 30528 bf16 with 20 alternatives 9 us.  Blocks of 128 threads
+// Measured: 8192 x 30528 bf16 106 us (4.7 TB/s, one exp a value keeps the SFUs 60 % busy), with 5 alternatives 125, its gradient 184 to
+// 198 us (5.1 to 5.4 TB/s); float32 164 us (6.1 TB/s), with 5 alternatives 188; one row of 30528 bf16 with 20 alternatives 9 us.  Blocks of 128 threads
 // rather than 256 (a row's start and end overlap with more other rows): 106 against 115 us.
 #include "common.cuh"
 
@@ -22,7 +22,7 @@ namespace lp {
 constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int GROUPS = 64;
-constexpr int SHARE = THREADS / GROUPS;   // threads of a group: 2 or 4
+constexpr int SHARE = THREADS / GROUPS;   // threads of a group
 constexpr int MAX_TOP = 32;              // <= GROUPS
 constexpr int CAND = 1024;               // candidates kept per block
 constexpr int MAX_SPLIT = 8;             // blocks of a cluster that share a row
