@@ -30,6 +30,8 @@ def _check(name, q, k, v, log_decay, dims):
         raise TypeError(f"{name}: q, k and v are all float32 or all bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
     if log_decay.shape != (H,):
         raise ValueError(f"{name}: log_decay has one value for each of the {H} heads, got shape {tuple(log_decay.shape)}")
+    if log_decay.is_complex():
+        raise TypeError(f"{name}: log_decay holds real numbers, got {log_decay.dtype}")
     dev = q.get_device()
     if dev < 0 or k.get_device() != dev or v.get_device() != dev or log_decay.get_device() != dev:
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
@@ -137,7 +139,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
         _state(name, initial_state, "initial_state", (B, H, dk, dv), q.get_device())
         initial_state = initial_state.contiguous()
     if lengths is not None:
-        if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != q.device:
+        if lengths.shape != (B,) or lengths.is_floating_point() or lengths.is_complex() or lengths.dtype == torch.bool or lengths.device != q.device:
             raise ValueError(f"{name}: lengths are ({B},) integers on {q.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
         lengths = lengths.to(torch.long).contiguous()
     q, k, v = _packed(q), _packed(k), _packed(v)

@@ -238,3 +238,10 @@ def test_an_infinity_stays_in_its_channels_and_behind_its_token(L, dtype):
     assert torch.equal(p[:, :, 1], o[:, :, 1]) and torch.equal(p[:, :37], o[:, :37]) and not torch.isfinite(p[0, 100:, 0, 3]).any()
     assert torch.equal(p[..., :3], o[..., :3]) and torch.equal(p[..., 4:], o[..., 4:])
     assert not torch.isfinite(t[0, 0, :, 3]).any() and torch.equal(t[..., :3], s[..., :3]) and torch.equal(t[..., 4:], s[..., 4:])
+
+
+def test_lengths_are_whole_numbers():
+    q, ld = torch.zeros(2, 3, 2, 8, device="cuda"), torch.zeros(2, device="cuda")
+    for dtype in (torch.complex64, torch.float32, torch.bool):
+        with pytest.raises(ValueError, match="lengths"):
+            m2_b200.linear_attention(q, q, q, ld, lengths=torch.ones(2, device="cuda").to(dtype))

@@ -1,8 +1,10 @@
-"""Workspaces of linear_attention and gated_residual_norm, and rows of token_logprobs, on the host: no GPU is touched."""
+"""Workspaces of linear_attention and gated_residual_norm, rows of token_logprobs, types of decays, on the host: no GPU is touched."""
 import ctypes as C
 
+import pytest
 import torch
 
+import m2_b200
 from m2_b200 import _lib, linear_attn, ops
 
 SOMEWHERE = 1 << 20                      # nothing is read: the calls are refused before any launch
@@ -86,3 +88,11 @@ def test_a_long_axis_is_cut_into_as_many_pieces_as_run_at_once():
         assert pieces(dk, dv, dtype, 0) <= an_sm * 148 // 2 < 1.1 * pieces(dk, dv, dtype, 0)
         tiles = 2 * ((dk + 63) // 64) + 1                  # of the three gradients
         assert pieces(dk, dv, dtype, 1) <= an_sm * 148 // (2 * tiles) < 1.1 * pieces(dk, dv, dtype, 1)
+
+
+def test_complex_decays_are_refused():
+    q, ld = torch.zeros(1, 2, 3, 8), torch.zeros(3, dtype=torch.complex64)
+    with pytest.raises(TypeError, match="log_decay"):
+        m2_b200.linear_attention(q, q, q, ld)
+    with pytest.raises(TypeError, match="log_decay"):
+        m2_b200.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], ld, torch.zeros(1, 3, 8, 8))
