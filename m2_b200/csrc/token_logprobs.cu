@@ -301,7 +301,7 @@ template <typename T> __device__ void select_top(Shared& sh, const Span<T>& sp, 
     unsigned long long top = 0;
     auto look = [&](float v, int id) {
       const unsigned long long q = rank_key(v, id);
-      if (q < last && q > top) top = q;
+      if ((q < last || r == 0) && q > top) top = q;    // a NaN at id 0 has the largest key there is
     };
     sp.ends(look);
     for (int i = tid; i < sp.pieces; i += THREADS) {

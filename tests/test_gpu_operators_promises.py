@@ -245,3 +245,20 @@ def test_lengths_are_whole_numbers():
     for dtype in (torch.complex64, torch.float32, torch.bool):
         with pytest.raises(ValueError, match="lengths"):
             m2_b200.linear_attention(q, q, q, ld, lengths=torch.ones(2, device="cuda").to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [700, 1500, 5000, 30528])
+def test_alternatives_of_rows_of_nan(V, dtype):
+    """NaN goes before all, by ascending id, however many there are."""
+    x = torch.randn(4, V, device="cuda").to(dtype)
+    x[0] = float("nan")
+    x[1, ::2] = float("nan")
+    x[2, 1::2] = float("nan")
+    x[3, 0] = float("nan")
+    out = m2_b200.token_logprobs(x, torch.zeros(4, dtype=torch.long, device="cuda"), top=32)
+    ids = torch.arange(32, device="cuda")
+    assert torch.equal(out.top_id[0], ids) and torch.equal(out.top_id[1], 2 * ids) and torch.equal(out.top_id[2], 2 * ids + 1)
+    rest = x[3, 1:].float().sort(descending=True, stable=True).indices[:31] + 1
+    assert out.top_id[3, 0] == 0 and torch.equal(out.top_id[3, 1:], rest)
+    assert torch.isnan(out.top_logprob).all() and torch.isnan(out.logprob).all()
