@@ -448,9 +448,9 @@ int m2_last_launches(void);
  * A NaN or an infinity in a token's v reaches, besides the tokens after it, outputs of up to 63 tokens before it (their weight
  * for it is 0, and 0 times it is NaN).  An infinity in k or v becomes an infinity or NaN in the channels of the state that it
  * meets (bf16: products are summed in parts, inf - inf among them; float32: a fading infinity is inf - inf).
- * bf16: float32 sums and state; the weights (q_i . k_j) decay^(i-j) and the state's copy that q meets are rounded to bf16, as
- * tensor-core operands; keys enter the state with all 24 bits of their product with the decay, but with 16 in gradients without
- * d_state_in, where the state serves those rounded copies alone.  float32: products and sums in float32 throughout.
+ * bf16: float32 sums and state; operands of the tensor cores that are no bf16 numbers, the weights (q_i . k_j) decay^(i-j) and the
+ * state's copy that q meets, keep 16 bits; keys enter the state with all 24 bits of their product with the decay, and with 16 in
+ * gradients without d_state_in, where the state serves those copies alone.  float32: products and sums in float32 throughout.
  * o has the same bits with and without state_out.  They go by the batch: a long axis is cut where the (sequence, head)
  * pairs do not fill the GPU, and sums are then taken in another order.
  * Gradients (m2_linear_attention_bwd): of q, k, v (packed, `dtype`) and of state_in (d_state_in: NULL or float32), from d_o

@@ -266,22 +266,23 @@ scan_f32_kernel(const __grid_constant__ Scans scans) {
 // A block of 4 warps keeps the columns [col0, col0 + 64) of one (sequence, head) and walks over the chunks; warp w has rows
 // 16 w .. 16 w + 15 of a chunk and rows w DK / 4 .. of the state, whose float32 values stay in its registers.  q, k and v tiles
 // arrive by cp.async one chunk ahead.  A chunk's weights P = (q k^T) decay never leave the registers: the accumulators of q k^T are
-// the operand of P v.  Every warp needs the whole state as an operand: it goes through shared memory as bf16, into the other one of
-// two buffers, so that a chunk has a single block barrier and the warps of the SM's blocks drift apart and fill each other's waits.
+// the operand of P v.  Every warp needs the whole state as an operand: it goes through shared memory, written behind a barrier that
+// all pass when they have read the one before.
 //
-// The state is a sum over thousands of tokens: l^(C-1-j) k_j goes into its product as three bf16 parts of 8 bits, all 24 of it, and
-// every chunk's sum starts from zero and is added in float32, as tensor cores cut their sums instead of rounding them.  A gradient's
-// state that goes nowhere but, rounded to bf16, into products has two parts, 16 bits.  Forward there are always three: o has the same
-// bits whether or not the state is asked for (two parts took 121 us where three take 137, 32 x 2048 tokens, 12 heads of 64).
+// Nothing but o is rounded to bf16.  P and the state's copy that q meets are two bf16 parts of 8 bits each, 16 bits (one part each:
+// o was 1.41 times as far from 64 bits as its own rounding takes it; 32 x 2048 tokens of 12 heads of 64 took 144 us, not 176, and
+// 16 x 2048 of 12 heads of 128 262 and 535 back, not 320 and 676).  The state itself is a sum over thousands of tokens:
+// l^(C-1-j) k_j goes into its product as three parts, all 24 bits of it, and every chunk's sum starts from zero and is added in
+// float32, as tensor cores cut their sums instead of rounding them.  A gradient's state that goes nowhere but into those copies of
+// 16 bits has two parts.  Forward there are always three: o has the same bits whether or not the state is asked for.
 //
 // Bound: a token and head of 64 + 64 channels moves 512 bytes, 64 of them 0.74 us of an SM's share of 6.5 TB/s; the products take
-// 0.55 us with two parts and 0.69 with three at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a chunk
-// unrolled (2.2 k instructions a warp) does not fit the SM's instruction cache and waited for it more than for anything else.  The
-// same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took longer.
-// Measured: 32 x 2048 tokens, 12 heads of 64: 137 to 145 us, 2.8 TB/s, the tensor pipe 42 % busy, 1.2 k instructions a warp and chunk,
-// which 12 warps an SM issue at 38 % of its rate (registers and shared memory admit no more); 16 x 2048, 12 heads of 128: 255 to 266 us,
-// the pipe 55 % busy, and its three scans back 535 us in one launch (741 in three).  Heads of 65 to 127 channels do the work of 128:
-// 96 take 268 us, 80 take 307 (their tiles are loaded as 128 channels with zeros behind).
+// 0.89 us (gradients 0.76) at the 555 TFLOP/s that mma.sync reaches on a B200.  What costs is the rest: loops are kept rolled, as a
+// chunk unrolled (2.2 k instructions a warp) does not fit the SM's instruction cache and waited for it more than for anything else.
+// The same scan on tcgen05 (chunks of 128, P and the state's parts through shared memory, five block barriers a chunk) took longer.
+// Measured: 32 x 2048 tokens, 12 heads of 64: 176 us, 2.3 TB/s, the tensor pipe 55 % busy, 1.3 k instructions a warp and chunk, which
+// 12 warps an SM issue at 41 % of its rate (registers and shared memory admit no more); 16 x 2048, 12 heads of 128: 320 us, the pipe
+// 60 % busy, and its three scans back 676 us in one launch.  Heads of 65 to 127 channels do the work of 128: 80 take 322 us.
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -432,17 +433,25 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
   const int r8 = lane & 7, half = (lane >> 3) & 1, quad = lane >> 4;
   const uint32_t off_a = (r8 + 8 * half) * 128 + ((quad ^ r8) << 4);                // 16 rows, two pieces: A, and B from rows of k
   const uint32_t off_b = (r8 + 8 * quad) * 128 + ((half ^ r8) << 4);                // the other order
-  auto write_state = [&](uint32_t to) {
+  auto write_state = [&]() {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int np = 0; np < NT / 2; ++np) {
-        const float (&x)[4] = s[mt][2 * np], (&y)[4] = s[mt][2 * np + 1];
-        stsm((to + off_a + (w * MT + mt) * 2048) ^ (np << 5), pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3]));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          f32x2 z = f2_pack(s[mt][2 * np + (x >> 1)][2 * (x & 1)], s[mt][2 * np + (x >> 1)][2 * (x & 1) + 1]);
+          hi[x] = cut_off(z);
+          lo[x] = pack_up(z);
+        }
+        const uint32_t to = (base + L::OFF_S + off_a + (w * MT + mt) * 2048) ^ (np << 5);
+        stsm(to, hi[0], hi[1], hi[2], hi[3]);
+        stsm(to + L::STATE, lo[0], lo[1], lo[2], lo[3]);
       }
   };
-  if (!SUMS) write_state(base + L::OFF_S);
-  uint32_t stage = 0, sbuf = 0;          // bytes to the buffers at hand
+  if (!SUMS) write_state();
+  uint32_t stage = 0;                    // bytes to the buffer at hand
   // o: rows 4 x + lane / 8 of this warp's 16, 16-byte piece lane & 7
   const int o_row = w * 16 + (lane >> 3), o_c = lane & 7;
   T* o_at = static_cast<T*>(a.o) + b * a.o_sb + (tok0 + (long long)o_row * dir) * a.o_st + h * a.o_sh + col0 + o_c * 8;
@@ -460,7 +469,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
     cp_wait0();
     __syncthreads();
     if (at + C < end) fetch(base + (L::STAGE - stage), end - at - C);
-    const uint32_t qs = base + stage, ks_ = qs + L::K, vs = ks_ + L::TILE, ss = base + L::OFF_S + sbuf;
+    const uint32_t qs = base + stage, ks_ = qs + L::K, vs = ks_ + L::TILE, ss = base + L::OFF_S;
     if (!SUMS) {
       const uint32_t q_a = qs + w * 2048 + off_a;
       uint32_t qf[MT][4][4];
@@ -473,12 +482,16 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
-            uint32_t f[4];
-            ldsm_t(f, (ss + off_a + (x * 4 + ks) * 2048) ^ (np << 5));
-            mma(o[2 * np], qf[x][ks], f[0], f[1]);
-            mma(o[2 * np + 1], qf[x][ks], f[2], f[3]);
+#pragma unroll
+            for (int y = 1; y >= 0; --y) {
+              uint32_t f[4];
+              ldsm_t(f, ((ss + off_a + (x * 4 + ks) * 2048) ^ (np << 5)) + y * L::STATE);
+              mma(o[2 * np], qf[x][ks], f[0], f[1]);
+              mma(o[2 * np + 1], qf[x][ks], f[2], f[3]);
+            }
           }
       }
+      __syncthreads();                   // the state has been read by all, and may be written anew
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         f2_unpack(f2_mul(f2_pack(o[nt][0], o[nt][1]), f2_splat(d0)), o[nt][0], o[nt][1]);
@@ -506,13 +519,22 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
             const int off = 8 * (e >> 1) - 8 * x - (e & 1);
             p[x][e] = gap + off >= 0 ? (p[x][e] + p2[x][e]) * f[off] : 0.f;
           }
-        const uint32_t pf[4] = {pack2(p[0][0], p[0][1]), pack2(p[0][2], p[0][3]), pack2(p[1][0], p[1][1]), pack2(p[1][2], p[1][3])};
+        uint32_t pf[2][4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          f32x2 z = f2_pack(p[x >> 1][2 * (x & 1)], p[x >> 1][2 * (x & 1) + 1]);
+          pf[0][x] = cut_off(z);
+          pf[1][x] = pack_up(z);
+        }
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
           uint32_t v[4];
           ldsm_t(v, v_a ^ (np << 5));
-          mma(o[2 * np], pf, v[0], v[1]);
-          mma(o[2 * np + 1], pf, v[2], v[3]);
+#pragma unroll
+          for (int y = 1; y >= 0; --y) {
+            mma(o[2 * np], pf[y], v[0], v[1]);
+            mma(o[2 * np + 1], pf[y], v[2], v[3]);
+          }
         }
       }
       if (a.o_f32) {
@@ -607,8 +629,7 @@ scan_mma_kernel(const __grid_constant__ Scans scans) {
           f2_unpack(f2_add(f2_fma(z, keep, z), f2_pack(acc[mt][nt][e], acc[mt][nt][e + 1])), s[mt][nt][e], s[mt][nt][e + 1]);
         }
     stage = L::STAGE - stage;
-    sbuf = L::STATE - sbuf;
-    if (!SUMS && at + C < end) write_state(base + L::OFF_S + sbuf);
+    if (!SUMS && at + C < end) write_state();
   }
   const float f = SUMS ? 1.f : a.final_scale * (a.reverse ? power(ld, n == 0 && a.init ? 0 : 1) : 1.f);
   float* to = SUMS ? a.segments + ((long long)bh * a.n_seg + seg) * a.dk * a.dv : a.final && last ? a.final + b * a.s_b + h * a.s_h : nullptr;

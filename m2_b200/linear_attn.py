@@ -121,11 +121,10 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
                    are zero and the state is that behind the last token
     return_state   also return the state behind the last token, (B, H, dk, dv) float32
 
-    Sums and states are float32.  bfloat16: the weights scale (q_i . k_j) exp(log_decay (i - j)) and the copy of the state that q
-    meets (in gradients, their counterparts) are rounded to bfloat16 as operands of the tensor cores, so that o is as far from the
-    exact value as two roundings to bfloat16 take it; float32 tensors have float32 products throughout.  Two calls give the same
-    bits, with or without the state; those of a text go by the batch it is in, as a long axis is cut where sequences and heads do
-    not fill the GPU, and the parts' sums are then added in another order.
+    Sums and states are float32, and o is rounded once.  bfloat16: operands of the tensor cores that are no bfloat16 numbers (the
+    weights scale (q_i . k_j) exp(log_decay (i - j)), the copy of the state that q meets) keep 16 bits; float32 tensors have
+    float32 products throughout.  Two calls give the same bits, with or without the state; those of a text go by the batch it is
+    in, as a long axis is cut where sequences and heads do not fill the GPU, and the parts' sums are then added in another order.
 
     A NaN or an infinity in v[:, t] reaches, besides the tokens after t, outputs of up to 63 tokens before it.  An infinity in k
     or v becomes an infinity or NaN in the channels of the state that it meets, and so in later outputs.

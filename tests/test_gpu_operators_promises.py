@@ -6,6 +6,7 @@ import torch
 
 import m2_b200
 from m2_b200 import ops
+from tests.test_gpu_linear_attention import U16, U32, definition, make, within
 
 pytestmark = pytest.mark.gpu
 
@@ -262,3 +263,27 @@ def test_alternatives_of_rows_of_nan(V, dtype):
     rest = x[3, 1:].float().sort(descending=True, stable=True).indices[:31] + 1
     assert out.top_id[3, 0] == 0 and torch.equal(out.top_id[3, 1:], rest)
     assert torch.isnan(out.top_logprob).all() and torch.isnan(out.logprob).all()
+
+
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("shape", [(3, 1, 4, 2, 64, 64), (2, 50, 4, 2, 64, 64), (2, 300, 4, 4, 64, 64), (1, 1100, 2, 1, 64, 64), (2, 200, 2, 2, 128, 128), (1, 700, 2, 2, 128, 64),
+                                   (1, 130, 2, 1, 80, 40)])
+def test_bfloat16_scans_round_to_bfloat16_once(shape, state):
+    """Operands of the tensor cores have two parts of 8 bits, the first cut and the second rounded: what is left out is below 2^-7 times
+    half a step, 2^-15 of the operand.  A product has up to two such operands (a weight's or the state's, and in gradients a key's in the
+    state): 2^-14 of M, what the operator gives for the absolute values; sums as in float32 but up to twice as far off; the output's half
+    step once."""
+    B, L, H, K, dk, dv = shape
+    q, k, v, ld, s0 = make(*shape, torch.bfloat16, seed=L)
+    leaves = [t.detach().requires_grad_() for t in ((q, k, v, s0) if state else (q, k, v))]
+    o, s = m2_b200.linear_attention(*leaves[:3], ld, initial_state=leaves[3] if state else None, return_state=True)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    do, ds = torch.randn(o.shape, device="cuda", generator=g).bfloat16(), torch.randn(s.shape, device="cuda", generator=g) * state
+    grads = torch.autograd.grad([o, s], leaves, [do, ds])
+    runs = []
+    for sign in (lambda t: t, torch.abs):
+        wide = [sign(t.detach().double()).requires_grad_() for t in leaves]
+        out = definition(*wide[:3], ld.double(), dk ** -0.5, wide[3] if state else None, None)
+        runs.append([out[0], *torch.autograd.grad(out, wide, [sign(do.double()), sign(ds.double())])[:3]])
+    for name, got, ref, M, d in zip(("o", "dq", "dk", "dv"), [o, *grads[:3]], *runs, (dk, dv, dv, dk)):
+        within(got, ref, U16 * ref.abs() + (2.0 ** -14 + 2 * (d + 64 + L / 32 + 16 + H // K) * U32) * M, name)
