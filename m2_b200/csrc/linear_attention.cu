@@ -78,7 +78,8 @@ __device__ __forceinline__ int seq_length(const Scan& a, int b) {
 // ---- float32: products on CUDA cores ---------------------------------------------------------------------------------------------------
 // 256 threads as 16 x 16, each with 4 x 4 outputs of a 64 x 64 product; operands lie in shared memory with the summed index outside
 // (two 16-byte loads for 16 products).  Bound by its instructions: 3.6 k FMAs and 1.9 k others a warp and chunk; 4 x 509 tokens of 12
-// heads of 64, cut into four segments: 67 us (sums 23, scan 47 under a profiler).  Tensor cores would take six products of bf16 parts for each of these.
+// heads of 64, cut into four segments: 67 us (sums 23, scan 47 under a profiler).  Tensor cores would take six products of bf16 parts
+// for each of these.
 constexpr int LD = 68;                   // row pitch of the tiles: 16-byte rows, spread over the banks
 
 __device__ __forceinline__ void mac(float (&acc)[4][4], const float4& a, const float4& b) {
@@ -755,8 +756,8 @@ step_kernel(const m2_linear_attention_step_args a) {
 // Segments: where the blocks of all (sequence, head) pairs and 64-column tiles do not fill the GPU, a long axis is cut; every
 // segment's own sum is made first (reading k and v once more) and the segments then run side by side.
 // A cut costs half as much again, so there is one only where all blocks still run at once: an SM holds three of them, two with
-// more than 64 channels, and of float32 two with up to 96 channels and one with more (cut for two of those: 4096 float32 tokens of 4 heads
-// of 128 150 us, gradients 400; for one 144 and 368).
+// more than 64 channels, and of float32 two with up to 96 channels and one with more (cut for two of those: 4096 float32 tokens of 4
+// heads of 128 150 us, gradients 400; for one 144 and 368).
 static size_t f32_smem(int dk) { return ((size_t)(3 * ((dk + 15) / 16 * 16) + 2 * C) * LD + C + 4) * sizeof(float); }
 static int blocks_an_sm(int dtype, int dk) {             // dk: of the launch's widest keys
   if (dtype == M2_BF16) return dk <= 64 ? 3 : 2;

@@ -7,12 +7,12 @@
 //     N'(d) = rstd (d w - mean(d w) - v^ mean(d w v^)),      dw = sum d v^,      db = sum d      (no mean(d w) for the RMS norm).
 //
 // Bound: every tensor crosses HBM once in each direction.  Forward: a warp has a row (forward_warp_kernel), 131072 x 1536 with a
-// float32 stream and a gate per token 500 to 550 us, 5.1 to 5.6 TB/s or 0.78 to 0.86 of the measured copy rate.  Gradient, and rows of other lengths: a
-// block of ceil(n / 256) warps walks over rows and a thread owns the same 8 columns of each: weights stay in its registers, and so do
-// the column sums of the gradient, which meet in a second, small launch that adds the blocks' sums in a fixed order (no atomics: two
-// runs give the same bits); 32768 x 768 144 to 150 us, 3.1 TB/s: 168 registers a thread admit 12 warps an SM, whose two sums over the row
-// then show (with the parameters in shared memory and 96 registers it spilled, 346 us).  Rows to come are copied ahead (cp.async).
-// Of those registers 48 are the six column sums, which are kept whether or not they are asked for.
+// float32 stream and a gate per token 500 to 550 us, 5.1 to 5.6 TB/s or 0.78 to 0.86 of the measured copy rate.  Gradient, and rows of
+// other lengths: a block of ceil(n / 256) warps walks over rows and a thread owns the same 8 columns of each: weights stay in its
+// registers, and so do the column sums of the gradient, which meet in a second, small launch that adds the blocks' sums in a fixed
+// order (no atomics: two runs give the same bits); 32768 x 768 144 to 150 us, 3.1 TB/s: 168 registers a thread, 48 of them the six
+// column sums whether or not they are asked for, admit 12 warps an SM, whose two sums over the row then show (with the parameters in
+// shared memory and 96 registers it spilled, 346 us).  Rows to come are copied ahead (cp.async).
 // Everything is float32 until the one rounding of each output.
 #include "common.cuh"
 
@@ -452,7 +452,7 @@ forward_warp_kernel(const Args a) {
 }
 
 // MAXT: 192 threads, up to 1536 columns, are the most of which two blocks an SM have 168 registers a thread (65,536 / 384); that form
-// spills 24 bytes.  512 threads have 128 and spill 400 to 480 bytes, 1024 have 64 and spill 1272; neither has been made to fit.  As rows
+// spills 24 bytes.  512 threads have 128 and spill 384 to 480 bytes, 1024 have 64 and spill 1272; neither has been made to fit.  As rows
 // get wider than the first form, 32768 x 1536 267 us becomes 757 at 2048 columns; 8192 x 8192 takes 1328 (floors 139, 185 and 185).
 template <typename TX, typename TY, int MODE, int MAXT>
 __global__ void __launch_bounds__(MAXT, (MAXT == 192 ? 2 : 1))

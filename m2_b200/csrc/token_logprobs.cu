@@ -12,8 +12,8 @@
 // below it look at their values once more, collect what is not below it, and these are ranked among one another.  Rows with so many
 // equal values that the list overflows are searched k times instead.
 // Measured: 8192 x 30528 bf16 106 us (4.7 TB/s, one exp a value keeps the SFUs 60 % busy), with 5 alternatives 125, its gradient 184 to
-// 198 us (5.1 to 5.4 TB/s); float32 164 us (6.1 TB/s), with 5 alternatives 188; one row of 30528 bf16 with 20 alternatives 9 us.  Blocks of 128 threads
-// rather than 256 (a row's start and end overlap with more other rows): 106 against 115 us.
+// 198 us (5.1 to 5.4 TB/s); float32 164 us (6.1 TB/s), with 5 alternatives 188; one row of 30528 bf16 with 20 alternatives 9 us.
+// Blocks of 128 threads rather than 256 (a row's start and end overlap with more other rows): 106 against 115 us.
 #include "common.cuh"
 
 namespace m2 {
@@ -446,7 +446,7 @@ backward_kernel(const BwdArgs a, int slices) {
   T* dx = static_cast<T*>(a.dx) + row * a.ldd;
   const int tid = threadIdx.x;
   const long long target = a.target[row];
-  if (target == a.ignore) {              // nothing is read: 8192 x 30528 bf16 with 85 % of the rows ignored 101 us, where reading them took 183
+  if (target == a.ignore) {              // nothing is read: 8192 x 30528 bf16, 85 % of the rows ignored, 101 us; reading them took 183
     const Span<T> z(dx, lo, hi);
     if (tid < z.head) st_from_float(dx + lo + tid, 0.f);
     if (z.tail() + tid < hi) st_from_float(dx + z.tail() + tid, 0.f);
