@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define M2_B200_ABI_VERSION 10
+#define M2_B200_ABI_VERSION 11
 
 typedef enum { M2_F32 = 0, M2_BF16 = 1, M2_F16 = 2 /* only where an entry point says so */ } m2_dtype;
 
@@ -44,7 +44,7 @@ typedef enum {
 #define M2_DEV_TIMEOUT_MMA   2   /* a wait for tensor-core work or a free accumulator ran out */
 #define M2_DEV_TIMEOUT_EPI   4   /* an epilogue's wait for an accumulator ran out */
 #define M2_DEV_TIMEOUT_EMPTY 8   /* a producer's wait for a free shared-memory stage ran out */
-#define M2_DEV_BAD_INDEX     16  /* m2_embed_layernorm_fwd met an id outside its table (clamped), or m2_token_logprobs_fwd a target outside the vocabulary */
+#define M2_DEV_BAD_INDEX     16  /* m2_embed_layernorm_fwd met an id outside its table (clamped), m2_token_logprobs_fwd a target outside the vocabulary, or m2_reorder_states a beam that is none */
 
 /* ABI version of the loaded library (== M2_B200_ABI_VERSION it was built with). */
 int m2_version(void);
@@ -427,7 +427,7 @@ long long m2_encoder_workspace(int batch, int pitch, int d_model, int inter);
 long long m2_encoder_workspace_f32(int batch, int seq_len, int d_model, int inter, int nblocks);
 int m2_encoder_fwd(const m2_encoder_args* args, void* stream);
 
-/* Kernels that this thread's last call of an m2_linear_attention_*, m2_residual_norm_* or m2_token_logprobs_* entry point launched:
+/* Kernels that this thread's last call of an entry point from here on launched:
  * their number goes by the shape (a long axis that is cut, shared heads, the sums of parameters' gradients). */
 int m2_last_launches(void);
 
@@ -580,6 +580,166 @@ typedef struct {
 
 int m2_token_logprobs_fwd(const m2_token_logprobs_args* args, void* stream);
 int m2_token_logprobs_bwd(const m2_token_logprobs_bwd_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Short causal convolution of every channel with its own taps, in front of a scan:
+ *   v_t = bias + sum_i weight[d, i] x_{t - taps + 1 + i},     y_t = v_t or (silu != 0) silu(v_t)
+ *   x (batch, seq_len, dim): `dtype` (M2_F32 or M2_BF16), strides in elements, contiguous channels.  y packed.  weight float32
+ *   (dim, taps), taps <= 8, bias float32 (dim) or NULL.
+ *   lengths   : NULL or int64 (batch), as m2_linear_attention_fwd takes them: what lies behind a text is not read, y (and gradients)
+ *               are zero there.
+ *   state_in  : NULL (zeros) or (batch, taps - 1, dim) of `dtype`, packed, oldest first: the inputs in front of x.  state_out: NULL or the
+ *               same for the next call: the last taps - 1 inputs of every text.  They may not be the same memory.  With one tap there are none.
+ * Products and sums are float32.  Gradients (m2_causal_conv_bwd): of x and state_in (`dtype`, packed) from d_y (`dtype`, strides) and
+ * d_state_out (NULL or packed); of weight and bias float32 sums in a fixed order (NULL: not wanted).
+ *   workspace: m2_causal_conv_workspace() bytes on a 16-byte boundary, asked for on the device that the call runs on.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  int batch, seq_len, dim, taps, silu;
+  m2_dtype dtype;
+  const void* x; long long x_sb, x_st;
+  const float *weight, *bias;
+  const void* lengths;     /* int64 */
+  const void* state_in;
+  void *y, *state_out;
+} m2_causal_conv_args;
+
+typedef struct {
+  const void* d_y; long long y_sb, y_st;
+  const void* d_state_out;
+  void *d_x, *d_state_in;
+  float *d_weight, *d_bias;
+  float* workspace; long long workspace_bytes;
+} m2_causal_conv_grads;
+
+/* One token of every sequence: x (batch, dim), y packed; `state` (taps - 1, dim) of each, s_b apart, loses its oldest input and takes x. */
+typedef struct {
+  int batch, dim, taps, silu;
+  m2_dtype dtype;
+  const void* x; long long x_sb;
+  const float *weight, *bias;
+  void* state; long long s_b;
+  void* y;
+} m2_causal_conv_step_args;
+
+int m2_causal_conv_fwd(const m2_causal_conv_args* args, void* stream);
+long long m2_causal_conv_workspace(int batch, int seq_len, int dim, int taps);
+int m2_causal_conv_bwd(const m2_causal_conv_args* args, const m2_causal_conv_grads* grads, void* stream);
+int m2_causal_conv_step(const m2_causal_conv_step_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Selective state space scan: a causal mixer in which every channel d has a state of `states` numbers that the token itself fades and feeds.
+ *   s_t = softplus(delta_t + delta_bias) or (softplus == 0) delta_t + delta_bias
+ *   h_t[n] = exp(s_t a[d, n]) h_{t-1}[n] + s_t x_t b_t[n],     y_t = (sum_n c_t[n] h_t[n] + skip x_t) silu(gate_t)
+ *   x, delta, gate (batch, seq_len, dim): `dtype`, strides in elements, contiguous channels; gate NULL: without.  b, c (batch, seq_len,
+ *   groups, states): `dtype`, strides, contiguous states; channel d reads group d / (dim / groups).  states <= 64.
+ *   a float32 (dim, states), packed, < 0 (or 0) for states that do not grow; skip, delta_bias float32 (dim) or NULL.
+ *   y packed.  lengths as above; the state is that behind a text's last token.
+ *   state_in  : NULL (zeros) or float32 (batch, dim, states), packed; state_out: NULL or the same.
+ *   saves     : NULL, or m2_selective_scan_saves() bytes on a 16-byte boundary: states along the axis, for the gradient.
+ *   workspace : m2_selective_scan_workspace() bytes on a 16-byte boundary (0: NULL).  Both sizes go by the multiprocessors of the current
+ *               device: ask for them on the device that the call runs on.
+ * Steps, states and sums are float32, each output is rounded once.  A long axis is cut where sequences and channels do not fill the GPU, so
+ * that a text's bits go by the batch that it is in; two runs of one call give the same bits.
+ * Gradients (m2_selective_scan_bwd), from d_y (`dtype`, strides) and d_state_out (NULL: zero): d_x, d_delta, d_gate, d_b, d_c of `dtype`, packed;
+ * d_a, d_skip, d_delta_bias, d_state_in float32 (NULL: not wanted).  Sums over channels, sequences and tokens are float32 in a fixed order.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  int batch, seq_len, dim, states, groups, softplus;
+  m2_dtype dtype;
+  const void* x; long long x_sb, x_st;
+  const void* delta; long long d_sb, d_st;
+  const void* gate; long long z_sb, z_st;
+  const void* b; long long b_sb, b_st, b_sg;
+  const void* c; long long c_sb, c_st, c_sg;
+  const float *a, *skip, *delta_bias;
+  const void* lengths;     /* int64 */
+  const float* state_in;
+  void* y;
+  float *state_out, *saves; long long saves_bytes;
+  float* workspace; long long workspace_bytes;
+} m2_selective_scan_args;
+
+typedef struct {
+  const void* d_y; long long y_sb, y_st;
+  const float* d_state_out;
+  void *d_x, *d_delta, *d_gate, *d_b, *d_c;
+  float *d_a, *d_skip, *d_delta_bias, *d_state_in;
+} m2_selective_scan_grads;
+
+/* One token of every sequence: x, delta, gate (batch, dim), b, c (batch, groups, states), y packed.  `state` float32 (dim, states) of each
+ * sequence, s_b apart, is read and replaced. */
+typedef struct {
+  int batch, dim, states, groups, softplus;
+  m2_dtype dtype;
+  const void* x; long long x_sb;
+  const void* delta; long long d_sb;
+  const void* gate; long long z_sb;
+  const void* b; long long b_sb, b_sg;
+  const void* c; long long c_sb, c_sg;
+  const float *a, *skip, *delta_bias;
+  float* state; long long s_b;
+  void* y;
+} m2_selective_scan_step_args;
+
+long long m2_selective_scan_saves(int batch, int seq_len, int dim, int states, int groups);
+long long m2_selective_scan_workspace(int batch, int seq_len, int dim, int states, int groups, int backward);
+int m2_selective_scan_fwd(const m2_selective_scan_args* args, void* stream);
+int m2_selective_scan_bwd(const m2_selective_scan_args* args, const m2_selective_scan_grads* grads, void* stream);
+int m2_selective_scan_step(const m2_selective_scan_step_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * One step of a beam search: the `keep` best (beam, token) pairs of each text by scores[beam] + log softmax(logits[beam])[token].
+ *   logits (batch, beams, vocab) of `dtype`, strides in elements, contiguous logits; scores float32 (batch, beams), packed.  beams, keep <= 32.
+ *   finished  : NULL, or bytes (batch, beams): a beam that has ended has one continuation, end_id at its own score; its logits are not read.
+ *   end_id    : the token that ends a text, or -1.
+ *   score float32, beam, token int64 (batch, keep), best first; done NULL, or bytes (batch, keep): whether the beam has ended now.
+ * A beam's tokens go by their logits, equal ones by ascending id; beams against one another by scores in 64 bits, equal ones by ascending
+ * beam; NaN goes before all (a NaN or +inf among a beam's logits makes all of that beam NaN).  A score of -inf is no candidate: where
+ * there are fewer than `keep`, the rest are beam 0, token end_id (0 without), score -inf.
+ *   workspace: m2_beam_select_workspace() bytes on a 16-byte boundary.
+ * m2_reorder_states: in each of `count` tensors of batch * beams rows, row (i, k) becomes what row (i, beam[i, k]) was; beam int64 (batch,
+ * beams).  A beam outside 0 .. beams-1 is clamped and M2_DEV_BAD_INDEX set.  `states` is host memory; rows of different tensors may not overlap.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  int batch, beams, vocab, keep;
+  m2_dtype dtype;
+  const void* logits; long long x_sb, x_sk;
+  const float* scores;
+  const void* finished;
+  long long end_id;
+  float* score; void *beam, *token, *done;
+  void* workspace; long long workspace_bytes;
+} m2_beam_select_args;
+
+typedef struct { void* p; long long row_bytes, stride_bytes; } m2_beam_state;
+typedef struct {
+  int batch, beams, count;
+  const void* beam;
+  const m2_beam_state* states;
+} m2_reorder_states_args;
+
+long long m2_beam_select_workspace(int batch, int beams, int vocab, int keep);
+int m2_beam_select(const m2_beam_select_args* args, void* stream);
+int m2_reorder_states(const m2_reorder_states_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Dropout (the reference: nn.Dropout in training, bert/src/bert_layers.py:487, 505) from a counter-based generator, Philox 4x32-10:
+ *   y = (kept(i) ? x / (1 - p) : 0) + residual
+ *   x, y, residual (NULL: none): n values of `dtype`, packed; y may be x or the residual.  p = threshold / 65536.
+ *   Element i is kept if 16 bits of the block that key `key` gives for the counter (i / 8, call) are not below the threshold: halves of the
+ *   four words in order, the low one first.  seed: NULL, or int64 (2) on the device: key and call are read there.
+ * The gradient of x is the same call on the gradient of y without a residual.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  long long n; int threshold;
+  m2_dtype dtype;
+  const void *x, *residual; void* y;
+  const void* seed;
+  unsigned long long key, call;
+} m2_dropout_args;
+
+int m2_dropout(const m2_dropout_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,10 +17,15 @@ from .graph import GraphedForward  # noqa: F401
 from .linear_attn import linear_attention, linear_attention_step  # noqa: F401
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from .residual_norm import gated_residual_norm  # noqa: F401
+from .short_conv import causal_conv, causal_conv_step  # noqa: F401
+from .state_scan import selective_scan, selective_scan_step  # noqa: F401
+from .beams import BeamStep, beam_select, reorder_states  # noqa: F401
+from .random_drop import dropout  # noqa: F401
 
 __all__ = [
     "MonarchMixerSequenceMixing", "HyenaFilter", "BlockdiagLinear", "StructuredLinear",
     "BertGatedLinearUnitMLP", "blockdiag_multiply", "Sin", "PositionalEmbedding",
     "ExponentialModulation", "OptimModule", "GraphedForward",
     "linear_attention", "linear_attention_step", "gated_residual_norm", "token_logprobs", "TokenLogprobs",
+    "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "beam_select", "BeamStep", "reorder_states", "dropout",
 ]

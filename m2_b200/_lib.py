@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libm2b200.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 M2_F32, M2_BF16, M2_F16 = 0, 1, 2
 
@@ -220,6 +220,86 @@ class TokenLogprobsBwdArgs(C.Structure):
     ]
 
 
+class CausalConvArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("seq_len", C.c_int), ("dim", C.c_int), ("taps", C.c_int), ("silu", C.c_int), ("dtype", C.c_int),
+        ("x", C.c_void_p), ("x_sb", C.c_longlong), ("x_st", C.c_longlong), ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("y", C.c_void_p), ("state_out", C.c_void_p),
+    ]
+
+
+class CausalConvGrads(C.Structure):
+    _fields_ = [
+        ("d_y", C.c_void_p), ("y_sb", C.c_longlong), ("y_st", C.c_longlong), ("d_state_out", C.c_void_p), ("d_x", C.c_void_p),
+        ("d_state_in", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_longlong),
+    ]
+
+
+class CausalConvStepArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("dim", C.c_int), ("taps", C.c_int), ("silu", C.c_int), ("dtype", C.c_int), ("x", C.c_void_p),
+        ("x_sb", C.c_longlong), ("weight", C.c_void_p), ("bias", C.c_void_p), ("state", C.c_void_p), ("s_b", C.c_longlong),
+        ("y", C.c_void_p),
+    ]
+
+
+class SelectiveScanArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("seq_len", C.c_int), ("dim", C.c_int), ("states", C.c_int), ("groups", C.c_int), ("softplus", C.c_int),
+        ("dtype", C.c_int), ("x", C.c_void_p), ("x_sb", C.c_longlong), ("x_st", C.c_longlong), ("delta", C.c_void_p), ("d_sb", C.c_longlong),
+        ("d_st", C.c_longlong), ("gate", C.c_void_p), ("z_sb", C.c_longlong), ("z_st", C.c_longlong), ("b", C.c_void_p),
+        ("b_sb", C.c_longlong), ("b_st", C.c_longlong), ("b_sg", C.c_longlong), ("c", C.c_void_p), ("c_sb", C.c_longlong),
+        ("c_st", C.c_longlong), ("c_sg", C.c_longlong), ("a", C.c_void_p), ("skip", C.c_void_p), ("delta_bias", C.c_void_p),
+        ("lengths", C.c_void_p), ("state_in", C.c_void_p), ("y", C.c_void_p), ("state_out", C.c_void_p), ("saves", C.c_void_p),
+        ("saves_bytes", C.c_longlong), ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+    ]
+
+
+class SelectiveScanGrads(C.Structure):
+    _fields_ = [
+        ("d_y", C.c_void_p), ("y_sb", C.c_longlong), ("y_st", C.c_longlong), ("d_state_out", C.c_void_p), ("d_x", C.c_void_p),
+        ("d_delta", C.c_void_p), ("d_gate", C.c_void_p), ("d_b", C.c_void_p), ("d_c", C.c_void_p), ("d_a", C.c_void_p),
+        ("d_skip", C.c_void_p), ("d_delta_bias", C.c_void_p), ("d_state_in", C.c_void_p),
+    ]
+
+
+class SelectiveScanStepArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("dim", C.c_int), ("states", C.c_int), ("groups", C.c_int), ("softplus", C.c_int), ("dtype", C.c_int),
+        ("x", C.c_void_p), ("x_sb", C.c_longlong), ("delta", C.c_void_p), ("d_sb", C.c_longlong), ("gate", C.c_void_p),
+        ("z_sb", C.c_longlong), ("b", C.c_void_p), ("b_sb", C.c_longlong), ("b_sg", C.c_longlong), ("c", C.c_void_p), ("c_sb", C.c_longlong),
+        ("c_sg", C.c_longlong), ("a", C.c_void_p), ("skip", C.c_void_p), ("delta_bias", C.c_void_p), ("state", C.c_void_p),
+        ("s_b", C.c_longlong), ("y", C.c_void_p),
+    ]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int), ("beams", C.c_int), ("vocab", C.c_int), ("keep", C.c_int), ("dtype", C.c_int), ("logits", C.c_void_p),
+        ("x_sb", C.c_longlong), ("x_sk", C.c_longlong), ("scores", C.c_void_p), ("finished", C.c_void_p), ("end_id", C.c_longlong),
+        ("score", C.c_void_p), ("beam", C.c_void_p), ("token", C.c_void_p), ("done", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_longlong),
+    ]
+
+
+class BeamState(C.Structure):
+    _fields_ = [
+        ("p", C.c_void_p), ("row_bytes", C.c_longlong), ("stride_bytes", C.c_longlong),
+    ]
+
+
+class ReorderStatesArgs(C.Structure):
+    _fields_ = [("batch", C.c_int), ("beams", C.c_int), ("count", C.c_int), ("beam", C.c_void_p), ("states", C.POINTER(BeamState))]
+
+
+class DropoutArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_longlong), ("threshold", C.c_int), ("dtype", C.c_int), ("x", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+        ("seed", C.c_void_p), ("key", C.c_ulonglong), ("call", C.c_ulonglong),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/m2_b200.h declares
 SYMBOLS = {
     "m2_version": (C.c_int, []),
@@ -262,6 +342,19 @@ SYMBOLS = {
     "m2_residual_norm_bwd": (C.c_int, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), C.c_void_p]),
     "m2_token_logprobs_fwd": (C.c_int, [C.POINTER(TokenLogprobsArgs), C.c_void_p]),
     "m2_token_logprobs_bwd": (C.c_int, [C.POINTER(TokenLogprobsBwdArgs), C.c_void_p]),
+    "m2_causal_conv_fwd": (C.c_int, [C.POINTER(CausalConvArgs), C.c_void_p]),
+    "m2_causal_conv_workspace": (C.c_longlong, [C.c_int] * 4),
+    "m2_causal_conv_bwd": (C.c_int, [C.POINTER(CausalConvArgs), C.POINTER(CausalConvGrads), C.c_void_p]),
+    "m2_causal_conv_step": (C.c_int, [C.POINTER(CausalConvStepArgs), C.c_void_p]),
+    "m2_selective_scan_saves": (C.c_longlong, [C.c_int] * 5),
+    "m2_selective_scan_workspace": (C.c_longlong, [C.c_int] * 6),
+    "m2_selective_scan_fwd": (C.c_int, [C.POINTER(SelectiveScanArgs), C.c_void_p]),
+    "m2_selective_scan_bwd": (C.c_int, [C.POINTER(SelectiveScanArgs), C.POINTER(SelectiveScanGrads), C.c_void_p]),
+    "m2_selective_scan_step": (C.c_int, [C.POINTER(SelectiveScanStepArgs), C.c_void_p]),
+    "m2_beam_select_workspace": (C.c_longlong, [C.c_int] * 4),
+    "m2_beam_select": (C.c_int, [C.POINTER(BeamSelectArgs), C.c_void_p]),
+    "m2_reorder_states": (C.c_int, [C.POINTER(ReorderStatesArgs), C.c_void_p]),
+    "m2_dropout": (C.c_int, [C.POINTER(DropoutArgs), C.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,119 @@
+"""One step of a beam search: the best of all (beam, token) pairs from logits, behind the decoder and beside token_logprobs, and the states of the
+chosen beams (of linear_attention, selective_scan, causal_conv) moved to their places.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib, ops
+
+MAX_BEAMS = 32
+_TYPES = {torch.float32: _lib.M2_F32, torch.bfloat16: _lib.M2_BF16}
+
+
+class BeamStep(NamedTuple):
+    """score float32; beam, the one that is continued, and token, int64; finished, bool, or None without end_id: all (B, keep), best first."""
+    score: torch.Tensor
+    beam: torch.Tensor
+    token: torch.Tensor
+    finished: Optional[torch.Tensor]
+
+
+def beam_select(logits, scores, *, keep=None, finished=None, end_id=None):
+    """The `keep` (default K, at most 32) best continuations of each text by scores[b, k] + log softmax(logits[b, k])[token], for logits
+    (B, K, V), float32 or bfloat16 (rows of adjacent logits are read in place, once), and scores (B, K); K <= 32.
+
+    end_id    None, or the id that ends a text: `finished` of the result says which beams have ended with this token or before
+    finished  None or (B, K) bool: an ended beam has one continuation, end_id at its own score; its logits are not read
+
+    A beam's tokens go by their logits, equal ones by ascending id; beams go by scores in 64 bits, equal ones by ascending beam.  A
+    score of -inf is no candidate (a text's first step: scores 0, -inf, -inf ... where all its beams are alike); where there are fewer
+    than `keep`, the rest are beam 0, token end_id (0 without it), score -inf.  NaN goes before all.  It has no gradient."""
+    name = "beam_select"
+    if logits.dim() != 3 or scores.shape != logits.shape[:2]:
+        raise ValueError(f"{name}: logits are (B, K, V) and scores (B, K), got {tuple(logits.shape)} and {tuple(scores.shape)}")
+    B, K, V = logits.shape
+    if logits.dtype not in _TYPES:
+        raise TypeError(f"{name}: logits are float32 or bfloat16, got {logits.dtype}")
+    if not scores.is_floating_point():
+        raise TypeError(f"{name}: scores are real numbers, got {scores.dtype}")
+    dev = logits.get_device()
+    if dev < 0 or scores.get_device() != dev or (finished is not None and finished.get_device() != dev):
+        raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
+    keep = K if keep is None else int(keep)
+    if V == 0 or not 1 <= K <= MAX_BEAMS or not 1 <= keep <= MAX_BEAMS:
+        raise ValueError(f"{name}: {keep} of {K} beams (1 to {MAX_BEAMS} each) and {V} logits")
+    if end_id is not None and not 0 <= int(end_id) < 1 << 62:
+        raise ValueError(f"{name}: end_id {end_id}")
+    if finished is not None:
+        if end_id is None:
+            raise ValueError(f"{name}: finished beams need an end_id")
+        if finished.shape != (B, K) or finished.dtype != torch.bool:
+            raise ValueError(f"{name}: finished is ({B}, {K}) bool, got {finished.dtype} {tuple(finished.shape)}")
+        finished = finished.contiguous()
+    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or pass detached tensors")
+    if logits.stride(2) != 1 and V > 1:
+        logits = logits.contiguous()
+    scores = (scores if scores.dtype == torch.float32 else scores.float()).contiguous()
+    score = scores.new_empty((B, keep))
+    beam, token = (torch.empty((B, keep), dtype=torch.long, device=logits.device) for _ in range(2))
+    done = torch.empty((B, keep), dtype=torch.bool, device=logits.device) if end_id is not None else None
+    size = _lib.lib().m2_beam_select_workspace(B, K, V, keep)
+    work = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    a = _lib.BeamSelectArgs(B, K, V, keep, _TYPES[logits.dtype], logits.data_ptr(), *logits.stride()[:2], scores.data_ptr(),
+                            finished.data_ptr() if finished is not None else None, -1 if end_id is None else int(end_id), score.data_ptr(), beam.data_ptr(),
+                            token.data_ptr(), done.data_ptr() if done is not None else None, work.data_ptr(), size)
+    ops._launch("m2_beam_select", logits, _lib.lib().m2_beam_select, C.byref(a), launches=None)
+    return BeamStep(score, beam, token, done)
+
+
+def _apart(states):
+    """Whether no element belongs to two of the states, each (pointer, bytes of a row, distance of rows, rows)."""
+    order = sorted((p, row, step, p + step * (n - 1) + row) for p, row, step, n in states if row and n)
+    for i, (p, row, step, end) in enumerate(order):
+        for q, row2, step2, _ in order[i + 1:]:
+            if q >= end:
+                break
+            at = (q - p) % step                                # rows of one cache, side by side
+            if step != step2 or at < row or at + row2 > step:
+                return False
+    return True
+
+
+def reorder_states(states, beam):
+    """In each tensor of `states`, (B * K, ...), row b K + k becomes what row b K + beam[b, k] was, in place and in one launch for all that are
+    laid out alike; beam (B, K) int64 as beam_select gives it, K <= 32.  Every row is packed; rows of one tensor lie a fixed distance
+    apart.  An entry of beam outside 0 .. K-1 is clamped and sets M2_DEV_BAD_INDEX (ops.device_status())."""
+    name = "reorder_states"
+    states = [states] if isinstance(states, torch.Tensor) else list(states)
+    if beam.dim() != 2 or beam.dtype != torch.long:
+        raise ValueError(f"{name}: beam is (B, K) int64, got {beam.dtype} {tuple(beam.shape)}")
+    B, K = beam.shape
+    if not 1 <= K <= MAX_BEAMS:
+        raise ValueError(f"{name}: {K} beams (1 to {MAX_BEAMS})")
+    dev = beam.get_device()
+    if dev < 0 or any(s.get_device() != dev for s in states):
+        raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
+    rows = (_lib.BeamState * max(len(states), 1))()
+    for i, s in enumerate(states):
+        if s.dim() < 1 or s.shape[0] != B * K:
+            raise ValueError(f"{name}: states have B * K = {B * K} rows, got {tuple(s.shape)}")
+        if torch.is_grad_enabled() and s.requires_grad:
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+        size = s.element_size()
+        n = s.numel() // (B * K) * size if B else 0
+        if B and not (s.is_contiguous() or (s[0].is_contiguous() and (B * K == 1 or s.stride(0) * size >= n))):
+            raise ValueError(f"{name}: a state is changed in place: its rows are packed and do not overlap, got {tuple(s.shape)} with strides {s.stride()}")
+        rows[i] = _lib.BeamState(s.data_ptr(), n, s.stride(0) * size if B * K > 1 else n)
+    if not _apart([(r.p or 0, r.row_bytes, r.stride_bytes, B * K) for r in rows[:len(states)]]):
+        raise ValueError(f"{name}: two states share memory")
+    beam = beam.contiguous()
+    a = _lib.ReorderStatesArgs(B, K, len(states), beam.data_ptr(), rows)
+    ops._launch("m2_reorder_states", beam, _lib.lib().m2_reorder_states, C.byref(a), launches=None)
+    for s in states:
+        if not s.is_inference():
+            torch.autograd.graph.increment_version(s)
