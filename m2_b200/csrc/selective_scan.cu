@@ -9,12 +9,13 @@ namespace m2 {
 namespace ss {
 
 constexpr int THREADS = 128;
-constexpr int CT = 64;                   // channels of a block: 16 a warp, two a thread
-constexpr int QL = 4;                    // lanes that share a channel's states
+constexpr int TT = 32;                   // tokens of a tile
 constexpr int MAX_STATES = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 
-__host__ __device__ constexpr int tile_of(int per_lane) { return per_lane == 16 ? 16 : 32; }       // tokens of a tile
+// A thread has two channels with S states of each; QL lanes share a channel's states.  4 x 4 for up to 16 states, 8 x 4 up to 32, 8 x 8 up to 64: sixteen
+// states a lane were tried and spilled hundreds of bytes.
+__host__ __device__ constexpr int channels_of(int ql) { return 256 / ql; }                          // of a block
 
 struct Rows { const void* p; long long sb, st; int vec; };           // vec: 16-byte pieces
 struct Group { const void* p; long long sb, st, sg; };
@@ -47,25 +48,49 @@ struct Grads {
 using lp::Piece;
 using lp::ex2;
 
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + ex2(-v * LOG2E)); }
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * LOG2E)); }
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|): log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3, and atanh(s) = s + s^3 P(s^2) with P a
+// least-squares fit in s^2 <= 1/9 that leaves 5e-9 of s: small steps keep their digits.
 __device__ __forceinline__ float step_of(float v, int softplus) {
-  return softplus ? fmaxf(v, 0.f) + log1pf(ex2(-fabsf(v) * LOG2E)) : v;
+  if (!softplus) return v;
+  const float e = ex2(-fabsf(v) * LOG2E), s = e * rcp(2.f + e), u = s * s;
+  float p = fmaf(0.140122298f, u, 0.139995704f);
+  p = fmaf(p, u, 0.200108495f);
+  p = fmaf(p, u, 0.333332066f);
+  return fmaxf(v, 0.f) + 2.f * fmaf(s * u, p, s);
 }
 
 template <typename T> __device__ __forceinline__ uint4 load_piece(const T* p, int valid, bool vec) {
   constexpr int E = Piece<T>::N;
   if (vec && valid >= E) return __ldg(reinterpret_cast<const uint4*>(p));
-  float f[E];
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int j = 0; j < E && j < valid; ++j) {
+    uint32_t u;
+    if constexpr (sizeof(T) == 4) u = __ldg(reinterpret_cast<const uint32_t*>(p) + j);
+    else u = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + j) << (j & 1) * 16;
+    const int at = j * (int)sizeof(T) / 4;
 #pragma unroll
-  for (int j = 0; j < E; ++j) f[j] = j < valid ? lp::load1(p + j) : 0.f;
-  return Piece<T>::put(f);
+    for (int q = 0; q < 4; ++q) w[q] |= q == at ? u : 0;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T> __device__ __forceinline__ void store_piece(T* p, const float (&f)[Piece<T>::N], int valid, bool vec) {
   constexpr int E = Piece<T>::N;
-  if (vec && valid >= E) { *reinterpret_cast<uint4*>(p) = Piece<T>::put(f); return; }
-#pragma unroll
-  for (int j = 0; j < E; ++j)
-    if (j < valid) st_from_float(p + j, f[j]);
+  const uint4 u = Piece<T>::put(f);
+  if (vec && valid >= E) { *reinterpret_cast<uint4*>(p) = u; return; }
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+  for (int j = 0; j < E && j < valid; ++j) {
+    const uint32_t word = j * sizeof(T) < 4 ? w[0] : j * sizeof(T) < 8 ? w[1] : j * sizeof(T) < 12 ? w[2] : w[3];
+    if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[j] = word;
+    else reinterpret_cast<uint16_t*>(p)[j] = (uint16_t)(word >> (j & 1) * 16);
+  }
 }
 template <int E> __device__ __forceinline__ void to_shared(float* p, const float (&f)[E]) {
 #pragma unroll
@@ -91,20 +116,37 @@ template <int S> __device__ __forceinline__ void ld_dup(const float* p, f32x2 (&
     v[i] = u.x; v[i + 1] = u.y;
   }
 }
+// What a token brings to a thread.  The loops ask for a token's operands one token ahead, for its step two ahead, and have the next token's decays
+// computed while this one's are used, so that neither shared memory nor the exps are waited for.
+template <int S, bool E, bool Cs> struct Token {
+  f32x2 x, e, B[S], C[S];
+  __device__ __forceinline__ void get(const float* dx, const float* ep, const float* b, const float* c) {
+    x = ld2(dx);
+    if constexpr (E) e = ld2(ep);
+    ld_dup<S>(b, B);
+    if constexpr (Cs) ld_dup<S>(c, C);
+  }
+};
+template <int S> __device__ __forceinline__ void decays(f32x2 dt, const f32x2 (&A)[S], f32x2 (&d)[S]) {
+#pragma unroll
+  for (int i = 0; i < S; ++i) d[i] = ex2_pair(f2_mul(dt, A[i]));
+}
 // The sum over the lanes of a channel's states of (v, w), a pair of channels each: lane bit 0 ends with the channel, bit 1 with v or w.
-__device__ __forceinline__ float sum_states(f32x2 v, f32x2 w, int lane) {
+template <int QL> __device__ __forceinline__ float sum_states(f32x2 v, f32x2 w, int lane) {
   float v0, v1, w0, w1;
   f2_unpack(v, v0, v1);
   f2_unpack(w, w0, w1);
   const bool hi = lane & 1, sec = lane & 2;
   const float p = (hi ? v1 : v0) + __shfl_xor_sync(~0u, hi ? v0 : v1, 1);
   const float q = (hi ? w1 : w0) + __shfl_xor_sync(~0u, hi ? w0 : w1, 1);
-  return (sec ? q : p) + __shfl_xor_sync(~0u, sec ? p : q, 2);
+  float r = (sec ? q : p) + __shfl_xor_sync(~0u, sec ? p : q, 2);
+  if constexpr (QL == 8) r += __shfl_xor_sync(~0u, r, 4);               // two lanes have the same sum
+  return r;
 }
 
 // Where a block works: blocks of one sequence and segment lie side by side, as they read the same b and c
 struct Place { int b, seg, g, tile, c0, valid, ch0; };
-__device__ __forceinline__ Place place_of(const Args& a) {
+template <int CT> __device__ __forceinline__ Place place_of(const Args& a) {
   Place p;
   unsigned i = blockIdx.x;
   p.tile = i % a.tiles; i /= a.tiles;
@@ -123,8 +165,8 @@ __device__ __forceinline__ int text_length(const Args& a, int b) {
 }
 
 // b and c of a tile, as pairs of equal numbers in shared memory
-template <typename T, int S, int TT> struct Coeffs {
-  static constexpr int NP = QL * S, PER = TT * NP / THREADS;
+template <typename T, int NP> struct Coeffs {
+  static constexpr int PER = TT * NP / THREADS;
   float v[PER];
   __device__ __forceinline__ void fetch(const Group& r, const Place& p, int t0, int n, int states) {
     const T* base = static_cast<const T*>(r.p) + p.b * r.sb + p.g * r.sg;
@@ -140,37 +182,56 @@ template <typename T, int S, int TT> struct Coeffs {
   }
 };
 
-template <typename T, int TT> struct Pieces {                           // a thread's part of a tile of x, delta, z or a gradient
+template <typename T, int CT> struct Pieces {                           // a thread's part of a tile of x, delta, z or a gradient
   static constexpr int E = Piece<T>::N, PPR = CT / E, ROWS = THREADS / PPR, P = TT / ROWS;
   uint4 v[P];
   __device__ __forceinline__ void fetch(const Rows& r, const Place& p, int t0, int n) {
     const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
+    const T* at = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col + (t0 + row) * r.st;
+    if (r.vec && p.valid == CT && t0 + TT <= n) {                        // for the whole block alike
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(at + i * ROWS * r.st));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < P; ++i) {
+        const uint4 u = t0 + row + i * ROWS < n ? load_piece<T>(at + i * ROWS * r.st, p.valid - col, r.vec) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (j == i) v[j] = u;
+      }
+    }
+  }
+  // into L2, so that fetch() waits less
+  static __device__ __forceinline__ void ask(const Rows& r, const Place& p, int t0, int n) {
+    const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
+    if (threadIdx.x % (PPR < 8 ? PPR : 8) || col >= p.valid) return;        // a line of 128 bytes each
     const T* base = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int t = t0 + row + i * ROWS;
-      v[i] = t < n ? load_piece<T>(base + t * r.st, p.valid - col, r.vec) : make_uint4(0, 0, 0, 0);
+      if (t >= 0 && t < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + t * r.st));
     }
   }
 };
 
 // A segment's part of y, or (SUMS) its own contribution to the state and the sum of its steps.
-template <typename T, int S, bool SUMS>
-__global__ void __launch_bounds__(THREADS, S == 4 ? 4 : 2)
+template <typename T, int S, int QL, bool SUMS>
+__global__ void __launch_bounds__(THREADS, S == 4 ? 3 : 2)
 scan_kernel(const Args a) {
-  constexpr int TT = tile_of(S), NP = QL * S;
-  using Px = Pieces<T, TT>;
+  constexpr int NP = QL * S, CT = channels_of(QL);
+  using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
-  __shared__ __align__(16) float s_dt[TT][CT], s_dx[TT][CT], s_y[TT][CT], s_b[TT][2 * NP], s_c[TT][2 * NP], s_bias[CT], s_skip[CT];
+  // two rows and one more than a tile has: what the loop asks for ahead of its end
+  __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_y[TT][CT], s_b[TT + 1][2 * NP], s_c[TT + 1][2 * NP], s_bias[CT], s_skip[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of(a);
+  const Place p = place_of<CT>(a);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) {
     s_bias[tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
     s_skip[tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
   }
-  const int cl = warp * 16 + (lane >> 2) * 2, q0 = (lane & 3) * S;      // the thread's two channels and S states
+  const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;      // the thread's two channels and S states
   f32x2 h[S], A[S];
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
 #pragma unroll
@@ -195,7 +256,7 @@ scan_kernel(const Args a) {
   const int col = tid % Px::PPR * E, row = tid / Px::PPR;
   T* y = static_cast<T*>(a.y) + (long long)p.b * a.len * a.dim + p.ch0 + col;
   Px x, delta, z;
-  Coeffs<T, S, TT> fb, fc;
+  Coeffs<T, NP> fb, fc;
   auto fetch = [&](int k) {
     x.fetch(a.x, p, k * TT, n);
     delta.fetch(a.delta, p, k * TT, n);
@@ -205,10 +266,13 @@ scan_kernel(const Args a) {
       fc.fetch(a.c, p, k * TT, n, a.states);
     }
   };
-  float steps[2] = {0.f, 0.f};
-  if (first < used) fetch(first);
+  f32x2 steps = 0;
   __syncthreads();
   for (int k = first; k < used; ++k) {
+    fetch(k);
+    f32x2 h0[S], own[S], cum = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) { h0[i] = h[i]; own[i] = 0; }
     if (!SUMS && a.saves) {              // the state in front of the tile, for the gradient
       float* to = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
 #pragma unroll
@@ -221,7 +285,6 @@ scan_kernel(const Args a) {
           if (cl + j < p.valid) *reinterpret_cast<float4*>(to + j * NP + i) = make_float4(f[j][0], f[j][1], f[j][2], f[j][3]);
       }
     }
-    Px x_now = x, z_now = z;
     {
       float bias[E];
       from_shared(s_bias + col, bias);
@@ -244,31 +307,55 @@ scan_kernel(const Args a) {
     fb.put(&s_b[0][0]);
     if constexpr (!SUMS) fc.put(&s_c[0][0]);
     __syncthreads();
-    if (k + 1 < used) fetch(k + 1);
-#pragma unroll 2
-    for (int t = 0; t < TT; t += 2) {
-      f32x2 sum[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const f32x2 dt = ld2(&s_dt[t + u][cl]), dx = ld2(&s_dx[t + u][cl]);
-        f32x2 B[S], C[S];
-        ld_dup<S>(&s_b[t + u][2 * q0], B);
-        if constexpr (!SUMS) ld_dup<S>(&s_c[t + u][2 * q0], C);
-        sum[u] = 0;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          h[i] = f2_fma(ex2_pair(f2_mul(dt, A[i])), h[i], f2_mul(dx, B[i]));
-          if constexpr (!SUMS) sum[u] = f2_fma(h[i], C[i], sum[u]);
-        }
-        if constexpr (SUMS) {
-          float d0, d1;
-          f2_unpack(dt, d0, d1);
-          steps[0] += d0;
-          steps[1] += d1;
-        }
-      }
-      if constexpr (!SUMS) s_y[t + ((lane >> 1) & 1)][cl + (lane & 1)] = sum_states(sum[0], sum[1], lane);
+    if (k + 1 < used) {
+      Px::ask(a.x, p, (k + 1) * TT, n);
+      Px::ask(a.delta, p, (k + 1) * TT, n);
+      if (!SUMS && a.z.p) Px::ask(a.z, p, (k + 1) * TT, n);
     }
+    {
+      constexpr int U = 4;
+      Token<S, false, !SUMS> next;
+      const float *p_dt = &s_dt[0][cl], *p_dx = &s_dx[0][cl], *p_b = &s_b[0][2 * q0], *p_c = &s_c[0][2 * q0];
+      float* p_y = &s_y[(lane >> 1) & 1][cl + (lane & 1)];
+      f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[S];
+      next.get(p_dx, nullptr, p_b, p_c);
+      decays<S>(dt, A, d_next);
+#pragma unroll 1
+      for (int t0 = 0; t0 < TT; t0 += U) {
+        f32x2 sum[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const Token<S, false, !SUMS> now = next;
+          f32x2 d[S];
+#pragma unroll
+          for (int i = 0; i < S; ++i) d[i] = d_next[i];
+          next.get(p_dx + (u + 1) * CT, nullptr, p_b + (u + 1) * 2 * NP, p_c + (u + 1) * 2 * NP);
+          cum = f2_add(cum, dt);
+          dt = dt_next;
+          dt_next = ld2(p_dt + (u + 2) * CT);
+          decays<S>(dt, A, d_next);
+          sum[u] = 0;
+#pragma unroll
+          for (int i = 0; i < S; ++i) {
+            const f32x2 fed = f2_mul(now.x, now.B[i]);
+            own[i] = f2_fma(d[i], own[i], fed);
+            if constexpr (!SUMS) {
+              h[i] = f2_fma(d[i], h[i], fed);
+              sum[u] = f2_fma(h[i], now.C[i], sum[u]);
+            }
+          }
+        }
+        if constexpr (!SUMS) {
+#pragma unroll
+          for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(sum[u], sum[u + 1], lane);
+        }
+        p_dt += U * CT; p_dx += U * CT; p_b += U * 2 * NP; p_c += U * 2 * NP; p_y += U * CT;
+      }
+    }
+    // the carried state meets the tile's decays in one product, so that its error grows with the tiles, not with the tokens
+#pragma unroll
+    for (int i = 0; i < S; ++i) h[i] = f2_fma(ex2_pair(f2_mul(cum, A[i])), h0[i], own[i]);
+    steps = f2_add(steps, cum);
     __syncthreads();
     if constexpr (!SUMS) {
       float skip[E];
@@ -279,11 +366,11 @@ scan_kernel(const Args a) {
         if (t >= a.len) continue;
         float f[E], u[E];
         from_shared(&s_y[row + i * Px::ROWS][col], f);
-        Piece<T>::get(x_now.v[i], u);
+        Piece<T>::get(x.v[i], u);
 #pragma unroll
         for (int j = 0; j < E; ++j) f[j] = fmaf(skip[j], u[j], f[j]);
         if (a.z.p) {
-          Piece<T>::get(z_now.v[i], u);
+          Piece<T>::get(z.v[i], u);
 #pragma unroll
           for (int j = 0; j < E; ++j) f[j] *= u[j] * sigmoid(u[j]);
         }
@@ -304,9 +391,11 @@ scan_kernel(const Args a) {
       for (int j = 0; j < 2; ++j)
         if (cl + j < p.valid) a.seg_state[(row_n + cl + j) * NP + q0 + i] = f[j];
     }
+    float f[2];
+    f2_unpack(steps, f[0], f[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if ((lane & 3) == 0 && cl + j < p.valid) a.seg_steps[row_n + cl + j] = steps[j];
+      if (lane % QL == 0 && cl + j < p.valid) a.seg_steps[row_n + cl + j] = f[j];
   } else {
     for (int t = max(used, first) * TT + row; t < min(last * TT, a.len); t += Px::ROWS) {      // behind the text
       const float f[E] = {};
@@ -345,19 +434,19 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
 }
 
 // The contribution of a segment's outputs to the gradient of the state in front of it, and the sum of its steps.
-template <typename T, int S>
+template <typename T, int S, int QL>
 __global__ void __launch_bounds__(THREADS, S == 4 ? 4 : 2)
 back_sums_kernel(const Args a, const Grads g) {
-  constexpr int TT = tile_of(S), NP = QL * S;
-  using Px = Pieces<T, TT>;
+  constexpr int NP = QL * S, CT = channels_of(QL);
+  using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
   __shared__ __align__(16) float s_dt[TT][CT], s_e[TT][CT], s_c[TT][2 * NP], s_bias[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of(a);
+  const Place p = place_of<CT>(a);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) s_bias[tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
-  const int cl = warp * 16 + (lane >> 2) * 2, q0 = (lane & 3) * S;
+  const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
   f32x2 G[S], A[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) {
@@ -372,7 +461,7 @@ back_sums_kernel(const Args a, const Grads g) {
   const int used = min(min(first + a.seg_tiles, total), (n + TT - 1) / TT);
   const int col = tid % Px::PPR * E, row = tid / Px::PPR;
   Px delta, dy, z;
-  Coeffs<T, S, TT> fc;
+  Coeffs<T, NP> fc;
   float steps[2] = {0.f, 0.f};
   __syncthreads();
   for (int k = used - 1; k >= first; --k) {
@@ -427,38 +516,53 @@ back_sums_kernel(const Args a, const Grads g) {
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if ((lane & 3) == 0 && cl + j < p.valid) a.seg_steps[row_n + cl + j] = steps[j];
+    if (lane % QL == 0 && cl + j < p.valid) a.seg_steps[row_n + cl + j] = steps[j];
 }
 
-template <int TT, int NP> struct BackShared {
-  float dt[TT][CT], dx[TT][CT], e[TT][CT], y[TT][CT], q[TT][CT], gb[TT][CT];
-  float b[TT][2 * NP], c[TT][2 * NP];
-  float db[4][TT][NP], dc[4][TT][NP];    // of each warp's channels
-  float bias[CT], skip[CT];
+template <int S, int QL> struct BackShared {
+  static constexpr int NP = QL * S, CT = channels_of(QL), U = 4, STEP = 32 / QL * NP + 16;      // STEP: steps side by side meet other banks
+  // the loops ask for two tokens more than the tile has: at either end there is other memory of this struct, which is not used
+  float bias[2][CT];
+  float dt[TT][CT], dx[TT][CT], e[TT][CT], y[TT][CT], q[TT][CT];       // dx becomes gb
+  float before[2 * NP], b[TT][2 * NP], c[TT][2 * NP];
+  float part[4][TT][NP];                 // db or dc of each warp's channels
+  float mid[4][U * STEP];                // four steps of each pair of channels
+  float da[S][THREADS][2];               // each thread's sums over the tiles
 };
 
-// Sums over a warp's channels of S values in each of two steps (pairs of channels), into out[state] of the steps.
-template <int S> __device__ __forceinline__ void sum_channels(const f32x2 (&v)[S], const f32x2 (&w)[S], int lane, float* to_v, float* to_w) {
-  float f[2 * S];
+// Four steps' values of a warp's pairs of channels are added up through shared memory: half the instructions of shuffles
+template <int S, int QL> __device__ __forceinline__ void put_channels(float* mid, const f32x2 (&v)[S], int lane) {
+  constexpr int NP = QL * S;
+  float* to = mid + lane / QL * NP + lane % QL * S;
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float x, y;
-    f2_unpack(v[i], x, y);
-    f[i] = x + y;
-    f2_unpack(w[i], x, y);
-    f[S + i] = x + y;
+  for (int i = 0; i < S; i += 4) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x, y;
+      f2_unpack(v[i + j], x, y);
+      f[j] = x + y;
+    }
+    *reinterpret_cast<float4*>(to + i) = make_float4(f[0], f[1], f[2], f[3]);
   }
-  constexpr int H = S;                   // of 2 S values half stay, a quarter, an eighth
-  const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
+}
+template <int S, int QL> __device__ __forceinline__ void sum_channels(const float* mid, float* to, int lane) {    // to: four rows of NP
+  constexpr int NP = QL * S, STEP = BackShared<S, QL>::STEP, C = 32 / QL;
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < H; ++i) f[i] = (b4 ? f[H + i] : f[i]) + __shfl_xor_sync(~0u, b4 ? f[i] : f[H + i], 16);
+  for (int j = 0; j < NP / 16; ++j) {
+    const int id = lane + 32 * j, u = id / (NP / 2), at = id % (NP / 2) * 2;
+    const float* from = mid + u * STEP + at;
+    f32x2 v[C];
 #pragma unroll
-  for (int i = 0; i < H / 2; ++i) f[i] = (b3 ? f[H / 2 + i] : f[i]) + __shfl_xor_sync(~0u, b3 ? f[i] : f[H / 2 + i], 8);
+    for (int c = 0; c < C; ++c) v[c] = ld2(from + c * NP);
 #pragma unroll
-  for (int i = 0; i < H / 4; ++i) f[i] = (b2 ? f[H / 4 + i] : f[i]) + __shfl_xor_sync(~0u, b2 ? f[i] : f[H / 4 + i], 4);
-  float* to = (b4 ? to_w : to_v) + (lane & 3) * S + (b3 ? S / 2 : 0) + (b2 ? S / 4 : 0);
+    for (int w = C / 2; w > 0; w /= 2)
 #pragma unroll
-  for (int i = 0; i < H / 4; ++i) to[i] = f[i];
+      for (int c = 0; c < w; ++c) v[c] = f2_add(v[c], v[c + w]);
+    *reinterpret_cast<f32x2*>(to + u * NP + at) = v[0];
+  }
+  __syncwarp();
 }
 
 // Gradients, a tile at a time from the last to the first.  With v_t = h_t c_t, e_t the gradient of sum c h, g_t that of h_t:
@@ -468,25 +572,25 @@ template <int S> __device__ __forceinline__ void sum_channels(const f32x2 (&v)[S
 // a tile sum_n a w_t is a sum of scalars of a channel from its end, where h and g are both at hand:
 //   sum_n a w_t = sum_n a g h (end) + sum_{r >= t} (q_r e_r - p_r s x),       da = sum_t s_t w_t = g h S + sum_r S_r (v_r e_r - g_r b_r s x)
 // with S_r the sum of the tile's steps up to r.
-template <typename T, int S>
-__global__ void __launch_bounds__(THREADS, S == 4 ? 3 : S == 8 ? 2 : 1)
+template <typename T, int S, int QL>
+__global__ void __launch_bounds__(THREADS, S == 4 && sizeof(T) == 2 ? 3 : 2)
 back_kernel(const Args a, const Grads g) {
-  constexpr int TT = tile_of(S), NP = QL * S;
-  using Px = Pieces<T, TT>;
+  constexpr int NP = QL * S, CT = channels_of(QL);
+  using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
   extern __shared__ __align__(16) unsigned char raw[];
-  BackShared<TT, NP>& sh = *reinterpret_cast<BackShared<TT, NP>*>(raw);
+  BackShared<S, QL>& sh = *reinterpret_cast<BackShared<S, QL>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of(a);
+  const Place p = place_of<CT>(a);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) {
-    sh.bias[tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
-    sh.skip[tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
+    sh.bias[0][tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
+    sh.bias[1][tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
   }
-  const int cl = warp * 16 + (lane >> 2) * 2, q0 = (lane & 3) * S;
+  const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
-  f32x2 G[S], A[S], dA[S];
+  f32x2 G[S], A[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) {
     float v[2], w[2];
@@ -501,7 +605,7 @@ back_kernel(const Args a, const Grads g) {
     }
     A[i] = f2_pack(v[0], v[1]);
     G[i] = f2_pack(w[0], w[1]);
-    dA[i] = 0;
+    *reinterpret_cast<f32x2*>(sh.da[i][tid]) = 0;
   }
   const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
   const int used = min(last, (n + TT - 1) / TT);
@@ -518,7 +622,7 @@ back_kernel(const Args a, const Grads g) {
     if (g.dz) store_piece<T>(dz + (long long)t * a.dim, f, p.valid - col, g.vec);
   }
   Px x, delta, z, dy;
-  Coeffs<T, S, TT> fb, fc;
+  Coeffs<T, NP> fb, fc;
   auto fetch = [&](int k) {
     x.fetch(a.x, p, k * TT, n);
     delta.fetch(a.delta, p, k * TT, n);
@@ -530,20 +634,21 @@ back_kernel(const Args a, const Grads g) {
   __syncthreads();
   for (int k = used - 1; k >= first; --k) {
     fetch(k);
-    f32x2 h[S];
-    {
-      const float* from = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
+    const float* saved = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
+    auto in_front = [&](f32x2 (&h)[S]) {
 #pragma unroll
       for (int i = 0; i < S; i += 4) {
         float4 f[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = cl + j < p.valid ? *reinterpret_cast<const float4*>(from + j * NP + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < 2; ++j) f[j] = cl + j < p.valid ? __ldg(reinterpret_cast<const float4*>(saved + j * NP + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
         h[i] = f2_pack(f[0].x, f[1].x); h[i + 1] = f2_pack(f[0].y, f[1].y); h[i + 2] = f2_pack(f[0].z, f[1].z); h[i + 3] = f2_pack(f[0].w, f[1].w);
       }
-    }
+    };
+    f32x2 h[S], dA[S];
+    in_front(h);
     {
       float bias[E];
-      from_shared(sh.bias + col, bias);
+      from_shared(sh.bias[0] + col, bias);
 #pragma unroll
       for (int i = 0; i < Px::P; ++i) {
         const int t = row + i * Px::ROWS;
@@ -572,88 +677,172 @@ back_kernel(const Args a, const Grads g) {
     fc.put(&sh.c[0][0]);
     __syncthreads();
     const int own_row = (lane >> 1) & 1, own_ch = cl + (lane & 1);
-    f32x2 cum = 0;
-    for (int t = 0; t < TT; t += 2) {
-      f32x2 U[2][S];
+    if (k > first) {
+      Px::ask(a.x, p, (k - 1) * TT, n);
+      Px::ask(a.delta, p, (k - 1) * TT, n);
+      Px::ask(g.dy, p, (k - 1) * TT, n);
+      if (a.z.p) Px::ask(a.z, p, (k - 1) * TT, n);
+    }
+    constexpr int U = BackShared<S, QL>::U, STEP = BackShared<S, QL>::STEP;
+    float* mid = sh.mid[warp];
+    f32x2 K[S];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const f32x2 dt = ld2(&sh.dt[t + u][cl]), xs = ld2(&sh.dx[t + u][cl]), e = ld2(&sh.e[t + u][cl]);
-        f32x2 B[S], C[S];
-        ld_dup<S>(&sh.b[t + u][2 * q0], B);
-        ld_dup<S>(&sh.c[t + u][2 * q0], C);
-        cum = f2_add(cum, dt);
-        const f32x2 ec = f2_mul(e, cum);
-        f32x2 y = 0, q = 0;
+    for (int i = 0; i < S; ++i) K[i] = dA[i] = 0;
+    float* to_yq = own_row ? &sh.q[0][own_ch] : &sh.y[0][own_ch];
+    {
+      Token<S, true, true> next;
+      const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][2 * q0], *p_c = &sh.c[0][2 * q0];
+      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt + CT), d_next[S];
+      next.get(p_dx, p_e, p_b, p_c);
+      decays<S>(dt_next, A, d_next);
+#pragma unroll 1
+      for (int t0 = 0; t0 < TT; t0 += U) {
+        f32x2 y[U], q[U];
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-          h[i] = f2_fma(ex2_pair(f2_mul(dt, A[i])), h[i], f2_mul(xs, B[i]));
-          U[u][i] = f2_mul(h[i], e);
-          const f32x2 v = f2_mul(h[i], C[i]);
-          y = f2_add(y, v);
-          q = f2_fma(v, A[i], q);
-          dA[i] = f2_fma(v, ec, dA[i]);
+        for (int u = 0; u < U; ++u) {
+          const Token<S, true, true> now = next;
+          const f32x2 dt = dt_next;
+          f32x2 d[S], hs[S];
+#pragma unroll
+          for (int i = 0; i < S; ++i) d[i] = d_next[i];
+          next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * 2 * NP, p_c + (u + 1) * 2 * NP);
+          dt_next = dt_far;
+          dt_far = ld2(p_dt + (u + 2) * CT);
+          decays<S>(dt_next, A, d_next);
+          y[u] = q[u] = 0;
+#pragma unroll
+          for (int i = 0; i < S; ++i) {
+            K[i] = f2_mul(d[i], f2_fma(dt, h[i], K[i]));
+            h[i] = f2_fma(d[i], h[i], f2_mul(now.x, now.B[i]));
+            hs[i] = f2_mul(h[i], now.e);
+            const f32x2 v = f2_mul(h[i], now.C[i]);
+            y[u] = f2_add(y[u], v);
+            q[u] = f2_fma(v, A[i], q[u]);
+            dA[i] = f2_fma(f2_mul(K[i], now.C[i]), now.e, dA[i]);
+          }
+          put_channels<S, QL>(mid + u * STEP, hs, lane);
         }
-        const float r = sum_states(y, q, lane);
-        (own_row ? sh.q : sh.y)[t + u][own_ch] = r;
-      }
-      sum_channels<S>(U[0], U[1], lane, sh.dc[warp][t], sh.dc[warp][t + 1]);
-    }
-    f32x2 end = 0;                       // sum a g h behind the tile's last token
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const f32x2 w = f2_mul(G[i], h[i]);
-      end = f2_fma(w, A[i], end);
-      dA[i] = f2_fma(w, cum, dA[i]);
-    }
-    const float w_end = sum_states(end, 0, lane);          // lanes with bit 1 clear
-    for (int t = TT - 2; t >= 0; t -= 2) {
-      f32x2 U[2][S];
-#pragma unroll
-      for (int u = 1; u >= 0; --u) {
-        const f32x2 dt = ld2(&sh.dt[t + u][cl]), xs = ld2(&sh.dx[t + u][cl]), e = ld2(&sh.e[t + u][cl]);
-        f32x2 B[S], C[S];
-        ld_dup<S>(&sh.b[t + u][2 * q0], B);
-        ld_dup<S>(&sh.c[t + u][2 * q0], C);
-        const f32x2 xc = f2_mul(f2_mul(xs, cum), f2_splat(-1.f));
-        cum = f2_fma(dt, f2_splat(-1.f), cum);
-        f32x2 gb = 0, q = 0;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          G[i] = f2_fma(e, C[i], G[i]);
-          U[u][i] = f2_mul(G[i], xs);
-          const f32x2 v = f2_mul(G[i], B[i]);
-          gb = f2_add(gb, v);
-          q = f2_fma(v, A[i], q);
-          dA[i] = f2_fma(v, xc, dA[i]);
-          G[i] = f2_mul(ex2_pair(f2_mul(dt, A[i])), G[i]);
-        }
-        const float r = sum_states(gb, q, lane);
-        if (own_row) sh.q[t + u][own_ch] = sh.q[t + u][own_ch] * sh.e[t + u][own_ch] - r * sh.dx[t + u][own_ch];
-        else sh.gb[t + u][own_ch] = r;
-      }
-      sum_channels<S>(U[0], U[1], lane, sh.db[warp][t], sh.db[warp][t + 1]);
-    }
-    __syncwarp();
-    if (own_row == 0 && (lane & 3) == (lane & 1)) {        // a channel's sums from the tile's end
-      float w = w_end;
-      for (int t = TT - 1; t >= 0; --t) {
-        w += sh.q[t][own_ch];
-        sh.q[t][own_ch] = w * LN2;
+        for (int u = 0; u < U; ++u) to_yq[u * CT] = sum_states<QL>(y[u], q[u], lane);
+        sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
+        to_yq += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * 2 * NP; p_c += U * 2 * NP;
       }
     }
     __syncthreads();
-    for (int i = tid; i < TT * NP; i += THREADS) {
-      const int t = k * TT + i / NP;
-      if (t < n) {
-        const long long at = ((((long long)p.tile * a.batch + p.b) * a.len + t) * a.groups + p.g) * NP + i % NP;
-        g.part_b[at] = (&sh.db[0][0][0])[i] + (&sh.db[1][0][0])[i] + (&sh.db[2][0][0])[i] + (&sh.db[3][0][0])[i];
-        g.part_c[at] = (&sh.dc[0][0][0])[i] + (&sh.dc[1][0][0])[i] + (&sh.dc[2][0][0])[i] + (&sh.dc[3][0][0])[i];
+    auto parts_to = [&](float* out) {
+      const long long row = (long long)a.groups * NP;
+      out += (((long long)p.tile * a.batch + p.b) * a.len + k * TT) * row + p.g * NP + tid % NP;
+#pragma unroll
+      for (int j = 0; j < TT * NP / THREADS; ++j) {
+        const int i = tid + j * THREADS;
+        if (k * TT + i / NP < n)
+          out[i / NP * row] = ((&sh.part[0][0][0])[i] + (&sh.part[1][0][0])[i]) + ((&sh.part[2][0][0])[i] + (&sh.part[3][0][0])[i]);
+      }
+    };
+    parts_to(g.part_c);
+    f32x2 end = 0;                       // sum a g h behind the tile's last token
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      end = f2_fma(f2_mul(G[i], h[i]), A[i], end);
+      f32x2* sum = reinterpret_cast<f32x2*>(sh.da[i][tid]);
+      *sum = f2_add(*sum, f2_fma(G[i], K[i], dA[i]));      // a tile's own sum first: 2048 tokens one by one lose half a digit
+    }
+    __syncthreads();
+    f32x2 G0[S], own[S], cum = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) { G0[i] = G[i]; own[i] = 0; }
+    {
+      Token<S, true, true> next;
+      constexpr int LAST = (TT - 1) * CT, LAST_N = (TT - 1) * 2 * NP;
+      float* to_gq = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
+      const float *p_dt = &sh.dt[0][cl] + LAST, *p_dx = &sh.dx[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][2 * q0] + LAST_N, *p_c = &sh.c[0][2 * q0] + LAST_N;
+      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt - CT), d_next[S];
+      next.get(p_dx, p_e, p_b, p_c);
+      decays<S>(dt_next, A, d_next);
+#pragma unroll 1
+      for (int t0 = TT - U; t0 >= 0; t0 -= U) {
+        f32x2 gb[U], q[U];
+        float q_h[U], xs[U], es[U];
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+          const int u = U - 1 - r;
+          const Token<S, true, true> now = next;
+          f32x2 d[S], gs[S];
+#pragma unroll
+          for (int i = 0; i < S; ++i) d[i] = d_next[i];
+          cum = f2_add(cum, dt_next);
+          next.get(p_dx - (r + 1) * CT, p_e - (r + 1) * CT, p_b - (r + 1) * 2 * NP, p_c - (r + 1) * 2 * NP);
+          dt_next = dt_far;
+          dt_far = ld2(p_dt - (r + 2) * CT);
+          q_h[u] = to_gq[-r * CT];
+          decays<S>(dt_next, A, d_next);
+          gb[u] = q[u] = 0;
+#pragma unroll
+          for (int i = 0; i < S; ++i) {
+            const f32x2 fed = f2_fma(now.e, now.C[i], G[i]);
+            own[i] = f2_mul(d[i], f2_fma(now.e, now.C[i], own[i]));
+            gs[i] = f2_mul(fed, now.x);
+            const f32x2 v = f2_mul(fed, now.B[i]);
+            gb[u] = f2_add(gb[u], v);
+            q[u] = f2_fma(v, A[i], q[u]);
+            G[i] = f2_mul(d[i], fed);
+          }
+          put_channels<S, QL>(mid + u * STEP, gs, lane);
+          float v0, v1;
+          f2_unpack(now.x, v0, v1);
+          xs[u] = lane & 1 ? v1 : v0;
+          f2_unpack(now.e, v0, v1);
+          es[u] = lane & 1 ? v1 : v0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float r = sum_states<QL>(gb[u], q[u], lane);
+          to_gq[(u - (U - 1)) * CT] = own_row ? fmaf(q_h[u], es[u], -r * xs[u]) : r;
+        }
+        sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
+        to_gq -= U * CT;
+        p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * 2 * NP; p_c -= U * 2 * NP;
       }
     }
+    // as in the forward pass: the carried gradient meets the tile's decays once
+#pragma unroll
+    for (int i = 0; i < S; ++i) G[i] = f2_fma(ex2_pair(f2_mul(cum, A[i])), G0[i], own[i]);
+    // a channel's sums, the second half of the tile from its end, the first from its start, where g and h are known too: rounding errors of the
+    // q_r e_r and p_r s x, which all later sums share, have half the way to pile up
+    in_front(h);
+    f32x2 start = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) start = f2_fma(f2_mul(G[i], h[i]), A[i], start);
+    float w = sum_states<QL>(start, end, lane);                // lanes with bit 1: the tile's second half
+    __syncwarp();
+    if (lane % QL >= 4) {
+      // its sums are another lane's too
+    } else if (own_row) {
+#pragma unroll 4
+      for (int t = TT - 1; t >= TT / 2; --t) {
+        w += sh.q[t][own_ch];
+        sh.q[t][own_ch] = w * LN2;
+      }
+    } else {
+#pragma unroll 4
+      for (int t = 0; t < TT / 2; ++t) {
+        const float r = sh.q[t][own_ch];
+        sh.q[t][own_ch] = w * LN2;
+        w -= r;
+      }
+    }
+    __syncthreads();
+    parts_to(g.part_b);
     {
+      x.fetch(a.x, p, k * TT, n);        // again: they would fill 32 registers meanwhile
+      delta.fetch(a.delta, p, k * TT, n);
+      if (a.z.p) {
+        dy.fetch(g.dy, p, k * TT, n);
+        z.fetch(a.z, p, k * TT, n);
+      }
       float bias[E], skip[E];
-      from_shared(sh.bias + col, bias);
-      from_shared(sh.skip + col, skip);
+      from_shared(sh.bias[0] + col, bias);
+      from_shared(sh.bias[1] + col, skip);
 #pragma unroll
       for (int i = 0; i < Px::P; ++i) {
         const int r = row + i * Px::ROWS, t = k * TT + r;
@@ -674,7 +863,7 @@ back_kernel(const Args a, const Grads g) {
           }
           store_piece<T>(dz + (long long)t * a.dim, o, p.valid - col, g.vec);
         }
-        from_shared(&sh.gb[r][col], gb);
+        from_shared(&sh.dx[r][col], gb);
         from_shared(&sh.dt[r][col], f);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
@@ -699,22 +888,22 @@ back_kernel(const Args a, const Grads g) {
   }
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    float f[2], w[2];
-    f2_unpack(dA[i], f[0], f[1]);
+    float w[2];
     f2_unpack(G[i], w[0], w[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (cl + j < p.valid) {
-        g.part_a[(row_n + cl + j) * NP + q0 + i] = f[j];
+        g.part_a[(row_n + cl + j) * NP + q0 + i] = sh.da[i][tid][j];
         if (g.d_state_in && p.seg == 0 && q0 + i < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + j) * a.states + q0 + i] = w[j];
       }
     }
   }
   float* sums = &sh.dt[0][0];            // [2][ROWS][CT]
-  static_assert(2 * Px::ROWS <= 6 * TT, "sums of the parameters");
+  static_assert(2 * Px::ROWS <= 5 * TT, "sums of the parameters");
   to_shared(sums + row * CT + col, d_skip);
   to_shared(sums + (Px::ROWS + row) * CT + col, d_bias);
   __syncthreads();
+  if (tid >= 2 * CT) return;
   const int c = tid % CT, which = tid / CT;
   float v = 0.f;
   for (int r = 0; r < Px::ROWS; ++r) v += sums[(which * Px::ROWS + r) * CT + c];
@@ -815,19 +1004,16 @@ step_kernel(const StepArgs a) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-static int per_lane(int states) { return states <= 16 ? 4 : states <= 32 ? 8 : 16; }
-
-struct Plan { int per_lane, np, tile, total, tiles, per_group, segs, seg_tiles; };
+struct Plan { int np, total, tiles, per_group, segs, seg_tiles; };
 // The axis is cut into segments where sequences and channels alone leave SMs without two blocks: what a segment adds to the state is then computed
 // first, at the price of a second exp for each token, channel and state.
 static Plan plan_of(int batch, int len, int dim, int states, int groups) {
   Plan p;
-  p.per_lane = per_lane(states);
-  p.np = QL * p.per_lane;
-  p.tile = tile_of(p.per_lane);
-  p.total = (len + p.tile - 1) / p.tile;
+  p.np = states <= 16 ? 16 : states <= 32 ? 32 : 64;
+  p.total = (len + TT - 1) / TT;
   p.per_group = dim / groups;
-  p.tiles = (p.per_group + CT - 1) / CT;
+  const int ct = channels_of(p.np == 64 ? 8 : 4);
+  p.tiles = (p.per_group + ct - 1) / ct;
   const long long blocks = (long long)batch * groups * p.tiles, want = 4LL * m2_sm_count();
   p.segs = 1;
   if (blocks < m2_sm_count() && p.total >= 8) {
@@ -846,28 +1032,28 @@ static long long grad_floats(const Plan& p, int batch, int len, int dim, int gro
   return seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
 }
 
-template <typename T, int S> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
+template <typename T, int S, int QL> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
   const long long blocks = (long long)a.batch * p.segs * a.groups * p.tiles, size = (long long)a.batch * a.len * a.dim;
   if (p.segs > 1) {
-    if (int rc = m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, true>, dim3((unsigned)blocks), THREADS, 0, st, a)) return rc;
+    if (int rc = m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, true>, dim3((unsigned)blocks), THREADS, 0, st, a)) return rc;
     const long long n = (long long)a.batch * a.dim * p.np;
     if (int rc = m2_launch("m2_selective_scan_fwd", size, join_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, a.a, a.seg_state, a.seg_steps,
                            a.state_in, a.batch, p.segs, a.dim, a.states, p.np, 0)) return rc;
   }
-  return m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, false>, dim3((unsigned)blocks), THREADS, 0, st, a);
+  return m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, false>, dim3((unsigned)blocks), THREADS, 0, st, a);
 }
 
-template <typename T, int S> static int backward(const Args& a, const Grads& g, const Plan& p, cudaStream_t st) {
+template <typename T, int S, int QL> static int backward(const Args& a, const Grads& g, const Plan& p, cudaStream_t st) {
   const long long blocks = (long long)a.batch * p.segs * a.groups * p.tiles, size = (long long)a.batch * a.len * a.dim;
   if (p.segs > 1) {
-    if (int rc = m2_launch("m2_selective_scan_bwd", size, back_sums_kernel<T, S>, dim3((unsigned)blocks), THREADS, 0, st, a, g)) return rc;
+    if (int rc = m2_launch("m2_selective_scan_bwd", size, back_sums_kernel<T, S, QL>, dim3((unsigned)blocks), THREADS, 0, st, a, g)) return rc;
     const long long n = (long long)a.batch * a.dim * p.np;
     if (int rc = m2_launch("m2_selective_scan_bwd", size, join_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, a.a, a.seg_state, a.seg_steps,
                            g.d_state_out, a.batch, p.segs, a.dim, a.states, p.np, 1)) return rc;
   }
-  constexpr size_t smem = sizeof(BackShared<tile_of(S), QL * S>);
-  M2_SMEM_ONCE((back_kernel<T, S>), smem);
-  if (int rc = m2_launch("m2_selective_scan_bwd", size, back_kernel<T, S>, dim3((unsigned)blocks), THREADS, smem, st, a, g)) return rc;
+  constexpr size_t smem = sizeof(BackShared<S, QL>);
+  M2_SMEM_ONCE((back_kernel<T, S, QL>), smem);
+  if (int rc = m2_launch("m2_selective_scan_bwd", size, back_kernel<T, S, QL>, dim3((unsigned)blocks), THREADS, smem, st, a, g)) return rc;
   const long long bc = ((long long)a.batch * a.len * a.groups * a.states + 255) / 256, par = ((long long)a.dim * (a.states + 2) + 255) / 256;
   return m2_launch("m2_selective_scan_bwd", size, finish_kernel<T>, dim3((unsigned)(bc + par)), 256, 0, st, a, g, p.np, (unsigned)bc);
 }
@@ -916,15 +1102,14 @@ extern "C" long long m2_selective_scan_saves(int batch, int seq_len, int dim, in
 
 extern "C" long long m2_selective_scan_workspace(int batch, int seq_len, int dim, int states, int groups, int backward) {
   using namespace m2::ss;
-  if (batch <= 0 || seq_len <= 0 || dim <= 0 || states <= 0 || states > MAX_STATES || groups <= 0 || dim % groups) return 0;
+  if (batch <= 0 || seq_len < 0 || dim <= 0 || states <= 0 || states > MAX_STATES || groups <= 0 || dim % groups) return 0;
   const Plan p = plan_of(batch, seq_len, dim, states, groups);
   return 4 * (backward ? grad_floats(p, batch, seq_len, dim, groups) : seg_floats(p, batch, dim));
 }
 
-#define M2_SS_DISPATCH(fn, ...)                                                                                           \
-  (g.dtype == M2_F32 ? (p.per_lane == 4 ? fn<float, 4>(__VA_ARGS__) : p.per_lane == 8 ? fn<float, 8>(__VA_ARGS__) : fn<float, 16>(__VA_ARGS__)) \
-                     : (p.per_lane == 4 ? fn<__nv_bfloat16, 4>(__VA_ARGS__) : p.per_lane == 8 ? fn<__nv_bfloat16, 8>(__VA_ARGS__)               \
-                                                                                     : fn<__nv_bfloat16, 16>(__VA_ARGS__)))
+#define M2_SS_DISPATCH(fn, ...)                                                                                            \
+  (g.dtype == M2_F32 ? (p.np == 16 ? fn<float, 4, 4>(__VA_ARGS__) : p.np == 32 ? fn<float, 8, 4>(__VA_ARGS__) : fn<float, 8, 8>(__VA_ARGS__)) \
+                     : (p.np == 16 ? fn<__nv_bfloat16, 4, 4>(__VA_ARGS__) : p.np == 32 ? fn<__nv_bfloat16, 8, 4>(__VA_ARGS__) : fn<__nv_bfloat16, 8, 8>(__VA_ARGS__)))
 
 extern "C" int m2_selective_scan_fwd(const m2_selective_scan_args* args, void* stream) {
   using namespace m2::ss;

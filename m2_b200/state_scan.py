@@ -131,7 +131,7 @@ def selective_scan(x, delta, a, b, c, *, skip=None, gate=None, delta_bias=None, 
 
     Steps, states and sums are float32, y is rounded once.  Two calls give the same bits; those of a text go by the batch it is in, as a long
     axis is cut where sequences and channels do not fill the GPU.  Differentiable in every tensor but lengths; for the gradient the state is kept
-    every 32 tokens (every 16 with more than 32 states) in float32."""
+    every 32 tokens in float32."""
     name = "selective_scan"
     b, c, a, skip, delta_bias = _check(name, x, delta, a, b, c, skip, gate, delta_bias, 3)
     B, L, D = x.shape
