@@ -109,33 +109,51 @@ __device__ __forceinline__ f32x2 ex2_pair(f32x2 v) {
   f2_unpack(v, x, y);
   return f2_pack(ex2(x), ex2(y));
 }
-template <int S> __device__ __forceinline__ void ld_dup(const float* p, f32x2 (&v)[S]) {      // pairs of equal numbers
+template <int H> __device__ __forceinline__ void ld_pairs(const float* p, f32x2 (&v)[H]) {
 #pragma unroll
-  for (int i = 0; i < S; i += 2) {
+  for (int i = 0; i < H; i += 2) {
     const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p + 2 * i);
     v[i] = u.x; v[i + 1] = u.y;
   }
 }
+template <int H> __device__ __forceinline__ void st_pairs(float* p, const f32x2 (&v)[H]) {
+#pragma unroll
+  for (int i = 0; i < H; i += 2) *reinterpret_cast<ulonglong2*>(p + 2 * i) = make_ulonglong2(v[i], v[i + 1]);
+}
+__device__ __forceinline__ float both(f32x2 v) {
+  float x, y;
+  f2_unpack(v, x, y);
+  return x + y;
+}
 // What a token brings to a thread.  The loops ask for a token's operands one token ahead, for its step two ahead, and have the next token's decays
 // computed while this one's are used, so that neither shared memory nor the exps are waited for.
-template <int S, bool E, bool Cs> struct Token {
-  f32x2 x, e, B[S], C[S];
+// H = S / 2 pairs of states; channels one by one.  Shared memory gives four bytes a lane and cycle whatever lanes share, so that b and c lie there
+// once, and the channels' numbers are doubled in registers.
+template <int H, bool E, bool Cs> struct Token {
+  f32x2 x, e, B[H], C[H];                // x, e: of the two channels
   __device__ __forceinline__ void get(const float* dx, const float* ep, const float* b, const float* c) {
     x = ld2(dx);
     if constexpr (E) e = ld2(ep);
-    ld_dup<S>(b, B);
-    if constexpr (Cs) ld_dup<S>(c, C);
+    ld_pairs<H>(b, B);
+    if constexpr (Cs) ld_pairs<H>(c, C);
   }
 };
-template <int S> __device__ __forceinline__ void decays(f32x2 dt, const f32x2 (&A)[S], f32x2 (&d)[S]) {
-#pragma unroll
-  for (int i = 0; i < S; ++i) d[i] = ex2_pair(f2_mul(dt, A[i]));
+__device__ __forceinline__ void splat2(f32x2 v, f32x2 (&s)[2]) {
+  float x, y;
+  f2_unpack(v, x, y);
+  s[0] = f2_splat(x);
+  s[1] = f2_splat(y);
 }
-// The sum over the lanes of a channel's states of (v, w), a pair of channels each: lane bit 0 ends with the channel, bit 1 with v or w.
-template <int QL> __device__ __forceinline__ float sum_states(f32x2 v, f32x2 w, int lane) {
-  float v0, v1, w0, w1;
-  f2_unpack(v, v0, v1);
-  f2_unpack(w, w0, w1);
+template <int H> __device__ __forceinline__ void decays(f32x2 dt, const f32x2 (&A)[2][H], f32x2 (&d)[2][H]) {
+  f32x2 s[2];
+  splat2(dt, s);
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < H; ++i) d[c][i] = ex2_pair(f2_mul(s[c], A[c][i]));
+}
+// The sum over the lanes of a channel's states of v and w, of two channels each: lane bit 0 ends with the channel, bit 1 with v or w.
+template <int QL> __device__ __forceinline__ float sum_states(float v0, float v1, float w0, float w1, int lane) {
   const bool hi = lane & 1, sec = lane & 2;
   const float p = (hi ? v1 : v0) + __shfl_xor_sync(~0u, hi ? v0 : v1, 1);
   const float q = (hi ? w1 : w0) + __shfl_xor_sync(~0u, hi ? w0 : w1, 1);
@@ -164,7 +182,7 @@ __device__ __forceinline__ int text_length(const Args& a, int b) {
   return (int)(n < 0 ? 0 : n > a.len ? a.len : n);
 }
 
-// b and c of a tile, as pairs of equal numbers in shared memory
+// b and c of a tile
 template <typename T, int NP> struct Coeffs {
   static constexpr int PER = TT * NP / THREADS;
   float v[PER];
@@ -178,7 +196,7 @@ template <typename T, int NP> struct Coeffs {
   }
   __device__ __forceinline__ void put(float* sm) const {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *reinterpret_cast<float2*>(sm + 2 * (threadIdx.x + i * THREADS)) = make_float2(v[i], v[i]);
+    for (int i = 0; i < PER; ++i) sm[threadIdx.x + i * THREADS] = v[i];
   }
 };
 
@@ -216,13 +234,13 @@ template <typename T, int CT> struct Pieces {                           // a thr
 
 // A segment's part of y, or (SUMS) its own contribution to the state and the sum of its steps.
 template <typename T, int S, int QL, bool SUMS>
-__global__ void __launch_bounds__(THREADS, S == 4 ? 3 : 2)
+__global__ void __launch_bounds__(THREADS, S == 4 ? 4 : 2)
 scan_kernel(const Args a) {
   constexpr int NP = QL * S, CT = channels_of(QL);
   using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
   // two rows and one more than a tile has: what the loop asks for ahead of its end
-  __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_y[TT][CT], s_b[TT + 1][2 * NP], s_c[TT + 1][2 * NP], s_bias[CT], s_skip[CT];
+  __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_y[TT][CT], s_b[TT + 1][NP], s_c[TT + 1][NP], s_bias[CT], s_skip[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place p = place_of<CT>(a);
   pdl_wait();
@@ -232,24 +250,29 @@ scan_kernel(const Args a) {
     s_skip[tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
   }
   const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;      // the thread's two channels and S states
-  f32x2 h[S], A[S];
+  constexpr int H = S / 2;
+  f32x2 h[2][H], A[2][H];
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float v[2], w[2];
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bool real = cl + j < p.valid && q0 + i < a.states;
-      const long long ch = p.ch0 + cl + j;
-      v[j] = real ? a.a[ch * a.states + q0 + i] * LOG2E : 0.f;
-      w[j] = 0.f;
-      if (!SUMS && real) {
-        if (a.segs > 1) w[j] = a.seg_state[(row_n + cl + j) * NP + q0 + i];
-        else if (a.state_in) w[j] = a.state_in[((long long)p.b * a.dim + ch) * a.states + q0 + i];
+    for (int i = 0; i < H; ++i) {
+      float v[2], w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = q0 + 2 * i + j;
+        const bool real = cl + c < p.valid && s < a.states;
+        const long long ch = p.ch0 + cl + c;
+        v[j] = real ? a.a[ch * a.states + s] * LOG2E : 0.f;
+        w[j] = 0.f;
+        if (!SUMS && real) {
+          if (a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
+          else if (a.state_in) w[j] = a.state_in[((long long)p.b * a.dim + ch) * a.states + s];
+        }
       }
+      A[c][i] = f2_pack(v[0], v[1]);
+      h[c][i] = f2_pack(w[0], w[1]);
     }
-    A[i] = f2_pack(v[0], v[1]);
-    h[i] = f2_pack(w[0], w[1]);
   }
   const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
   const int used = min(last, (n + TT - 1) / TT);
@@ -270,20 +293,16 @@ scan_kernel(const Args a) {
   __syncthreads();
   for (int k = first; k < used; ++k) {
     fetch(k);
-    f32x2 h0[S], own[S], cum = 0;
+    f32x2 h0[2][H], own[2][H], cum = 0;
 #pragma unroll
-    for (int i = 0; i < S; ++i) { h0[i] = h[i]; own[i] = 0; }
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < H; ++i) { h0[c][i] = h[c][i]; own[c][i] = 0; }
     if (!SUMS && a.saves) {              // the state in front of the tile, for the gradient
       float* to = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
 #pragma unroll
-      for (int i = 0; i < S; i += 4) {
-        float f[2][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f2_unpack(h[i + j], f[0][j], f[1][j]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (cl + j < p.valid) *reinterpret_cast<float4*>(to + j * NP + i) = make_float4(f[j][0], f[j][1], f[j][2], f[j][3]);
-      }
+      for (int c = 0; c < 2; ++c)
+        if (cl + c < p.valid) st_pairs<H>(to + c * NP, h[c]);
     }
     {
       float bias[E];
@@ -314,47 +333,58 @@ scan_kernel(const Args a) {
     }
     {
       constexpr int U = 4;
-      Token<S, false, !SUMS> next;
-      const float *p_dt = &s_dt[0][cl], *p_dx = &s_dx[0][cl], *p_b = &s_b[0][2 * q0], *p_c = &s_c[0][2 * q0];
+      Token<H, false, !SUMS> next;
+      const float *p_dt = &s_dt[0][cl], *p_dx = &s_dx[0][cl], *p_b = &s_b[0][q0], *p_c = &s_c[0][q0];
       float* p_y = &s_y[(lane >> 1) & 1][cl + (lane & 1)];
-      f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[S];
+      f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[2][H];
       next.get(p_dx, nullptr, p_b, p_c);
-      decays<S>(dt, A, d_next);
+      decays<H>(dt, A, d_next);
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += U) {
-        f32x2 sum[U];
+        float sum[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const Token<S, false, !SUMS> now = next;
-          f32x2 d[S];
+          const Token<H, false, !SUMS> now = next;
+          f32x2 d[2][H], x[2];
 #pragma unroll
-          for (int i = 0; i < S; ++i) d[i] = d_next[i];
-          next.get(p_dx + (u + 1) * CT, nullptr, p_b + (u + 1) * 2 * NP, p_c + (u + 1) * 2 * NP);
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
+          next.get(p_dx + (u + 1) * CT, nullptr, p_b + (u + 1) * NP, p_c + (u + 1) * NP);
           cum = f2_add(cum, dt);
           dt = dt_next;
           dt_next = ld2(p_dt + (u + 2) * CT);
-          decays<S>(dt, A, d_next);
-          sum[u] = 0;
+          decays<H>(dt, A, d_next);
+          splat2(now.x, x);
 #pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const f32x2 fed = f2_mul(now.x, now.B[i]);
-            own[i] = f2_fma(d[i], own[i], fed);
-            if constexpr (!SUMS) {
-              h[i] = f2_fma(d[i], h[i], fed);
-              sum[u] = f2_fma(h[i], now.C[i], sum[u]);
+          for (int c = 0; c < 2; ++c) {
+            f32x2 y = 0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+              const f32x2 fed = f2_mul(x[c], now.B[i]);
+              own[c][i] = f2_fma(d[c][i], own[c][i], fed);
+              if constexpr (!SUMS) {
+                h[c][i] = f2_fma(d[c][i], h[c][i], fed);
+                y = i ? f2_fma(h[c][i], now.C[i], y) : f2_mul(h[c][i], now.C[i]);
+              }
             }
+            sum[u][c] = both(y);
           }
         }
         if constexpr (!SUMS) {
 #pragma unroll
-          for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(sum[u], sum[u + 1], lane);
+          for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(sum[u][0], sum[u][1], sum[u + 1][0], sum[u + 1][1], lane);
         }
-        p_dt += U * CT; p_dx += U * CT; p_b += U * 2 * NP; p_c += U * 2 * NP; p_y += U * CT;
+        p_dt += U * CT; p_dx += U * CT; p_b += U * NP; p_c += U * NP; p_y += U * CT;
       }
     }
     // the carried state meets the tile's decays in one product, so that its error grows with the tiles, not with the tokens
+    f32x2 through[2][H];
+    decays<H>(cum, A, through);
 #pragma unroll
-    for (int i = 0; i < S; ++i) h[i] = f2_fma(ex2_pair(f2_mul(cum, A[i])), h0[i], own[i]);
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < H; ++i) h[c][i] = f2_fma(through[c][i], h0[c][i], own[c][i]);
     steps = f2_add(steps, cum);
     __syncthreads();
     if constexpr (!SUMS) {
@@ -384,13 +414,8 @@ scan_kernel(const Args a) {
   }
   if constexpr (SUMS) {
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      float f[2];
-      f2_unpack(h[i], f[0], f[1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (cl + j < p.valid) a.seg_state[(row_n + cl + j) * NP + q0 + i] = f[j];
-    }
+    for (int c = 0; c < 2; ++c)
+      if (cl + c < p.valid) st_pairs<H>(a.seg_state + (row_n + cl + c) * NP + q0, h[c]);
     float f[2];
     f2_unpack(steps, f[0], f[1]);
 #pragma unroll
@@ -403,12 +428,15 @@ scan_kernel(const Args a) {
     }
     if (a.state_out && p.seg == a.segs - 1) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        float f[2];
-        f2_unpack(h[i], f[0], f[1]);
+      for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (cl + j < p.valid && q0 + i < a.states) a.state_out[((long long)p.b * a.dim + p.ch0 + cl + j) * a.states + q0 + i] = f[j];
+        for (int i = 0; i < H; ++i) {
+          float f[2];
+          f2_unpack(h[c][i], f[0], f[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (cl + c < p.valid && q0 + 2 * i + j < a.states) a.state_out[((long long)p.b * a.dim + p.ch0 + cl + c) * a.states + q0 + 2 * i + j] = f[j];
+        }
       }
     }
   }
@@ -425,11 +453,27 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
   const bool real = s < states;
   const float A = real ? a[(long long)d * states + s] * LOG2E : 0.f;
   float h = real && edge ? edge[((long long)b * dim + d) * states + s] : 0.f;
-  for (int k = 0; k < segs; ++k) {
-    const long long at = ((long long)b * segs + (reverse ? segs - 1 - k : k)) * dim + d;
-    const float own = seg_state[at * np + s];
-    seg_state[at * np + s] = h;
-    h = fmaf(exp2f(A * seg_steps[at]), h, own);
+  // several segments' loads are under way together
+  constexpr int U = 8;
+  const long long step = reverse ? -(long long)dim : dim;
+  long long at = ((long long)b * segs + (reverse ? segs - 1 : 0)) * dim + d;
+  for (int k = 0; k < segs; k += U) {
+    float own[U], decay[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      own[u] = k + u < segs ? seg_state[(at + u * step) * np + s] : 0.f;
+      decay[u] = k + u < segs ? seg_steps[at + u * step] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) decay[u] = exp2f(A * decay[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k + u < segs) {
+        seg_state[(at + u * step) * np + s] = h;
+        h = fmaf(decay[u], h, own[u]);
+      }
+    }
+    at += U * step;
   }
 }
 
@@ -440,29 +484,35 @@ back_sums_kernel(const Args a, const Grads g) {
   constexpr int NP = QL * S, CT = channels_of(QL);
   using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
-  __shared__ __align__(16) float s_dt[TT][CT], s_e[TT][CT], s_c[TT][2 * NP], s_bias[CT];
+  __shared__ __align__(16) float s_dt[TT][CT], s_e[TT][CT], s_c[TT][NP], s_bias[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place p = place_of<CT>(a);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) s_bias[tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
   const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
-  f32x2 G[S], A[S];
+  constexpr int H = S / 2;
+  f32x2 G[2][H], A[2][H];
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float v[2];
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      v[j] = cl + j < p.valid && q0 + i < a.states ? a.a[(long long)(p.ch0 + cl + j) * a.states + q0 + i] * LOG2E : 0.f;
-    A[i] = f2_pack(v[0], v[1]);
-    G[i] = 0;
+    for (int i = 0; i < H; ++i) {
+      float v[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = q0 + 2 * i + j;
+        v[j] = cl + c < p.valid && s < a.states ? a.a[(long long)(p.ch0 + cl + c) * a.states + s] * LOG2E : 0.f;
+      }
+      A[c][i] = f2_pack(v[0], v[1]);
+      G[c][i] = 0;
+    }
   }
   const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles;
   const int used = min(min(first + a.seg_tiles, total), (n + TT - 1) / TT);
   const int col = tid % Px::PPR * E, row = tid / Px::PPR;
   Px delta, dy, z;
   Coeffs<T, NP> fc;
-  float steps[2] = {0.f, 0.f};
+  f32x2 steps = 0;
   __syncthreads();
   for (int k = used - 1; k >= first; --k) {
     delta.fetch(a.delta, p, k * TT, n);
@@ -491,32 +541,31 @@ back_sums_kernel(const Args a, const Grads g) {
     }
     fc.put(&s_c[0][0]);
     __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
     for (int t = TT - 1; t >= 0; --t) {
-      const f32x2 dt = ld2(&s_dt[t][cl]), e = ld2(&s_e[t][cl]);
-      f32x2 C[S];
-      ld_dup<S>(&s_c[t][2 * q0], C);
+      const f32x2 dt = ld2(&s_dt[t][cl]);
+      f32x2 C[H], d[2][H], e[2];
+      splat2(ld2(&s_e[t][cl]), e);
+      ld_pairs<H>(&s_c[t][q0], C);
+      decays<H>(dt, A, d);
 #pragma unroll
-      for (int i = 0; i < S; ++i) G[i] = f2_mul(ex2_pair(f2_mul(dt, A[i])), f2_fma(e, C[i], G[i]));
-      float d0, d1;
-      f2_unpack(dt, d0, d1);
-      steps[0] += d0;
-      steps[1] += d1;
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < H; ++i) G[c][i] = f2_mul(d[c][i], f2_fma(e[c], C[i], G[c][i]));
+      steps = f2_add(steps, dt);
     }
     __syncthreads();
   }
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
+  float f[2];
+  f2_unpack(steps, f[0], f[1]);
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float f[2];
-    f2_unpack(G[i], f[0], f[1]);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (cl + j < p.valid) a.seg_state[(row_n + cl + j) * NP + q0 + i] = f[j];
+  for (int c = 0; c < 2; ++c) {
+    if (cl + c < p.valid) {
+      st_pairs<H>(a.seg_state + (row_n + cl + c) * NP + q0, G[c]);
+      if (lane % QL == 0) a.seg_steps[row_n + cl + c] = f[c];
+    }
   }
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (lane % QL == 0 && cl + j < p.valid) a.seg_steps[row_n + cl + j] = steps[j];
 }
 
 template <int S, int QL> struct BackShared {
@@ -524,27 +573,15 @@ template <int S, int QL> struct BackShared {
   // the loops ask for two tokens more than the tile has: at either end there is other memory of this struct, which is not used
   float bias[2][CT];
   float dt[TT][CT], dx[TT][CT], e[TT][CT], y[TT][CT], q[TT][CT];       // dx becomes gb
-  float before[2 * NP], b[TT][2 * NP], c[TT][2 * NP];
+  float before[NP], b[TT][NP], c[TT][NP];
   float part[4][TT][NP];                 // db or dc of each warp's channels
   float mid[4][U * STEP];                // four steps of each pair of channels
   float da[S][THREADS][2];               // each thread's sums over the tiles
 };
 
 // Four steps' values of a warp's pairs of channels are added up through shared memory: half the instructions of shuffles
-template <int S, int QL> __device__ __forceinline__ void put_channels(float* mid, const f32x2 (&v)[S], int lane) {
-  constexpr int NP = QL * S;
-  float* to = mid + lane / QL * NP + lane % QL * S;
-#pragma unroll
-  for (int i = 0; i < S; i += 4) {
-    float f[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float x, y;
-      f2_unpack(v[i + j], x, y);
-      f[j] = x + y;
-    }
-    *reinterpret_cast<float4*>(to + i) = make_float4(f[0], f[1], f[2], f[3]);
-  }
+template <int S, int QL> __device__ __forceinline__ void put_channels(float* mid, const f32x2 (&v)[S / 2], int lane) {
+  st_pairs<S / 2>(mid + lane / QL * (QL * S) + lane % QL * S, v);
 }
 template <int S, int QL> __device__ __forceinline__ void sum_channels(const float* mid, float* to, int lane) {    // to: four rows of NP
   constexpr int NP = QL * S, STEP = BackShared<S, QL>::STEP, C = 32 / QL;
@@ -590,22 +627,27 @@ back_kernel(const Args a, const Grads g) {
   }
   const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
-  f32x2 G[S], A[S];
+  constexpr int H = S / 2;
+  f32x2 G[2][H], A[2][H];
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float v[2], w[2];
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bool real = cl + j < p.valid && q0 + i < a.states;
-      const long long ch = p.ch0 + cl + j;
-      v[j] = real ? a.a[ch * a.states + q0 + i] * LOG2E : 0.f;
-      w[j] = 0.f;
-      if (real && a.segs > 1) w[j] = a.seg_state[(row_n + cl + j) * NP + q0 + i];
-      else if (real && g.d_state_out) w[j] = g.d_state_out[((long long)p.b * a.dim + ch) * a.states + q0 + i];
+    for (int i = 0; i < H; ++i) {
+      float v[2], w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = q0 + 2 * i + j;
+        const bool real = cl + c < p.valid && s < a.states;
+        const long long ch = p.ch0 + cl + c;
+        v[j] = real ? a.a[ch * a.states + s] * LOG2E : 0.f;
+        w[j] = 0.f;
+        if (real && a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
+        else if (real && g.d_state_out) w[j] = g.d_state_out[((long long)p.b * a.dim + ch) * a.states + s];
+      }
+      A[c][i] = f2_pack(v[0], v[1]);
+      G[c][i] = f2_pack(w[0], w[1]);
+      *reinterpret_cast<f32x2*>(sh.da[c * H + i][tid]) = 0;
     }
-    A[i] = f2_pack(v[0], v[1]);
-    G[i] = f2_pack(w[0], w[1]);
-    *reinterpret_cast<f32x2*>(sh.da[i][tid]) = 0;
   }
   const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
   const int used = min(last, (n + TT - 1) / TT);
@@ -635,16 +677,16 @@ back_kernel(const Args a, const Grads g) {
   for (int k = used - 1; k >= first; --k) {
     fetch(k);
     const float* saved = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
-    auto in_front = [&](f32x2 (&h)[S]) {
+    auto in_front = [&](f32x2 (&h)[2][H]) {
 #pragma unroll
-      for (int i = 0; i < S; i += 4) {
-        float4 f[2];
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = cl + j < p.valid ? __ldg(reinterpret_cast<const float4*>(saved + j * NP + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        h[i] = f2_pack(f[0].x, f[1].x); h[i + 1] = f2_pack(f[0].y, f[1].y); h[i + 2] = f2_pack(f[0].z, f[1].z); h[i + 3] = f2_pack(f[0].w, f[1].w);
-      }
+        for (int i = 0; i < H; i += 2) {
+          const ulonglong2 u = cl + c < p.valid ? __ldg(reinterpret_cast<const ulonglong2*>(saved + c * NP + 2 * i)) : make_ulonglong2(0, 0);
+          h[c][i] = u.x; h[c][i + 1] = u.y;
+        }
     };
-    f32x2 h[S], dA[S];
+    f32x2 h[2][H], dA[2][H];
     in_front(h);
     {
       float bias[E];
@@ -685,47 +727,58 @@ back_kernel(const Args a, const Grads g) {
     }
     constexpr int U = BackShared<S, QL>::U, STEP = BackShared<S, QL>::STEP;
     float* mid = sh.mid[warp];
-    f32x2 K[S];
+    f32x2 K[2][H];
 #pragma unroll
-    for (int i = 0; i < S; ++i) K[i] = dA[i] = 0;
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < H; ++i) K[c][i] = dA[c][i] = 0;
     float* to_yq = own_row ? &sh.q[0][own_ch] : &sh.y[0][own_ch];
     {
-      Token<S, true, true> next;
-      const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][2 * q0], *p_c = &sh.c[0][2 * q0];
-      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt + CT), d_next[S];
+      Token<H, true, true> next;
+      const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][q0], *p_c = &sh.c[0][q0];
+      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt + CT), d_next[2][H];
       next.get(p_dx, p_e, p_b, p_c);
-      decays<S>(dt_next, A, d_next);
+      decays<H>(dt_next, A, d_next);
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += U) {
-        f32x2 y[U], q[U];
+        float y[U][2], q[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const Token<S, true, true> now = next;
-          const f32x2 dt = dt_next;
-          f32x2 d[S], hs[S];
+          const Token<H, true, true> now = next;
+          f32x2 d[2][H], hs[H], dt[2], x[2], e[2];
+          splat2(dt_next, dt);
 #pragma unroll
-          for (int i = 0; i < S; ++i) d[i] = d_next[i];
-          next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * 2 * NP, p_c + (u + 1) * 2 * NP);
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
+          next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * NP, p_c + (u + 1) * NP);
           dt_next = dt_far;
           dt_far = ld2(p_dt + (u + 2) * CT);
-          decays<S>(dt_next, A, d_next);
-          y[u] = q[u] = 0;
+          decays<H>(dt_next, A, d_next);
+          splat2(now.x, x);
+          splat2(now.e, e);
 #pragma unroll
-          for (int i = 0; i < S; ++i) {
-            K[i] = f2_mul(d[i], f2_fma(dt, h[i], K[i]));
-            h[i] = f2_fma(d[i], h[i], f2_mul(now.x, now.B[i]));
-            hs[i] = f2_mul(h[i], now.e);
-            const f32x2 v = f2_mul(h[i], now.C[i]);
-            y[u] = f2_add(y[u], v);
-            q[u] = f2_fma(v, A[i], q[u]);
-            dA[i] = f2_fma(f2_mul(K[i], now.C[i]), now.e, dA[i]);
+          for (int c = 0; c < 2; ++c) {
+            f32x2 yy, qq;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+              K[c][i] = f2_mul(d[c][i], f2_fma(dt[c], h[c][i], K[c][i]));
+              h[c][i] = f2_fma(d[c][i], h[c][i], f2_mul(x[c], now.B[i]));
+              hs[i] = c ? f2_fma(h[c][i], e[c], hs[i]) : f2_mul(h[c][i], e[c]);
+              const f32x2 v = f2_mul(h[c][i], now.C[i]);
+              yy = i ? f2_add(yy, v) : v;
+              qq = i ? f2_fma(v, A[c][i], qq) : f2_mul(v, A[c][i]);
+              dA[c][i] = f2_fma(f2_mul(K[c][i], now.C[i]), e[c], dA[c][i]);
+            }
+            y[u][c] = both(yy);
+            q[u][c] = both(qq);
           }
           put_channels<S, QL>(mid + u * STEP, hs, lane);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) to_yq[u * CT] = sum_states<QL>(y[u], q[u], lane);
+        for (int u = 0; u < U; ++u) to_yq[u * CT] = sum_states<QL>(y[u][0], y[u][1], q[u][0], q[u][1], lane);
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        to_yq += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * 2 * NP; p_c += U * 2 * NP;
+        to_yq += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * NP; p_c += U * NP;
       }
     }
     __syncthreads();
@@ -740,52 +793,65 @@ back_kernel(const Args a, const Grads g) {
       }
     };
     parts_to(g.part_c);
-    f32x2 end = 0;                       // sum a g h behind the tile's last token
+    float end[2];                        // sum a g h behind the tile's last token
+    f32x2 G0[2][H], own[2][H], cum = 0;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      end = f2_fma(f2_mul(G[i], h[i]), A[i], end);
-      f32x2* sum = reinterpret_cast<f32x2*>(sh.da[i][tid]);
-      *sum = f2_add(*sum, f2_fma(G[i], K[i], dA[i]));      // a tile's own sum first: 2048 tokens one by one lose half a digit
+    for (int c = 0; c < 2; ++c) {
+      f32x2 v = 0;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
+        f32x2* sum = reinterpret_cast<f32x2*>(sh.da[c * H + i][tid]);
+        *sum = f2_add(*sum, f2_fma(G[c][i], K[c][i], dA[c][i]));      // a tile's own sum first: 2048 tokens one by one lose half a digit
+        G0[c][i] = G[c][i];
+        own[c][i] = 0;
+      }
+      end[c] = both(v);
     }
     __syncthreads();
-    f32x2 G0[S], own[S], cum = 0;
-#pragma unroll
-    for (int i = 0; i < S; ++i) { G0[i] = G[i]; own[i] = 0; }
     {
-      Token<S, true, true> next;
-      constexpr int LAST = (TT - 1) * CT, LAST_N = (TT - 1) * 2 * NP;
+      Token<H, true, true> next;
+      constexpr int LAST = (TT - 1) * CT, LAST_N = (TT - 1) * NP;
       float* to_gq = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
-      const float *p_dt = &sh.dt[0][cl] + LAST, *p_dx = &sh.dx[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][2 * q0] + LAST_N, *p_c = &sh.c[0][2 * q0] + LAST_N;
-      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt - CT), d_next[S];
+      const float *p_dt = &sh.dt[0][cl] + LAST, *p_dx = &sh.dx[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][q0] + LAST_N, *p_c = &sh.c[0][q0] + LAST_N;
+      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt - CT), d_next[2][H];
       next.get(p_dx, p_e, p_b, p_c);
-      decays<S>(dt_next, A, d_next);
+      decays<H>(dt_next, A, d_next);
 #pragma unroll 1
       for (int t0 = TT - U; t0 >= 0; t0 -= U) {
-        f32x2 gb[U], q[U];
-        float q_h[U], xs[U], es[U];
+        float gb[U][2], q[U][2], q_h[U], xs[U], es[U];
 #pragma unroll
         for (int r = 0; r < U; ++r) {
           const int u = U - 1 - r;
-          const Token<S, true, true> now = next;
-          f32x2 d[S], gs[S];
+          const Token<H, true, true> now = next;
+          f32x2 d[2][H], gs[H], x[2], e[2];
 #pragma unroll
-          for (int i = 0; i < S; ++i) d[i] = d_next[i];
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
           cum = f2_add(cum, dt_next);
-          next.get(p_dx - (r + 1) * CT, p_e - (r + 1) * CT, p_b - (r + 1) * 2 * NP, p_c - (r + 1) * 2 * NP);
+          next.get(p_dx - (r + 1) * CT, p_e - (r + 1) * CT, p_b - (r + 1) * NP, p_c - (r + 1) * NP);
           dt_next = dt_far;
           dt_far = ld2(p_dt - (r + 2) * CT);
           q_h[u] = to_gq[-r * CT];
-          decays<S>(dt_next, A, d_next);
-          gb[u] = q[u] = 0;
+          decays<H>(dt_next, A, d_next);
+          splat2(now.x, x);
+          splat2(now.e, e);
 #pragma unroll
-          for (int i = 0; i < S; ++i) {
-            const f32x2 fed = f2_fma(now.e, now.C[i], G[i]);
-            own[i] = f2_mul(d[i], f2_fma(now.e, now.C[i], own[i]));
-            gs[i] = f2_mul(fed, now.x);
-            const f32x2 v = f2_mul(fed, now.B[i]);
-            gb[u] = f2_add(gb[u], v);
-            q[u] = f2_fma(v, A[i], q[u]);
-            G[i] = f2_mul(d[i], fed);
+          for (int c = 0; c < 2; ++c) {
+            f32x2 bb, qq;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+              const f32x2 fed = f2_fma(e[c], now.C[i], G[c][i]);
+              own[c][i] = f2_mul(d[c][i], f2_fma(e[c], now.C[i], own[c][i]));
+              gs[i] = c ? f2_fma(fed, x[c], gs[i]) : f2_mul(fed, x[c]);
+              const f32x2 v = f2_mul(fed, now.B[i]);
+              bb = i ? f2_add(bb, v) : v;
+              qq = i ? f2_fma(v, A[c][i], qq) : f2_mul(v, A[c][i]);
+              G[c][i] = f2_mul(d[c][i], fed);
+            }
+            gb[u][c] = both(bb);
+            q[u][c] = both(qq);
           }
           put_channels<S, QL>(mid + u * STEP, gs, lane);
           float v0, v1;
@@ -796,24 +862,34 @@ back_kernel(const Args a, const Grads g) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float r = sum_states<QL>(gb[u], q[u], lane);
+          const float r = sum_states<QL>(gb[u][0], gb[u][1], q[u][0], q[u][1], lane);
           to_gq[(u - (U - 1)) * CT] = own_row ? fmaf(q_h[u], es[u], -r * xs[u]) : r;
         }
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        to_gq -= U * CT;
-        p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * 2 * NP; p_c -= U * 2 * NP;
+        to_gq -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
       }
     }
     // as in the forward pass: the carried gradient meets the tile's decays once
+    {
+      f32x2 through[2][H];
+      decays<H>(cum, A, through);
 #pragma unroll
-    for (int i = 0; i < S; ++i) G[i] = f2_fma(ex2_pair(f2_mul(cum, A[i])), G0[i], own[i]);
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < H; ++i) G[c][i] = f2_fma(through[c][i], G0[c][i], own[c][i]);
+    }
     // a channel's sums, the second half of the tile from its end, the first from its start, where g and h are known too: rounding errors of the
     // q_r e_r and p_r s x, which all later sums share, have half the way to pile up
     in_front(h);
-    f32x2 start = 0;
+    float start[2];
 #pragma unroll
-    for (int i = 0; i < S; ++i) start = f2_fma(f2_mul(G[i], h[i]), A[i], start);
-    float w = sum_states<QL>(start, end, lane);                // lanes with bit 1: the tile's second half
+    for (int c = 0; c < 2; ++c) {
+      f32x2 v = 0;
+#pragma unroll
+      for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
+      start[c] = both(v);
+    }
+    float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane);    // lanes with bit 1: the tile's second half
     __syncwarp();
     if (lane % QL >= 4) {
       // its sums are another lane's too
@@ -887,14 +963,17 @@ back_kernel(const Args a, const Grads g) {
     __syncthreads();
   }
 #pragma unroll
-  for (int i = 0; i < S; ++i) {
-    float w[2];
-    f2_unpack(G[i], w[0], w[1]);
+  for (int c = 0; c < 2; ++c) {
+    if (cl + c >= p.valid) continue;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (cl + j < p.valid) {
-        g.part_a[(row_n + cl + j) * NP + q0 + i] = sh.da[i][tid][j];
-        if (g.d_state_in && p.seg == 0 && q0 + i < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + j) * a.states + q0 + i] = w[j];
+    for (int i = 0; i < H; ++i) {
+      float w[2];
+      f2_unpack(G[c][i], w[0], w[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = q0 + 2 * i + j;
+        g.part_a[(row_n + cl + c) * NP + s] = sh.da[c * H + i][tid][j];
+        if (g.d_state_in && p.seg == 0 && s < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + c) * a.states + s] = w[j];
       }
     }
   }
@@ -949,7 +1028,7 @@ finish_kernel(const Args a, const Grads g, int np, unsigned bc_blocks) {
   }
 }
 
-// One token: four threads a channel, a piece of its states each.
+// One token: four threads a channel, four of its states each at a time.
 struct StepArgs {
   int batch, dim, states, groups, per_group, softplus;
   const void *x, *delta, *z, *b, *c;
@@ -959,54 +1038,96 @@ struct StepArgs {
   void* y;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+template <typename T> __device__ __forceinline__ void load4(const T* p, bool vec, float (&f)[4]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+      f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+      f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = lp::load1(p + j);
+  }
+}
+
+constexpr int STEP_THREADS = 256, STEP_UNROLL = 2, STEP_CHANNELS = STEP_THREADS / 4 * STEP_UNROLL;      // of a block
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(STEP_THREADS)
 step_kernel(const StepArgs a) {
   pdl_wait();
-  const long long i = blockIdx.x * 64LL + threadIdx.x / 4;
   const int part = threadIdx.x % 4;
-  const bool live = i < (long long)a.batch * a.dim;
-  const int b = live ? (int)(i / a.dim) : 0, d = live ? (int)(i % a.dim) : 0, grp = d / a.per_group;
-  const float x = lp::load1(static_cast<const T*>(a.x) + b * a.x_sb + d);
-  const float dt = step_of(lp::load1(static_cast<const T*>(a.delta) + b * a.d_sb + d) + (a.bias ? a.bias[d] : 0.f), a.softplus);
-  const float dx = dt * x;
-  const T* B = static_cast<const T*>(a.b) + b * a.b_sb + grp * a.b_sg;
-  const T* C = static_cast<const T*>(a.c) + b * a.c_sb + grp * a.c_sg;
-  float* h = a.state + b * a.s_b + (long long)d * a.states;
-  const float* A = a.a + (long long)d * a.states;
-  float y = 0.f;
-  auto one = [&](float hh, float aa, int s) {
-    hh = fmaf(ex2(dt * (aa * LOG2E)), hh, dx * lp::load1(B + s));
-    y = fmaf(hh, lp::load1(C + s), y);
-    return hh;
-  };
-  if (live) {
-    if (a.states % 4 == 0 && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(A)) & 15) == 0) {
-      for (int s = part * 4; s < a.states; s += 16) {
-        float4 v = *reinterpret_cast<float4*>(h + s);
-        const float4 w = __ldg(reinterpret_cast<const float4*>(A + s));
-        v.x = one(v.x, w.x, s); v.y = one(v.y, w.y, s + 1); v.z = one(v.z, w.z, s + 2); v.w = one(v.w, w.w, s + 3);
-        *reinterpret_cast<float4*>(h + s) = v;
+  const long long n = (long long)a.batch * a.dim, first = blockIdx.x * (long long)STEP_CHANNELS + threadIdx.x / 4;
+  int b[STEP_UNROLL], d[STEP_UNROLL];
+  float x[STEP_UNROLL], v[STEP_UNROLL], z[STEP_UNROLL], h[STEP_UNROLL][4], A[STEP_UNROLL][4], B[STEP_UNROLL][4], C[STEP_UNROLL][4];
+  bool live[STEP_UNROLL];
+  auto group = [&](int u, long long sb, long long sg, const void* p) { return static_cast<const T*>(p) + b[u] * sb + d[u] / a.per_group * sg; };
+#pragma unroll
+  for (int u = 0; u < STEP_UNROLL; ++u) {  // the first states of all channels are under way together
+    const long long i = first + u * (STEP_THREADS / 4);
+    live[u] = i < n;
+    b[u] = live[u] ? (int)(i / a.dim) : 0;
+    d[u] = live[u] ? (int)(i - (long long)b[u] * a.dim) : 0;
+    x[u] = lp::load1(static_cast<const T*>(a.x) + b[u] * a.x_sb + d[u]);
+    v[u] = lp::load1(static_cast<const T*>(a.delta) + b[u] * a.d_sb + d[u]) + (a.bias ? a.bias[d[u]] : 0.f);
+    z[u] = a.z ? lp::load1(static_cast<const T*>(a.z) + b[u] * a.z_sb + d[u]) : 0.f;
+    if constexpr (VEC) {
+      if (part * 4 < a.states) {
+        load4(a.state + b[u] * a.s_b + (long long)d[u] * a.states + part * 4, true, h[u]);
+        load4(a.a + (long long)d[u] * a.states + part * 4, true, A[u]);
+        load4(group(u, a.b_sb, a.b_sg, a.b) + part * 4, true, B[u]);
+        load4(group(u, a.c_sb, a.c_sg, a.c) + part * 4, true, C[u]);
       }
-    } else {
-      for (int s = part; s < a.states; s += 4) h[s] = one(h[s], A[s], s);
     }
   }
-  y += __shfl_xor_sync(~0u, y, 1);
-  y += __shfl_xor_sync(~0u, y, 2);
-  if (!live || part) return;
-  if (a.skip) y = fmaf(a.skip[d], x, y);
-  if (a.z) {
-    const float z = lp::load1(static_cast<const T*>(a.z) + b * a.z_sb + d);
-    y *= z * sigmoid(z);
+#pragma unroll
+  for (int u = 0; u < STEP_UNROLL; ++u) {
+    const float dt = step_of(v[u], a.softplus), dx = dt * x[u];
+    float* state = a.state + b[u] * a.s_b + (long long)d[u] * a.states;
+    const float* decay = a.a + (long long)d[u] * a.states;
+    float y = 0.f;
+    if (live[u]) {
+      if constexpr (VEC) {
+        for (int s = part * 4; s < a.states; s += 16) {
+          if (s >= 16) {
+            load4(state + s, true, h[u]);
+            load4(decay + s, true, A[u]);
+            load4(group(u, a.b_sb, a.b_sg, a.b) + s, true, B[u]);
+            load4(group(u, a.c_sb, a.c_sg, a.c) + s, true, C[u]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            h[u][j] = fmaf(ex2(dt * (A[u][j] * LOG2E)), h[u][j], dx * B[u][j]);
+            y = fmaf(h[u][j], C[u][j], y);
+          }
+          *reinterpret_cast<float4*>(state + s) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
+        }
+      } else {
+        const T *pb = group(u, a.b_sb, a.b_sg, a.b), *pc = group(u, a.c_sb, a.c_sg, a.c);
+        for (int s = part; s < a.states; s += 4) {
+          const float hh = fmaf(ex2(dt * (decay[s] * LOG2E)), state[s], dx * lp::load1(pb + s));
+          state[s] = hh;
+          y = fmaf(hh, lp::load1(pc + s), y);
+        }
+      }
+    }
+    y += __shfl_xor_sync(~0u, y, 1);
+    y += __shfl_xor_sync(~0u, y, 2);
+    if (!live[u] || part) continue;
+    if (a.skip) y = fmaf(a.skip[d[u]], x[u], y);
+    if (a.z) y *= z[u] * sigmoid(z[u]);
+    st_from_float(static_cast<T*>(a.y) + (long long)b[u] * a.dim + d[u], y);
   }
-  st_from_float(static_cast<T*>(a.y) + i, y);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 struct Plan { int np, total, tiles, per_group, segs, seg_tiles; };
-// The axis is cut into segments where sequences and channels alone leave SMs without two blocks: what a segment adds to the state is then computed
-// first, at the price of a second exp for each token, channel and state.
+// The axis is cut into segments where sequences and channels alone are fewer blocks than SMs, into as many as run at once: what a segment adds to the
+// state is then computed first, at the price of a second exp for each token, channel and state.
 static Plan plan_of(int batch, int len, int dim, int states, int groups) {
   Plan p;
   p.np = states <= 16 ? 16 : states <= 32 ? 32 : 64;
@@ -1014,7 +1135,7 @@ static Plan plan_of(int batch, int len, int dim, int states, int groups) {
   p.per_group = dim / groups;
   const int ct = channels_of(p.np == 64 ? 8 : 4);
   p.tiles = (p.per_group + ct - 1) / ct;
-  const long long blocks = (long long)batch * groups * p.tiles, want = 4LL * m2_sm_count();
+  const long long blocks = (long long)batch * groups * p.tiles, want = (p.np == 16 ? 4LL : 2LL) * m2_sm_count();
   p.segs = 1;
   if (blocks < m2_sm_count() && p.total >= 8) {
     long long s = want / (blocks > 0 ? blocks : 1);
@@ -1171,7 +1292,7 @@ extern "C" int m2_selective_scan_step(const m2_selective_scan_step_args* args, v
              "m2_selective_scan_step: %d sequences, %d channels, %d states, %d groups", g.batch, g.dim, g.states, g.groups);
   M2_REQUIRE(g.states <= MAX_STATES, M2_ERR_UNSUPPORTED, "m2_selective_scan_step: %d states (at most %d)", g.states, MAX_STATES);
   M2_REQUIRE(g.dtype == M2_F32 || g.dtype == M2_BF16, M2_ERR_UNSUPPORTED, "m2_selective_scan_step: tensors are float32 or bf16");
-  const long long blocks = ((long long)g.batch * g.dim + 63) / 64;
+  const long long blocks = ((long long)g.batch * g.dim + STEP_CHANNELS - 1) / STEP_CHANNELS;
   M2_REQUIRE(blocks <= 0x7fffffffLL && g.dim <= 1 << 24, M2_ERR_UNSUPPORTED, "m2_selective_scan_step: %d sequences of %d channels are more than the grid takes", g.batch, g.dim);
   if (g.batch == 0) return M2_OK;
   M2_REQUIRE(g.x && g.delta && g.a && g.b && g.c && g.state && g.y, M2_ERR_ARG, "m2_selective_scan_step: a tensor is NULL");
@@ -1182,7 +1303,10 @@ extern "C" int m2_selective_scan_step(const m2_selective_scan_step_args* args, v
   const StepArgs a = {g.batch, g.dim, g.states, g.groups, g.dim / g.groups, g.softplus, g.x, g.delta, g.gate, g.b, g.c,
                       g.x_sb, g.d_sb, g.z_sb, g.b_sb, g.b_sg, g.c_sb, g.c_sg, g.a, g.skip, g.delta_bias, g.state, g.s_b, g.y};
   const long long elements = (long long)g.batch * g.dim * g.states;
+  auto fours = [&](const void* p, long long sb, long long sg, int bytes) { return m2_aligned(p, 4 * bytes) && sb % 4 == 0 && sg % 4 == 0; };
+  const bool vec = g.states % 4 == 0 && fours(g.state, g.s_b, 0, 4) && fours(g.a, 0, 0, 4) && fours(g.b, g.b_sb, g.b_sg, size) && fours(g.c, g.c_sb, g.c_sg, size);
   const cudaStream_t st = (cudaStream_t)stream;
-  return g.dtype == M2_F32 ? m2_launch("m2_selective_scan_step", elements, step_kernel<float>, dim3((unsigned)blocks), 256, 0, st, a)
-                           : m2_launch("m2_selective_scan_step", elements, step_kernel<__nv_bfloat16>, dim3((unsigned)blocks), 256, 0, st, a);
+  auto go = [&](auto kernel) { return m2_launch("m2_selective_scan_step", elements, kernel, dim3((unsigned)blocks), STEP_THREADS, 0, st, a); };
+  if (g.dtype == M2_F32) return vec ? go(step_kernel<float, true>) : go(step_kernel<float, false>);
+  return vec ? go(step_kernel<__nv_bfloat16, true>) : go(step_kernel<__nv_bfloat16, false>);
 }
