@@ -71,12 +71,13 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_id=None):
     return BeamStep(score, beam, token, done)
 
 
-def _apart(states):
-    """Whether no element belongs to two of the states, each (pointer, bytes of a row, distance of rows, rows)."""
-    order = sorted((p, row, step, p + step * (n - 1) + row) for p, row, step, n in states if row and n)
-    for i, (p, row, step, end) in enumerate(order):
-        for q, row2, step2, _ in order[i + 1:]:
-            if q >= end:
+def _apart(states, rows):
+    """Whether no element belongs to two of the states, each (pointer, bytes of a row, distance of rows), of `rows` rows."""
+    order = sorted((p, row, step) for p, row, step in states if row)
+    ends = [p + step * (rows - 1) + row for p, row, step in order]
+    for i, (p, row, step) in enumerate(order):
+        for q, row2, step2 in order[i + 1:]:
+            if q >= ends[i]:
                 break
             at = (q - p) % step                                # rows of one cache, side by side
             if step != step2 or at < row or at + row2 > step:
@@ -96,24 +97,30 @@ def reorder_states(states, beam):
     if not 1 <= K <= MAX_BEAMS:
         raise ValueError(f"{name}: {K} beams (1 to {MAX_BEAMS})")
     dev = beam.get_device()
-    if dev < 0 or any(s.get_device() != dev for s in states):
+    if dev < 0 or [s for s in states if s.get_device() != dev]:
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
-    rows = (_lib.BeamState * max(len(states), 1))()
-    for i, s in enumerate(states):
-        if s.dim() < 1 or s.shape[0] != B * K:
-            raise ValueError(f"{name}: states have B * K = {B * K} rows, got {tuple(s.shape)}")
-        if torch.is_grad_enabled() and s.requires_grad:
-            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
-        size = s.element_size()
-        n = s.numel() // (B * K) * size if B else 0
-        if B and not (s.is_contiguous() or (s[0].is_contiguous() and (B * K == 1 or s.stride(0) * size >= n))):
-            raise ValueError(f"{name}: a state is changed in place: its rows are packed and do not overlap, got {tuple(s.shape)} with strides {s.stride()}")
-        rows[i] = _lib.BeamState(s.data_ptr(), n, s.stride(0) * size if B * K > 1 else n)
-    if not _apart([(r.p or 0, r.row_bytes, r.stride_bytes, B * K) for r in rows[:len(states)]]):
-        raise ValueError(f"{name}: two states share memory")
-    beam = beam.contiguous()
-    a = _lib.ReorderStatesArgs(B, K, len(states), beam.data_ptr(), rows)
-    ops._launch("m2_reorder_states", beam, _lib.lib().m2_reorder_states, C.byref(a), launches=None)
+    rows, numbers, grad = B * K, [], torch.is_grad_enabled()
     for s in states:
-        if not s.is_inference():
-            torch.autograd.graph.increment_version(s)
+        if s.dim() < 1 or s.shape[0] != rows:
+            raise ValueError(f"{name}: states have B * K = {rows} rows, got {tuple(s.shape)}")
+        if grad and s.requires_grad:
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+        if rows == 0:
+            continue
+        n = s.nbytes // rows
+        if s.is_contiguous():
+            numbers.append((s.data_ptr(), n, n))
+            continue
+        step = s.stride(0) * s.element_size()
+        if not s[0].is_contiguous() or (rows > 1 and step < n):
+            raise ValueError(f"{name}: a state is changed in place: its rows are packed and do not overlap, got {tuple(s.shape)} with strides {s.stride()}")
+        numbers.append((s.data_ptr(), n, step if rows > 1 else n))
+    if not _apart(numbers, rows):
+        raise ValueError(f"{name}: two states share memory")
+    if not numbers:
+        return
+    beam = beam.contiguous()
+    table = (_lib.BeamState * len(numbers))(*numbers)
+    a = _lib.ReorderStatesArgs(B, K, len(numbers), beam.data_ptr(), table)
+    ops._launch("m2_reorder_states", beam, _lib.lib().m2_reorder_states, C.byref(a), launches=None)
+    torch.autograd.graph.increment_version([s for s in states if not s.is_inference()])

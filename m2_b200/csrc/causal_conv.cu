@@ -3,8 +3,9 @@
 // its gradients, and one token at a time.  x_{-W+1} .. x_{-1} are the inputs that earlier calls left.  (The reference's short convolution,
 // bert/src/mm/monarch_mixer_sequence_mixer.py:118-121, has three taps around a token and lies inside m2_longconv_fwd.)
 //
-// Bound: memory, x in and y out (gradients: x and dy in, dx out).  A thread walks through CHUNK tokens of a few adjacent channels with the last W - 1
-// inputs in registers, so that a token is read once but for the W - 1 in front of a chunk.
+// Bound: memory, x in and y out (gradients: x and dy in, dx out).  A thread walks through a chunk of tokens of a few adjacent channels with the last W - 1
+// inputs in registers, so that a token is read once but for the W - 1 in front of a chunk; the next four tokens are under way while four are computed,
+// in pairs of channels.
 #include "common.cuh"
 
 namespace m2 {
@@ -29,42 +30,86 @@ struct Grads {
   float *dw, *d_bias;
 };
 
-template <typename T, int V> struct Vec {                              // V adjacent channels
-  static constexpr int BYTES = V * (int)sizeof(T);
-  static __device__ __forceinline__ void get(const T* p, float (&f)[V]) {
+// V adjacent channels as they lie in memory, and as P pairs of float32
+template <typename T, int V> struct Vec {
+  static constexpr int BYTES = V * (int)sizeof(T), P = (V + 1) / 2, WORDS = (BYTES + 3) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
     if constexpr (BYTES == 16) {
-      lp::Piece<T>::get(__ldg(reinterpret_cast<const uint4*>(p)), f);
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
     } else if constexpr (BYTES == 8) {
       const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-      if constexpr (sizeof(T) == 2) {
-        f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
-        f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
-      } else {
-        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y);
-      }
+      w[0] = u.x; w[1] = u.y;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
     } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = lp::load1(p + j);
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
     }
   }
-  static __device__ __forceinline__ void put(T* p, const float (&f)[V]) {
-    if constexpr (BYTES == 16) {
-      *reinterpret_cast<uint4*>(p) = lp::Piece<T>::put(f);
-    } else if constexpr (BYTES == 8) {
-      if constexpr (sizeof(T) == 2) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
-        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      } else {
-        *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
-      }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void get(f32x2 (&f)[P]) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) f[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) st_from_float(p + j, f[j]);
+      for (int i = 0; i < P; ++i) f[i] = f2_pack(__uint_as_float(w[2 * i]), V > 1 ? __uint_as_float(w[(2 * i + 1) % WORDS]) : 0.f);
     }
+  }
+  static __device__ __forceinline__ void put(T* p, const f32x2 (&f)[P]) {
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float x, y;
+      f2_unpack(f[i], x, y);
+      if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        w[2 * i] = __float_as_uint(x);
+        if constexpr (V > 1) w[2 * i + 1] = __float_as_uint(y);
+      }
+    }
+    if constexpr (BYTES == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
   }
 };
 
+// a number of each of V channels, step apart
+template <int V> __device__ __forceinline__ void channels(const float* p, int step, f32x2 (&f)[(V + 1) / 2]) {
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) f[i] = p ? f2_pack(__ldg(p + 2 * i * step), V > 1 ? __ldg(p + (2 * i + 1) * step) : 0.f) : 0;
+}
+// the taps of V channels, (dim, W): four at once where they are on 16 bytes
+template <int V, int W> __device__ __forceinline__ void taps_of(const float* p, f32x2 (&w)[W][(V + 1) / 2]) {
+  if constexpr (W % 4 == 0 && V > 1) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+#pragma unroll
+        for (int k = 0; k < W; k += 4) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(p + 2 * i * W + k)), b = __ldg(reinterpret_cast<const float4*>(p + (2 * i + 1) * W + k));
+          w[k][i] = f2_pack(a.x, b.x); w[k + 1][i] = f2_pack(a.y, b.y); w[k + 2][i] = f2_pack(a.z, b.z); w[k + 3][i] = f2_pack(a.w, b.w);
+        }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) channels<V>(p + k, W, w[k]);
+}
+
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + lp::ex2(-v * lp::LOG2E)); }
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 v) {
+  float x, y;
+  f2_unpack(v, x, y);
+  return f2_pack(sigmoid(x), sigmoid(y));
+}
 __device__ __forceinline__ int text_length(const Args& a, int b) {
   if (!a.lengths) return a.len;
   const long long n = a.lengths[b];
@@ -77,13 +122,62 @@ template <typename T, int V, int W> struct Line {
   long long st; int dim, n;
   __device__ Line(const Args& a, int b, int c, int n_) : x(static_cast<const T*>(a.x) + b * a.x_sb + c),
       before(a.state_in ? static_cast<const T*>(a.state_in) + (long long)b * (W - 1) * a.dim + c : nullptr), st(a.x_st), dim(a.dim), n(n_) {}
-  __device__ __forceinline__ void get(int t, float (&f)[V]) const {
-    if (t >= 0 && t < n) { Vec<T, V>::get(x + t * st, f); return; }
-    if (t < 0 && before) { Vec<T, V>::get(before + (long long)(t + W - 1) * dim, f); return; }
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = 0.f;
+  __device__ __forceinline__ const T* at(int t) const {                // NULL: zero
+    return t >= 0 && t < n ? x + t * st : t < 0 && t > -W && before ? before + (long long)(t + W - 1) * dim : nullptr;
+  }
+  __device__ __forceinline__ void get(int t, f32x2 (&f)[(V + 1) / 2]) const {
+    Vec<T, V> v;
+    const T* p = at(t);
+    if (p) v.load(p);
+    else v.clear();
+    v.get(f);
   }
 };
+
+// The next R times U tokens of a thread: copies under way into its own part of shared memory, or (pieces below 8 bytes) U of them in registers.
+constexpr int U = 4, R = 4;
+template <typename T, int V> struct Ring {
+  static constexpr bool ASYNC = Vec<T, V>::BYTES >= 8;
+  static constexpr int DEPTH = ASYNC ? R : 1, WORDS = Vec<T, V>::WORDS, SIZE = ASYNC ? R * U * THREADS * WORDS : 1;     // words of shared memory
+  uint32_t* sm;
+  Vec<T, V> reg[ASYNC ? 1 : U];
+  __device__ __forceinline__ Ring(uint32_t* s) : sm(s + threadIdx.x * WORDS) {}
+  __device__ __forceinline__ uint32_t* at(int stage, int u) const { return sm + (stage * U + u) * THREADS * WORDS; }
+  __device__ __forceinline__ void put(int stage, int u, const T* from) {       // NULL: zero
+    if constexpr (ASYNC) {
+      uint32_t* to = at(stage, u);
+      if (from) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(Vec<T, V>::BYTES) : "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) to[i] = 0;
+      }
+    } else {
+      if (from) reg[u].load(from);
+      else reg[u].clear();
+    }
+  }
+  __device__ __forceinline__ void get(int stage, int u, f32x2 (&f)[Vec<T, V>::P]) const {
+    if constexpr (ASYNC) {
+      Vec<T, V> v;
+      const uint32_t* from = at(stage, u);
+      if constexpr (WORDS == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(from);
+        v.w[0] = w.x; v.w[1] = w.y; v.w[2] = w.z; v.w[3] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(from);
+        v.w[0] = w.x; v.w[1] = w.y;
+      }
+      v.get(f);
+    } else {
+      reg[u].get(f);
+    }
+  }
+};
+template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <bool B> struct Const { static constexpr bool value = B; };
 
 struct Place { int b, chunk, c; bool live; };
 template <int V> __device__ __forceinline__ Place place_of(const Args& a) {       // lanes go over channels first
@@ -99,65 +193,90 @@ template <int V> __device__ __forceinline__ Place place_of(const Args& a) {     
 }
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, V > 1 && W <= 4 ? 5 : 1)
 conv_kernel(const Args a) {
-  constexpr int U = 4;                   // tokens whose loads are under way together
+  constexpr int P = (V + 1) / 2;
+  using X = Vec<T, V>;
   pdl_wait();
   const Place p = place_of<V>(a);
   if (!p.live) return;
   const int n = text_length(a, p.b);
   const Line<T, V, W> line(a, p.b, p.c, n);
   const int first = p.chunk * a.chunk, end = min(first + a.chunk, a.len), last = min(end, n);
-  float w[W][V], bias[V];
+  constexpr int D = Ring<T, V>::DEPTH, AHEAD = D * U;
+  __shared__ __align__(16) uint32_t s_ring[Ring<T, V>::SIZE];
+  Ring<T, V> next(s_ring);
+  const T* x_at = line.x + first * a.x_st;
+  int stage = 0;
+  for (int s = 0; s < D; ++s) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    bias[j] = a.bias ? __ldg(a.bias + p.c + j) : 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) w[i][j] = __ldg(a.w + (long long)(p.c + j) * W + i);
+    for (int u = 0; u < U; ++u)
+      if (first + s * U + u < last) next.put(s, u, x_at + u * a.x_st);
+    x_at += U * a.x_st;
+    copies_end();
   }
-  float x[W - 1 + U][V];
+  f32x2 x[W - 1 + U][P];
 #pragma unroll
   for (int i = 0; i < W - 1; ++i) line.get(first - (W - 1) + i, x[i]);
-  T* y = static_cast<T*>(a.y) + (long long)p.b * a.len * a.dim + p.c;
-  for (int t = first; t < last; t += U) {
+  f32x2 w[W][P], bias[P];
+  channels<V>(a.bias ? a.bias + p.c : nullptr, 1, bias);
+  taps_of<V, W>(a.w + (long long)p.c * W, w);
+  T* y = static_cast<T*>(a.y) + ((long long)p.b * a.len + first) * a.dim + p.c;
+  // ALL: neither these U tokens nor those that are asked for now end the chunk
+  auto tokens = [&](int t, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    copies_but<D - 1>();
 #pragma unroll
-    for (int u = 0; u < U; ++u) line.get(t + u < last ? t + u : n, x[W - 1 + u]);
+    for (int u = 0; u < U; ++u) next.get(stage, u, x[W - 1 + u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ALL || t + AHEAD + u < last) next.put(stage, u, x_at + u * a.x_st);
+    copies_end();
+    x_at += U * a.x_st;
+    stage = stage + 1 < D ? stage + 1 : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (t + u >= last) break;
-      float v[V];
+      if (!ALL && t + u >= last) break;
+      f32x2 v[P];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < P; ++j) {
         v[j] = bias[j];
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[j] = fmaf(w[i][j], x[u + i][j], v[j]);
-        if (a.silu) v[j] *= sigmoid(v[j]);
+        for (int i = 0; i < W; ++i) v[j] = f2_fma(w[i][j], x[u + i][j], v[j]);
+        if (a.silu) v[j] = f2_mul(v[j], sigmoid2(v[j]));
       }
-      Vec<T, V>::put(y + (long long)(t + u) * a.dim, v);
+      X::put(y + u * a.dim, v);
     }
+    y += U * a.dim;
 #pragma unroll
     for (int i = 0; i < W - 1; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = x[i + U][j];
-  }
-  const float zero[V] = {};
-  for (int t = max(first, last); t < end; ++t) Vec<T, V>::put(y + (long long)t * a.dim, zero);
+      for (int j = 0; j < P; ++j) x[i][j] = x[i + U][j];
+  };
+  int t = first;
+  for (; t + AHEAD + U <= last; t += U) tokens(t, Const<true>());
+  for (; t < last; t += U) tokens(t, Const<false>());
+  const f32x2 zero[P] = {};
+  y = static_cast<T*>(a.y) + (long long)p.b * a.len * a.dim + p.c;
+  for (t = max(first, last); t < end; ++t) X::put(y + (long long)t * a.dim, zero);
   if (a.state_out && p.chunk == 0) {
     T* s = static_cast<T*>(a.state_out) + (long long)p.b * (W - 1) * a.dim + p.c;
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
-      float v[V];
+      f32x2 v[P];
       line.get(n - (W - 1) + i, v);
-      Vec<T, V>::put(s + (long long)i * a.dim, v);
+      X::put(s + (long long)i * a.dim, v);
     }
   }
 }
 
 // dx_s = sum_i w_i dv_{s+W-1-i}, dv = dy silu'(v), with v computed again; a chunk's tokens s and the W - 1 behind them are walked through, so that
-// every chunk has all that its own dx need.  Sums of dw and dbias over a block's chunks of one column of channels, then over the blocks.
+// every chunk has all that its own dx need.  A thread's sums of dw and dbias are its chunk's part.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, V > 1 && W <= 4 ? 3 : 1)
 back_kernel(const Args a, const Grads g) {
+  constexpr int P = (V + 1) / 2;
+  using X = Vec<T, V>;
   pdl_wait();
   const Place p = place_of<V>(a);
   if (!p.live) return;
@@ -166,88 +285,133 @@ back_kernel(const Args a, const Grads g) {
   const T* dy = static_cast<const T*>(g.dy) + p.b * g.y_sb + p.c;
   const T* ds = g.d_state_out ? static_cast<const T*>(g.d_state_out) + (long long)p.b * (W - 1) * a.dim + p.c : nullptr;
   const int first = p.chunk * a.chunk, end = min(first + a.chunk, a.len), last = min(end, n);
-  float w[W][V], bias[V], dw[W][V], db[V];
+  // the first chunk also has the inputs in front of the sequence
+  const int lo = p.chunk == 0 ? -(W - 1) : first;
+  const int stop = max(last, p.chunk == 0 ? 0 : first) + W - 1;        // the last s whose gradient is not zero by its place, and what it needs
+  constexpr int D = Ring<T, V>::DEPTH, AHEAD = D * U;
+  __shared__ __align__(16) uint32_t s_x[Ring<T, V>::SIZE], s_y[Ring<T, V>::SIZE];
+  Ring<T, V> next_x(s_x), next_y(s_y);
+  auto ask = [&](int stage, int t0) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    bias[j] = a.bias ? __ldg(a.bias + p.c + j) : 0.f;
-    db[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      w[i][j] = __ldg(a.w + (long long)(p.c + j) * W + i);
-      dw[i][j] = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u;
+      next_x.put(stage, u, t < stop ? line.at(t) : nullptr);
+      next_y.put(stage, u, t >= 0 && t < n && t < stop ? dy + t * g.y_st : nullptr);
     }
+    copies_end();
+  };
+  for (int s = 0; s < D; ++s) ask(s, lo + s * U);
+  int stage = 0;
+  f32x2 w[W][P], bias[P], dw[W][P], db[P];
+  channels<V>(a.bias ? a.bias + p.c : nullptr, 1, bias);
+  taps_of<V, W>(a.w + (long long)p.c * W, w);
+  f32x2 x[W - 1 + U][P], dv[W - 1 + U][P];                             // x_{t-W+1} .. x_{t+U-1} and dv of the same
+#pragma unroll
+  for (int i = 0; i < W - 1; ++i) {
+    line.get(p.chunk == 0 ? n : lo - (W - 1) + i, x[i]);               // in front of what lies in front of a text: zero
+#pragma unroll
+    for (int j = 0; j < P; ++j) dv[i][j] = 0;
+  }
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    db[j] = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) dw[i][j] = 0;
   }
   T* dx = static_cast<T*>(g.dx) + (long long)p.b * a.len * a.dim + p.c;
   T* d_before = g.d_state_in ? static_cast<T*>(g.d_state_in) + (long long)p.b * (W - 1) * a.dim + p.c : nullptr;
-  // the first chunk also has the inputs in front of the sequence
-  const int lo = p.chunk == 0 ? -(W - 1) : first;
-  float x[W][V], dv[W][V];               // x_{t-W+1} .. x_t; dv_{t-W+1} .. dv_t
+  // ALL: these U tokens, the W - 1 in front of them and those that are asked for now are the chunk's own
+  const T *x_at = line.x + (lo + AHEAD) * a.x_st, *y_at = dy + (lo + AHEAD) * g.y_st;
+  T* o_at = dx + (long long)(lo - (W - 1)) * a.dim;
+  auto tokens = [&](int t0, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    copies_but<D - 1>();
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    if (i > 0) line.get(lo - W + i < -(W - 1) ? n : lo - W + i, x[i]);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (i == 0 || lo - W + i < -(W - 1)) x[i][j] = 0.f;
-      dv[i][j] = 0.f;
+    for (int u = 0; u < U; ++u) {
+      next_x.get(stage, u, x[W - 1 + u]);
+      next_y.get(stage, u, dv[W - 1 + u]);
     }
-  }
-  const int stop = max(last, p.chunk == 0 ? 0 : first);                // one behind the last s whose gradient is not zero by its place
-  for (int t = lo; t < stop + W - 1; ++t) {
+    if constexpr (ALL) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        next_x.put(stage, u, x_at + u * a.x_st);
+        next_y.put(stage, u, y_at + u * g.y_st);
+      }
+      copies_end();
+    } else {
+      ask(stage, t0 + AHEAD);
+    }
+    stage = stage + 1 < D ? stage + 1 : 0;
+    x_at += U * a.x_st;
+    y_at += U * g.y_st;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u;
+      if (!ALL && t >= stop) break;
+      const bool own = ALL || (t >= max(first, 0) && t < last);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        f32x2 e = dv[W - 1 + u][j];                                    // dy, 0 where there is none
+        if (a.silu) {
+          f32x2 v = bias[j];
+#pragma unroll
+          for (int i = 0; i < W; ++i) v = f2_fma(w[i][j], x[u + i][j], v);
+          const f32x2 s = sigmoid2(v);
+          // silu' = s (1 + v (1 - s))
+          const f32x2 rest = f2_fma(s, f2_splat(-1.f), f2_splat(1.f));
+          const f32x2 slope = f2_mul(s, f2_fma(v, rest, f2_splat(1.f)));
+          if (ALL || (t >= 0 && t < n)) e = f2_mul(e, slope);          // elsewhere x may be anything
+          dv[W - 1 + u][j] = e;
+        }
+        if (own) {
+          db[j] = f2_add(db[j], e);
+#pragma unroll
+          for (int i = 0; i < W; ++i) dw[i][j] = f2_fma(e, x[u + i][j], dw[i][j]);
+        }
+      }
+      const int s = t - (W - 1);
+      if (ALL || (s >= lo && (s >= 0 || d_before))) {
+        f32x2 o[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          o[j] = f2_mul(w[0][j], dv[W - 1 + u][j]);
+#pragma unroll
+          for (int i = 1; i < W; ++i) o[j] = f2_fma(w[i][j], dv[W - 1 + u - i][j], o[j]);
+        }
+        if (!ALL && ds && s >= n - (W - 1) && s < n) {
+          X v;
+          f32x2 q[P];
+          v.load(ds + (long long)(s - n + W - 1) * a.dim);
+          v.get(q);
+#pragma unroll
+          for (int j = 0; j < P; ++j) o[j] = f2_add(o[j], q[j]);
+        }
+        if (ALL || s >= 0) { if (ALL || s < last) X::put(o_at + u * a.dim, o); }
+        else X::put(d_before + (long long)(s + W - 1) * a.dim, o);
+      }
+    }
+    o_at += U * a.dim;
 #pragma unroll
     for (int i = 0; i < W - 1; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) { x[i][j] = x[i + 1][j]; dv[i][j] = dv[i + 1][j]; }
-    line.get(t, x[W - 1]);
-    const bool in = t >= 0 && t < n, own = in && t >= first && t < last;
-    float d[V];
-    if (in) Vec<T, V>::get(dy + t * g.y_st, d);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float e = 0.f;
-      if (in) {
-        e = d[j];
-        if (a.silu) {
-          float v = bias[j];
-#pragma unroll
-          for (int i = 0; i < W; ++i) v = fmaf(w[i][j], x[i][j], v);
-          const float s = sigmoid(v);
-          e *= s * fmaf(v, 1.f - s, 1.f);
-        }
-      }
-      dv[W - 1][j] = e;
-      if (own) {
-        db[j] += e;
-#pragma unroll
-        for (int i = 0; i < W; ++i) dw[i][j] = fmaf(e, x[i][j], dw[i][j]);
-      }
-    }
-    const int s = t - (W - 1);
-    if (s >= lo && (s >= 0 || d_before)) {
-      float o[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        o[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) o[j] = fmaf(w[i][j], dv[W - 1 - i][j], o[j]);
-      }
-      if (ds && s >= n - (W - 1) && s < n) {
-        float q[V];
-        Vec<T, V>::get(ds + (long long)(s - n + W - 1) * a.dim, q);
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] += q[j];
-      }
-      if (s >= 0) { if (s < last) Vec<T, V>::put(dx + (long long)s * a.dim, o); }
-      else Vec<T, V>::put(d_before + (long long)(s + W - 1) * a.dim, o);
-    }
-  }
-  const float zero[V] = {};
-  for (int t = max(first, last); t < end; ++t) Vec<T, V>::put(dx + (long long)t * a.dim, zero);
+      for (int j = 0; j < P; ++j) { x[i][j] = x[i + U][j]; dv[i][j] = dv[i + U][j]; }
+  };
+  int t0 = lo;
+  for (; t0 < max(lo, 0) + W - 1 && t0 < stop; t0 += U) tokens(t0, Const<false>());
+  for (; t0 + AHEAD + U <= last; t0 += U) tokens(t0, Const<true>());
+  for (; t0 < stop; t0 += U) tokens(t0, Const<false>());
+  const f32x2 zero[P] = {};
+  for (int t = max(first, last); t < end; ++t) X::put(dx + (long long)t * a.dim, zero);
   float* part = g.part + ((long long)p.b * a.chunks + p.chunk) * (W + 1) * a.dim + p.c;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
+  for (int i = 0; i <= W; ++i) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) part[(long long)i * a.dim + j] = dw[i][j];
-    part[(long long)W * a.dim + j] = db[j];
+    for (int j = 0; j < P; ++j) {
+      float f[2];
+      f2_unpack(i < W ? dw[i % W][j] : db[j], f[0], f[1]);
+      part[(long long)i * a.dim + 2 * j] = f[0];
+      if (V > 1) part[(long long)i * a.dim + 2 * j + 1] = f[1];
+    }
   }
 }
 
@@ -288,50 +452,58 @@ step_kernel(const StepArgs a) {
   const long long i = blockIdx.x * (long long)THREADS + threadIdx.x;
   if (i >= (long long)a.batch * cols) return;
   const int b = (int)(i / cols), c = (int)(i % cols) * V, W = a.taps;
+  constexpr int P = (V + 1) / 2;
+  using X = Vec<T, V>;
   T* s = static_cast<T*>(a.state) + b * a.s_b + c;
-  float x[MAX_TAPS][V], v[V];
+  X x[MAX_TAPS], last;
 #pragma unroll
-  for (int k = 0; k < MAX_TAPS; ++k) {
-    if (k < W - 1) {
+  for (int k = 0; k < MAX_TAPS - 1; ++k)
+    if (k < W - 1) x[k].load(s + (long long)k * a.dim);
+  last.load(static_cast<const T*>(a.x) + b * a.x_sb + c);
+  f32x2 v[P];
+  channels<V>(a.bias ? a.bias + c : nullptr, 1, v);
+  auto add = [&](const X& in, int k) {
+    f32x2 f[P], w[P];
+    in.get(f);
+    channels<V>(a.w + (long long)c * W + k, W, w);
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = 0.f;
-      Vec<T, V>::get(s + (long long)k * a.dim, x[k]);
-    }
+    for (int j = 0; j < P; ++j) v[j] = f2_fma(w[j], f[j], v[j]);
+  };
+#pragma unroll
+  for (int k = 0; k < MAX_TAPS - 1; ++k)
+    if (k < W - 1) add(x[k], k);
+  add(last, W - 1);
+  if (a.silu) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) v[j] = f2_mul(v[j], sigmoid2(v[j]));
   }
-  float last[V];
-  Vec<T, V>::get(static_cast<const T*>(a.x) + b * a.x_sb + c, last);
+  X::put(static_cast<T*>(a.y) + (long long)b * a.dim + c, v);
+  auto keep = [&](const X& in, int k) {
+    f32x2 f[P];
+    in.get(f);
+    X::put(s + (long long)k * a.dim, f);
+  };
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    v[j] = a.bias ? __ldg(a.bias + c + j) : 0.f;
-#pragma unroll
-    for (int k = 0; k < MAX_TAPS; ++k)
-      if (k < W - 1) v[j] = fmaf(__ldg(a.w + (long long)(c + j) * W + k), x[k][j], v[j]);
-    v[j] = fmaf(__ldg(a.w + (long long)(c + j) * W + W - 1), last[j], v[j]);
-    if (a.silu) v[j] *= sigmoid(v[j]);
-  }
-  Vec<T, V>::put(static_cast<T*>(a.y) + (long long)b * a.dim + c, v);
-#pragma unroll
-  for (int k = 1; k < MAX_TAPS; ++k)
-    if (k < W - 1) Vec<T, V>::put(s + (long long)(k - 1) * a.dim, x[k]);
-  if (W > 1) Vec<T, V>::put(s + (long long)(W - 2) * a.dim, last);
+  for (int k = 1; k < MAX_TAPS - 1; ++k)
+    if (k < W - 1) keep(x[k], k - 1);
+  if (W > 1) keep(last, W - 2);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-// Tokens of a thread: 32, fewer where that leaves SMs without 8 warps (two of 128 tokens have W - 1 in front of them read twice).
-static int chunk_of(int batch, int len, int dim, int v) {
-  const long long cols = (dim + v - 1) / v;
-  int chunk = 32;
-  while (chunk > 4 && (long long)batch * cols * ((len + chunk - 1) / chunk) < 256LL * m2_sm_count()) chunk /= 2;
-  return chunk;
+// Tokens of a thread: as many as let all threads run at once (a block that starts waits for its taps and its first tokens: 16 x 2048 x 1536 in four
+// rounds of 32 tokens took 55 us), but 8 at least, as W - 1 in front of them are read twice.
+static int chunk_of(int batch, int len, int dim, int v, int an_sm, int least) {
+  const long long cols = (dim + v - 1) / v, threads = (long long)an_sm * THREADS * m2_sm_count();
+  long long chunks = threads / (batch * cols);
+  if (chunks < 1) chunks = 1;
+  const long long chunk = (len + chunks - 1) / chunks;
+  return chunk < least ? least : (int)chunk;
 }
-// Of the gradients: their parameters' sums leave W + 1 numbers a channel and chunk.
-static int back_chunk_of(int batch, int len, int dim) {
-  int chunk = 256;
-  while (chunk > 16 && (long long)batch * dim / 4 * ((len + chunk - 1) / chunk) < 512LL * m2_sm_count()) chunk /= 2;
-  return chunk;
-}
+// Of the gradients: their parameters' sums leave W + 1 numbers a channel and chunk, and each chunk walks W - 1 tokens further.  The width of a
+// thread goes by the tensors' alignment, the workspace does not: chunks are those of the widest.
+static int back_chunk_of(int batch, int len, int dim) { return chunk_of(batch, len, dim, 4, 3, 16); }
 
-// channels of a thread: 16 bytes, fewer with many taps and in the gradient (registers); one where a row does not allow it
+// channels of a thread: 8 bytes (float32 forward with few taps 16); one where a row does not allow it
 static bool wide(const void* p, long long sb, long long st, int dim, int size, int bytes) {
   return !p || (m2_aligned(p, bytes) && sb * size % bytes == 0 && st * size % bytes == 0 && (long long)dim * size % bytes == 0);
 }
@@ -400,14 +572,14 @@ extern "C" int m2_causal_conv_fwd(const m2_causal_conv_args* args, void* stream)
   M2_REQUIRE(g.y || g.seq_len == 0, M2_ERR_ARG, "m2_causal_conv_fwd: y is NULL");
   const int size = g.dtype == M2_F32 ? 4 : 2;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int bytes = g.taps <= 4 ? 16 : 8;
+  const int bytes = g.dtype == M2_F32 && g.taps <= 4 ? 16 : 8;
   const bool vec = wide(g.x, g.x_sb, g.x_st, g.dim, size, bytes) && wide(a.state_in, 0, 0, g.dim, size, bytes) && wide(g.y, 0, 0, g.dim, size, bytes) &&
                    wide(a.state_out, 0, 0, g.dim, size, bytes);
-  a.chunk = chunk_of(g.batch, g.seq_len, g.dim, vec ? bytes / size : 1);
+  a.chunk = chunk_of(g.batch, g.seq_len, g.dim, vec ? bytes / size : 1, 5, 8);
   a.chunks = g.seq_len > 0 ? (g.seq_len + a.chunk - 1) / a.chunk : 1;
   const Grads none = {};
   if (g.dtype == M2_F32) return vec ? by_taps<float, 4, 2, false>(a, none, st) : by_taps<float, 1, 1, false>(a, none, st);
-  return vec ? by_taps<__nv_bfloat16, 8, 4, false>(a, none, st) : by_taps<__nv_bfloat16, 1, 1, false>(a, none, st);
+  return vec ? by_taps<__nv_bfloat16, 4, 4, false>(a, none, st) : by_taps<__nv_bfloat16, 1, 1, false>(a, none, st);
 }
 
 extern "C" int m2_causal_conv_bwd(const m2_causal_conv_args* args, const m2_causal_conv_grads* grads, void* stream) {

@@ -36,14 +36,23 @@ def _check(name, x, delta, a, b, c, skip, gate, delta_bias, dims):
     G = b.shape[-2]
     if G == 0 or D % G:
         raise ValueError(f"{name}: {G} groups of b and c do not divide {D} channels")
-    tensors = [x, delta, b, c] + ([gate] if gate is not None else [])
-    if any(t.dtype not in _TYPES or t.dtype != x.dtype for t in tensors):
-        raise TypeError(f"{name}: x, delta, b, c and gate are all float32 or all bfloat16, got {[t.dtype for t in tensors]}")
-    dev = x.get_device()
-    if dev < 0 or a.get_device() != dev or any(t.get_device() != dev for t in tensors):
+    dtype, dev = x.dtype, x.get_device()
+    if dtype not in _TYPES or delta.dtype != dtype or b.dtype != dtype or c.dtype != dtype or (gate is not None and gate.dtype != dtype):
+        raise TypeError(f"{name}: x, delta, b, c and gate are all float32 or all bfloat16, got {dtype}, {delta.dtype}, {b.dtype}, {c.dtype}"
+                        f"{'' if gate is None else f' and {gate.dtype}'}")
+    if dev < 0 or a.get_device() != dev or delta.get_device() != dev or b.get_device() != dev or c.get_device() != dev or \
+            (gate is not None and gate.get_device() != dev):
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
     return (b, c, _vector(name, "a", a, (D, N), dev), _vector(name, "skip", skip, (D,), dev) if skip is not None else None,
             _vector(name, "delta_bias", delta_bias, (D,), dev) if delta_bias is not None else None)
+
+
+def _wants_gradient(tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _two(t):
@@ -141,7 +150,7 @@ def selective_scan(x, delta, a, b, c, *, skip=None, gate=None, delta_bias=None, 
     lengths = _lengths(name, lengths, B, x)
     x, delta, b, c, gate = _packed(x), _packed(delta), _packed(b), _packed(c), _packed(gate) if gate is not None else None
     tensors = (x, delta, a, b, c, skip, gate, delta_bias, initial_state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _wants_gradient(tensors):
         y, state = _SelectiveScan.apply(*tensors, bool(softplus), lengths, return_state)
     else:
         y, state, _ = _forward(*tensors[:8], bool(softplus), initial_state, lengths, return_state, False)
@@ -158,7 +167,7 @@ def selective_scan_step(x, delta, a, b, c, state, *, skip=None, gate=None, delta
     s_b, s_d, s_n = state.stride()
     if (s_n != 1 and N > 1) or (s_d != N and D > 1) or (B > 1 and s_b < D * N):
         raise ValueError(f"{name}: state is updated in place: its last two dimensions are packed and no two sequences overlap, got strides {state.stride()}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, a, b, c, skip, gate, delta_bias, state)):
+    if _wants_gradient((x, delta, a, b, c, skip, gate, delta_bias, state)):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or selective_scan with initial_state")
     x, delta, b, c, gate = _packed(x), _packed(delta), _packed(b), _packed(c), _packed(gate) if gate is not None else None
     y = x.new_empty((B, D))

@@ -77,12 +77,12 @@ def test_beams_and_dropout_refuse():
 
 
 def test_states_that_share_memory_are_found():
-    assert beams._apart([(0, 16, 16, 4), (64, 16, 16, 4)]) and not beams._apart([(0, 16, 16, 4), (48, 16, 16, 4)])
-    assert not beams._apart([(0, 16, 16, 4), (0, 16, 16, 4)])
-    assert beams._apart([(0, 16, 64, 4), (16, 16, 64, 4), (48, 16, 64, 4), (32, 16, 64, 4)])       # rows side by side
-    assert not beams._apart([(0, 16, 64, 4), (8, 16, 64, 4)]) and not beams._apart([(0, 16, 64, 4), (56, 16, 64, 4)])
-    assert not beams._apart([(0, 16, 64, 4), (32, 16, 32, 4)])
-    assert beams._apart([(0, 0, 0, 4), (0, 16, 16, 4)])
+    assert beams._apart([(0, 16, 16), (64, 16, 16)], 4) and not beams._apart([(0, 16, 16), (48, 16, 16)], 4)
+    assert not beams._apart([(0, 16, 16), (0, 16, 16)], 4)
+    assert beams._apart([(0, 16, 64), (16, 16, 64), (48, 16, 64), (32, 16, 64)], 4)                 # rows side by side
+    assert not beams._apart([(0, 16, 64), (8, 16, 64)], 4) and not beams._apart([(0, 16, 64), (56, 16, 64)], 4)
+    assert not beams._apart([(0, 16, 64), (32, 16, 32)], 4)
+    assert beams._apart([(0, 0, 0), (0, 16, 16)], 4)
 
 
 def test_c_entries_refuse_before_any_launch():
