@@ -726,7 +726,7 @@ int m2_reorder_states(const m2_reorder_states_args* args, void* stream);
 /* ---------------------------------------------------------------------------------------
  * Dropout (the reference: nn.Dropout in training, bert/src/bert_layers.py:487, 505) from a counter-based generator, Philox 4x32-10:
  *   y = (kept(i) ? x / (1 - p) : 0) + residual
- *   x, y, residual (NULL: none): n values of `dtype`, packed; y may be x or the residual.  p = threshold / 65536.
+ *   x, y, residual (NULL: none): n values of `dtype`, packed, y in memory of its own.  p = threshold / 65536.
  *   Element i is kept if 16 bits of the block that key `key` gives for the counter (i / 8, call) are not below the threshold: halves of the
  *   four words in order, the low one first.  seed: NULL, or int64 (2) on the device: key and call are read there.
  * The gradient of x is the same call on the gradient of y without a residual.

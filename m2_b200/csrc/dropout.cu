@@ -11,7 +11,7 @@ namespace m2 {
 namespace drop {
 
 constexpr int THREADS = 256;
-constexpr int UNROLL = 2;                // groups of eight of a thread
+constexpr int AN_SM = 5;                 // blocks of an SM
 
 struct Args {
   const void *x, *residual;
@@ -39,66 +39,84 @@ __device__ __forceinline__ uint4 philox(unsigned long long counter, unsigned lon
   return make_uint4(c0, c1, c2, c3);
 }
 
-template <typename T> __device__ __forceinline__ void get8(const T* p, int valid, bool vec, float (&f)[8]) {
-  constexpr int E = lp::Piece<T>::N;
-  if (vec && valid >= 8) {
+template <typename T> struct Eight {     // elements as they lie in memory
+  static constexpr int E = lp::Piece<T>::N, P = 8 / E;
+  uint4 v[P];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 8; i += E) {
-      float v[E];
-      lp::Piece<T>::get(__ldcs(reinterpret_cast<const uint4*>(p + i)), v);
+    for (int i = 0; i < P; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
 #pragma unroll
-      for (int j = 0; j < E; ++j) f[i + j] = v[j];
+    for (int i = 0; i < P; ++i) {
+      float w[E];
+      lp::Piece<T>::get(v[i], w);
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[i * E + j] = w[j];
     }
-  } else {
+  }
+  static __device__ __forceinline__ void put(T* p, const float (&f)[8]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = j < valid ? lp::load1(p + j) : 0.f;
+    for (int i = 0; i < P; ++i) {
+      float w[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) w[j] = f[i * E + j];
+      reinterpret_cast<uint4*>(p)[i] = lp::Piece<T>::put(w);
+    }
+  }
+};
+
+// y of a group from its numbers
+template <bool RES> __device__ __forceinline__ void apply(const uint4& w, unsigned threshold, float scale, float (&f)[8], const float (&r)[8]) {
+  const uint32_t bits[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = j & 1 ? bits[j / 2] >> 16 : bits[j / 2] & 0xffffu;
+    const float v = b >= threshold ? f[j] * scale : 0.f;
+    f[j] = RES ? v + r[j] : v;
   }
 }
 
+// A thread takes one group after another; the next group's elements are under way while this one's numbers are made.
 template <typename T, bool RES>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, AN_SM)
 dropout_kernel(const Args a) {
-  constexpr int E = lp::Piece<T>::N;
   pdl_wait();
   const unsigned long long key = a.seed ? a.seed[0] : a.key, call = a.seed ? a.seed[1] : a.call;
-  const long long first = blockIdx.x * (long long)(THREADS * UNROLL) + threadIdx.x;
+  const long long step = (long long)gridDim.x * THREADS, whole = a.vec ? a.n / 8 : 0;     // whole groups on 16 bytes
   const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.residual);
   T* y = static_cast<T*>(a.y);
-  float f[UNROLL][8], r[UNROLL][8];
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const long long g = first + u * THREADS;
-    const int valid = g < a.groups ? (int)min(8LL, a.n - g * 8) : 0;
-    get8<T>(x + g * 8, valid, a.vec, f[u]);
-    if constexpr (RES) get8<T>(res + g * 8, valid, a.vec, r[u]);
+  long long g = blockIdx.x * (long long)THREADS + threadIdx.x;
+  Eight<T> next, next_r;
+  if (g < whole) {
+    next.load(x + g * 8);
+    if constexpr (RES) next_r.load(res + g * 8);
   }
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const long long g = first + u * THREADS;
-    if (g >= a.groups) return;
-    const int valid = (int)min(8LL, a.n - g * 8);
+  for (; g < whole; g += step) {
+    const Eight<T> now = next, now_r = next_r;
+    if (g + step < whole) {
+      next.load(x + (g + step) * 8);
+      if constexpr (RES) next_r.load(res + (g + step) * 8);
+    }
     const uint4 w = philox((unsigned long long)g, call, key);
-    const uint32_t bits[4] = {w.x, w.y, w.z, w.w};
+    float f[8], r[8];
+    now.get(f);
+    if constexpr (RES) now_r.get(r);
+    apply<RES>(w, a.threshold, a.scale, f, r);
+    Eight<T>::put(y + g * 8, f);
+  }
+  for (; g < a.groups; g += step) {        // one by one: the last group, or all where a tensor is not on 16 bytes
+    const uint4 w = philox((unsigned long long)g, call, key);
+    float f[8], r[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t b = j & 1 ? bits[j / 2] >> 16 : bits[j / 2] & 0xffffu;
-      const float v = b >= a.threshold ? f[u][j] * a.scale : 0.f;
-      f[u][j] = RES ? v + r[u][j] : v;
+      f[j] = g * 8 + j < a.n ? lp::load1(x + g * 8 + j) : 0.f;
+      if constexpr (RES) r[j] = g * 8 + j < a.n ? lp::load1(res + g * 8 + j) : 0.f;
     }
-    T* to = y + g * 8;
-    if (a.vec && valid == 8) {
+    apply<RES>(w, a.threshold, a.scale, f, r);
 #pragma unroll
-      for (int i = 0; i < 8; i += E) {
-        float v[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = f[u][i + j];
-        __stcs(reinterpret_cast<uint4*>(to + i), lp::Piece<T>::put(v));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < valid) st_from_float(to + j, f[u][j]);
-    }
+    for (int j = 0; j < 8; ++j)
+      if (g * 8 + j < a.n) st_from_float(y + g * 8 + j, f[j]);
   }
 }
 
@@ -119,8 +137,7 @@ extern "C" int m2_dropout(const m2_dropout_args* args, void* stream) {
              "m2_dropout: a tensor is not aligned to its type");
   Args a = {g.x, g.residual, g.y, g.n, (g.n + 7) / 8, (unsigned)g.threshold, g.threshold < 65536 ? 65536.f / (65536 - g.threshold) : 0.f,
             (const unsigned long long*)g.seed, g.key, g.call, m2_aligned(g.x, 16) && m2_aligned(g.y, 16) && m2_aligned(g.residual, 16)};
-  const long long blocks = (a.groups + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-  M2_REQUIRE(blocks <= 0x7fffffffLL, M2_ERR_UNSUPPORTED, "m2_dropout: %lld values are more than the grid takes", g.n);
+  const long long need = (a.groups + THREADS - 1) / THREADS, most = (long long)AN_SM * m2_sm_count(), blocks = need < most ? need : most;
   const cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto kernel) { return m2_launch("m2_dropout", g.n, kernel, dim3((unsigned)blocks), THREADS, 0, st, a); };
   if (g.dtype == M2_F32) return g.residual ? go(dropout_kernel<float, true>) : go(dropout_kernel<float, false>);
