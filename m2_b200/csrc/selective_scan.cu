@@ -577,6 +577,7 @@ template <int S, int QL> struct BackShared {
   float part[4][TT][NP];                 // db or dc of each warp's channels
   float mid[4][U * STEP];                // four steps of each pair of channels
   float da[S][THREADS][2];               // each thread's sums over the tiles
+  float middle[S][THREADS][2];           // its states in front of the tile's second half
 };
 
 // Four steps' values of a warp's pairs of channels are added up through shared memory: half the instructions of shuffles
@@ -741,6 +742,12 @@ back_kernel(const Args a, const Grads g) {
       decays<H>(dt_next, A, d_next);
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += U) {
+        if (t0 == TT / 2) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) *reinterpret_cast<f32x2*>(sh.middle[c * H + i][tid]) = h[c][i];
+        }
         float y[U][2], q[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -793,7 +800,7 @@ back_kernel(const Args a, const Grads g) {
       }
     };
     parts_to(g.part_c);
-    float end[2];                        // sum a g h behind the tile's last token
+    float end[2], middle[2];             // sum a g h behind the tile's last token, and in front of its second half
     f32x2 G0[2][H], own[2][H], cum = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -866,6 +873,15 @@ back_kernel(const Args a, const Grads g) {
           to_gq[(u - (U - 1)) * CT] = own_row ? fmaf(q_h[u], es[u], -r * xs[u]) : r;
         }
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
+        if (t0 == TT / 2) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            f32x2 v = 0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], ld2(sh.middle[c * H + i][tid])), A[c][i], v);
+            middle[c] = both(v);
+          }
+        }
         to_gq -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
       }
     }
@@ -878,8 +894,8 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
         for (int i = 0; i < H; ++i) G[c][i] = f2_fma(through[c][i], G0[c][i], own[c][i]);
     }
-    // a channel's sums, the second half of the tile from its end, the first from its start, where g and h are known too: rounding errors of the
-    // q_r e_r and p_r s x, which all later sums share, have half the way to pile up
+    // a channel's sums, in quarters of the tile from its ends and its middle, where g and h are both known: rounding errors of the q_r e_r and p_r s x,
+    // which all later sums share, have eight tokens to pile up
     in_front(h);
     float start[2];
 #pragma unroll
@@ -889,22 +905,32 @@ back_kernel(const Args a, const Grads g) {
       for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
       start[c] = both(v);
     }
-    float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane);    // lanes with bit 1: the tile's second half
+    float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane), m = sum_states<QL>(middle[0], middle[1], middle[0], middle[1], lane);
     __syncwarp();
-    if (lane % QL >= 4) {
-      // its sums are another lane's too
-    } else if (own_row) {
-#pragma unroll 4
-      for (int t = TT - 1; t >= TT / 2; --t) {
-        w += sh.q[t][own_ch];
-        sh.q[t][own_ch] = w * LN2;
-      }
-    } else {
-#pragma unroll 4
-      for (int t = 0; t < TT / 2; ++t) {
-        const float r = sh.q[t][own_ch];
-        sh.q[t][own_ch] = w * LN2;
-        w -= r;
+    if (lane % QL < 4) {                 // of eight lanes two have the same sums
+      constexpr int Q = TT / 4;
+      float* q = &sh.q[0][own_ch];
+      auto down = [&](int t, float v) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          v += q[(t - 1 - i) * CT];
+          q[(t - 1 - i) * CT] = v * LN2;
+        }
+      };
+      auto up = [&](int t, float v) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const float r = q[(t + i) * CT];
+          q[(t + i) * CT] = v * LN2;
+          v -= r;
+        }
+      };
+      if (own_row) {
+        down(TT, w);
+        up(2 * Q, m);
+      } else {
+        up(0, w);
+        down(2 * Q, m);
       }
     }
     __syncthreads();
