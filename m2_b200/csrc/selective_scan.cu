@@ -1152,18 +1152,19 @@ step_kernel(const StepArgs a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 struct Plan { int np, total, tiles, per_group, segs, seg_tiles; };
-// The axis is cut into segments where sequences and channels alone are fewer blocks than SMs, into as many as run at once: what a segment adds to the
-// state is then computed first, at the price of a second exp for each token, channel and state.
-static Plan plan_of(int batch, int len, int dim, int states, int groups) {
+// The axis is cut into segments where sequences and channels alone are fewer blocks than one and a half times the SMs, into as many as run at once: what a
+// segment adds to the state (its gradient) is then computed first, at the price of another exp for each token, channel and state.  With 144 blocks
+// (6 x 2048 x 1536) cut: 265 us and 643 back; with 168, not cut: 356 and 1030; with 288, not cut: 375 and 1046, where cut blocks would take about 530 and 1290.
+static Plan plan_of(int batch, int len, int dim, int states, int groups, bool backward) {
   Plan p;
   p.np = states <= 16 ? 16 : states <= 32 ? 32 : 64;
   p.total = (len + TT - 1) / TT;
   p.per_group = dim / groups;
   const int ct = channels_of(p.np == 64 ? 8 : 4);
   p.tiles = (p.per_group + ct - 1) / ct;
-  const long long blocks = (long long)batch * groups * p.tiles, want = (p.np == 16 ? 4LL : 2LL) * m2_sm_count();
+  const long long blocks = (long long)batch * groups * p.tiles, sms = m2_sm_count(), want = (p.np == 16 ? (backward ? 3 : 4) : 2) * sms;
   p.segs = 1;
-  if (blocks < m2_sm_count() && p.total >= 8) {
+  if (2 * blocks < 3 * sms && p.total >= 8) {
     long long s = want / (blocks > 0 ? blocks : 1);
     if (s > p.total / 2) s = p.total / 2;
     p.segs = s > 1 ? (int)s : 1;
@@ -1209,13 +1210,13 @@ static bool in_pieces(const void* p, long long sb, long long st, int per_group, 
   return m2_aligned(p, 16) && sb * size % 16 == 0 && st * size % 16 == 0 && (long long)per_group * size % 16 == 0;
 }
 
-static int check(const char* name, const m2_selective_scan_args& g, Args& a, Plan& p) {
+static int check(const char* name, const m2_selective_scan_args& g, Args& a, Plan& p, bool backward) {
   M2_REQUIRE(g.batch >= 0 && g.seq_len >= 0 && g.dim >= 1 && g.states >= 1 && g.groups >= 1 && g.dim % g.groups == 0, M2_ERR_ARG,
              "%s: %d sequences of %d tokens, %d channels, %d states, %d groups", name, g.batch, g.seq_len, g.dim, g.states, g.groups);
   M2_REQUIRE(g.states <= MAX_STATES, M2_ERR_UNSUPPORTED, "%s: %d states (at most %d)", name, g.states, MAX_STATES);
   M2_REQUIRE(g.dtype == M2_F32 || g.dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: tensors are float32 or bf16", name);
   M2_REQUIRE(g.seq_len <= 1 << 28 && g.dim <= 1 << 24, M2_ERR_UNSUPPORTED, "%s: %d tokens of %d channels", name, g.seq_len, g.dim);
-  p = plan_of(g.batch, g.seq_len, g.dim, g.states, g.groups);
+  p = plan_of(g.batch, g.seq_len, g.dim, g.states, g.groups, backward);
   M2_REQUIRE((long long)g.batch * p.segs * g.groups * p.tiles <= 0x7fffffffLL && ((long long)g.batch * g.dim * p.np + 255) / 256 <= 0x7fffffffLL &&
                  ((long long)g.batch * g.seq_len * g.groups * g.states + 255) / 256 <= 0x3fffffffLL,
              M2_ERR_UNSUPPORTED, "%s: %d sequences of %d channels are more than the grid takes", name, g.batch, g.dim);
@@ -1244,13 +1245,13 @@ static int check(const char* name, const m2_selective_scan_args& g, Args& a, Pla
 extern "C" long long m2_selective_scan_saves(int batch, int seq_len, int dim, int states, int groups) {
   using namespace m2::ss;
   if (batch <= 0 || seq_len <= 0 || dim <= 0 || states <= 0 || states > MAX_STATES || groups <= 0 || dim % groups) return 0;
-  return 4 * saves_floats(plan_of(batch, seq_len, dim, states, groups), batch, dim);
+  return 4 * saves_floats(plan_of(batch, seq_len, dim, states, groups, false), batch, dim);
 }
 
 extern "C" long long m2_selective_scan_workspace(int batch, int seq_len, int dim, int states, int groups, int backward) {
   using namespace m2::ss;
   if (batch <= 0 || seq_len < 0 || dim <= 0 || states <= 0 || states > MAX_STATES || groups <= 0 || dim % groups) return 0;
-  const Plan p = plan_of(batch, seq_len, dim, states, groups);
+  const Plan p = plan_of(batch, seq_len, dim, states, groups, backward != 0);
   return 4 * (backward ? grad_floats(p, batch, seq_len, dim, groups) : seg_floats(p, batch, dim));
 }
 
@@ -1265,7 +1266,7 @@ extern "C" int m2_selective_scan_fwd(const m2_selective_scan_args* args, void* s
   const m2_selective_scan_args& g = *args;
   Args a;
   Plan p;
-  if (int rc = check("m2_selective_scan_fwd", g, a, p)) return rc;
+  if (int rc = check("m2_selective_scan_fwd", g, a, p, false)) return rc;
   if (g.batch == 0) return M2_OK;
   M2_REQUIRE(g.y || g.seq_len == 0, M2_ERR_ARG, "m2_selective_scan_fwd: y is NULL");
   const long long need = 4 * seg_floats(p, g.batch, g.dim), keep = 4 * saves_floats(p, g.batch, g.dim);
@@ -1284,7 +1285,7 @@ extern "C" int m2_selective_scan_bwd(const m2_selective_scan_args* args, const m
   const m2_selective_scan_grads& o = *grads;
   Args a;
   Plan p;
-  if (int rc = check("m2_selective_scan_bwd", g, a, p)) return rc;
+  if (int rc = check("m2_selective_scan_bwd", g, a, p, true)) return rc;
   if (g.batch == 0) return M2_OK;
   M2_REQUIRE(g.seq_len == 0 || (o.d_y && o.d_x && o.d_delta && o.d_b && o.d_c && (!g.gate == !o.d_gate)), M2_ERR_ARG,
              "m2_selective_scan_bwd: d_y or a gradient is NULL");
