@@ -134,11 +134,12 @@ template <typename T, int V, int W> struct Line {
   }
 };
 
-// The next R times U tokens of a thread: copies under way into its own part of shared memory, or (pieces below 8 bytes) U of them in registers.
-constexpr int U = 4, R = 4;
+// The next tokens of a thread, U at a time: copies under way into its own part of shared memory, a ring of R stages of which one is being used, one was
+// used before and is asked for anew, and the others are under way; or (pieces below 8 bytes) U of them in registers.
+constexpr int U = 4, R = 5;
 template <typename T, int V> struct Ring {
   static constexpr bool ASYNC = Vec<T, V>::BYTES >= 8;
-  static constexpr int DEPTH = ASYNC ? R : 1, WORDS = Vec<T, V>::WORDS, SIZE = ASYNC ? R * U * THREADS * WORDS : 1;     // words of shared memory
+  static constexpr int DEPTH = ASYNC ? R : 1, UNDER_WAY = ASYNC ? R - 1 : 1, WORDS = Vec<T, V>::WORDS, SIZE = ASYNC ? R * U * THREADS * WORDS : 1;     // words of shared memory
   uint32_t* sm;
   Vec<T, V> reg[ASYNC ? 1 : U];
   __device__ __forceinline__ Ring(uint32_t* s) : sm(s + threadIdx.x * WORDS) {}
@@ -203,12 +204,12 @@ conv_kernel(const Args a) {
   const int n = text_length(a, p.b);
   const Line<T, V, W> line(a, p.b, p.c, n);
   const int first = p.chunk * a.chunk, end = min(first + a.chunk, a.len), last = min(end, n);
-  constexpr int D = Ring<T, V>::DEPTH, AHEAD = D * U;
+  constexpr int D = Ring<T, V>::DEPTH, M = Ring<T, V>::UNDER_WAY, AHEAD = M * U;
   __shared__ __align__(16) uint32_t s_ring[Ring<T, V>::SIZE];
   Ring<T, V> next(s_ring);
   const T* x_at = line.x + first * a.x_st;
   int stage = 0;
-  for (int s = 0; s < D; ++s) {
+  for (int s = 0; s < M; ++s) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (first + s * U + u < last) next.put(s, u, x_at + u * a.x_st);
@@ -225,12 +226,13 @@ conv_kernel(const Args a) {
   // ALL: neither these U tokens nor those that are asked for now end the chunk
   auto tokens = [&](int t, auto all) {
     constexpr bool ALL = decltype(all)::value;
-    copies_but<D - 1>();
+    copies_but<M - 1>();
 #pragma unroll
     for (int u = 0; u < U; ++u) next.get(stage, u, x[W - 1 + u]);
+    const int used = stage > 0 ? stage - 1 : D - 1;          // by the tokens before these
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (ALL || t + AHEAD + u < last) next.put(stage, u, x_at + u * a.x_st);
+      if (ALL || t + AHEAD + u < last) next.put(used, u, x_at + u * a.x_st);
     copies_end();
     x_at += U * a.x_st;
     stage = stage + 1 < D ? stage + 1 : 0;
@@ -288,7 +290,7 @@ back_kernel(const Args a, const Grads g) {
   // the first chunk also has the inputs in front of the sequence
   const int lo = p.chunk == 0 ? -(W - 1) : first;
   const int stop = max(last, p.chunk == 0 ? 0 : first) + W - 1;        // the last s whose gradient is not zero by its place, and what it needs
-  constexpr int D = Ring<T, V>::DEPTH, AHEAD = D * U;
+  constexpr int D = Ring<T, V>::DEPTH, M = Ring<T, V>::UNDER_WAY, AHEAD = M * U;
   __shared__ __align__(16) uint32_t s_x[Ring<T, V>::SIZE], s_y[Ring<T, V>::SIZE];
   Ring<T, V> next_x(s_x), next_y(s_y);
   auto ask = [&](int stage, int t0) {
@@ -300,7 +302,7 @@ back_kernel(const Args a, const Grads g) {
     }
     copies_end();
   };
-  for (int s = 0; s < D; ++s) ask(s, lo + s * U);
+  for (int s = 0; s < M; ++s) ask(s, lo + s * U);
   int stage = 0;
   f32x2 w[W][P], bias[P], dw[W][P], db[P];
   channels<V>(a.bias ? a.bias + p.c : nullptr, 1, bias);
@@ -325,21 +327,22 @@ back_kernel(const Args a, const Grads g) {
   T* o_at = dx + (long long)(lo - (W - 1)) * a.dim;
   auto tokens = [&](int t0, auto all) {
     constexpr bool ALL = decltype(all)::value;
-    copies_but<D - 1>();
+    copies_but<M - 1>();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       next_x.get(stage, u, x[W - 1 + u]);
       next_y.get(stage, u, dv[W - 1 + u]);
     }
+    const int used = stage > 0 ? stage - 1 : D - 1;          // by the tokens before these
     if constexpr (ALL) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        next_x.put(stage, u, x_at + u * a.x_st);
-        next_y.put(stage, u, y_at + u * g.y_st);
+        next_x.put(used, u, x_at + u * a.x_st);
+        next_y.put(used, u, y_at + u * g.y_st);
       }
       copies_end();
     } else {
-      ask(stage, t0 + AHEAD);
+      ask(used, t0 + AHEAD);
     }
     stage = stage + 1 < D ? stage + 1 : 0;
     x_at += U * a.x_st;
