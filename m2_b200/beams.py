@@ -73,7 +73,14 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_id=None):
 
 def _apart(states, rows):
     """Whether no element belongs to two of the states, each (pointer, bytes of a row, distance of rows), of `rows` rows."""
-    order = sorted((p, row, step) for p, row, step in states if row)
+    order, last = sorted(states), 0
+    for p, row, step in order:
+        if p < last and row:
+            break
+        last = p + step * (rows - 1) + row if row else last
+    else:
+        return True                                            # one behind the other
+    order = [s for s in order if s[1]]
     ends = [p + step * (rows - 1) + row for p, row, step in order]
     for i, (p, row, step) in enumerate(order):
         for q, row2, step2 in order[i + 1:]:

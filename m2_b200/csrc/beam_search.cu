@@ -8,6 +8,8 @@
 // that the order is that of exact scores but for gaps below about 1e-7.
 // States: a thread owns a few bytes of the rows of all beams of one text; it reads the rows that its beams come from before it writes any,
 // so that nothing waits and no second buffer is needed.  Rows that stay are neither read nor written.
+// Measured: selection for one text of four beams 17 us, for 32 of eight beams (float32, 31 MB) 27; states of 12 layers of the latter (256 rows of 58 KB a layer) 40 us,
+// 0.97 of the measured copy rate counted as if all rows moved.
 #include "common.cuh"
 
 namespace m2 {
@@ -297,7 +299,9 @@ extern "C" int m2_beam_select(const m2_beam_select_args* args, void* stream) {
   Args a = {g.logits, g.x_sb, g.x_sk, g.batch, g.beams, g.vocab, g.keep, g.keep < g.vocab ? g.keep : g.vocab, 1, g.scores, (const unsigned char*)g.finished, g.end_id,
             reinterpret_cast<float*>(w + up16(rows * 8)), reinterpret_cast<double*>(w), reinterpret_cast<unsigned long long*>(w + up16(rows * 8) + up16(rows * 4)),
             g.score, (long long*)g.beam, (long long*)g.token, (unsigned char*)g.done};
-  while (a.split < m2::lp::MAX_SPLIT && rows * a.split < 2LL * m2_sm_count() && g.vocab / (a.split * 2) >= 4096) a.split *= 2;
+  // a row is shared by the blocks of a cluster where the rows alone do not fill the GPU, each block with 2048 logits at least (one text of four beams, 30528
+  // logits: 13 us with slices of 2048, 15 with 4096); shared further than to two blocks an SM, 256 rows took 30 us instead of 22
+  while (a.split < m2::lp::MAX_SPLIT && rows * a.split < 2LL * m2_sm_count() && g.vocab / (a.split * 2) >= 2048) a.split *= 2;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * a.split));

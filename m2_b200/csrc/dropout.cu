@@ -4,7 +4,8 @@
 // counter the number of a group of eight elements and the number of the call; each of the four words serves two elements, 16 bits each.  An element is
 // kept if its 16 bits are not below p 2^16, so that p is a multiple of 2^-16 and 1 / (1 - p) is that p's.
 // The reference drops out with torch's nn.Dropout (bert/src/bert_layers.py:487, 505).
-// Bound: memory; ten rounds of two products for eight elements.
+// Bound: memory; ten rounds of two products, some 190 instructions in all, for eight elements.  Measured: 16 x 2048 x 1536 bf16 with a residual 57 us
+// (302 MB, 5.3 TB/s), its gradient 42 (201 MB).  Two groups a thread and many short blocks took 70 and 51.
 #include "common.cuh"
 
 namespace m2 {
