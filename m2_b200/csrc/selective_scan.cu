@@ -28,7 +28,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 __host__ __device__ constexpr int channels_of(int ql) { return 256 / ql; }                          // of a block
 
 struct Rows { const void* p; long long sb, st; int vec; };           // vec: 16-byte pieces
-struct Group { const void* p; long long sb, st, sg; };
+struct Group { const void* p; long long sb, st, sg; int vec; };       // vec: four states at once
 
 struct Args {
   int batch, len, dim, states, groups, per_group, tiles, softplus;   // per_group: channels of a group; tiles: blocks that share them
@@ -192,21 +192,81 @@ __device__ __forceinline__ int text_length(const Args& a, int b) {
   return (int)(n < 0 ? 0 : n > a.len ? a.len : n);
 }
 
-// b and c of a tile
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+
+// b or c of a tile: PER times four states of a token a thread
 template <typename T, int NP> struct Coeffs {
-  static constexpr int PER = TT * NP / THREADS;
-  float v[PER];
+  static constexpr int PER = TT * NP / 4 / THREADS, WORDS = (int)sizeof(T);           // words of four states
+  uint32_t w[PER][WORDS];
+  static __device__ __forceinline__ int token(int i) { return (threadIdx.x + i * THREADS) / (NP / 4); }
+  static __device__ __forceinline__ int state(int i) { return (threadIdx.x + i * THREADS) % (NP / 4) * 4; }
+  static __device__ __forceinline__ const T* at(const Group& r, const Place& p, int t0, int i) {
+    return static_cast<const T*>(r.p) + p.b * r.sb + p.g * r.sg + (t0 + token(i)) * r.st + state(i);
+  }
+  // four states whose rows are in no such pieces, or end among them
+  __device__ __forceinline__ void one_by_one(const T* from, int i, int live) {
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) w[i][j] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= live) continue;
+      if constexpr (sizeof(T) == 4) w[i][j] = __ldg(reinterpret_cast<const uint32_t*>(from) + j);
+      else w[i][j / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(from) + j) << (j & 1) * 16;
+    }
+  }
   __device__ __forceinline__ void fetch(const Group& r, const Place& p, int t0, int n, int states) {
-    const T* base = static_cast<const T*>(r.p) + p.b * r.sb + p.g * r.sg;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = threadIdx.x + i * THREADS, t = t0 + at / NP, s = at % NP;
-      v[i] = t < n && s < states ? lp::load1(base + t * r.st + s) : 0.f;
+      const T* from = at(r, p, t0, i);
+      const int live = t0 + token(i) < n ? states - state(i) : 0;
+      if (r.vec && live >= 4) {
+        if constexpr (sizeof(T) == 4) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(from));
+          w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+        } else {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(from));
+          w[i][0] = u.x; w[i][1] = u.y;
+        }
+      } else {
+        one_by_one(from, i, live);
+      }
     }
   }
   __device__ __forceinline__ void put(float* sm) const {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sm[threadIdx.x + i * THREADS] = v[i];
+    for (int i = 0; i < PER; ++i) {
+      float4 v;
+      if constexpr (sizeof(T) == 4) {
+        v = make_float4(__uint_as_float(w[i][0]), __uint_as_float(w[i][1]), __uint_as_float(w[i][2]), __uint_as_float(w[i][3]));
+      } else {
+        v = make_float4(__uint_as_float(w[i][0] << 16), __uint_as_float(w[i][0] & 0xffff0000u), __uint_as_float(w[i][1] << 16), __uint_as_float(w[i][1] & 0xffff0000u));
+      }
+      *reinterpret_cast<float4*>(sm + 4 * (threadIdx.x + i * THREADS)) = v;
+    }
+  }
+  // under way into a place of the thread's own in shared memory, and out of it
+  __device__ __forceinline__ void ask(uint2* slot, const Group& r, const Place& p, int t0, int n, int states) {
+    static_assert(sizeof(T) == 2, "float32 is fetched");
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const T* from = at(r, p, t0, i);
+      const int live = t0 + token(i) < n ? states - state(i) : 0;
+      if (r.vec && live >= 4) {
+        copy_async<8>(slot + i * THREADS, from);
+      } else {
+        one_by_one(from, i, live);
+        slot[i * THREADS] = make_uint2(w[i][0], w[i][1]);
+      }
+    }
+  }
+  __device__ __forceinline__ void take(const uint2* slot) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint2 u = slot[i * THREADS];
+      w[i][0] = u.x; w[i][1] = u.y;
+    }
   }
 };
 
@@ -229,6 +289,23 @@ template <typename T, int CT> struct Pieces {                           // a thr
       }
     }
   }
+  // under way into a place of the thread's own in shared memory, and out of it
+  __device__ __forceinline__ void ask(uint4* slot, const Rows& r, const Place& p, int t0, int n) {
+    const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
+    const T* at = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col + (t0 + row) * r.st;
+    if (r.vec && p.valid == CT && t0 + TT <= n) {                        // for the whole block alike
+#pragma unroll
+      for (int i = 0; i < P; ++i) copy_async<16>(slot + i * THREADS, at + i * ROWS * r.st);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < P; ++i)
+        slot[i * THREADS] = t0 + row + i * ROWS < n ? load_piece<T>(at + i * ROWS * r.st, p.valid - col, r.vec) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void take(const uint4* slot) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = slot[i * THREADS];
+  }
   // into L2, so that fetch() waits less
   static __device__ __forceinline__ void ask(const Rows& r, const Place& p, int t0, int n) {
     const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
@@ -242,6 +319,16 @@ template <typename T, int CT> struct Pieces {                           // a thr
   }
 };
 
+// A block's next tile while one is computed: two places in turn for a thread's pieces of x, delta and z and its states of b and c.  (float32 and more states fetch
+// theirs when a tile begins: registers and shared memory are full.)
+template <typename T, int S, int QL> struct Ahead {
+  static constexpr bool USED = sizeof(T) == 2 && S == 4;
+  static constexpr int P = Pieces<T, channels_of(QL)>::P, PER = Coeffs<T, QL * S>::PER;
+  uint4 rows[2][3][P * THREADS];
+  uint2 states[2][2][PER * THREADS];
+  static constexpr size_t bytes() { return USED ? sizeof(Ahead) : 0; }
+};
+
 // A segment's part of y, or (SUMS) its own contribution to the state and the sum of its steps.
 template <typename T, int S, int QL, bool SUMS>
 __global__ void __launch_bounds__(THREADS, S == 4 ? 4 : 2)
@@ -249,8 +336,8 @@ scan_kernel(const Args a) {
   constexpr int NP = QL * S, CT = channels_of(QL);
   using Px = Pieces<T, CT>;
   constexpr int E = Px::E;
-  // two rows and one more than a tile has: what the loop asks for ahead of its end
-  __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_y[TT][CT], s_b[TT + 1][NP], s_c[TT + 1][NP], s_bias[CT], s_skip[CT];
+  // two rows and one more than a tile has: what the loop asks for ahead of its end.  y takes the place of s x.
+  __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_b[TT + 1][NP], s_c[TT + 1][NP], s_bias[CT], s_skip[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place p = place_of<CT>(a);
   pdl_wait();
@@ -290,16 +377,49 @@ scan_kernel(const Args a) {
   T* y = static_cast<T*>(a.y) + (long long)p.b * a.len * a.dim + p.ch0 + col;
   Px x, delta, z;
   Coeffs<T, NP> fb, fc;
+  extern __shared__ __align__(16) unsigned char s_ahead[];
+  constexpr bool AHEAD = Ahead<T, S, QL>::USED;
+  auto& ahead = *reinterpret_cast<Ahead<T, S, QL>*>(s_ahead);
+  auto ask = [&](int k) {
+    if constexpr (AHEAD) {
+      uint4* rows = &ahead.rows[k & 1][0][tid];
+      uint2* states = &ahead.states[k & 1][0][tid];
+      constexpr int R = Px::P * THREADS, C = Coeffs<T, NP>::PER * THREADS;
+      x.ask(rows, a.x, p, k * TT, n);
+      delta.ask(rows + R, a.delta, p, k * TT, n);
+      fb.ask(states, a.b, p, k * TT, n, a.states);
+      if constexpr (!SUMS) {
+        if (a.z.p) z.ask(rows + 2 * R, a.z, p, k * TT, n);
+        fc.ask(states + C, a.c, p, k * TT, n, a.states);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
   auto fetch = [&](int k) {
-    x.fetch(a.x, p, k * TT, n);
-    delta.fetch(a.delta, p, k * TT, n);
-    fb.fetch(a.b, p, k * TT, n, a.states);
-    if constexpr (!SUMS) {
-      if (a.z.p) z.fetch(a.z, p, k * TT, n);
-      fc.fetch(a.c, p, k * TT, n, a.states);
+    if constexpr (AHEAD) {
+      const uint4* rows = &ahead.rows[k & 1][0][tid];
+      const uint2* states = &ahead.states[k & 1][0][tid];
+      constexpr int R = Px::P * THREADS, C = Coeffs<T, NP>::PER * THREADS;
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      x.take(rows);
+      delta.take(rows + R);
+      fb.take(states);
+      if constexpr (!SUMS) {
+        if (a.z.p) z.take(rows + 2 * R);
+        fc.take(states + C);
+      }
+    } else {
+      x.fetch(a.x, p, k * TT, n);
+      delta.fetch(a.delta, p, k * TT, n);
+      fb.fetch(a.b, p, k * TT, n, a.states);
+      if constexpr (!SUMS) {
+        if (a.z.p) z.fetch(a.z, p, k * TT, n);
+        fc.fetch(a.c, p, k * TT, n, a.states);
+      }
     }
   };
   f32x2 steps = 0;
+  if (first < used) ask(first);
   __syncthreads();
   for (int k = first; k < used; ++k) {
     fetch(k);
@@ -337,15 +457,19 @@ scan_kernel(const Args a) {
     if constexpr (!SUMS) fc.put(&s_c[0][0]);
     __syncthreads();
     if (k + 1 < used) {
-      Px::ask(a.x, p, (k + 1) * TT, n);
-      Px::ask(a.delta, p, (k + 1) * TT, n);
-      if (!SUMS && a.z.p) Px::ask(a.z, p, (k + 1) * TT, n);
+      if constexpr (AHEAD) {             // into the place that the tile before this one had
+        ask(k + 1);
+      } else {
+        Px::ask(a.x, p, (k + 1) * TT, n);
+        Px::ask(a.delta, p, (k + 1) * TT, n);
+        if (!SUMS && a.z.p) Px::ask(a.z, p, (k + 1) * TT, n);
+      }
     }
     {
       constexpr int U = 4;
       Token<H, false, !SUMS> next;
       const float *p_dt = &s_dt[0][cl], *p_dx = &s_dx[0][cl], *p_b = &s_b[0][q0], *p_c = &s_c[0][q0];
-      float* p_y = &s_y[(lane >> 1) & 1][cl + (lane & 1)];
+      float* p_y = &s_dx[(lane >> 1) & 1][cl + (lane & 1)];
       f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[2][H];
       next.get(p_dx, nullptr, p_b, p_c);
       decays<H>(dt, A, d_next);
@@ -405,7 +529,7 @@ scan_kernel(const Args a) {
         const int t = k * TT + row + i * Px::ROWS;
         if (t >= a.len) continue;
         float f[E], u[E];
-        from_shared(&s_y[row + i * Px::ROWS][col], f);
+        from_shared(&s_dx[row + i * Px::ROWS][col], f);
         Piece<T>::get(x.v[i], u);
 #pragma unroll
         for (int j = 0; j < E; ++j) f[j] = fmaf(skip[j], u[j], f[j]);
@@ -1172,14 +1296,17 @@ static long long grad_floats(const Plan& p, int batch, int len, int dim, int gro
 }
 
 template <typename T, int S, int QL> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
+  constexpr size_t smem = Ahead<T, S, QL>::bytes();
   const long long blocks = (long long)a.batch * p.segs * a.groups * p.tiles, size = (long long)a.batch * a.len * a.dim;
   if (p.segs > 1) {
-    if (int rc = m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, true>, dim3((unsigned)blocks), THREADS, 0, st, a)) return rc;
+    if (smem) M2_SMEM_ONCE((scan_kernel<T, S, QL, true>), smem);
+    if (int rc = m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, true>, dim3((unsigned)blocks), THREADS, smem, st, a)) return rc;
     const long long n = (long long)a.batch * a.dim * p.np;
     if (int rc = m2_launch("m2_selective_scan_fwd", size, join_kernel, dim3((unsigned)((n + 255) / 256)), 256, 0, st, a.a, a.seg_state, a.seg_steps,
                            a.state_in, a.batch, p.segs, a.dim, a.states, p.np, 0)) return rc;
   }
-  return m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, false>, dim3((unsigned)blocks), THREADS, 0, st, a);
+  if (smem) M2_SMEM_ONCE((scan_kernel<T, S, QL, false>), smem);
+  return m2_launch("m2_selective_scan_fwd", size, scan_kernel<T, S, QL, false>, dim3((unsigned)blocks), THREADS, smem, st, a);
 }
 
 template <typename T, int S, int QL> static int backward(const Args& a, const Grads& g, const Plan& p, cudaStream_t st) {
@@ -1222,7 +1349,8 @@ static int check(const char* name, const m2_selective_scan_args& g, Args& a, Pla
   a.batch = g.batch; a.len = g.seq_len; a.dim = g.dim; a.states = g.states; a.groups = g.groups; a.per_group = p.per_group; a.tiles = p.tiles;
   a.softplus = g.softplus;
   a.x = rows(g.x, g.x_sb, g.x_st); a.delta = rows(g.delta, g.d_sb, g.d_st); a.z = rows(g.gate, g.z_sb, g.z_st);
-  a.b = {g.b, g.b_sb, g.b_st, g.b_sg}; a.c = {g.c, g.c_sb, g.c_st, g.c_sg};
+  auto fours = [&](const void* q, long long sb, long long st, long long sg) { return m2_aligned(q, 4 * size) && sb % 4 == 0 && st % 4 == 0 && sg % 4 == 0; };
+  a.b = {g.b, g.b_sb, g.b_st, g.b_sg, fours(g.b, g.b_sb, g.b_st, g.b_sg)}; a.c = {g.c, g.c_sb, g.c_st, g.c_sg, fours(g.c, g.c_sb, g.c_st, g.c_sg)};
   a.a = g.a; a.skip = g.skip; a.bias = g.delta_bias; a.lengths = (const long long*)g.lengths; a.state_in = g.state_in;
   a.y = g.y; a.state_out = g.state_out; a.saves = g.saves; a.segs = p.segs; a.seg_tiles = p.seg_tiles;
   a.seg_state = g.workspace; a.seg_steps = g.workspace ? g.workspace + (long long)g.batch * p.segs * g.dim * p.np : nullptr;
