@@ -8,11 +8,11 @@
 // it: 20 packed FMAs, 8 exps, 4 loads from shared memory for 16 channels and 16 states a token, 70 to 80 in all, 240 back.  No tensor cores: every channel has
 // decays of its own, so that no product shares an operand.  A block has 64 channels and takes 32 tokens at a time: elementwise part (steps, gates) by
 // pieces of 16 bytes, then the recurrence with two channels and four states a thread, in registers; y is summed over four lanes.
-// Measured (bf16, 16 states): 16 x 2048 x 1536 forward 465 us (exps alone 179), gradients 1370 (358); 64 x 512 x 1536 forward 386; 1 x 32768 x 768 forward 344 us in
-// three launches (179, as the sums of the segments need the exps too).  At all SMs' full the forward kernel issues in 56 % of the cycles, exps 58 %, FMAs 43 %,
-// shared memory 53 %; back 57, 40, 51 and 67.  An exp in four as a polynomial on the FMA pipe: 526 us instead of 481; operands doubled in shared memory for packed
-// FMAs: 479 and 1457 instead of 465 and 1370; reductions of y and q through shared memory instead of shuffles: 1749 back; the next tile's pieces held in
-// registers: 512.
+// Measured (bf16, 16 states): 16 x 2048 x 1536 forward 432 us (exps alone 179), gradients 1360 (358); 1 x 32768 x 768 forward 332 us in three launches (179, as the
+// sums of the segments need the exps too).  With all SMs full the forward kernel issued in 56 % of the cycles, exps 58 %, FMAs 43 %, shared memory 53 % (before the
+// next tile's pieces were copied ahead); back 57, 40, 51 and 67.  An exp in four as a polynomial on the FMA pipe: 526 us where the exps alone took 481; operands doubled
+// in shared memory for packed FMAs: 479 and 1457 where 465 and 1370 were; reductions of y and q through shared memory instead of shuffles: 1749 back; the next
+// tile's pieces held in registers: 512 where 465 were.
 #include "common.cuh"
 
 namespace m2 {
@@ -51,6 +51,7 @@ struct Grads {
   int vec;                               // packed outputs in 16-byte pieces
   float *part_b, *part_c;                // (tiles, batch, len, groups, NP)
   float *part_a, *part_skip, *part_bias; // (batch * segs, dim, NP), (batch * segs, dim) twice
+  float* quarters;                       // more than 16 states: (blocks, 2, S, THREADS, 2), each thread's states after a quarter and three of a tile
   void *db, *dc;
   float *da, *d_skip, *d_bias, *d_state_in;
 };
@@ -753,6 +754,8 @@ back_kernel(const Args a, const Grads g) {
   constexpr int E = Px::E;
   extern __shared__ __align__(16) unsigned char raw[];
   BackShared<S, QL>& sh = *reinterpret_cast<BackShared<S, QL>*>(raw);
+  constexpr bool QUARTERS = S > 4;       // its own loads and stores only, but through L2: shared memory has no room for them
+  f32x2* quarter = reinterpret_cast<f32x2*>(g.quarters) + (long long)blockIdx.x * (2 * S * THREADS) + threadIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place p = place_of<CT>(a);
   pdl_wait();
@@ -883,6 +886,12 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
             for (int i = 0; i < H; ++i) *reinterpret_cast<f32x2*>(sh.middle[c * H + i][tid]) = h[c][i];
         }
+        if (QUARTERS && t0 % (TT / 2) == TT / 4) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) quarter[(t0 / (TT / 2) * S + c * H + i) * THREADS] = h[c][i];
+        }
         float y[U][2], q[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -935,7 +944,7 @@ back_kernel(const Args a, const Grads g) {
       }
     };
     parts_to(g.part_c);
-    float end[2], middle[2];             // sum a g h behind the tile's last token, and in front of its second half
+    float end[2], middle[2], low[2] = {0.f, 0.f}, high[2] = {0.f, 0.f};     // sum a g h behind the tile's last token, in front of its second half and of its quarters
     f32x2 G0[2][H], own[2][H], cum = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -1017,6 +1026,15 @@ back_kernel(const Args a, const Grads g) {
             middle[c] = both(v);
           }
         }
+        if (QUARTERS && t0 % (TT / 2) == TT / 4) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            f32x2 v = 0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], quarter[(t0 / (TT / 2) * S + c * H + i) * THREADS]), A[c][i], v);
+            (t0 > TT / 2 ? high : low)[c] = both(v);
+          }
+        }
         to_gq -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
       }
     }
@@ -1029,8 +1047,8 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
         for (int i = 0; i < H; ++i) G[c][i] = f2_fma(through[c][i], G0[c][i], own[c][i]);
     }
-    // a channel's sums, in quarters of the tile from its ends and its middle, where g and h are both known: rounding errors of the q_r e_r and p_r s x,
-    // which all later sums share, have eight tokens to pile up
+    // a channel's sums, in pieces of the tile from its ends and its middle (with more than 16 states from its quarters too), where g and h are both known: rounding
+    // errors of the q_r e_r and p_r s x, which all later sums share, have eight (four) tokens to pile up
     in_front(h);
     float start[2];
 #pragma unroll
@@ -1040,11 +1058,12 @@ back_kernel(const Args a, const Grads g) {
       for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
       start[c] = both(v);
     }
-    float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane), m = sum_states<QL>(middle[0], middle[1], middle[0], middle[1], lane);
+    const float from = sum_states<QL>(start[0], start[1], middle[0], middle[1], lane), till = sum_states<QL>(middle[0], middle[1], end[0], end[1], lane);
+    const float inner = QUARTERS ? sum_states<QL>(low[0], low[1], high[0], high[1], lane) : 0.f;
     __syncwarp();
-    if (lane % QL < 4) {                 // of eight lanes two have the same sums
-      constexpr int Q = TT / 4;
-      float* q = &sh.q[0][own_ch];
+    if (lane % QL < 4) {                 // of eight lanes two have the same sums; lanes with bit 1 have the second half
+      constexpr int Q = QUARTERS ? TT / 8 : TT / 4;
+      float* q = &sh.q[0][own_ch] + own_row * (TT / 2) * CT;
       auto down = [&](int t, float v) {
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
@@ -1060,13 +1079,12 @@ back_kernel(const Args a, const Grads g) {
           v -= r;
         }
       };
-      if (own_row) {
-        down(TT, w);
-        up(2 * Q, m);
-      } else {
-        up(0, w);
-        down(2 * Q, m);
+      up(0, from);
+      if constexpr (QUARTERS) {
+        down(TT / 4, inner);
+        up(TT / 4, inner);
       }
+      down(TT / 2, till);
     }
     __syncthreads();
     parts_to(g.part_b);
@@ -1269,7 +1287,7 @@ step_kernel(const StepArgs a) {
 struct Plan { int np, total, tiles, per_group, segs, seg_tiles; };
 // The axis is cut into segments where sequences and channels alone are fewer blocks than one and a half times the SMs, into as many as run at once: what a
 // segment adds to the state (its gradient) is then computed first, at the price of another exp for each token, channel and state.  With 144 blocks
-// (6 x 2048 x 1536) cut: 265 us and 643 back; with 168, not cut: 356 and 1030; with 288, not cut: 375 and 1046, where cut blocks would take about 530 and 1290.
+// (6 x 2048 x 1536) cut: 265 us and 623 back; with 168, cut: 358 and 885, not cut: 356 and 1030; with 240, not cut: 375 and 1038, about what cut ones would take.
 static Plan plan_of(int batch, int len, int dim, int states, int groups, bool backward) {
   Plan p;
   p.np = states <= 16 ? 16 : states <= 32 ? 32 : 64;
@@ -1291,8 +1309,9 @@ static Plan plan_of(int batch, int len, int dim, int states, int groups, bool ba
 
 static long long seg_floats(const Plan& p, int batch, int dim) { return p.segs > 1 ? (long long)batch * p.segs * dim * (p.np + 1) : 0; }
 static long long saves_floats(const Plan& p, int batch, int dim) { return (long long)batch * p.total * dim * p.np; }
+static long long quarter_floats(const Plan& p, int batch, int groups) { return p.np > 16 ? (long long)batch * p.segs * groups * p.tiles * (2 * 8 * THREADS * 2) : 0; }
 static long long grad_floats(const Plan& p, int batch, int len, int dim, int groups) {
-  return seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
+  return quarter_floats(p, batch, groups) + seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
 }
 
 template <typename T, int S, int QL> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
@@ -1421,7 +1440,11 @@ extern "C" int m2_selective_scan_bwd(const m2_selective_scan_args* args, const m
   r.d_state_out = o.d_state_out;
   r.dx = o.d_x; r.d_delta = o.d_delta; r.dz = o.d_gate;
   r.vec = m2_aligned(o.d_x, 16) && m2_aligned(o.d_delta, 16) && m2_aligned(o.d_gate, 16) && (long long)p.per_group * size % 16 == 0;
-  float* w = g.workspace + seg_floats(p, g.batch, g.dim);
+  r.quarters = g.workspace;              // on 16 bytes, as a multiple of that many floats
+  float* w = g.workspace + quarter_floats(p, g.batch, g.groups);
+  a.seg_state = w;
+  a.seg_steps = w + (long long)g.batch * p.segs * g.dim * p.np;
+  w += seg_floats(p, g.batch, g.dim);
   const long long bc = (long long)p.tiles * g.batch * g.seq_len * g.groups * p.np, parts = (long long)g.batch * p.segs * g.dim;
   r.part_b = w; r.part_c = w + bc; r.part_a = w + 2 * bc; r.part_skip = r.part_a + parts * p.np; r.part_bias = r.part_skip + parts;
   r.db = o.d_b; r.dc = o.d_c; r.da = o.d_a; r.d_skip = o.d_skip; r.d_bias = o.d_delta_bias; r.d_state_in = o.d_state_in;
