@@ -59,7 +59,6 @@ __device__ __forceinline__ Sum join(Sum a, Sum b) {
 struct Shared {
   lp::Shared top;
   Sum warp[lp::WARPS], mine;
-  float lo[lp::WARPS];
 };
 
 template <typename T>

@@ -163,6 +163,16 @@ template <int H> __device__ __forceinline__ void decays(f32x2 dt, const f32x2 (&
 #pragma unroll
     for (int i = 0; i < H; ++i) d[c][i] = ex2_pair(f2_mul(s[c], A[c][i]));
 }
+// What was carried, by the decays that it met, and what came since.  Nothing carried is nothing, also where states that grow would make infinity of it.
+__device__ __forceinline__ float carry(float through, float before, float own) { return before == 0.f ? own : fmaf(through, before, own); }
+__device__ __forceinline__ f32x2 carry2(f32x2 through, f32x2 before, f32x2 own) {
+  float t[2], b[2], o[2];
+  f2_unpack(through, t[0], t[1]);
+  f2_unpack(before, b[0], b[1]);
+  f2_unpack(own, o[0], o[1]);
+  return f2_pack(carry(t[0], b[0], o[0]), carry(t[1], b[1], o[1]));
+}
+
 // The sum over the lanes of a channel's states of v and w, of two channels each: lane bit 0 ends with the channel, bit 1 with v or w.
 template <int QL> __device__ __forceinline__ float sum_states(float v0, float v1, float w0, float w1, int lane) {
   const bool hi = lane & 1, sec = lane & 2;
@@ -519,7 +529,7 @@ scan_kernel(const Args a) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int i = 0; i < H; ++i) h[c][i] = f2_fma(through[c][i], h0[c][i], own[c][i]);
+      for (int i = 0; i < H; ++i) h[c][i] = carry2(through[c][i], h0[c][i], own[c][i]);
     steps = f2_add(steps, cum);
     __syncthreads();
     if constexpr (!SUMS) {
@@ -605,7 +615,7 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
     for (int u = 0; u < U; ++u) {
       if (k + u < segs) {
         seg_state[(at + u * step) * np + s] = h;
-        h = fmaf(decay[u], h, own[u]);
+        h = carry(decay[u], h, own[u]);
       }
     }
     at += U * step;
@@ -1045,7 +1055,7 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; ++i) G[c][i] = f2_fma(through[c][i], G0[c][i], own[c][i]);
+        for (int i = 0; i < H; ++i) G[c][i] = carry2(through[c][i], G0[c][i], own[c][i]);
     }
     // a channel's sums, in pieces of the tile from its ends and its middle (with more than 16 states from its quarters too), where g and h are both known: rounding
     // errors of the q_r e_r and p_r s x, which all later sums share, have eight (four) tokens to pile up

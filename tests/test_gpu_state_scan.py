@@ -280,6 +280,23 @@ def test_states_that_do_not_fade_and_fade_at_once():
     assert torch.equal(s[..., 1::2], ((t["delta"] * t["x"])[..., None] * t["b"])[:, -1][..., 1::2])
 
 
+@pytest.mark.parametrize("L", [100, 700])
+def test_an_empty_state_that_would_grow_stays_empty(L):
+    """Factors of e^20 a token: what is never fed is zero, not infinity times zero, forwards and back."""
+    t = make(1, L, 64, 4, 1, torch.float32, plain=True)
+    t["a"] = torch.tensor([20.0, -1.0, 20.0, -1.0], device="cuda").expand(64, 4).contiguous()
+    t["delta"] = torch.ones_like(t["delta"])
+    t["b"][..., ::2] = 0
+    t["c"][..., ::2] = 0
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y, s = m2_b200.selective_scan(**leaves, return_state=True)
+    fading = {**t, "a": t["a"][:, 1::2].contiguous(), "b": t["b"][..., 1::2], "c": t["c"][..., 1::2]}
+    p, q = m2_b200.selective_scan(**fading, return_state=True)
+    assert not s[..., ::2].any() and (s[..., 1::2] - q).abs().max() <= 2 * eps(L, 4) * 40 and (y - p).abs().max() <= 2 * eps(L, 4) * 100
+    d = torch.autograd.grad(y, [leaves["x"], leaves["delta"]], torch.ones_like(y))
+    assert all(torch.isfinite(v).all() for v in d)
+
+
 def test_a_state_is_handed_on():
     """Two halves with the state between them are the whole, forwards and in the gradients, within the bounds of both."""
     B, L, D, N = 2, 128, 64, 16
