@@ -51,7 +51,7 @@ struct Grads {
   int vec;                               // packed outputs in 16-byte pieces
   float *part_b, *part_c;                // (tiles, batch, len, groups, NP)
   float *part_a, *part_skip, *part_bias; // (batch * segs, dim, NP), (batch * segs, dim) twice
-  float* quarters;                       // more than 16 states: (blocks, 2, S, THREADS, 2), each thread's states after a quarter and three of a tile
+  float* between;                        // more than 16 states: (blocks, 7, S, THREADS, 2), each thread's states behind every fourth token of a tile
   void *db, *dc;
   float *da, *d_skip, *d_bias, *d_state_in;
 };
@@ -722,7 +722,8 @@ template <int S, int QL> struct BackShared {
   float part[4][TT][NP];                 // db or dc of each warp's channels
   float mid[4][U * STEP];                // four steps of each pair of channels
   float da[S][THREADS][2];               // each thread's sums over the tiles
-  float middle[S][THREADS][2];           // its states in front of the tile's second half
+  float middle[S > 4 ? 1 : S][THREADS][2];            // its states in front of the tile's second half
+  float known[S > 4 ? TT / 4 + 1 : 1][CT];            // sum a w in front of every fourth token
 };
 
 // Four steps' values of a warp's pairs of channels are added up through shared memory: half the instructions of shuffles
@@ -754,7 +755,7 @@ template <int S, int QL> __device__ __forceinline__ void sum_channels(const floa
 // The gradient of s_t needs w_t = g_t exp(s_t a) h_{t-1} for every state, so h and g at one time.  But w_{t+1} = w_t + g_t b_t s x - v_t e_t, so that inside
 // a tile sum_n a w_t is a sum of scalars of a channel from its end, where h and g are both at hand:
 //   sum_n a w_t = sum_n a g h (end) + sum_{r >= t} (q_r e_r - p_r s x),
-// and likewise from the tile's start and middle.  da goes forwards, with k_t = dh_t / da by the tile's own decays, exp(s a) (k_{t-1} + s h_{t-1}):
+// and likewise from other places where h is kept.  da goes forwards, with k_t = dh_t / da by the tile's own decays, exp(s a) (k_{t-1} + s h_{t-1}):
 //   da = sum_t k_t c_t e_t + g k (end): nothing cancels.
 template <typename T, int S, int QL>
 __global__ void __launch_bounds__(THREADS, S == 4 && sizeof(T) == 2 ? 3 : 2)
@@ -764,8 +765,8 @@ back_kernel(const Args a, const Grads g) {
   constexpr int E = Px::E;
   extern __shared__ __align__(16) unsigned char raw[];
   BackShared<S, QL>& sh = *reinterpret_cast<BackShared<S, QL>*>(raw);
-  constexpr bool QUARTERS = S > 4;       // its own loads and stores only, but through L2: shared memory has no room for them
-  f32x2* quarter = reinterpret_cast<f32x2*>(g.quarters) + (long long)blockIdx.x * (2 * S * THREADS) + threadIdx.x;
+  constexpr bool OFTEN = S > 4;          // a thread's own loads and stores, but through L2: shared memory has no room for them
+  f32x2* between = reinterpret_cast<f32x2*>(g.between) + (long long)blockIdx.x * (7 * S * THREADS) + threadIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place p = place_of<CT>(a);
   pdl_wait();
@@ -890,17 +891,14 @@ back_kernel(const Args a, const Grads g) {
       decays<H>(dt_next, A, d_next);
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += U) {
-        if (t0 == TT / 2) {
+        if (OFTEN ? t0 > 0 : t0 == TT / 2) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < H; ++i) *reinterpret_cast<f32x2*>(sh.middle[c * H + i][tid]) = h[c][i];
-        }
-        if (QUARTERS && t0 % (TT / 2) == TT / 4) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < H; ++i) quarter[(t0 / (TT / 2) * S + c * H + i) * THREADS] = h[c][i];
+            for (int i = 0; i < H; ++i) {
+              if constexpr (OFTEN) between[((t0 / U - 1) * S + c * H + i) * THREADS] = h[c][i];
+              else *reinterpret_cast<f32x2*>(sh.middle[c * H + i][tid]) = h[c][i];
+            }
         }
         float y[U][2], q[U][2];
 #pragma unroll
@@ -954,7 +952,7 @@ back_kernel(const Args a, const Grads g) {
       }
     };
     parts_to(g.part_c);
-    float end[2], middle[2], low[2] = {0.f, 0.f}, high[2] = {0.f, 0.f};     // sum a g h behind the tile's last token, in front of its second half and of its quarters
+    float end[2], middle[2] = {0.f, 0.f};            // sum a g h behind the tile's last token, and in front of its second half
     f32x2 G0[2][H], own[2][H], cum = 0;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -1027,22 +1025,22 @@ back_kernel(const Args a, const Grads g) {
           to_gq[(u - (U - 1)) * CT] = own_row ? fmaf(q_h[u], es[u], -r * xs[u]) : r;
         }
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        if (t0 == TT / 2) {
+        if (OFTEN ? t0 > 0 : t0 == TT / 2) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             f32x2 v = 0;
 #pragma unroll
-            for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], ld2(sh.middle[c * H + i][tid])), A[c][i], v);
+            for (int i = 0; i < H; ++i) {
+              f32x2 hh;
+              if constexpr (OFTEN) hh = between[((t0 / U - 1) * S + c * H + i) * THREADS];
+              else hh = ld2(sh.middle[c * H + i][tid]);
+              v = f2_fma(f2_mul(G[c][i], hh), A[c][i], v);
+            }
             middle[c] = both(v);
           }
-        }
-        if (QUARTERS && t0 % (TT / 2) == TT / 4) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 v = 0;
-#pragma unroll
-            for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], quarter[(t0 / (TT / 2) * S + c * H + i) * THREADS]), A[c][i], v);
-            (t0 > TT / 2 ? high : low)[c] = both(v);
+          if constexpr (OFTEN) {
+            const float w = sum_states<QL>(middle[0], middle[1], middle[0], middle[1], lane);
+            if (lane % QL < 2) sh.known[t0 / U][own_ch] = w;
           }
         }
         to_gq -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
@@ -1057,8 +1055,8 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
         for (int i = 0; i < H; ++i) G[c][i] = carry2(through[c][i], G0[c][i], own[c][i]);
     }
-    // a channel's sums, in pieces of the tile from its ends and its middle (with more than 16 states from its quarters too), where g and h are both known: rounding
-    // errors of the q_r e_r and p_r s x, which all later sums share, have eight (four) tokens to pile up
+    // a channel's sums, in pieces of the tile from its ends and its middle (with more than 16 states from every fourth token), where g and h are both known:
+    // rounding errors of the q_r e_r and p_r s x, which all later sums share, have eight (two) tokens to pile up
     in_front(h);
     float start[2];
 #pragma unroll
@@ -1068,33 +1066,40 @@ back_kernel(const Args a, const Grads g) {
       for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
       start[c] = both(v);
     }
-    const float from = sum_states<QL>(start[0], start[1], middle[0], middle[1], lane), till = sum_states<QL>(middle[0], middle[1], end[0], end[1], lane);
-    const float inner = QUARTERS ? sum_states<QL>(low[0], low[1], high[0], high[1], lane) : 0.f;
-    __syncwarp();
-    if (lane % QL < 4) {                 // of eight lanes two have the same sums; lanes with bit 1 have the second half
-      constexpr int Q = QUARTERS ? TT / 8 : TT / 4;
-      float* q = &sh.q[0][own_ch] + own_row * (TT / 2) * CT;
-      auto down = [&](int t, float v) {
+    float* q = &sh.q[0][own_ch] + own_row * (TT / 2) * CT;              // lanes with bit 1 have the tile's second half
+    auto down = [&](int t, int tokens, float v) {
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          v += q[(t - 1 - i) * CT];
-          q[(t - 1 - i) * CT] = v * LN2;
-        }
-      };
-      auto up = [&](int t, float v) {
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          const float r = q[(t + i) * CT];
-          q[(t + i) * CT] = v * LN2;
-          v -= r;
-        }
-      };
-      up(0, from);
-      if constexpr (QUARTERS) {
-        down(TT / 4, inner);
-        up(TT / 4, inner);
+      for (int i = 0; i < tokens; ++i) {
+        v += q[(t - 1 - i) * CT];
+        q[(t - 1 - i) * CT] = v * LN2;
       }
-      down(TT / 2, till);
+    };
+    auto up = [&](int t, int tokens, float v) {
+#pragma unroll
+      for (int i = 0; i < tokens; ++i) {
+        const float r = q[(t + i) * CT];
+        q[(t + i) * CT] = v * LN2;
+        v -= r;
+      }
+    };
+    if constexpr (OFTEN) {
+      const float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane);
+      if (lane % QL < 4) sh.known[own_row * (TT / U)][own_ch] = w;
+      __syncwarp();
+      if (lane % QL < 4) {                                                // of eight lanes two have the same sums
+        const float* known = &sh.known[own_row * (TT / U / 2)][own_ch];
+#pragma unroll
+        for (int j = 0; j < TT / U / 2; ++j) {
+          up(j * U, U / 2, known[j * CT]);
+          down((j + 1) * U, U / 2, known[(j + 1) * CT]);
+        }
+      }
+    } else {
+      static_assert(OFTEN || QL == 4, "every lane has a half of its own");
+      const float from = sum_states<QL>(start[0], start[1], middle[0], middle[1], lane), till = sum_states<QL>(middle[0], middle[1], end[0], end[1], lane);
+      __syncwarp();
+      up(0, TT / 4, from);
+      down(TT / 2, TT / 4, till);
     }
     __syncthreads();
     parts_to(g.part_b);
@@ -1319,9 +1324,9 @@ static Plan plan_of(int batch, int len, int dim, int states, int groups, bool ba
 
 static long long seg_floats(const Plan& p, int batch, int dim) { return p.segs > 1 ? (long long)batch * p.segs * dim * (p.np + 1) : 0; }
 static long long saves_floats(const Plan& p, int batch, int dim) { return (long long)batch * p.total * dim * p.np; }
-static long long quarter_floats(const Plan& p, int batch, int groups) { return p.np > 16 ? (long long)batch * p.segs * groups * p.tiles * (2 * 8 * THREADS * 2) : 0; }
+static long long between_floats(const Plan& p, int batch, int groups) { return p.np > 16 ? (long long)batch * p.segs * groups * p.tiles * (7 * 8 * THREADS * 2) : 0; }
 static long long grad_floats(const Plan& p, int batch, int len, int dim, int groups) {
-  return quarter_floats(p, batch, groups) + seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
+  return between_floats(p, batch, groups) + seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
 }
 
 template <typename T, int S, int QL> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
@@ -1450,8 +1455,8 @@ extern "C" int m2_selective_scan_bwd(const m2_selective_scan_args* args, const m
   r.d_state_out = o.d_state_out;
   r.dx = o.d_x; r.d_delta = o.d_delta; r.dz = o.d_gate;
   r.vec = m2_aligned(o.d_x, 16) && m2_aligned(o.d_delta, 16) && m2_aligned(o.d_gate, 16) && (long long)p.per_group * size % 16 == 0;
-  r.quarters = g.workspace;              // on 16 bytes, as a multiple of that many floats
-  float* w = g.workspace + quarter_floats(p, g.batch, g.groups);
+  r.between = g.workspace;               // on 16 bytes, as a multiple of that many floats
+  float* w = g.workspace + between_floats(p, g.batch, g.groups);
   a.seg_state = w;
   a.seg_steps = w + (long long)g.batch * p.segs * g.dim * p.np;
   w += seg_floats(p, g.batch, g.dim);

@@ -47,7 +47,7 @@ def test_a_long_axis_is_cut_into_as_many_pieces_as_run_at_once():
         if backward:                     # without the parts of the gradients: of b and c for each tile, of the parameters for each segment
             tiles = -(-dim // groups // (32 if np == 64 else 64))
             size -= 2 * tiles * batch * (1 << 15) * groups * np
-            return size / (batch * dim * (np + 1 + np + 2) + (batch * groups * tiles * 4096 if np > 16 else 0))
+            return size / (batch * dim * (np + 1 + np + 2) + (batch * groups * tiles * 14336 if np > 16 else 0))
         return size / (batch * dim * (np + 1))
 
     for batch, dim, states, groups, blocks, an_sm in ((1, 768, 16, 1, 12, 4), (2, 768, 11, 2, 24, 4), (1, 768, 20, 1, 12, 2), (1, 768, 50, 1, 24, 2), (3, 100, 16, 1, 6, 4)):
