@@ -633,7 +633,7 @@ int m2_causal_conv_step(const m2_causal_conv_step_args* args, void* stream);
  *   h_t[n] = exp(s_t a[d, n]) h_{t-1}[n] + s_t x_t b_t[n],     y_t = (sum_n c_t[n] h_t[n] + skip x_t) silu(gate_t)
  *   x, delta, gate (batch, seq_len, dim): `dtype`, strides in elements, contiguous channels; gate NULL: without.  b, c (batch, seq_len,
  *   groups, states): `dtype`, strides, contiguous states; channel d reads group d / (dim / groups).  states <= 64.
- *   a float32 (dim, states), packed, < 0 (or 0) for states that do not grow; skip, delta_bias float32 (dim) or NULL.
+ *   a float32 (dim, states), packed, < 0 (or 0) for states that do not grow; an infinity counts as the largest number; skip, delta_bias float32 (dim) or NULL.
  *   y packed.  lengths as above; the state is that behind a text's last token.
  *   state_in  : NULL (zeros) or float32 (batch, dim, states), packed; state_out: NULL or the same.
  *   saves     : NULL, or m2_selective_scan_saves() bytes on a 16-byte boundary: states along the axis, for the gradient.

@@ -131,6 +131,12 @@ template <int H> __device__ __forceinline__ void st_pairs(float* p, const f32x2 
 #pragma unroll
   for (int i = 0; i < H; i += 2) *reinterpret_cast<ulonglong2*>(p + 2 * i) = make_ulonglong2(v[i], v[i + 1]);
 }
+// a in units of a factor of two, within float32: a step of 0 fades nothing, also where log2(e) would make an infinity of a (below -2.36e38) or a is one
+__device__ __forceinline__ float rate(float a) {
+  constexpr float MOST = 3.402823466e38f;
+  const float v = a * LOG2E;
+  return v < -MOST ? -MOST : v > MOST ? MOST : v;                        // NaN stays
+}
 __device__ __forceinline__ float both(f32x2 v) {
   float x, y;
   f2_unpack(v, x, y);
@@ -371,7 +377,7 @@ scan_kernel(const Args a) {
         const int s = q0 + 2 * i + j;
         const bool real = cl + c < p.valid && s < a.states;
         const long long ch = p.ch0 + cl + c;
-        v[j] = real ? a.a[ch * a.states + s] * LOG2E : 0.f;
+        v[j] = real ? rate(a.a[ch * a.states + s]) : 0.f;
         w[j] = 0.f;
         if (!SUMS && real) {
           if (a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
@@ -596,7 +602,7 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
   if (i >= (long long)batch * dim * np) return;
   const int s = (int)(i % np), d = (int)(i / np % dim), b = (int)(i / np / dim);
   const bool real = s < states;
-  const float A = real ? a[(long long)d * states + s] * LOG2E : 0.f;
+  const float A = real ? rate(a[(long long)d * states + s]) : 0.f;
   float h = real && edge ? edge[((long long)b * dim + d) * states + s] : 0.f;
   // several segments' loads are under way together
   constexpr int U = 8;
@@ -646,7 +652,7 @@ back_sums_kernel(const Args a, const Grads g) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int s = q0 + 2 * i + j;
-        v[j] = cl + c < p.valid && s < a.states ? a.a[(long long)(p.ch0 + cl + c) * a.states + s] * LOG2E : 0.f;
+        v[j] = cl + c < p.valid && s < a.states ? rate(a.a[(long long)(p.ch0 + cl + c) * a.states + s]) : 0.f;
       }
       A[c][i] = f2_pack(v[0], v[1]);
       G[c][i] = 0;
@@ -789,7 +795,7 @@ back_kernel(const Args a, const Grads g) {
         const int s = q0 + 2 * i + j;
         const bool real = cl + c < p.valid && s < a.states;
         const long long ch = p.ch0 + cl + c;
-        v[j] = real ? a.a[ch * a.states + s] * LOG2E : 0.f;
+        v[j] = real ? rate(a.a[ch * a.states + s]) : 0.f;
         w[j] = 0.f;
         if (real && a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
         else if (real && g.d_state_out) w[j] = g.d_state_out[((long long)p.b * a.dim + ch) * a.states + s];
@@ -1277,14 +1283,14 @@ step_kernel(const StepArgs a) {
         if (s >= 16) load(s);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          h[j] = fmaf(ex2(dt * (A[j] * LOG2E)), h[j], dx * B[j]);
+          h[j] = fmaf(ex2(dt * rate(A[j])), h[j], dx * B[j]);
           y = fmaf(h[j], C[j], y);
         }
         *reinterpret_cast<float4*>(state + s) = make_float4(h[0], h[1], h[2], h[3]);
       }
     } else {
       for (int s = part; s < a.states; s += 4) {
-        const float hh = fmaf(ex2(dt * (decay[s] * LOG2E)), state[s], dx * lp::load1(pb + s));
+        const float hh = fmaf(ex2(dt * rate(decay[s])), state[s], dx * lp::load1(pb + s));
         state[s] = hh;
         y = fmaf(hh, lp::load1(pc + s), y);
       }

@@ -130,7 +130,8 @@ def selective_scan(x, delta, a, b, c, *, skip=None, gate=None, delta_bias=None, 
     """y (B, L, D) for x, delta (B, L, D) and b, c (B, L, N) or (B, L, G, N), all float32 or all bfloat16, any strides (contiguous channels and
     states are read in place); channel d reads group d // (D // G), N <= 64.
 
-    a              (D, N) float: exp(s a) fades a state with every token; < 0 for states that do not grow
+    a              (D, N) float: exp(s a) fades a state with every token; < 0 for states that do not grow.  An infinity counts as float32's
+                   largest number, so that a step of 0 changes nothing
     skip           None or (D,): x's own share of y;   gate  None or x's shape and type: y is multiplied by silu(gate)
     delta_bias     None or (D,), added to delta;       softplus  whether the step s is softplus of that sum, or the sum itself
     initial_state  None (zero) or (B, D, N) float32: what earlier calls left
