@@ -27,6 +27,13 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 // states a lane were tried and spilled hundreds of bytes.
 __host__ __device__ constexpr int channels_of(int ql) { return 256 / ql; }                          // of a block
 
+// Blocks of the gradients' kernel that an SM holds: 168 registers and 74 KB of shared memory up to 16 states, 255 and 92 to 96 beyond
+__host__ __device__ constexpr int back_blocks(int np) { return np == 16 ? 3 : 2; }
+// Tokens whose states are at hand at one time: four, or two where a lane has twice the states
+__host__ __device__ constexpr int few(int np) { return np == 16 ? 4 : 2; }
+constexpr int ASIDE = TT / 4 - 1;        // more than 16 states: places for states in front of every fourth token of a tile but its first
+constexpr int PLACES = 4096;             // such blocks, 235 MB (with as many as run at once, 64 ragged texts of 768 channels and 64 states took 1760 us instead of 1610)
+
 struct Rows { const void* p; long long sb, st; int vec; };           // vec: 16-byte pieces
 struct Group { const void* p; long long sb, st, sg; int vec; };       // vec: four states at once
 
@@ -51,7 +58,7 @@ struct Grads {
   int vec;                               // packed outputs in 16-byte pieces
   float *part_b, *part_c;                // (tiles, batch, len, groups, NP)
   float *part_a, *part_skip, *part_bias; // (batch * segs, dim, NP), (batch * segs, dim) twice
-  float* between;                        // more than 16 states: (blocks, 7, S, THREADS, 2), each thread's states behind every fourth token of a tile
+  float* aside;                          // more than 16 states: (blocks, ASIDE, S, THREADS, 2), each thread's states in front of every fourth token of a tile
   void *db, *dc;
   float *da, *d_skip, *d_bias, *d_state_in;
 };
@@ -137,6 +144,16 @@ __device__ __forceinline__ float rate(float a) {
   const float v = a * LOG2E;
   return v < -MOST ? -MOST : v > MOST ? MOST : v;                        // NaN stays
 }
+// adds to a thread's own numbers in memory; nothing is waited for, and one thread's additions to one place keep their order
+template <int H> __device__ __forceinline__ void add_pairs(float* p, const f32x2 (&v)[H]) {
+#pragma unroll
+  for (int i = 0; i < H; i += 2) {
+    float f[4];
+    f2_unpack(v[i], f[0], f[1]);
+    f2_unpack(v[i + 1], f[2], f[3]);
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + 2 * i), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+  }
+}
 __device__ __forceinline__ float both(f32x2 v) {
   float x, y;
   f2_unpack(v, x, y);
@@ -191,9 +208,8 @@ template <int QL> __device__ __forceinline__ float sum_states(float v0, float v1
 
 // Where a block works: blocks of one sequence and segment lie side by side, as they read the same b and c
 struct Place { int b, seg, g, tile, c0, valid, ch0; };
-template <int CT> __device__ __forceinline__ Place place_of(const Args& a) {
+template <int CT> __device__ __forceinline__ Place place_of(const Args& a, unsigned i) {
   Place p;
-  unsigned i = blockIdx.x;
   p.tile = i % a.tiles; i /= a.tiles;
   p.g = i % a.groups; i /= a.groups;
   p.seg = i % a.segs;
@@ -287,13 +303,13 @@ template <typename T, int NP> struct Coeffs {
   }
 };
 
-template <typename T, int CT> struct Pieces {                           // a thread's part of a tile of x, delta, z or a gradient
-  static constexpr int E = Piece<T>::N, PPR = CT / E, ROWS = THREADS / PPR, P = TT / ROWS;
+template <typename T, int CT, int PARTS = 1> struct Pieces {            // a thread's part of a tile (or of one of PARTS) of x, delta, z or a gradient
+  static constexpr int E = Piece<T>::N, PPR = CT / E, ROWS = THREADS / PPR, SPAN = TT / PARTS, P = SPAN / ROWS;
   uint4 v[P];
   __device__ __forceinline__ void fetch(const Rows& r, const Place& p, int t0, int n) {
     const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
     const T* at = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col + (t0 + row) * r.st;
-    if (r.vec && p.valid == CT && t0 + TT <= n) {                        // for the whole block alike
+    if (r.vec && p.valid == CT && t0 + SPAN <= n) {                        // for the whole block alike
 #pragma unroll
       for (int i = 0; i < P; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(at + i * ROWS * r.st));
     } else {
@@ -310,7 +326,7 @@ template <typename T, int CT> struct Pieces {                           // a thr
   __device__ __forceinline__ void ask(uint4* slot, const Rows& r, const Place& p, int t0, int n) {
     const int col = threadIdx.x % PPR * E, row = threadIdx.x / PPR;
     const T* at = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col + (t0 + row) * r.st;
-    if (r.vec && p.valid == CT && t0 + TT <= n) {                        // for the whole block alike
+    if (r.vec && p.valid == CT && t0 + SPAN <= n) {                        // for the whole block alike
 #pragma unroll
       for (int i = 0; i < P; ++i) copy_async<16>(slot + i * THREADS, at + i * ROWS * r.st);
     } else {
@@ -329,7 +345,7 @@ template <typename T, int CT> struct Pieces {                           // a thr
     if (threadIdx.x % (PPR < 8 ? PPR : 8) || col >= p.valid) return;        // a line of 128 bytes each
     const T* base = static_cast<const T*>(r.p) + p.b * r.sb + p.ch0 + col;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
+    for (int i = 0; i < P * PARTS; ++i) {
       const int t = t0 + row + i * ROWS;
       if (t >= 0 && t < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + t * r.st));
     }
@@ -356,7 +372,7 @@ scan_kernel(const Args a) {
   // two rows and one more than a tile has: what the loop asks for ahead of its end.  y takes the place of s x.
   __shared__ __align__(16) float s_dt[TT + 2][CT], s_dx[TT + 1][CT], s_b[TT + 1][NP], s_c[TT + 1][NP], s_bias[CT], s_skip[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of<CT>(a);
+  const Place p = place_of<CT>(a, blockIdx.x);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) {
@@ -637,7 +653,7 @@ back_sums_kernel(const Args a, const Grads g) {
   constexpr int E = Px::E;
   __shared__ __align__(16) float s_dt[TT][CT], s_e[TT][CT], s_c[TT][NP], s_bias[CT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of<CT>(a);
+  const Place p = place_of<CT>(a, blockIdx.x);
   pdl_wait();
   const int n = text_length(a, p.b);
   if (tid < CT) s_bias[tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
@@ -720,16 +736,15 @@ back_sums_kernel(const Args a, const Grads g) {
 }
 
 template <int S, int QL> struct BackShared {
-  static constexpr int NP = QL * S, CT = channels_of(QL), U = 4, STEP = 32 / QL * NP + 16;      // STEP: steps side by side meet other banks
-  // the loops ask for two tokens more than the tile has: at either end there is other memory of this struct, which is not used
+  static constexpr int NP = QL * S, CT = channels_of(QL), U = 4, FEW = few(QL * S), STEP = 32 / QL * NP + 16;      // STEP: steps side by side meet other banks
+  // the loop forwards asks for two tokens more than the tile has: at its end there is other memory of this struct, which is not used
   float bias[2][CT];
   float dt[TT][CT], dx[TT][CT], e[TT][CT], y[TT][CT], q[TT][CT];       // dx becomes gb
-  float before[NP], b[TT][NP], c[TT][NP];
+  float b[TT][NP], c[TT][NP];
   float part[4][TT][NP];                 // db or dc of each warp's channels
   float mid[4][U * STEP];                // four steps of each pair of channels
-  float da[S][THREADS][2];               // each thread's sums over the tiles
-  float middle[S > 4 ? 1 : S][THREADS][2];            // its states in front of the tile's second half
-  float known[S > 4 ? TT / 4 + 1 : 1][CT];            // sum a w in front of every fourth token
+  float aside[S > 4 ? 1 : 2][2][THREADS][4];          // up to 16 states: each thread's in front of the tile's tokens 8 and 24; then 0 in the place of 24
+  float behind[S][THREADS][2];           // the gradient of the state behind the tile
 };
 
 // Four steps' values of a warp's pairs of channels are added up through shared memory: half the instructions of shuffles
@@ -756,26 +771,30 @@ template <int S, int QL> __device__ __forceinline__ void sum_channels(const floa
 }
 
 // Gradients, a tile at a time from the last to the first.  With v_t = h_t c_t, e_t the gradient of sum c h, g_t that of h_t:
-//   forwards   h_t again from the saved state in front of the tile: y, dc_t = sum_d h_t e_t, and q_t = sum_n a v_t
-//   backwards  g_t = c_t e_t + exp(s a)_{t+1} g_{t+1}: gb_t = sum_n g_t b_t, db_t = sum_d g_t s x, and p_t = sum_n a g_t b_t
-// The gradient of s_t needs w_t = g_t exp(s_t a) h_{t-1} for every state, so h and g at one time.  But w_{t+1} = w_t + g_t b_t s x - v_t e_t, so that inside
-// a tile sum_n a w_t is a sum of scalars of a channel from its end, where h and g are both at hand:
-//   sum_n a w_t = sum_n a g h (end) + sum_{r >= t} (q_r e_r - p_r s x),
-// and likewise from other places where h is kept.  da goes forwards, with k_t = dh_t / da by the tile's own decays, exp(s a) (k_{t-1} + s h_{t-1}):
-//   da = sum_t k_t c_t e_t + g k (end): nothing cancels.
+//   forwards   h_t again from the saved state in front of the tile: y and dc_t = sum_d h_t e_t; h in front of every eighth token is put aside
+//   backwards  four tokens at a time, f_t = exp(s_t a) h_{t-1} of each from what was put aside, then g_t = c_t e_t + exp(s a)_{t+1} g_{t+1}:
+//              gb_t = sum_n g_t b_t, db_t = sum_d g_t s x, and from w_t = g_t f_t both da = sum_t s_t w_t and sum_n a w_t, the part of the step's gradient beside gb_t x_t.
+// w is one product of what belongs to its own token.  (w_{t+1} = w_t + g_t b_t s x - v_t e_t, v = c h, makes sum_n a w_t a running sum of scalars and saves the states, but
+// what is left of it where a state fades fast, or beside a token that outweighs its neighbours, is the others' roundings: it was off by 1e-5 for a s = -50, by more than
+// the gradient itself from -1e6 on.)
+// Measured (bf16, 16 states, 16 x 2048 x 1536): 1459 us, the running sum took 1343.  Half of the tokens' h are computed once more on the way from one place to the next
+// (73 us; places in front of more tokens do not fit, and those that fit gained nothing); the exps of the next tokens under way while some are computed: spills, 1700.
+// With more than 16 states: in front of every fourth token, two tokens at a time.  What is put aside then goes through L2, 57 KB a block, and blocks beyond PLACES
+// of them take one piece of work after another.
 template <typename T, int S, int QL>
-__global__ void __launch_bounds__(THREADS, S == 4 && sizeof(T) == 2 ? 3 : 2)
-back_kernel(const Args a, const Grads g) {
+__global__ void __launch_bounds__(THREADS, back_blocks(QL * S))
+back_kernel(const Args a, const Grads g, const unsigned work) {
   constexpr int NP = QL * S, CT = channels_of(QL);
-  using Px = Pieces<T, CT>;
+  constexpr int PARTS = sizeof(T) / 2;   // float32's twice as many pieces are in registers one half after the other
+  using Px = Pieces<T, CT, PARTS>;
   constexpr int E = Px::E;
   extern __shared__ __align__(16) unsigned char raw[];
   BackShared<S, QL>& sh = *reinterpret_cast<BackShared<S, QL>*>(raw);
-  constexpr bool OFTEN = S > 4;          // a thread's own loads and stores, but through L2: shared memory has no room for them
-  f32x2* between = reinterpret_cast<f32x2*>(g.between) + (long long)blockIdx.x * (7 * S * THREADS) + threadIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of<CT>(a);
+  float* const far_aside = g.aside + (long long)blockIdx.x * (ASIDE * 2 * S * THREADS) + 4 * threadIdx.x;
   pdl_wait();
+  for (unsigned item = blockIdx.x; item < work; item += gridDim.x) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Place p = place_of<CT>(a, item);
   const int n = text_length(a, p.b);
   if (tid < CT) {
     sh.bias[0][tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
@@ -802,7 +821,6 @@ back_kernel(const Args a, const Grads g) {
       }
       A[c][i] = f2_pack(v[0], v[1]);
       G[c][i] = f2_pack(w[0], w[1]);
-      *reinterpret_cast<f32x2*>(sh.da[c * H + i][tid]) = 0;
     }
   }
   const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
@@ -810,9 +828,7 @@ back_kernel(const Args a, const Grads g) {
   const int col = tid % Px::PPR * E, row = tid / Px::PPR;
   const long long out0 = (long long)p.b * a.len * a.dim + p.ch0 + col;
   T *dx = static_cast<T*>(g.dx) + out0, *dd = static_cast<T*>(g.d_delta) + out0, *dz = static_cast<T*>(g.dz) + out0;
-  float d_skip[E], d_bias[E];
-#pragma unroll
-  for (int j = 0; j < E; ++j) d_skip[j] = d_bias[j] = 0.f;
+  float sum = 0.f;                       // threads below CT: the gradient of a channel's skip, the next CT: of its delta_bias
   for (int t = max(used, first) * TT + row; t < min(last * TT, a.len); t += Px::ROWS) {       // behind the text
     const float f[E] = {};
     store_piece<T>(dx + (long long)t * a.dim, f, p.valid - col, g.vec);
@@ -821,17 +837,10 @@ back_kernel(const Args a, const Grads g) {
   }
   Px x, delta, z, dy;
   Coeffs<T, NP> fb, fc;
-  auto fetch = [&](int k) {
-    x.fetch(a.x, p, k * TT, n);
-    delta.fetch(a.delta, p, k * TT, n);
-    dy.fetch(g.dy, p, k * TT, n);
-    if (a.z.p) z.fetch(a.z, p, k * TT, n);
-    fb.fetch(a.b, p, k * TT, n, a.states);
-    fc.fetch(a.c, p, k * TT, n, a.states);
-  };
   __syncthreads();
   for (int k = used - 1; k >= first; --k) {
-    fetch(k);
+    fb.fetch(a.b, p, k * TT, n, a.states);
+    fc.fetch(a.c, p, k * TT, n, a.states);
     const float* saved = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
     auto in_front = [&](f32x2 (&h)[2][H]) {
 #pragma unroll
@@ -842,14 +851,19 @@ back_kernel(const Args a, const Grads g) {
           h[c][i] = u.x; h[c][i + 1] = u.y;
         }
     };
-    f32x2 h[2][H], dA[2][H];
+    f32x2 h[2][H];
     in_front(h);
-    {
+#pragma unroll 1
+    for (int part = 0; part < TT; part += Px::SPAN) {
+      x.fetch(a.x, p, k * TT + part, n);
+      delta.fetch(a.delta, p, k * TT + part, n);
+      dy.fetch(g.dy, p, k * TT + part, n);
+      if (a.z.p) z.fetch(a.z, p, k * TT + part, n);
       float bias[E];
       from_shared(sh.bias[0] + col, bias);
 #pragma unroll
       for (int i = 0; i < Px::P; ++i) {
-        const int t = row + i * Px::ROWS;
+        const int t = part + row + i * Px::ROWS;
         const bool in = k * TT + t < n;
         float f[E], d[E], e[E];
         Piece<T>::get(x.v[i], f);
@@ -881,71 +895,80 @@ back_kernel(const Args a, const Grads g) {
       Px::ask(g.dy, p, (k - 1) * TT, n);
       if (a.z.p) Px::ask(a.z, p, (k - 1) * TT, n);
     }
-    constexpr int U = BackShared<S, QL>::U, STEP = BackShared<S, QL>::STEP;
+    constexpr int U = BackShared<S, QL>::U, FEW = BackShared<S, QL>::FEW, STEP = BackShared<S, QL>::STEP;
     float* mid = sh.mid[warp];
-    f32x2 K[2][H];
+    // h in front of token t, a multiple of PART: a thread's own loads and stores, 16 bytes each
+    constexpr int PART = 2 * FEW;
+    auto place = [&](int t, int c) {
+      if constexpr (S > 4) return far_aside + (t / PART - 1) * (2 * S * THREADS) + c * (S * THREADS);
+      // token 16's lies in the first half of q, in the warp's own columns: by the time that half gets its own numbers it has been used
+      else return t == 16 ? &sh.q[c * 8 + lane / 4][warp * (CT / 4) + lane % 4 * 4] : sh.aside[t != 8][c][tid];
+    };
+    auto put_aside = [&](int t) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c) {
+        float* to = place(t, c);
 #pragma unroll
-      for (int i = 0; i < H; ++i) K[c][i] = dA[c][i] = 0;
-    float* to_yq = own_row ? &sh.q[0][own_ch] : &sh.y[0][own_ch];
+        for (int i = 0; i < H; i += 2) *reinterpret_cast<ulonglong2*>(to + i / 2 * (4 * THREADS)) = make_ulonglong2(h[c][i], h[c][i + 1]);
+      }
+    };
+    auto take_aside = [&](int t) {
+      if (S > 4 && t == 0) { in_front(h); return; }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float* from = place(t, c);
+#pragma unroll
+        for (int i = 0; i < H; i += 2) {
+          const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(from + i / 2 * (4 * THREADS));
+          h[c][i] = u.x; h[c][i + 1] = u.y;
+        }
+      }
+    };
     {
       Token<H, true, true> next;
       const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][q0], *p_c = &sh.c[0][q0];
-      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt + CT), d_next[2][H];
+      float* p_y = &sh.y[own_row][own_ch];
+      f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[2][H];
       next.get(p_dx, p_e, p_b, p_c);
-      decays<H>(dt_next, A, d_next);
+      decays<H>(dt, A, d_next);
 #pragma unroll 1
       for (int t0 = 0; t0 < TT; t0 += U) {
-        if (OFTEN ? t0 > 0 : t0 == TT / 2) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-              if constexpr (OFTEN) between[((t0 / U - 1) * S + c * H + i) * THREADS] = h[c][i];
-              else *reinterpret_cast<f32x2*>(sh.middle[c * H + i][tid]) = h[c][i];
-            }
-        }
-        float y[U][2], q[U][2];
+        float y[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          if (u == 0 && t0 > 0 && t0 % PART == 0) put_aside(t0);
           const Token<H, true, true> now = next;
-          f32x2 d[2][H], hs[H], dt[2], x[2], e[2];
-          splat2(dt_next, dt);
+          f32x2 d[2][H], hs[H], x[2], e[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
           next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * NP, p_c + (u + 1) * NP);
-          dt_next = dt_far;
-          dt_far = ld2(p_dt + (u + 2) * CT);
-          decays<H>(dt_next, A, d_next);
+          dt = dt_next;
+          dt_next = ld2(p_dt + (u + 2) * CT);
+          decays<H>(dt, A, d_next);
           splat2(now.x, x);
           splat2(now.e, e);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            f32x2 yy, qq;
+            f32x2 yy;
 #pragma unroll
             for (int i = 0; i < H; ++i) {
-              K[c][i] = f2_mul(d[c][i], f2_fma(dt[c], h[c][i], K[c][i]));
               h[c][i] = f2_fma(d[c][i], h[c][i], f2_mul(x[c], now.B[i]));
               hs[i] = c ? f2_fma(h[c][i], e[c], hs[i]) : f2_mul(h[c][i], e[c]);
-              const f32x2 v = f2_mul(h[c][i], now.C[i]);
-              yy = i ? f2_add(yy, v) : v;
-              qq = i ? f2_fma(v, A[c][i], qq) : f2_mul(v, A[c][i]);
-              dA[c][i] = f2_fma(f2_mul(K[c][i], now.C[i]), e[c], dA[c][i]);
+              yy = i ? f2_fma(h[c][i], now.C[i], yy) : f2_mul(h[c][i], now.C[i]);
             }
             y[u][c] = both(yy);
-            q[u][c] = both(qq);
           }
           put_channels<S, QL>(mid + u * STEP, hs, lane);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) to_yq[u * CT] = sum_states<QL>(y[u][0], y[u][1], q[u][0], q[u][1], lane);
+        for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(y[u][0], y[u][1], y[u + 1][0], y[u + 1][1], lane);
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        to_yq += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * NP; p_c += U * NP;
+        p_y += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * NP; p_c += U * NP;
       }
     }
+    take_aside(TT - PART);
     __syncthreads();
     auto parts_to = [&](float* out) {
       const long long row = (long long)a.groups * NP;
@@ -958,99 +981,115 @@ back_kernel(const Args a, const Grads g) {
       }
     };
     parts_to(g.part_c);
-    float end[2], middle[2] = {0.f, 0.f};            // sum a g h behind the tile's last token, and in front of its second half
-    f32x2 G0[2][H], own[2][H], cum = 0;
+    f32x2 own[2][H], dA[2][H], cum = 0;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      f32x2 v = 0;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
-        f32x2* sum = reinterpret_cast<f32x2*>(sh.da[c * H + i][tid]);
-        *sum = f2_add(*sum, f2_fma(G[c][i], K[c][i], dA[c][i]));      // a tile's own sum first: 2048 tokens one by one lose half a digit
-        G0[c][i] = G[c][i];
-        own[c][i] = 0;
+        *reinterpret_cast<f32x2*>(sh.behind[c * H + i][tid]) = G[c][i];
+        own[c][i] = dA[c][i] = 0;
       }
-      end[c] = both(v);
-    }
     __syncthreads();
     {
-      Token<H, true, true> next;
-      constexpr int LAST = (TT - 1) * CT, LAST_N = (TT - 1) * NP;
-      float* to_gq = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
-      const float *p_dt = &sh.dt[0][cl] + LAST, *p_dx = &sh.dx[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][q0] + LAST_N, *p_c = &sh.c[0][q0] + LAST_N;
-      f32x2 dt_next = ld2(p_dt), dt_far = ld2(p_dt - CT), d_next[2][H];
-      next.get(p_dx, p_e, p_b, p_c);
-      decays<H>(dt_next, A, d_next);
+      constexpr int LAST = (TT - U) * CT, LAST_N = (TT - U) * NP;
+      const float *p_dt = &sh.dt[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][q0] + LAST_N, *p_c = &sh.c[0][q0] + LAST_N;
+      const float* p_dx = &sh.dx[0][cl] + LAST;
+      float* to = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
+      constexpr int HALVES = PART > U ? 2 : 1;
 #pragma unroll 1
-      for (int t0 = TT - U; t0 >= 0; t0 -= U) {
-        float gb[U][2], q[U][2], q_h[U], xs[U], es[U];
+      for (int t1 = TT - U; t1 >= 0; t1 -= HALVES * U)
 #pragma unroll
-        for (int r = 0; r < U; ++r) {
-          const int u = U - 1 - r;
-          const Token<H, true, true> now = next;
-          f32x2 d[2][H], gs[H], x[2], e[2];
+      for (int half = 0; half < HALVES; ++half) {
+        const int t0 = t1 - half * U;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+        for (int u0 = U - FEW; u0 >= 0; u0 -= FEW) {
+          f32x2 d[FEW][2][H], f[FEW][2][H];
+          float gb[2][2], q[2][2];
+          const bool second = PART > U ? half == 0 : u0 > 0;        // half of the part
+          if (second) {
 #pragma unroll
-            for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
-          cum = f2_add(cum, dt_next);
-          next.get(p_dx - (r + 1) * CT, p_e - (r + 1) * CT, p_b - (r + 1) * NP, p_c - (r + 1) * NP);
-          dt_next = dt_far;
-          dt_far = ld2(p_dt - (r + 2) * CT);
-          q_h[u] = to_gq[-r * CT];
-          decays<H>(dt_next, A, d_next);
-          splat2(now.x, x);
-          splat2(now.e, e);
+            for (int v = 0; v < FEW; ++v) {
+              const int u = u0 - FEW + v;
+              f32x2 x[2], B[H];
+              decays<H>(ld2(p_dt + u * CT), A, d[0]);
+              splat2(ld2(p_dx + u * CT), x);
+              ld_pairs<H>(p_b + u * NP, B);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 bb, qq;
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < H; ++i) {
-              const f32x2 fed = f2_fma(e[c], now.C[i], G[c][i]);
-              own[c][i] = f2_mul(d[c][i], f2_fma(e[c], now.C[i], own[c][i]));
-              gs[i] = c ? f2_fma(fed, x[c], gs[i]) : f2_mul(fed, x[c]);
-              const f32x2 v = f2_mul(fed, now.B[i]);
-              bb = i ? f2_add(bb, v) : v;
-              qq = i ? f2_fma(v, A[c][i], qq) : f2_mul(v, A[c][i]);
-              G[c][i] = f2_mul(d[c][i], fed);
+                for (int i = 0; i < H; ++i) h[c][i] = f2_fma(d[0][c][i], h[c][i], f2_mul(x[c], B[i]));
             }
-            gb[u][c] = both(bb);
-            q[u][c] = both(qq);
           }
-          put_channels<S, QL>(mid + u * STEP, gs, lane);
-          float v0, v1;
-          f2_unpack(now.x, v0, v1);
-          xs[u] = lane & 1 ? v1 : v0;
-          f2_unpack(now.e, v0, v1);
-          es[u] = lane & 1 ? v1 : v0;
-        }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float r = sum_states<QL>(gb[u][0], gb[u][1], q[u][0], q[u][1], lane);
-          to_gq[(u - (U - 1)) * CT] = own_row ? fmaf(q_h[u], es[u], -r * xs[u]) : r;
+          for (int v = 0; v < FEW; ++v) {
+            const int u = u0 + v;
+            f32x2 x[2], B[H];
+            decays<H>(ld2(p_dt + u * CT), A, d[v]);
+            splat2(ld2(p_dx + u * CT), x);
+            ld_pairs<H>(p_b + u * NP, B);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < H; ++i) {
+                f[v][c][i] = f2_mul(d[v][c][i], h[c][i]);
+                if (v < FEW - 1) h[c][i] = f2_fma(x[c], B[i], f[v][c][i]);
+              }
+          }
+          if (S == 4 && t0 == 24) {                                      // its states have been used
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (cl + c < p.valid) copy_async<16>(sh.aside[1][c][tid], saved + c * NP);
+              else *reinterpret_cast<float4*>(sh.aside[1][c][tid]) = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+          if (S == 4 && t0 == 8) asm volatile("cp.async.wait_all;" ::: "memory");
+          if (t0 + u0 > 0) take_aside(t0 + u0 - (second ? FEW : PART));  // under way meanwhile
+#pragma unroll
+          for (int v = FEW - 1; v >= 0; --v) {
+            const int u = u0 + v;
+            Token<H, true, true> now;
+            now.get(p_dx + u * CT, p_e + u * CT, p_b + u * NP, p_c + u * NP);
+            f32x2 gs[H], x[2], e[2], dt[2];
+            const f32x2 steps = ld2(p_dt + u * CT);
+            cum = f2_add(cum, steps);
+            splat2(steps, dt);
+            splat2(now.x, x);
+            splat2(now.e, e);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              f32x2 bb, qq;
+#pragma unroll
+              for (int i = 0; i < H; ++i) {
+                const f32x2 fed = f2_fma(e[c], now.C[i], G[c][i]), w = f2_mul(fed, f[v][c][i]);
+                own[c][i] = f2_mul(d[v][c][i], f2_fma(e[c], now.C[i], own[c][i]));
+                gs[i] = c ? f2_fma(fed, x[c], gs[i]) : f2_mul(fed, x[c]);
+                bb = i ? f2_fma(fed, now.B[i], bb) : f2_mul(fed, now.B[i]);
+                qq = i ? f2_fma(w, A[c][i], qq) : f2_mul(w, A[c][i]);
+                dA[c][i] = f2_fma(dt[c], w, dA[c][i]);
+                G[c][i] = f2_mul(d[v][c][i], fed);
+              }
+              gb[v % 2][c] = both(bb);
+              q[v % 2][c] = both(qq);
+            }
+            put_channels<S, QL>(mid + u * STEP, gs, lane);
+            if (v % 2 == 0) {
+              __syncwarp();                                              // all of the warp have read these tokens' s x
+#pragma unroll
+              for (int j = 0; j < 2; ++j) to[(u + j) * CT] = sum_states<QL>(gb[j][0], gb[j][1], q[j][0], q[j][1], lane);
+            }
+          }
         }
         sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        if (OFTEN ? t0 > 0 : t0 == TT / 2) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 v = 0;
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-              f32x2 hh;
-              if constexpr (OFTEN) hh = between[((t0 / U - 1) * S + c * H + i) * THREADS];
-              else hh = ld2(sh.middle[c * H + i][tid]);
-              v = f2_fma(f2_mul(G[c][i], hh), A[c][i], v);
-            }
-            middle[c] = both(v);
-          }
-          if constexpr (OFTEN) {
-            const float w = sum_states<QL>(middle[0], middle[1], middle[0], middle[1], lane);
-            if (lane % QL < 2) sh.known[t0 / U][own_ch] = w;
-          }
-        }
-        to_gq -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
+        to -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
       }
+    }
+    // a tile's own sum first: 2048 tokens one by one lose half a digit
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (cl + c >= p.valid) continue;
+      float* to = g.part_a + (row_n + cl + c) * NP + q0;
+      if (k < used - 1) add_pairs<H>(to, dA[c]);
+      else st_pairs<H>(to, dA[c]);
     }
     // as in the forward pass: the carried gradient meets the tile's decays once
     {
@@ -1059,71 +1098,36 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; ++i) G[c][i] = carry2(through[c][i], G0[c][i], own[c][i]);
-    }
-    // a channel's sums, in pieces of the tile from its ends and its middle (with more than 16 states from every fourth token), where g and h are both known:
-    // rounding errors of the q_r e_r and p_r s x, which all later sums share, have eight (two) tokens to pile up
-    in_front(h);
-    float start[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      f32x2 v = 0;
-#pragma unroll
-      for (int i = 0; i < H; ++i) v = f2_fma(f2_mul(G[c][i], h[c][i]), A[c][i], v);
-      start[c] = both(v);
-    }
-    float* q = &sh.q[0][own_ch] + own_row * (TT / 2) * CT;              // lanes with bit 1 have the tile's second half
-    auto down = [&](int t, int tokens, float v) {
-#pragma unroll
-      for (int i = 0; i < tokens; ++i) {
-        v += q[(t - 1 - i) * CT];
-        q[(t - 1 - i) * CT] = v * LN2;
-      }
-    };
-    auto up = [&](int t, int tokens, float v) {
-#pragma unroll
-      for (int i = 0; i < tokens; ++i) {
-        const float r = q[(t + i) * CT];
-        q[(t + i) * CT] = v * LN2;
-        v -= r;
-      }
-    };
-    if constexpr (OFTEN) {
-      const float w = sum_states<QL>(start[0], start[1], end[0], end[1], lane);
-      if (lane % QL < 4) sh.known[own_row * (TT / U)][own_ch] = w;
-      __syncwarp();
-      if (lane % QL < 4) {                                                // of eight lanes two have the same sums
-        const float* known = &sh.known[own_row * (TT / U / 2)][own_ch];
-#pragma unroll
-        for (int j = 0; j < TT / U / 2; ++j) {
-          up(j * U, U / 2, known[j * CT]);
-          down((j + 1) * U, U / 2, known[(j + 1) * CT]);
-        }
-      }
-    } else {
-      static_assert(OFTEN || QL == 4, "every lane has a half of its own");
-      const float from = sum_states<QL>(start[0], start[1], middle[0], middle[1], lane), till = sum_states<QL>(middle[0], middle[1], end[0], end[1], lane);
-      __syncwarp();
-      up(0, TT / 4, from);
-      down(TT / 2, TT / 4, till);
+        for (int i = 0; i < H; ++i) G[c][i] = carry2(through[c][i], ld2(sh.behind[c * H + i][tid]), own[c][i]);
     }
     __syncthreads();
     parts_to(g.part_b);
-    {
-      x.fetch(a.x, p, k * TT, n);        // again: they would fill 32 registers meanwhile
-      delta.fetch(a.delta, p, k * TT, n);
+#pragma unroll 1
+    for (int part = 0; part < TT; part += Px::SPAN) {
+      x.fetch(a.x, p, k * TT + part, n);      // again: they would fill 32 registers meanwhile
+      delta.fetch(a.delta, p, k * TT + part, n);
       if (a.z.p) {
-        dy.fetch(g.dy, p, k * TT, n);
-        z.fetch(a.z, p, k * TT, n);
+        dy.fetch(g.dy, p, k * TT + part, n);
+        z.fetch(a.z, p, k * TT + part, n);
       }
       float bias[E], skip[E];
       from_shared(sh.bias[0] + col, bias);
       from_shared(sh.bias[1] + col, skip);
 #pragma unroll
       for (int i = 0; i < Px::P; ++i) {
-        const int r = row + i * Px::ROWS, t = k * TT + r;
-        if (t >= a.len) continue;
+        const int r = part + row + i * Px::ROWS, t = k * TT + r;
         const bool in = t < n;
+        if (!in) {                         // for the sums
+          const float zero[E] = {};
+          to_shared(&sh.y[r][col], zero);
+          to_shared(&sh.q[r][col], zero);
+          if (t < a.len) {
+            store_piece<T>(dx + (long long)t * a.dim, zero, p.valid - col, g.vec);
+            store_piece<T>(dd + (long long)t * a.dim, zero, p.valid - col, g.vec);
+            if (g.dz) store_piece<T>(dz + (long long)t * a.dim, zero, p.valid - col, g.vec);
+          }
+          continue;
+        }
         float u[E], e[E], gb[E], f[E], o[E];
         Piece<T>::get(x.v[i], u);
         from_shared(&sh.e[r][col], e);
@@ -1135,7 +1139,7 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
           for (int j = 0; j < E; ++j) {
             const float s = sigmoid(zz[j]), yy = fmaf(skip[j], u[j], f[j]);
-            o[j] = in ? dout[j] * yy * s * (1.f + zz[j] * (1.f - s)) : 0.f;
+            o[j] = dout[j] * yy * s * (1.f + zz[j] * (1.f - s));
           }
           store_piece<T>(dz + (long long)t * a.dim, o, p.valid - col, g.vec);
         }
@@ -1143,24 +1147,33 @@ back_kernel(const Args a, const Grads g) {
         from_shared(&sh.dt[r][col], f);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          o[j] = in ? fmaf(f[j], gb[j], skip[j] * e[j]) : 0.f;
-          d_skip[j] = fmaf(e[j], u[j], d_skip[j]);
+          o[j] = fmaf(f[j], gb[j], skip[j] * e[j]);
+          e[j] *= u[j];
         }
+        to_shared(&sh.y[r][col], e);
         store_piece<T>(dx + (long long)t * a.dim, o, p.valid - col, g.vec);
         from_shared(&sh.q[r][col], f);
         float d[E];
         Piece<T>::get(delta.v[i], d);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          o[j] = fmaf(gb[j], u[j], f[j]);
+          o[j] = fmaf(gb[j], u[j], f[j] * LN2);          // a's unit was a factor of two
           if (a.softplus) o[j] *= sigmoid(d[j] + bias[j]);
-          if (!in) o[j] = 0.f;
-          d_bias[j] += o[j];
         }
+        to_shared(&sh.q[r][col], o);
         store_piece<T>(dd + (long long)t * a.dim, o, p.valid - col, g.vec);
       }
     }
     __syncthreads();
+    if (tid < 2 * CT) {                  // a tile's own sums
+      const float* from = tid < CT ? &sh.y[0][tid] : &sh.q[0][tid - CT];
+      float v[4] = {};
+#pragma unroll
+      for (int r = 0; r < TT; r += 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += from[(r + j) * CT];
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -1172,21 +1185,14 @@ back_kernel(const Args a, const Grads g) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int s = q0 + 2 * i + j;
-        g.part_a[(row_n + cl + c) * NP + s] = sh.da[c * H + i][tid][j];
+        if (used <= first) g.part_a[(row_n + cl + c) * NP + s] = 0.f;
         if (g.d_state_in && p.seg == 0 && s < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + c) * a.states + s] = w[j];
       }
     }
   }
-  float* sums = &sh.dt[0][0];            // [2][ROWS][CT]
-  static_assert(2 * Px::ROWS <= 5 * TT, "sums of the parameters");
-  to_shared(sums + row * CT + col, d_skip);
-  to_shared(sums + (Px::ROWS + row) * CT + col, d_bias);
+  if (tid < 2 * CT && tid % CT < p.valid) (tid < CT ? g.part_skip : g.part_bias)[row_n + tid % CT] = sum;
   __syncthreads();
-  if (tid >= 2 * CT) return;
-  const int c = tid % CT, which = tid / CT;
-  float v = 0.f;
-  for (int r = 0; r < Px::ROWS; ++r) v += sums[(which * Px::ROWS + r) * CT + c];
-  if (c < p.valid) (which ? g.part_bias : g.part_skip)[row_n + c] = v;
+  }
 }
 
 // The blocks' parts of the gradients of b, c and of the parameters, added in one order.
@@ -1316,7 +1322,7 @@ static Plan plan_of(int batch, int len, int dim, int states, int groups, bool ba
   p.per_group = dim / groups;
   const int ct = channels_of(p.np == 64 ? 8 : 4);
   p.tiles = (p.per_group + ct - 1) / ct;
-  const long long blocks = (long long)batch * groups * p.tiles, sms = m2_sm_count(), want = (p.np == 16 ? (backward ? 3 : 4) : 2) * sms;
+  const long long blocks = (long long)batch * groups * p.tiles, sms = m2_sm_count(), want = (backward ? back_blocks(p.np) : p.np == 16 ? 4 : 2) * sms;
   p.segs = 1;
   if (2 * blocks < 3 * sms && p.total >= 8) {
     long long s = want / (blocks > 0 ? blocks : 1);
@@ -1330,9 +1336,14 @@ static Plan plan_of(int batch, int len, int dim, int states, int groups, bool ba
 
 static long long seg_floats(const Plan& p, int batch, int dim) { return p.segs > 1 ? (long long)batch * p.segs * dim * (p.np + 1) : 0; }
 static long long saves_floats(const Plan& p, int batch, int dim) { return (long long)batch * p.total * dim * p.np; }
-static long long between_floats(const Plan& p, int batch, int groups) { return p.np > 16 ? (long long)batch * p.segs * groups * p.tiles * (7 * 8 * THREADS * 2) : 0; }
+static long long work_of(const Plan& p, int batch, int groups) { return (long long)batch * p.segs * groups * p.tiles; }
+static long long back_grid(const Plan& p, int batch, int groups) {
+  const long long work = work_of(p, batch, groups);
+  return p.np == 16 || work < PLACES ? work : PLACES;
+}
+static long long aside_floats(const Plan& p, int batch, int groups) { return p.np == 16 ? 0 : back_grid(p, batch, groups) * (ASIDE * 8 * THREADS * 2); }
 static long long grad_floats(const Plan& p, int batch, int len, int dim, int groups) {
-  return between_floats(p, batch, groups) + seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
+  return aside_floats(p, batch, groups) + seg_floats(p, batch, dim) + 2LL * p.tiles * batch * len * groups * p.np + (long long)batch * p.segs * dim * (p.np + 2);
 }
 
 template <typename T, int S, int QL> static int forward(const Args& a, const Plan& p, cudaStream_t st) {
@@ -1359,7 +1370,7 @@ template <typename T, int S, int QL> static int backward(const Args& a, const Gr
   }
   constexpr size_t smem = sizeof(BackShared<S, QL>);
   M2_SMEM_ONCE((back_kernel<T, S, QL>), smem);
-  if (int rc = m2_launch("m2_selective_scan_bwd", size, back_kernel<T, S, QL>, dim3((unsigned)blocks), THREADS, smem, st, a, g)) return rc;
+  if (int rc = m2_launch("m2_selective_scan_bwd", size, back_kernel<T, S, QL>, dim3((unsigned)back_grid(p, a.batch, a.groups)), THREADS, smem, st, a, g, (unsigned)blocks)) return rc;
   const long long bc = ((long long)a.batch * a.len * a.groups * a.states + 255) / 256, par = ((long long)a.dim * (a.states + 2) + 255) / 256;
   return m2_launch("m2_selective_scan_bwd", size, finish_kernel<T>, dim3((unsigned)(bc + par)), 256, 0, st, a, g, p.np, (unsigned)bc);
 }
@@ -1461,13 +1472,13 @@ extern "C" int m2_selective_scan_bwd(const m2_selective_scan_args* args, const m
   r.d_state_out = o.d_state_out;
   r.dx = o.d_x; r.d_delta = o.d_delta; r.dz = o.d_gate;
   r.vec = m2_aligned(o.d_x, 16) && m2_aligned(o.d_delta, 16) && m2_aligned(o.d_gate, 16) && (long long)p.per_group * size % 16 == 0;
-  r.between = g.workspace;               // on 16 bytes, as a multiple of that many floats
-  float* w = g.workspace + between_floats(p, g.batch, g.groups);
-  a.seg_state = w;
-  a.seg_steps = w + (long long)g.batch * p.segs * g.dim * p.np;
-  w += seg_floats(p, g.batch, g.dim);
+  // aside, part_a and seg_state on 16 bytes: multiples of that many floats
   const long long bc = (long long)p.tiles * g.batch * g.seq_len * g.groups * p.np, parts = (long long)g.batch * p.segs * g.dim;
-  r.part_b = w; r.part_c = w + bc; r.part_a = w + 2 * bc; r.part_skip = r.part_a + parts * p.np; r.part_bias = r.part_skip + parts;
+  float* w = g.workspace;
+  r.aside = w; w += aside_floats(p, g.batch, g.groups);
+  r.part_a = w; w += parts * p.np;
+  a.seg_state = w; a.seg_steps = w + parts * p.np; w += seg_floats(p, g.batch, g.dim);
+  r.part_b = w; r.part_c = w + bc; r.part_skip = w + 2 * bc; r.part_bias = r.part_skip + parts;
   r.db = o.d_b; r.dc = o.d_c; r.da = o.d_a; r.d_skip = o.d_skip; r.d_bias = o.d_delta_bias; r.d_state_in = o.d_state_in;
   const cudaStream_t st = (cudaStream_t)stream;
   return M2_SS_DISPATCH(backward, a, r, p, st);

@@ -66,3 +66,103 @@ def test_a_step_of_zero_changes_no_state(N, value):
     assert torch.equal(own, state)
     _, s = m2_b200.selective_scan(**t, initial_state=state, return_state=True)
     assert torch.equal(s, state)
+
+
+FADING = [(-1e2, 5.0), (-16.0, 5.0), (-1e4, 1.0), (-1e30, 0.1), (LOWEST, 0.1)]
+
+
+@pytest.mark.parametrize("a,step", FADING)
+@pytest.mark.parametrize("L,N", [(64, 4), (45, 4), (600, 4), (64, 20), (70, 40)])
+def test_steps_of_states_that_fade_fast(L, N, a, step):
+    """The gradient of a step is sum_n a g exp(s a) h + x sum_n g b.  Where a state forgets, the first part is next to nothing and the second is left, whatever a is."""
+    B, D = 2, 24
+    t = make(B, L, D, N, 1, torch.float32, plain=True)
+    t["a"] = torch.full((D, N), a, device="cuda") * (0.5 + torch.rand(D, N, device="cuda") * 0.5)
+    t["delta"] = step * (1 + torch.rand(B, L, D, device="cuda"))
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y, s = m2_b200.selective_scan(**leaves, return_state=True)
+    up, d_s = torch.randn_like(y), torch.randn_like(s)
+    grads = dict(zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [up, d_s])))
+    ref, M = (definition(t, False, None, up, d_s, size) for size in (False, True))
+    for k in ("delta", "x", "a"):
+        within(grads[k], ref[k], U32 * ref[k].abs() + (3 * strong(N) + (B * L * U32 if k == "a" else 0.0)) * M[k], k)
+
+
+@pytest.mark.parametrize("what", ["dy", "x", "both"])
+@pytest.mark.parametrize("L,N", [(64, 4), (600, 4), (64, 20), (70, 40)])
+def test_a_token_that_outweighs_the_others_leaves_their_gradients_alone(L, N, what):
+    """One gradient of y, or one x, a million times the others': tokens behind the first, and in front of the second, do not depend on it."""
+    B, D = 2, 24
+    t = make(B, L, D, N, 1, torch.float32, plain=True)
+    t["a"] = -1 - torch.rand(D, N, device="cuda")
+    t["delta"] = 1 + torch.rand(B, L, D, device="cuda")
+    up, d_s = torch.randn(B, L, D, device="cuda"), torch.randn(B, D, N, device="cuda")
+    for at in (5, 18, 27, 43):
+        if what != "x":
+            up[:, at, ::3] *= 1e6
+        if what != "dy":
+            t["x"][:, at, ::3] *= 1e6
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y, s = m2_b200.selective_scan(**leaves, return_state=True)
+    grads = dict(zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [up, d_s])))
+    ref, M = (definition(t, False, None, up, d_s, size) for size in (False, True))
+    for k in ("delta", "x", "a"):
+        within(grads[k], ref[k], U32 * ref[k].abs() + (3 * strong(N) + (B * L * U32 if k == "a" else 0.0)) * M[k], k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L,N", [(60, 16), (700, 16), (100, 20), (60, 40)])
+def test_what_is_not_finite_reaches_no_gradient_that_does_not_depend_on_it(L, N, dtype):
+    """A gradient of y at one token: gradients of its channel up to this token.  An x: gradients of its channel behind it (and its own).  Bits of all others stay."""
+    D, T, CH = 70, 37, 5
+    t = make(1, L, D, N, 1, dtype)
+
+    def run(t, up):
+        leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+        y, s = m2_b200.selective_scan(**leaves, softplus=True, return_state=True)
+        return dict(zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [up, torch.ones_like(s)])))
+
+    up = torch.randn(1, L, D, device="cuda").to(dtype)
+    ref = run(t, up)
+    others = [i for i in range(D) if i != CH]
+    for value in (float("nan"), float("inf")):
+        bad = up.clone()
+        bad[0, T, CH] = value
+        got = run(t, bad)
+        for k in ("x", "delta", "gate"):
+            assert torch.equal(got[k][..., others], ref[k][..., others]) and torch.equal(got[k][:, T + 1:], ref[k][:, T + 1:]), k
+        assert torch.equal(got["gate"][:, :T], ref["gate"][:, :T]) and torch.equal(got["b"][:, T + 1:], ref["b"][:, T + 1:])
+        assert torch.equal(got["c"][:, :T], ref["c"][:, :T]) and torch.equal(got["c"][:, T + 1:], ref["c"][:, T + 1:])
+        assert not torch.isfinite(got["x"][0, T, CH]) and not torch.isfinite(got["delta"][0, T, CH])
+        bad = {k: v.clone() for k, v in t.items()}
+        bad["x"][0, T, CH] = value
+        got = run(bad, up)
+        for k in ("x", "delta", "gate"):
+            assert torch.equal(got[k][..., others], ref[k][..., others]) and torch.equal(got[k][:, :T], ref[k][:, :T]), k
+        assert torch.equal(got["x"][:, T + 1:], ref["x"][:, T + 1:])
+        assert torch.equal(got["b"][:, :T], ref["b"][:, :T]) and torch.equal(got["b"][:, T + 1:], ref["b"][:, T + 1:])
+        assert torch.equal(got["c"][:, :T], ref["c"][:, :T])
+
+
+@pytest.mark.parametrize("L,N", [(100, 4), (700, 4), (100, 20), (60, 40)])
+def test_gradients_beside_an_empty_state_that_would_grow(L, N):
+    """Factors of e^20 a token on states that are neither fed nor read: all gradients are those of the fading states alone, and theirs are zero."""
+    D = 64
+    t = make(1, L, D, N, 1, torch.float32, plain=True)
+    t["a"] = -1 - torch.rand(D, N, device="cuda")
+    t["a"][:, ::2] = 20.0
+    t["delta"] = torch.ones_like(t["delta"])
+    t["b"][..., ::2] = 0
+    t["c"][..., ::2] = 0
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y = m2_b200.selective_scan(**leaves)
+    up = torch.randn_like(y)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), up)))
+    fading = {**t, "a": t["a"][:, 1::2], "b": t["b"][..., 1::2], "c": t["c"][..., 1::2]}
+    ref, M = (definition(fading, False, None, up, None, size) for size in (False, True))
+    for k, v in grads.items():
+        if k in ("a", "b", "c"):
+            assert not v[..., ::2].any(), k
+            v = v[..., 1::2]
+        terms = {"b": D, "c": D, "a": L}.get(k, 0)
+        within(v, ref[k], U32 * ref[k].abs() + (3 * strong(N) + terms * U32) * M[k], k)
