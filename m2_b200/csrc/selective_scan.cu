@@ -186,14 +186,29 @@ template <int H> __device__ __forceinline__ void decays(f32x2 dt, const f32x2 (&
 #pragma unroll
     for (int i = 0; i < H; ++i) d[c][i] = ex2_pair(f2_mul(s[c], A[c][i]));
 }
-// What was carried, by the decays that it met, and what came since.  Nothing carried is nothing, also where states that grow would make infinity of it.
-__device__ __forceinline__ float carry(float through, float before, float own) { return before == 0.f ? own : fmaf(through, before, own); }
-__device__ __forceinline__ f32x2 carry2(f32x2 through, f32x2 before, f32x2 own) {
-  float t[2], b[2], o[2];
-  f2_unpack(through, t[0], t[1]);
-  f2_unpack(before, b[0], b[1]);
-  f2_unpack(own, o[0], o[1]);
-  return f2_pack(carry(t[0], b[0], o[0]), carry(t[1], b[1], o[1]));
+// What was carried, by 2^x for the decays that it met, and what came since.  Nothing carried is nothing, also where states that grow would make infinity of it; a
+// factor beyond float32 is met in two halves, as a small state (a large one) may well have grown (faded) by it.
+__device__ __forceinline__ float part_of(float x) { return fabsf(x) > 120.f ? 0.5f : 1.f; }
+__device__ __forceinline__ float carry(float part, float f, float before, float own) {             // f = 2^(part x)
+  return before == 0.f ? own : fmaf(part < 1.f ? before * f : before, f, own);
+}
+__device__ __forceinline__ float carry(float x, float before, float own) {
+  const float part = part_of(x);
+  return carry(part, ex2(part * x), before, own);
+}
+template <int H> __device__ __forceinline__ void carry_pairs(f32x2 dt, const f32x2 (&A)[2][H], f32x2 (&h)[2][H], const f32x2 (&own)[2][H]) {      // h becomes the sum
+  float s[2];
+  f2_unpack(dt, s[0], s[1]);
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      float x[2], b[2], o[2];
+      f2_unpack(f2_mul(f2_splat(s[c]), A[c][i]), x[0], x[1]);
+      f2_unpack(h[c][i], b[0], b[1]);
+      f2_unpack(own[c][i], o[0], o[1]);
+      h[c][i] = f2_pack(carry(x[0], b[0], o[0]), carry(x[1], b[1], o[1]));
+    }
 }
 
 // The sum over the lanes of a channel's states of v and w, of two channels each: lane bit 0 ends with the channel, bit 1 with v or w.
@@ -546,12 +561,11 @@ scan_kernel(const Args a) {
       }
     }
     // the carried state meets the tile's decays in one product, so that its error grows with the tiles, not with the tokens
-    f32x2 through[2][H];
-    decays<H>(cum, A, through);
+    carry_pairs<H>(cum, A, h0, own);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int i = 0; i < H; ++i) h[c][i] = carry2(through[c][i], h0[c][i], own[c][i]);
+      for (int i = 0; i < H; ++i) h[c][i] = h0[c][i];
     steps = f2_add(steps, cum);
     __syncthreads();
     if constexpr (!SUMS) {
@@ -625,19 +639,22 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
   const long long step = reverse ? -(long long)dim : dim;
   long long at = ((long long)b * segs + (reverse ? segs - 1 : 0)) * dim + d;
   for (int k = 0; k < segs; k += U) {
-    float own[U], decay[U];
+    float own[U], decay[U], part[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       own[u] = k + u < segs ? seg_state[(at + u * step) * np + s] : 0.f;
       decay[u] = k + u < segs ? seg_steps[at + u * step] : 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) decay[u] = exp2f(A * decay[u]);
+    for (int u = 0; u < U; ++u) {
+      part[u] = part_of(A * decay[u]);
+      decay[u] = exp2f(part[u] * (A * decay[u]));
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (k + u < segs) {
         seg_state[(at + u * step) * np + s] = h;
-        h = carry(decay[u], h, own[u]);
+        h = carry(part[u], decay[u], h, own[u]);
       }
     }
     at += U * step;
@@ -1092,14 +1109,11 @@ back_kernel(const Args a, const Grads g, const unsigned work) {
       else st_pairs<H>(to, dA[c]);
     }
     // as in the forward pass: the carried gradient meets the tile's decays once
-    {
-      f32x2 through[2][H];
-      decays<H>(cum, A, through);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; ++i) G[c][i] = carry2(through[c][i], ld2(sh.behind[c * H + i][tid]), own[c][i]);
-    }
+      for (int i = 0; i < H; ++i) G[c][i] = ld2(sh.behind[c * H + i][tid]);
+    carry_pairs<H>(cum, A, G, own);
     __syncthreads();
     parts_to(g.part_b);
 #pragma unroll 1

@@ -166,3 +166,27 @@ def test_gradients_beside_an_empty_state_that_would_grow(L, N):
             v = v[..., 1::2]
         terms = {"b": D, "c": D, "a": L}.get(k, 0)
         within(v, ref[k], U32 * ref[k].abs() + (3 * strong(N) + terms * U32) * M[k], k)
+
+
+@pytest.mark.parametrize("L,N", [(64, 4), (700, 16), (64, 20), (100, 40)])
+@pytest.mark.parametrize("rate,start", [(1.0, 1e-30), (-1.0, 1e30)])
+def test_factors_beyond_float32_between_states_within_it(L, N, rate, start):
+    """exp(a times the steps of a tile, or of a segment) is e^128 or e^-128, beyond float32; the state of 1e-30 (1e30) in front and that behind are not.
+    Errors: 2^-22 for each of the 64 decays of a step that is not 0, and 128 times what the exponents are off by: two roundings, and one for each of the 64 sums on the way
+    to the sum of the steps (all steps are equal, so these may all go one way)."""
+    B, D = 2, 24
+    t = make(B, L, D, N, 1, torch.float32, plain=True)
+    t["a"] = torch.full((D, N), 20.0 * rate, device="cuda")
+    t["delta"] = torch.zeros(B, L, D, device="cuda")
+    first, tokens, step = (64, 64, 0.1) if L > 100 else (32, 20, 0.32)
+    t["delta"][:, first:first + tokens] = step
+    t["x"].zero_()
+    t["initial_state"] = start * (1 + torch.rand(B, D, N, device="cuda"))
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y, s = m2_b200.selective_scan(**leaves, return_state=True)
+    d_s = start * torch.randn(B, D, N, device="cuda").sign()
+    (g,) = torch.autograd.grad(s, [leaves["initial_state"]], d_s)
+    total = (t["delta"].double()[..., None] * t["a"].double()).sum(1)
+    one = 64 * 2.0 ** -22 + 128 * (2 + 64) * U32 + 64 * U32
+    within(s, t["initial_state"].double() * torch.exp(total), one * (t["initial_state"].double() * torch.exp(total)).abs(), "state")
+    within(g, d_s.double() * torch.exp(total), one * (d_s.double() * torch.exp(total)).abs(), "gradient")
