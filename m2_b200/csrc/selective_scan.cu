@@ -725,6 +725,11 @@ back_sums_kernel(const Args a, const Grads g) {
     }
     fc.put(&s_c[0][0]);
     __syncthreads();
+    f32x2 own[2][H], cum = 0;            // the tile's, as in the forward pass
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < H; ++i) own[c][i] = 0;
 #pragma unroll 4
     for (int t = TT - 1; t >= 0; --t) {
       const f32x2 dt = ld2(&s_dt[t][cl]);
@@ -735,9 +740,11 @@ back_sums_kernel(const Args a, const Grads g) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; ++i) G[c][i] = f2_mul(d[c][i], f2_fma(e[c], C[i], G[c][i]));
-      steps = f2_add(steps, dt);
+        for (int i = 0; i < H; ++i) own[c][i] = f2_mul(d[c][i], f2_fma(e[c], C[i], own[c][i]));
+      cum = f2_add(cum, dt);
     }
+    carry_pairs<H>(cum, A, G, own);
+    steps = f2_add(steps, cum);
     __syncthreads();
   }
   const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;

@@ -1,0 +1,38 @@
+"""Long sums whose roundings all go one way: softmax denominators of peaked and of rising rows, and parameters' gradients over long and over many sequences."""
+import pytest
+import torch
+
+import m2_b200
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+
+
+def score_errors(logits, keep=2):
+    B, K, V = logits.shape
+    got = m2_b200.beam_select(logits, torch.zeros(B, K, device="cuda"), keep=keep)
+    lp = torch.log_softmax(logits.double(), -1)
+    ref = lp[torch.arange(B, device="cuda")[:, None], got.beam, got.token]
+    return (got.score.double() - ref).abs(), ref
+
+
+# 1 + 2^-12 + 2^-14, four thousand times one by one in float32, is off by 0.75, three eighths of a step of the sum each time
+ODD = 1 + 2.0 ** -12 + 2.0 ** -14
+
+
+def test_gradients_along_a_long_axis_are_handed_on_by_tiles():
+    """The gradient of the initial state through 16384 tokens that hardly fade, in two segments, all terms of one sign: every tile of 32 tokens of a segment rounds what it
+    carries by its decays' 2^-22 and two roundings more, and its own terms by 40 of each; token by token the same decay's rounding, up to 2^-25, would come 8192 times."""
+    L, G, N = 16384, 200, 16
+    delta = torch.ones(1, 1, G, device="cuda").expand(1, L, G)
+    a = -(torch.arange(1, N + 1, device="cuda") * 2.0 ** -15 * 1.1).expand(G, N).contiguous()
+    b, c = torch.zeros(1, 1, G, N, device="cuda").expand(1, L, G, N), torch.ones(1, 1, G, N, device="cuda").expand(1, L, G, N)
+    initial = torch.zeros(1, G, N, device="cuda", requires_grad=True)
+    y = m2_b200.selective_scan(delta, delta, a, b, c, initial_state=initial)
+    (got,) = torch.autograd.grad(y, [initial], torch.ones_like(y))
+    ages = torch.arange(1, L + 1, dtype=torch.float64, device="cuda")
+    terms = torch.exp(a.double()[0, :, None] * ages)
+    ref, age = terms.sum(1), (terms * (ages % (L // 2))).sum(1) / terms.sum(1)          # of the terms within their segments
+    off = ((got[0].double() - ref).abs() / ref).amax(0)
+    bound = age / 32 * (2.0 ** -22 + 2 * U32) + 40 * U32
+    assert (off <= bound).all(), (off / bound).tolist()
