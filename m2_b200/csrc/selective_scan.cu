@@ -648,7 +648,7 @@ join_kernel(const float* __restrict__ a, float* __restrict__ seg_state, const fl
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       part[u] = part_of(A * decay[u]);
-      decay[u] = exp2f(part[u] * (A * decay[u]));
+      decay[u] = ex2(part[u] * (A * decay[u]));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1216,7 +1216,7 @@ back_kernel(const Args a, const Grads g, const unsigned work) {
   }
 }
 
-// The blocks' parts of the gradients of b, c and of the parameters, added in one order.
+// The blocks' parts of the gradients of b, c and of the parameters, added in one order; those of the parameters, one for each sequence and segment, in 64 bits.
 template <typename T>
 __global__ void __launch_bounds__(256)
 finish_kernel(const Args a, const Grads g, int np, unsigned bc_blocks) {
@@ -1241,17 +1241,21 @@ finish_kernel(const Args a, const Grads g, int np, unsigned bc_blocks) {
   const long long i = (blockIdx.x - bc_blocks) * 256LL + threadIdx.x, d = i / (a.states + 2);
   const int s = (int)(i - d * (a.states + 2)), parts = a.batch * a.segs;
   if (d >= a.dim) return;
-  float v = 0.f;
+  auto total = [&](const float* from, long long step) {                  // eight at a time, whose loads are under way together
+    double v = 0.0;
+    for (int k = 0; k < parts; k += 8) {
+      float eight = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) eight += k + j < parts ? from[(k + j) * step] : 0.f;
+      v += eight;
+    }
+    return (float)v;
+  };
   if (s < a.states) {
-    if (!g.da) return;
-    for (int k = 0; k < parts; ++k) v += g.part_a[((long long)k * a.dim + d) * np + s];
-    g.da[d * a.states + s] = v;
+    if (g.da) g.da[d * a.states + s] = total(g.part_a + d * np + s, (long long)a.dim * np);
   } else {
-    const float* from = s == a.states ? g.part_skip : g.part_bias;
     float* to = s == a.states ? g.d_skip : g.d_bias;
-    if (!to) return;
-    for (int k = 0; k < parts; ++k) v += from[(long long)k * a.dim + d];
-    to[d] = v;
+    if (to) to[d] = total((s == a.states ? g.part_skip : g.part_bias) + d, a.dim);
   }
 }
 

@@ -20,6 +20,22 @@ def score_errors(logits, keep=2):
 ODD = 1 + 2.0 ** -12 + 2.0 ** -14
 
 
+@pytest.mark.parametrize("B,L,D,N", [(32768, 2, 8, 4), (8192, 40, 8, 20)])
+def test_parameters_gradients_of_scans_over_many_sequences(B, L, D, N):
+    """The sums of the sequences are added in 64 bits; within one there are L terms."""
+    x = torch.ones(1, 1, 1, device="cuda").expand(B, L, D)
+    b = torch.ones(1, 1, 1, device="cuda").expand(B, L, N)
+    a, skip, bias = torch.zeros(D, N, device="cuda", requires_grad=True), torch.zeros(D, device="cuda", requires_grad=True), torch.zeros(D, device="cuda", requires_grad=True)
+    initial = torch.ones(1, 1, 1, device="cuda").expand(B, D, N)
+    y = m2_b200.selective_scan(x, x, a, b, b, skip=skip, delta_bias=bias, initial_state=initial)
+    grads = torch.autograd.grad(y, [a, skip, bias], torch.full((1, 1, 1), ODD, device="cuda").expand(B, L, D))
+    t = torch.arange(1, L + 1, dtype=torch.float64)
+    # steps 1 and no fading: h_t = 1 + t, dy_t / da = sum_{s <= t} h_{s-1} = sum_{s <= t} s, dy_t / dstep_s = 1 a state for s <= t
+    want = [B * ODD * (t * (t + 1) / 2).sum().item(), B * L * ODD, B * ODD * N * t.sum().item()]
+    for got, ref in zip(grads, want):
+        assert (got.double() - ref).abs().max() <= (2 * L + N + 8) * U32 * ref
+
+
 def test_gradients_along_a_long_axis_are_handed_on_by_tiles():
     """The gradient of the initial state through 16384 tokens that hardly fade, in two segments, all terms of one sign: every tile of 32 tokens of a segment rounds what it
     carries by its decays' 2^-22 and two roundings more, and its own terms by 40 of each; token by token the same decay's rounding, up to 2^-25, would come 8192 times."""
