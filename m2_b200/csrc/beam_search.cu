@@ -4,12 +4,13 @@
 //
 // Selection in two kernels.  The first reads each beam's logits once (a cluster of blocks a row where there are few rows): maximum, sum of
 // exponentials, and its `keep` best tokens, found without sorting as in token_logprobs.cu.  The second, a warp a text, merges the beams' sorted lists: a
-// lane a beam, the best head `keep` times.  Scores are compared in 64 bits, exponentials are within a rounding of float32 and summed in pairs, so
-// that the order is that of exact scores but for gaps below about 1e-7.
+// lane a beam, the best head `keep` times.  Scores are compared in 64 bits.  Their sums of exponentials are within 5 2^-24 (3e-7) of themselves, however many logits there
+// are and however they lie: each exponential within 2 2^-24 (what its argument's subtraction rounds off is put back), those of 16 bytes added in float32 as a
+// tree, and from there on in 64 bits, without being scaled again by float32 factors on the way.  So the order is that of exact scores but for gaps below that.
 // States: a thread owns a few bytes of the rows of all beams of one text; it reads the rows that its beams come from before it writes any,
 // so that nothing waits and no second buffer is needed.  Rows that stay are neither read nor written.
-// Measured: selection for one text of four beams 17 us, for 32 of eight beams (float32, 31 MB) 27; states of 12 layers of the latter (256 rows of 58 KB a layer) 40 us,
-// 0.97 of the measured copy rate counted as if all rows moved.
+// Measured: selection for one text of four beams 17 us, for 32 of eight beams (float32, 31 MB) 27; states of 12 layers of the latter (256 rows of 58 KB a layer,
+// of which two in three move) 40 us.
 #include "common.cuh"
 
 namespace m2 {
@@ -26,17 +27,20 @@ struct Args {
   const float* scores;
   const unsigned char* finished;
   long long end_id;                               // -1: none
-  float* row_max; double* row_sum;                // (batch * beams)
+  float* row_max; double* row_sum;                // (batch * beams): sums of exponentials of differences to a logit that is the largest but for 32
   unsigned long long* best;                       // (batch * beams, list)
   float* score;
   long long *beam, *token;
   unsigned char* done;
 };
 
-// exp(d) for d <= 0: 2^i 2^f with the powers of ln 2 for 2^f, |f| <= 1/2, cut where the next is below 1e-8; 0 below exp(-87), NaN stays NaN
-__device__ __forceinline__ float exp_near(float d) {
+// exp(v - m) for v - m < 64: 2^i 2^f with the powers of ln 2 for 2^f, |f| <= 1/2, cut where the next is below 1e-8; 0 below exp(-87), NaN stays NaN
+__device__ __forceinline__ float exp_near(float v, float m) {
+  const float d = v - m;
+  // the sum of two numbers exactly (D. E. Knuth): back is v as d has it, and what d lost is v - back less m - (back - d)
+  const float back = d + m, lost = (v - back) - (m - (back - d));
   const float i = rintf(d * lp::LOG2E);
-  const float f = fmaf(d, lp::LOG2E, -i) + d * 1.92596299e-8f;       // LOG2E and what float32 leaves of it
+  const float f = fmaf(d, lp::LOG2E, -i) + fmaf(d, 1.92596299e-8f, lost * lp::LOG2E);       // LOG2E and what float32 leaves of it
   float p = 1.52527338e-5f;
   p = fmaf(p, f, 1.54035304e-4f);
   p = fmaf(p, f, 1.33335581e-3f);
@@ -49,12 +53,8 @@ __device__ __forceinline__ float exp_near(float d) {
 }
 
 struct Sum { float m; double s; };
-__device__ __forceinline__ Sum join(Sum a, Sum b) {
-  const float m = fmaxf(a.m, b.m);
-  // the lowest finite value stands for no maximum: its sum is 0 or NaN
-  const double fa = a.m < m ? (double)exp_near(a.m - m) : 1.0, fb = b.m < m ? (double)exp_near(b.m - m) : 1.0;
-  return {m, a.s * fa + b.s * fb};
-}
+// s of m becomes that of a larger maximum
+__device__ __forceinline__ double at_maximum(Sum a, float m) { return a.m < m ? a.s * exp((double)a.m - (double)m) : a.s; }
 
 struct Shared {
   lp::Shared top;
@@ -75,12 +75,15 @@ rows_kernel(const Args a) {
   const int per = ((a.vocab + split - 1) / split + 63) / 64 * 64;
   const int lo = min((int)part * per, a.vocab), hi = min(lo + per, a.vocab);
   const lp::Span<T> sp(x, lo, hi);
-  float m = lp::LOWEST, s = 0.f;                  // a NaN or +inf makes s NaN
-  auto add = [&](float v) {
-    if (v > m) { s *= exp_near(m - v); m = v; }
-    s += exp_near(v - m);
+  // exponentials of differences to m, which stays while no logit is more than RISE above it; vmax is the largest logit.  A NaN or +inf makes s NaN.
+  constexpr float RISE = 32.f;
+  float m = lp::LOWEST, vmax = lp::LOWEST;
+  double s = 0.0;
+  auto look = [&](float big) {
+    if (big > vmax) vmax = big;
+    if (big > m + RISE) { s = at_maximum({m, s}, big); m = big; }
   };
-  sp.ends([&](float v, int) { add(v); });
+  sp.ends([&](float v, int) { look(v); s += exp_near(v, m); });
   const uint4* body = reinterpret_cast<const uint4*>(x + sp.body());
   constexpr int U = 4;
   uint4 now[U], next[U];
@@ -97,38 +100,46 @@ rows_kernel(const Args a) {
       if (i + j * THREADS < sp.pieces) {
         float f[N];
         Piece<T>::get(now[j], f);
-        const float big = lp::largest(now[j], f);
-        if (big > m) { s *= exp_near(m - big); m = big; }
-        float e = 0.f;
+        look(lp::largest(now[j], f));
 #pragma unroll
-        for (int q = 0; q < N; ++q) e += exp_near(f[q] - m);
-        s += e;
+        for (int q = 0; q < N; ++q) f[q] = exp_near(f[q], m);
+#pragma unroll
+        for (int w = N / 2; w > 0; w /= 2)
+#pragma unroll
+          for (int q = 0; q < w; ++q) f[q] += f[q + w];
+        s += f[0];
       }
       now[j] = next[j];
     }
   }
-  Sum st = {m, (double)s};
-  const float vmax = m;
   const bool nan = s != s;
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sum b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o)};
-    st = join(st, b);
-  }
+  Sum st = {m, s};
+  auto warp_sum = [&](int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    s = at_maximum(st, m);
+    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    st = {m, s};
+  };
+  warp_sum(32);
   if (lane == 0) sh.warp[warp] = st;
   __syncthreads();
-  if (tid == 0) {
-    st = sh.warp[0];
-    for (int w = 1; w < lp::WARPS; ++w) st = join(st, sh.warp[w]);
-    sh.mine = st;
+  if (warp == 0) {
+    st = lane < lp::WARPS ? sh.warp[lane] : Sum{lp::LOWEST, 0.0};
+    m = st.m;
+    warp_sum(32);
+    if (lane == 0) sh.mine = st;
   }
   lp::select_top<T>(sh.top, sp, a.list, vmax, nan);
   if (split > 1) lp::cluster_barrier(); else __syncthreads();
   if (part == 0) {
-    if (tid == 0) {
-      st = sh.mine;
-      for (int r = 1; r < split; ++r) st = join(st, *lp::in_cta(&sh.mine, r));
-      a.row_max[row] = st.m;
-      a.row_sum[row] = st.s;
+    if (warp == 0) {
+      st = lane < split ? *lp::in_cta(&sh.mine, lane) : Sum{lp::LOWEST, 0.0};
+      m = st.m;
+      warp_sum(32);
+      if (lane == 0) {
+        a.row_max[row] = st.m;
+        a.row_sum[row] = st.s;
+      }
     }
     if (split == 1) {
       if (tid < a.list) a.best[row * a.list + tid] = sh.top.best[tid];

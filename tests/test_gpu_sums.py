@@ -16,6 +16,28 @@ def score_errors(logits, keep=2):
     return (got.score.double() - ref).abs(), ref
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,K", [(1, 4), (40, 8)])              # a row is shared by blocks, and is not
+@pytest.mark.parametrize("V", [30528, 131072])
+def test_scores_of_peaked_and_rising_rows(B, K, V, dtype):
+    """Every exponential is within 2 2^-24 of its own size (its argument's rounding is added back), sums of a piece's up to 8 take 3 more, and what follows is in 64
+    bits: 5 2^-24 of the sum, below 2^-21, whatever the number of logits; the score itself is rounded once."""
+    at = torch.arange(B * K, device="cuda").view(B, K, 1) * 3001 % V
+    rows = []
+    for high, low in ((0.0, -18.1), (2.2, -9.3), (1.7, -8.9), (30.3, 19.1), (0.1, 0.0)):
+        x = torch.full((B, K, V), low, device="cuda")
+        rows.append(x.scatter_(2, at, high))
+    rows.append((torch.arange(V, device="cuda") * 2.0 ** -20).expand(B, K, V).contiguous())
+    rows.append((torch.arange(V, device="cuda") * 2.0 ** -10).expand(B, K, V).contiguous())
+    rows.append((torch.arange(V, device="cuda") * -2.0 ** -14).expand(B, K, V).contiguous())
+    rows.append(torch.randn(B, K, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V)) * 4)
+    worst = []
+    for x in rows:
+        off, ref = score_errors(x.to(dtype))
+        worst.append(((off - U32 * ref.abs()) / 2.0 ** -21).max().item())
+    assert max(worst) <= 1, worst
+
+
 # 1 + 2^-12 + 2^-14, four thousand times one by one in float32, is off by 0.75, three eighths of a step of the sum each time
 ODD = 1 + 2.0 ** -12 + 2.0 ** -14
 
