@@ -418,16 +418,22 @@ back_kernel(const Args a, const Grads g) {
   }
 }
 
-// Sums of the chunks' parts: 32 columns a block, 8 parts side by side, then these in order.
+// Sums of the chunks' parts: 32 columns a block, 8 threads a column, eight parts of each at a time in float32, these in 64 bits and in order.
 __global__ void __launch_bounds__(256)
 sum_kernel(const float* __restrict__ part, float* dw, float* d_bias, int parts, int taps, int dim) {
-  __shared__ float s[8][32];
+  __shared__ double s[8][32];
   pdl_wait();
   const long long i = blockIdx.x * 32LL + (threadIdx.x & 31), n = (long long)(taps + 1) * dim;
   const int y = threadIdx.x >> 5;
-  float v = 0.f;
-  if (i < n)
-    for (int k = y; k < parts; k += 8) v += part[k * n + i];
+  double v = 0.0;
+  if (i < n) {
+    for (int k = y; k < parts; k += 64) {
+      float eight = 0.f;
+#pragma unroll
+      for (int j = 0; j < 64; j += 8) eight += k + j < parts ? part[(k + j) * n + i] : 0.f;
+      v += eight;
+    }
+  }
   s[y][threadIdx.x & 31] = v;
   __syncthreads();
   if (y || i >= n) return;
@@ -435,8 +441,8 @@ sum_kernel(const float* __restrict__ part, float* dw, float* d_bias, int parts, 
 #pragma unroll
   for (int k = 1; k < 8; ++k) v += s[k][threadIdx.x];
   const int tap = (int)(i / dim), c = (int)(i % dim);
-  if (tap < taps) { if (dw) dw[(long long)c * taps + tap] = v; }
-  else if (d_bias) d_bias[c] = v;
+  if (tap < taps) { if (dw) dw[(long long)c * taps + tap] = (float)v; }
+  else if (d_bias) d_bias[c] = (float)v;
 }
 
 struct StepArgs {
@@ -504,7 +510,12 @@ static int chunk_of(int batch, int len, int dim, int v, int an_sm, int least) {
 }
 // Of the gradients: their parameters' sums leave W + 1 numbers a channel and chunk, and each chunk walks W - 1 tokens further.  The width of a
 // thread goes by the tensors' alignment, the workspace does not: chunks are those of the widest.
-static int back_chunk_of(int batch, int len, int dim) { return chunk_of(batch, len, dim, 4, 3, 16); }
+// A thread adds at most 256 tokens one by one: 8192 in one round of threads were off by 1e-4 where all roundings go one way (and slower: 64 x 8192 x 1536 bf16 in chunks of
+// 4096 took 1123 us, in chunks of 256 1079).
+static int back_chunk_of(int batch, int len, int dim) {
+  const int chunk = chunk_of(batch, len, dim, 4, 3, 16), parts = (len + 255) / 256;
+  return chunk <= 256 ? chunk : (len + parts - 1) / parts;
+}
 
 // channels of a thread: 8 bytes (float32 forward with few taps 16); one where a row does not allow it
 static bool wide(const void* p, long long sb, long long st, int dim, int size, int bytes) {

@@ -42,6 +42,19 @@ def test_scores_of_peaked_and_rising_rows(B, K, V, dtype):
 ODD = 1 + 2.0 ** -12 + 2.0 ** -14
 
 
+@pytest.mark.parametrize("B,L,D", [(56, 8192, 2048), (65536, 16, 8), (2, 8192, 64)])   # a thread for each long sequence; many short ones; cut
+def test_taps_gradients_over_long_and_many_sequences(B, L, D):
+    """A thread adds at most 256 tokens in float32 (256 2^-24 of the sum, were all roundings to go one way), the threads' sums are added in 64 bits."""
+    x = torch.ones(1, 1, D, device="cuda").expand(B, L, D)
+    w, bias = torch.zeros(D, 4, device="cuda", requires_grad=True), torch.zeros(D, device="cuda", requires_grad=True)
+    y = m2_b200.causal_conv(x, w, bias)
+    d_w, d_b = torch.autograd.grad(y, [w, bias], torch.full((1, 1, D), ODD, device="cuda").expand(B, L, D))
+    for i in range(4):
+        n = B * (L - (3 - i))
+        assert (d_w[:, i].double() - n * ODD).abs().max() <= 257 * U32 * n * ODD
+    assert (d_b.double() - B * L * ODD).abs().max() <= 257 * U32 * B * L * ODD
+
+
 @pytest.mark.parametrize("B,L,D,N", [(32768, 2, 8, 4), (8192, 40, 8, 20)])
 def test_parameters_gradients_of_scans_over_many_sequences(B, L, D, N):
     """The sums of the sequences are added in 64 bits; within one there are L terms."""
