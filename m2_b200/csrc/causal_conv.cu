@@ -14,6 +14,12 @@ namespace cc {
 constexpr int THREADS = 128;
 constexpr int MAX_TAPS = 8;
 
+// Blocks that an SM holds at least, by the registers of their taps and windows: what the kernels are bounded to, and what a thread's chunk goes by
+__host__ __device__ constexpr int fwd_blocks(int size, int v, int taps) {
+  return taps <= 4 || (size == 4 && v > 1) ? 5 : v == 1 ? (taps <= 7 ? 5 : 4) : taps <= 6 ? 4 : 3;
+}
+__host__ __device__ constexpr int back_blocks(int size, int taps) { return taps <= 4 || size == 4 ? 3 : 2; }
+
 struct Args {
   int batch, len, dim, taps, silu, chunk, chunks;
   const void* x; long long x_sb, x_st;
@@ -194,7 +200,7 @@ template <int V> __device__ __forceinline__ Place place_of(const Args& a) {     
 }
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS, V > 1 && W <= 4 ? 5 : 1)
+__global__ void __launch_bounds__(THREADS, fwd_blocks(sizeof(T), V, W))
 conv_kernel(const Args a) {
   constexpr int P = (V + 1) / 2;
   using X = Vec<T, V>;
@@ -275,7 +281,7 @@ conv_kernel(const Args a) {
 // dx_s = sum_i w_i dv_{s+W-1-i}, dv = dy silu'(v), with v computed again; a chunk's tokens s and the W - 1 behind them are walked through, so that
 // every chunk has all that its own dx need.  A thread's sums of dw and dbias are its chunk's part.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(THREADS, V > 1 && W <= 4 ? 3 : 1)
+__global__ void __launch_bounds__(THREADS, back_blocks(sizeof(T), W))
 back_kernel(const Args a, const Grads g) {
   constexpr int P = (V + 1) / 2;
   using X = Vec<T, V>;
@@ -509,13 +515,14 @@ static int chunk_of(int batch, int len, int dim, int v, int an_sm, int least) {
   return chunk < least ? least : (int)chunk;
 }
 // Of the gradients: their parameters' sums leave W + 1 numbers a channel and chunk, and each chunk walks W - 1 tokens further.  The width of a
-// thread goes by the tensors' alignment, the workspace does not: chunks are those of the widest.
+// thread goes by the tensors' alignment, chunks do not, as the bits of the parameters' sums go by them: they are those of the widest thread of the type (size bytes a value).
 // A thread adds at most 256 tokens one by one: 8192 in one round of threads were off by 1e-4 where all roundings go one way (and slower: 64 x 8192 x 1536 bf16 in chunks of
 // 4096 took 1123 us, in chunks of 256 1079).
-static int back_chunk_of(int batch, int len, int dim) {
-  const int chunk = chunk_of(batch, len, dim, 4, 3, 16), parts = (len + 255) / 256;
-  return chunk <= 256 ? chunk : (len + parts - 1) / parts;
+static int back_chunk_of(int batch, int len, int dim, int taps, int size) {
+  const int chunk = chunk_of(batch, len, dim, 8 / size, back_blocks(size, taps), 16), rounds = (chunk + 255) / 256;
+  return (chunk + rounds - 1) / rounds;
 }
+static int chunks_of(int len, int chunk) { return len > 0 ? (len + chunk - 1) / chunk : 1; }
 
 // channels of a thread: 8 bytes (float32 forward with few taps 16); one where a row does not allow it
 static bool wide(const void* p, long long sb, long long st, int dim, int size, int bytes) {
@@ -571,8 +578,8 @@ static int check(const char* name, const m2_causal_conv_args& g, Args& a) {
 extern "C" long long m2_causal_conv_workspace(int batch, int seq_len, int dim, int taps) {
   using namespace m2::cc;
   if (batch <= 0 || seq_len < 0 || dim <= 0 || taps <= 0 || taps > MAX_TAPS) return 0;
-  const int chunk = back_chunk_of(batch, seq_len, dim), chunks = seq_len > 0 ? (seq_len + chunk - 1) / chunk : 1;
-  return 4LL * batch * chunks * (taps + 1) * dim;
+  const int few = chunks_of(seq_len, back_chunk_of(batch, seq_len, dim, taps, 4)), many = chunks_of(seq_len, back_chunk_of(batch, seq_len, dim, taps, 2));
+  return 4LL * batch * (few > many ? few : many) * (taps + 1) * dim;       // of either type
 }
 
 extern "C" int m2_causal_conv_fwd(const m2_causal_conv_args* args, void* stream) {
@@ -589,8 +596,9 @@ extern "C" int m2_causal_conv_fwd(const m2_causal_conv_args* args, void* stream)
   const int bytes = g.dtype == M2_F32 && g.taps <= 4 ? 16 : 8;
   const bool vec = wide(g.x, g.x_sb, g.x_st, g.dim, size, bytes) && wide(a.state_in, 0, 0, g.dim, size, bytes) && wide(g.y, 0, 0, g.dim, size, bytes) &&
                    wide(a.state_out, 0, 0, g.dim, size, bytes);
-  a.chunk = chunk_of(g.batch, g.seq_len, g.dim, vec ? bytes / size : 1, 5, 8);
-  a.chunks = g.seq_len > 0 ? (g.seq_len + a.chunk - 1) / a.chunk : 1;
+  const int v = vec ? bytes / size : 1;
+  a.chunk = chunk_of(g.batch, g.seq_len, g.dim, v, fwd_blocks(size, v, g.taps), 8);
+  a.chunks = chunks_of(g.seq_len, a.chunk);
   const Grads none = {};
   if (g.dtype == M2_F32) return vec ? by_taps<float, 4, 2, false>(a, none, st) : by_taps<float, 1, 1, false>(a, none, st);
   return vec ? by_taps<__nv_bfloat16, 4, 4, false>(a, none, st) : by_taps<__nv_bfloat16, 1, 1, false>(a, none, st);
@@ -616,8 +624,8 @@ extern "C" int m2_causal_conv_bwd(const m2_causal_conv_args* args, const m2_caus
   const int bytes = 8;
   const bool vec = wide(g.x, g.x_sb, g.x_st, g.dim, size, bytes) && wide(a.state_in, 0, 0, g.dim, size, bytes) && wide(o.d_y, o.y_sb, o.y_st, g.dim, size, bytes) &&
                    wide(o.d_x, 0, 0, g.dim, size, bytes) && wide(r.d_state_out, 0, 0, g.dim, size, bytes) && wide(r.d_state_in, 0, 0, g.dim, size, bytes);
-  a.chunk = back_chunk_of(g.batch, g.seq_len, g.dim);
-  a.chunks = g.seq_len > 0 ? (g.seq_len + a.chunk - 1) / a.chunk : 1;
+  a.chunk = back_chunk_of(g.batch, g.seq_len, g.dim, g.taps, size);
+  a.chunks = chunks_of(g.seq_len, a.chunk);
   const cudaStream_t st = (cudaStream_t)stream;
   if (g.dtype == M2_F32) return vec ? by_taps<float, 2, 2, true>(a, r, st) : by_taps<float, 1, 1, true>(a, r, st);
   return vec ? by_taps<__nv_bfloat16, 4, 4, true>(a, r, st) : by_taps<__nv_bfloat16, 1, 1, true>(a, r, st);
