@@ -56,6 +56,7 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_id=None):
         finished = finished.contiguous()
     if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or pass detached tensors")
+    ops._no_tangents(name, logits, scores)
     if logits.stride(2) != 1 and V > 1:
         logits = logits.contiguous()
     scores = (scores if scores.dtype == torch.float32 else scores.float()).contiguous()
@@ -106,6 +107,7 @@ def reorder_states(states, beam):
     dev = beam.get_device()
     if dev < 0 or [s for s in states if s.get_device() != dev]:
         raise RuntimeError(f"{name}: m2_b200 kernels need CUDA tensors of one device; there is no CPU fallback")
+    ops._no_tangents(name, *states)
     rows, numbers, grad = B * K, [], torch.is_grad_enabled()
     for s in states:
         if s.dim() < 1 or s.shape[0] != rows:

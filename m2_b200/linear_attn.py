@@ -141,6 +141,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
         if lengths.shape != (B,) or lengths.is_floating_point() or lengths.is_complex() or lengths.dtype == torch.bool or lengths.device != q.device:
             raise ValueError(f"{name}: lengths are ({B},) integers on {q.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
         lengths = lengths.to(torch.long).contiguous()
+    ops._no_tangents(name, q, k, v, log_decay, initial_state)
     q, k, v = _packed(q), _packed(k), _packed(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (initial_state is not None and initial_state.requires_grad)):
         o, state = _LinearAttention.apply(q, k, v, _decay(log_decay), scale, initial_state, lengths, return_state)
@@ -162,6 +163,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
         raise ValueError(f"{name}: state is updated in place: its last two dimensions are packed and no two heads overlap, got strides {state.stride()}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or linear_attention with initial_state")
+    ops._no_tangents(name, q, k, v, log_decay, state)
     scale = dk ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -100 <= abs(scale) <= 2.0 ** 100:
         raise ValueError(f"{name}: scale {scale}")

@@ -111,6 +111,7 @@ def token_logprobs(logits, targets, *, top=0, ignore_index=-100):
         raise ValueError(f"{name}: {top} alternatives of {V} logits (0 to {MAX_TOP}, no more than there are)")
     if targets.dtype != torch.long or not targets.is_contiguous():
         targets = targets.to(torch.long).contiguous()
+    ops._no_tangents(name, logits)
     x = _readable(logits)
     if x.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(x, targets, top, int(ignore_index)))

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import M2_BF16, M2_F16, M2_F32
@@ -59,6 +60,14 @@ def _on_device(index, fn, *args):
         return fn(*args)
     with torch.cuda.device(index):
         return fn(*args)
+
+
+def _no_tangents(name, *tensors):
+    """Forward-mode derivatives: a kernel that is given a dual tensor's memory would return a value without its tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: pass forward_ad.unpack_dual(t).primal")
 
 
 def _observed_launch(name, index, fn, args):

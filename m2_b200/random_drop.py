@@ -71,6 +71,7 @@ def dropout(x, p, seed, *, residual=None):
         if not -(1 << 63) <= seed < 1 << 64:
             raise ValueError(f"{name}: seed {seed} has more than 64 bits")
         seed &= (1 << 64) - 1
+    ops._no_tangents(name, x, residual)
     threshold = round(p * 65536)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None

@@ -155,6 +155,7 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, after_weight=Non
     for i in range(3, 8):
         if tensors[i] is not None:
             tensors[i] = _vector(name, _VECTORS[i - 3], tensors[i], n, dev)
+    ops._no_tangents(name, *tensors)
     number = float(residual_scale) if tensors[3] is None else 1.0
     if torch.is_grad_enabled():
         for t in tensors:

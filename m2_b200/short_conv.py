@@ -125,6 +125,7 @@ def causal_conv(x, weight, bias=None, *, activation=None, initial_state=None, le
             raise ValueError(f"{name}: initial_state is {x.dtype} {(B, W - 1, D)} on {x.device}, got {initial_state.dtype} {tuple(initial_state.shape)} on {initial_state.device}")
         initial_state = initial_state.contiguous()
     lengths = _lengths(name, lengths, B, x)
+    ops._no_tangents(name, x, weight, bias, initial_state)
     x = _packed(x)
     silu = activation is not None
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
@@ -148,6 +149,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None):
         raise ValueError(f"{name}: state is updated in place: its last two dimensions are packed and no two sequences overlap, got strides {state.stride()}")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or state.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or causal_conv with initial_state")
+    ops._no_tangents(name, x, state, weight, bias)
     x = _packed(x)
     y = x.new_empty((B, D))
     a = _lib.CausalConvStepArgs(B, D, W, activation is not None, _TYPES[x.dtype], x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias), state.data_ptr(), s_b,

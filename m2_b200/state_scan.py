@@ -151,6 +151,7 @@ def selective_scan(x, delta, a, b, c, *, skip=None, gate=None, delta_bias=None, 
     lengths = _lengths(name, lengths, B, x)
     x, delta, b, c, gate = _packed(x), _packed(delta), _packed(b), _packed(c), _packed(gate) if gate is not None else None
     tensors = (x, delta, a, b, c, skip, gate, delta_bias, initial_state)
+    ops._no_tangents(name, *tensors)
     if _wants_gradient(tensors):
         y, state = _SelectiveScan.apply(*tensors, bool(softplus), lengths, return_state)
     else:
@@ -170,6 +171,7 @@ def selective_scan_step(x, delta, a, b, c, state, *, skip=None, gate=None, delta
         raise ValueError(f"{name}: state is updated in place: its last two dimensions are packed and no two sequences overlap, got strides {state.stride()}")
     if _wants_gradient((x, delta, a, b, c, skip, gate, delta_bias, state)):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or selective_scan with initial_state")
+    ops._no_tangents(name, x, delta, a, b, c, skip, gate, delta_bias, state)
     x, delta, b, c, gate = _packed(x), _packed(delta), _packed(b), _packed(c), _packed(gate) if gate is not None else None
     y = x.new_empty((B, D))
     args = _lib.SelectiveScanStepArgs(
