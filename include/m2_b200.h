@@ -699,7 +699,7 @@ int m2_selective_scan_step(const m2_selective_scan_step_args* args, void* stream
  * there are fewer than `keep`, the rest are beam 0, token end_id (0 without), score -inf.
  *   workspace: m2_beam_select_workspace() bytes on a 16-byte boundary.
  * m2_reorder_states: in each of `count` tensors of batch * beams rows, row (i, k) becomes what row (i, beam[i, k]) was; beam int64 (batch,
- * beams).  A beam outside 0 .. beams-1 is clamped and M2_DEV_BAD_INDEX set.  `states` is host memory; rows of different tensors may not overlap.
+ * beams).  A beam outside 0 .. beams-1 is clamped and M2_DEV_BAD_INDEX set.  `states` is host memory; rows of different tensors, and `beam`, may not overlap.
  * ------------------------------------------------------------------------------------- */
 typedef struct {
   int batch, beams, vocab, keep;

@@ -24,12 +24,12 @@ class BeamStep(NamedTuple):
 
 def beam_select(logits, scores, *, keep=None, finished=None, end_id=None):
     """The `keep` (default K, at most 32) best continuations of each text by scores[b, k] + log softmax(logits[b, k])[token], for logits
-    (B, K, V), float32 or bfloat16 (rows of adjacent logits are read in place, once), and scores (B, K); K <= 32.
+    (B, K, V), float32 or bfloat16 (rows of adjacent logits are read in place, once), and scores (B, K), taken as float32; K <= 32.
 
     end_id    None, or the id that ends a text: `finished` of the result says which beams have ended with this token or before
     finished  None or (B, K) bool: an ended beam has one continuation, end_id at its own score; its logits are not read
 
-    A beam's tokens go by their logits, equal ones by ascending id; beams go by scores in 64 bits, equal ones by ascending beam.  A
+    A beam's tokens go by their logits, equal ones by ascending id; beams go by the sums in 64 bits, equal ones by ascending beam.  A
     score of -inf is no candidate (a text's first step: scores 0, -inf, -inf ... where all its beams are alike); where there are fewer
     than `keep`, the rest are beam 0, token end_id (0 without it), score -inf.  NaN goes before all.  It has no gradient."""
     name = "beam_select"
@@ -96,7 +96,7 @@ def _apart(states, rows):
 def reorder_states(states, beam):
     """In each tensor of `states`, (B * K, ...), row b K + k becomes what row b K + beam[b, k] was, in place and in one launch for all that are
     laid out alike; beam (B, K) int64 as beam_select gives it, K <= 32.  Every row is packed; rows of one tensor lie a fixed distance
-    apart.  An entry of beam outside 0 .. K-1 is clamped and sets M2_DEV_BAD_INDEX (ops.device_status())."""
+    apart, and share no memory with beam.  An entry of beam outside 0 .. K-1 is clamped and sets M2_DEV_BAD_INDEX (ops.device_status())."""
     name = "reorder_states"
     states = [states] if isinstance(states, torch.Tensor) else list(states)
     if beam.dim() != 2 or beam.dtype != torch.long:
@@ -124,11 +124,11 @@ def reorder_states(states, beam):
         if not s[0].is_contiguous() or (rows > 1 and step < n):
             raise ValueError(f"{name}: a state is changed in place: its rows are packed and do not overlap, got {tuple(s.shape)} with strides {s.stride()}")
         numbers.append((s.data_ptr(), n, step if rows > 1 else n))
-    if not _apart(numbers, rows):
-        raise ValueError(f"{name}: two states share memory")
+    beam = beam.contiguous()
+    if not _apart(numbers + [(beam.data_ptr(), 8, 8)] if rows else [], rows):        # beam is read while states are written
+        raise ValueError(f"{name}: two states, or a state and beam, share memory")
     if not numbers:
         return
-    beam = beam.contiguous()
     table = (_lib.BeamState * len(numbers))(*numbers)
     a = _lib.ReorderStatesArgs(B, K, len(numbers), beam.data_ptr(), table)
     ops._launch("m2_reorder_states", beam, _lib.lib().m2_reorder_states, C.byref(a), launches=None)
