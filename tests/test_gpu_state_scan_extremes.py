@@ -190,3 +190,47 @@ def test_factors_beyond_float32_between_states_within_it(L, N, rate, start):
     one = 64 * 2.0 ** -22 + 128 * (2 + 64) * U32 + 64 * U32
     within(s, t["initial_state"].double() * torch.exp(total), one * (t["initial_state"].double() * torch.exp(total)).abs(), "state")
     within(g, d_s.double() * torch.exp(total), one * (d_s.double() * torch.exp(total)).abs(), "gradient")
+
+
+def test_more_blocks_than_places_for_what_they_put_aside():
+    """With more than 16 states blocks beyond 4096 take one sequence after another: each sequence's gradients are those of a smaller batch."""
+    B, L, D, N, G = 1100, 40, 16, 20, 4                        # 4400 blocks; 2200 in each half
+    t = make(B, L, D, N, G, torch.float32)
+    lengths = torch.randint(0, L + 1, (B,), device="cuda")
+    up, d_s = torch.randn(B, L, D, device="cuda"), torch.randn(B, D, N, device="cuda")
+
+    def run(part):
+        leaves = {k: (v if k in ("a", "skip", "delta_bias") else v[part]).clone().requires_grad_() for k, v in t.items()}
+        y, s = m2_b200.selective_scan(**leaves, softplus=True, lengths=lengths[part], return_state=True)
+        return dict(zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [up[part], d_s[part]])))
+
+    whole, halves = run(slice(None)), [run(slice(0, B // 2)), run(slice(B // 2, B))]
+    M = definition(t, True, lengths, up, d_s, size=True)
+    for k, v in whole.items():
+        if k in ("a", "skip", "delta_bias"):
+            within(v, sum(h[k].double() for h in halves), 32 * U32 * M[k], k)      # the same parts, in eights of other neighbours
+        else:
+            assert torch.equal(v, torch.cat([h[k] for h in halves])), k
+
+
+@pytest.mark.parametrize("B,L,D,N,G", [(2, 512, 64, 16, 1), (1, 2048, 64, 16, 1), (2, 512, 64, 20, 1), (2, 512, 64, 40, 2)])
+def test_roundings_in_training_add_up_as_independent_ones_do(B, L, D, N, G):
+    """Steps of 0.001 to 0.1 and a of -1 to -N, as models begin with.  A value is a nest of sums of 32 tokens of a tile, at three roundings each, of the tiles that a state
+    lives through, of N states or D channels and of a handful around them: k below 3 32 + 2 N + D + 16 roundings and exps in a row that matter, each 2^-24 in size (the exps'
+    2^-22 at most, and 2^-24 in the mean).  Independent ones add up to k^(1/2) 2^-24 of the sum of sizes, in the 2-norm; a bias, or a difference of large terms, does not."""
+    g = torch.Generator(device="cuda").manual_seed(L + N)
+
+    def rnd(*s, std=1.0, mean=0.0):
+        return torch.randn(s, device="cuda", generator=g) * std + mean
+
+    steps = torch.exp(torch.rand(D, device="cuda", generator=g) * 4.6 - 6.9)
+    t = dict(x=rnd(B, L, D), delta=rnd(B, L, D, std=0.5), a=-torch.arange(1, N + 1, device="cuda") * torch.exp(rnd(D, N, std=0.05)), b=rnd(B, L, G, N), c=rnd(B, L, G, N),
+             skip=rnd(D, mean=1.0, std=0.1), delta_bias=steps + torch.log(-torch.expm1(-steps)), gate=rnd(B, L, D), initial_state=rnd(B, D, N, std=0.5))
+    leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+    y, s = m2_b200.selective_scan(**leaves, softplus=True, return_state=True)
+    up, d_s = torch.randn(B, L, D, device="cuda", generator=g), torch.randn(B, D, N, device="cuda", generator=g)
+    got = dict(zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [up, d_s])), y=y.detach(), state=s.detach())
+    ref, M = (definition(t, True, None, up, d_s, size) for size in (False, True))
+    most = (3 * 32 + 2 * N + D + 16) ** 0.5 * U32
+    found = {k: ((v.double() - ref[k]).norm() / (most * M[k].norm())).item() for k, v in got.items()}
+    assert max(found.values()) <= 1, found
