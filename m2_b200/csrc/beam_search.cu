@@ -10,7 +10,7 @@
 // States: a thread owns a few bytes of the rows of all beams of one text; it reads the rows that its beams come from before it writes any,
 // so that nothing waits and no second buffer is needed.  Rows that stay are neither read nor written.
 // Measured: selection for one text of four beams 17 us, for 32 of eight beams (float32, 31 MB) 27; states of 12 layers of the latter (256 rows of 58 KB a layer,
-// of which two in three move) 40 us.
+// some 227 of which are replaced, by 75 different ones: 212 MB) 40 us, 5.3 TB/s.
 #include "common.cuh"
 
 namespace m2 {

@@ -5,13 +5,13 @@
 // (bert/src/mm/monarch_mixer_sequence_mixer.py:100-154).
 //
 // Bound: one exp for each token, channel and state (the special functions give 16 a cycle and SM), three with the gradients; then the instructions around
-// it: 20 packed FMAs, 8 exps, 4 loads from shared memory for 16 channels and 16 states a token, 70 to 80 in all, 240 back.  No tensor cores: every channel has
+// it: 20 packed FMAs, 8 exps, 4 loads from shared memory for 16 channels and 16 states a token, 80 in all, 235 back.  No tensor cores: every channel has
 // decays of its own, so that no product shares an operand.  A block has 64 channels and takes 32 tokens at a time: elementwise part (steps, gates) by
 // pieces of 16 bytes, then the recurrence with two channels and four states a thread, in registers; y is summed over four lanes.
-// Measured (bf16, 16 states): 16 x 2048 x 1536 forward 432 us (exps alone 179), gradients 1360 (358); 1 x 32768 x 768 forward 332 us in three launches (179, as the
-// sums of the segments need the exps too).  With all SMs full the forward kernel issued in 56 % of the cycles, exps 58 %, FMAs 43 %, shared memory 53 % (before the
-// next tile's pieces were copied ahead); back 57, 40, 51 and 67.  An exp in four as a polynomial on the FMA pipe: 526 us where the exps alone took 481; operands doubled
-// in shared memory for packed FMAs: 479 and 1457 where 465 and 1370 were; reductions of y and q through shared memory instead of shuffles: 1749 back; the next
+// Measured (bf16, 16 states): 16 x 2048 x 1536 forward 432 us (exps alone 179), gradients 1460 (447, as half of the exps come twice); 1 x 32768 x 768 forward 336 us in three
+// launches (179, as the sums of the segments need the exps too).  Where SMs are full the forward kernel issues in 62 % of the cycles, exps 65 %, shared memory 52 %; back 56, 47
+// and 63, in wait for the results of instructions before.  An exp in four as a polynomial on the FMA pipe: 526 us where the exps alone took 481; operands doubled
+// in shared memory for packed FMAs: 479 where 465 were; reductions of y and q through shared memory instead of shuffles: 1749 back; the next
 // tile's pieces held in registers: 512 where 465 were.
 #include "common.cuh"
 
@@ -27,7 +27,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 // states a lane were tried and spilled hundreds of bytes.
 __host__ __device__ constexpr int channels_of(int ql) { return 256 / ql; }                          // of a block
 
-// Blocks of the gradients' kernel that an SM holds: 168 registers and 74 KB of shared memory up to 16 states, 255 and 92 to 96 beyond
+// Blocks of the gradients' kernel that an SM holds: 168 registers and 74 KB of shared memory up to 16 states, 255 and 90 to 93 beyond; none spills
 __host__ __device__ constexpr int back_blocks(int np) { return np == 16 ? 3 : 2; }
 // Tokens whose states are at hand at one time: four, or two where a lane has twice the states
 __host__ __device__ constexpr int few(int np) { return np == 16 ? 4 : 2; }
@@ -767,7 +767,7 @@ template <int S, int QL> struct BackShared {
   float b[TT][NP], c[TT][NP];
   float part[4][TT][NP];                 // db or dc of each warp's channels
   float mid[4][U * STEP];                // four steps of each pair of channels
-  float aside[S > 4 ? 1 : 2][2][THREADS][4];          // up to 16 states: each thread's in front of the tile's tokens 8 and 24; then 0 in the place of 24
+  float aside[2][2][S > 4 ? 1 : THREADS][4];          // up to 16 states: each thread's in front of the tile's tokens 8 and 24; then 0 in the place of 24
   float behind[S][THREADS][2];           // the gradient of the state behind the tile
 };
 
@@ -1059,14 +1059,16 @@ back_kernel(const Args a, const Grads g, const unsigned work) {
                 if (v < FEW - 1) h[c][i] = f2_fma(x[c], B[i], f[v][c][i]);
               }
           }
-          if (S == 4 && t0 == 24) {                                      // its states have been used
+          if constexpr (S == 4) {
+            if (t0 == 24) {                                              // its states have been used
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (cl + c < p.valid) copy_async<16>(sh.aside[1][c][tid], saved + c * NP);
-              else *reinterpret_cast<float4*>(sh.aside[1][c][tid]) = make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int c = 0; c < 2; ++c) {
+                if (cl + c < p.valid) copy_async<16>(sh.aside[1][c][tid], saved + c * NP);
+                else *reinterpret_cast<float4*>(sh.aside[1][c][tid]) = make_float4(0.f, 0.f, 0.f, 0.f);
+              }
             }
+            if (t0 == 8) asm volatile("cp.async.wait_all;" ::: "memory");
           }
-          if (S == 4 && t0 == 8) asm volatile("cp.async.wait_all;" ::: "memory");
           if (t0 + u0 > 0) take_aside(t0 + u0 - (second ? FEW : PART));  // under way meanwhile
 #pragma unroll
           for (int v = FEW - 1; v >= 0; --v) {
