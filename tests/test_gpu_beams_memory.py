@@ -7,6 +7,13 @@ import m2_b200
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    with torch.random.fork_rng():                              # other files' random numbers are those they would have alone
+        torch.manual_seed(0)
+        yield
+
+
 def test_a_state_that_holds_beam_is_refused():
     beam = torch.tensor([[1, 0], [0, 0]], device="cuda")
     state = torch.randn(4, 6, device="cuda")

@@ -8,6 +8,13 @@ import m2_b200
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    with torch.random.fork_rng():                              # other files' random numbers are those they would have alone
+        torch.manual_seed(0)
+        yield
+
+
 def calls():
     x, w = torch.randn(2, 5, 8, device="cuda"), torch.randn(8, 4, device="cuda")
     a, b = -torch.rand(8, 4, device="cuda"), torch.randn(2, 5, 4, device="cuda")

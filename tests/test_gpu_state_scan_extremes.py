@@ -18,7 +18,9 @@ LOWEST, NONE = torch.finfo(torch.float32).min, -float("inf")
 
 @pytest.fixture(autouse=True)
 def seeded():
-    torch.manual_seed(0)
+    with torch.random.fork_rng():                              # other files' random numbers are those they would have alone
+        torch.manual_seed(0)
+        yield
 
 
 def strong(N):

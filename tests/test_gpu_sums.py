@@ -8,6 +8,13 @@ pytestmark = pytest.mark.gpu
 U32 = 2.0 ** -24
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    with torch.random.fork_rng():                              # other files' random numbers are those they would have alone
+        torch.manual_seed(0)
+        yield
+
+
 def score_errors(logits, keep=2):
     B, K, V = logits.shape
     got = m2_b200.beam_select(logits, torch.zeros(B, K, device="cuda"), keep=keep)
