@@ -817,404 +817,404 @@ back_kernel(const Args a, const Grads g, const unsigned work) {
   float* const far_aside = g.aside + (long long)blockIdx.x * (ASIDE * 2 * S * THREADS) + 4 * threadIdx.x;
   pdl_wait();
   for (unsigned item = blockIdx.x; item < work; item += gridDim.x) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Place p = place_of<CT>(a, item);
-  const int n = text_length(a, p.b);
-  if (tid < CT) {
-    sh.bias[0][tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
-    sh.bias[1][tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
-  }
-  const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
-  const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
-  constexpr int H = S / 2;
-  f32x2 G[2][H], A[2][H];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      float v[2], w[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int s = q0 + 2 * i + j;
-        const bool real = cl + c < p.valid && s < a.states;
-        const long long ch = p.ch0 + cl + c;
-        v[j] = real ? rate(a.a[ch * a.states + s]) : 0.f;
-        w[j] = 0.f;
-        if (real && a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
-        else if (real && g.d_state_out) w[j] = g.d_state_out[((long long)p.b * a.dim + ch) * a.states + s];
-      }
-      A[c][i] = f2_pack(v[0], v[1]);
-      G[c][i] = f2_pack(w[0], w[1]);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Place p = place_of<CT>(a, item);
+    const int n = text_length(a, p.b);
+    if (tid < CT) {
+      sh.bias[0][tid] = a.bias && tid < p.valid ? a.bias[p.ch0 + tid] : 0.f;
+      sh.bias[1][tid] = a.skip && tid < p.valid ? a.skip[p.ch0 + tid] : 0.f;
     }
-  }
-  const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
-  const int used = min(last, (n + TT - 1) / TT);
-  const int col = tid % Px::PPR * E, row = tid / Px::PPR;
-  const long long out0 = (long long)p.b * a.len * a.dim + p.ch0 + col;
-  T *dx = static_cast<T*>(g.dx) + out0, *dd = static_cast<T*>(g.d_delta) + out0, *dz = static_cast<T*>(g.dz) + out0;
-  float sum = 0.f;                       // threads below CT: the gradient of a channel's skip, the next CT: of its delta_bias
-  for (int t = max(used, first) * TT + row; t < min(last * TT, a.len); t += Px::ROWS) {       // behind the text
-    const float f[E] = {};
-    store_piece<T>(dx + (long long)t * a.dim, f, p.valid - col, g.vec);
-    store_piece<T>(dd + (long long)t * a.dim, f, p.valid - col, g.vec);
-    if (g.dz) store_piece<T>(dz + (long long)t * a.dim, f, p.valid - col, g.vec);
-  }
-  Px x, delta, z, dy;
-  Coeffs<T, NP> fb, fc;
-  __syncthreads();
-  for (int k = used - 1; k >= first; --k) {
-    fb.fetch(a.b, p, k * TT, n, a.states);
-    fc.fetch(a.c, p, k * TT, n, a.states);
-    const float* saved = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
-    auto in_front = [&](f32x2 (&h)[2][H]) {
+    const int cl = warp * (CT / 4) + lane / QL * 2, q0 = lane % QL * S;
+    const long long row_n = ((long long)p.b * a.segs + p.seg) * a.dim + p.ch0;
+    constexpr int H = S / 2;
+    f32x2 G[2][H], A[2][H];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        float v[2], w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int s = q0 + 2 * i + j;
+          const bool real = cl + c < p.valid && s < a.states;
+          const long long ch = p.ch0 + cl + c;
+          v[j] = real ? rate(a.a[ch * a.states + s]) : 0.f;
+          w[j] = 0.f;
+          if (real && a.segs > 1) w[j] = a.seg_state[(row_n + cl + c) * NP + s];
+          else if (real && g.d_state_out) w[j] = g.d_state_out[((long long)p.b * a.dim + ch) * a.states + s];
+        }
+        A[c][i] = f2_pack(v[0], v[1]);
+        G[c][i] = f2_pack(w[0], w[1]);
+      }
+    }
+    const int total = (a.len + TT - 1) / TT, first = p.seg * a.seg_tiles, last = min(first + a.seg_tiles, total);
+    const int used = min(last, (n + TT - 1) / TT);
+    const int col = tid % Px::PPR * E, row = tid / Px::PPR;
+    const long long out0 = (long long)p.b * a.len * a.dim + p.ch0 + col;
+    T *dx = static_cast<T*>(g.dx) + out0, *dd = static_cast<T*>(g.d_delta) + out0, *dz = static_cast<T*>(g.dz) + out0;
+    float sum = 0.f;                       // threads below CT: the gradient of a channel's skip, the next CT: of its delta_bias
+    for (int t = max(used, first) * TT + row; t < min(last * TT, a.len); t += Px::ROWS) {       // behind the text
+      const float f[E] = {};
+      store_piece<T>(dx + (long long)t * a.dim, f, p.valid - col, g.vec);
+      store_piece<T>(dd + (long long)t * a.dim, f, p.valid - col, g.vec);
+      if (g.dz) store_piece<T>(dz + (long long)t * a.dim, f, p.valid - col, g.vec);
+    }
+    Px x, delta, z, dy;
+    Coeffs<T, NP> fb, fc;
+    __syncthreads();
+    for (int k = used - 1; k >= first; --k) {
+      fb.fetch(a.b, p, k * TT, n, a.states);
+      fc.fetch(a.c, p, k * TT, n, a.states);
+      const float* saved = a.saves + (((long long)p.b * total + k) * a.dim + p.ch0 + cl) * NP + q0;
+      auto in_front = [&](f32x2 (&h)[2][H]) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < H; i += 2) {
+            const ulonglong2 u = cl + c < p.valid ? __ldg(reinterpret_cast<const ulonglong2*>(saved + c * NP + 2 * i)) : make_ulonglong2(0, 0);
+            h[c][i] = u.x; h[c][i + 1] = u.y;
+          }
+      };
+      f32x2 h[2][H];
+      in_front(h);
+#pragma unroll 1
+      for (int part = 0; part < TT; part += Px::SPAN) {
+        x.fetch(a.x, p, k * TT + part, n);
+        delta.fetch(a.delta, p, k * TT + part, n);
+        dy.fetch(g.dy, p, k * TT + part, n);
+        if (a.z.p) z.fetch(a.z, p, k * TT + part, n);
+        float bias[E];
+        from_shared(sh.bias[0] + col, bias);
+#pragma unroll
+        for (int i = 0; i < Px::P; ++i) {
+          const int t = part + row + i * Px::ROWS;
+          const bool in = k * TT + t < n;
+          float f[E], d[E], e[E];
+          Piece<T>::get(x.v[i], f);
+          Piece<T>::get(delta.v[i], d);
+          Piece<T>::get(dy.v[i], e);
+          if (a.z.p) {
+            float u[E];
+            Piece<T>::get(z.v[i], u);
+#pragma unroll
+            for (int j = 0; j < E; ++j) e[j] *= u[j] * sigmoid(u[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            d[j] = in ? step_of(d[j] + bias[j], a.softplus) : 0.f;
+            f[j] *= d[j];
+          }
+          to_shared(&sh.dt[t][col], d);
+          to_shared(&sh.dx[t][col], f);
+          to_shared(&sh.e[t][col], e);
+        }
+      }
+      fb.put(&sh.b[0][0]);
+      fc.put(&sh.c[0][0]);
+      __syncthreads();
+      const int own_row = (lane >> 1) & 1, own_ch = cl + (lane & 1);
+      if (k > first) {
+        Px::ask(a.x, p, (k - 1) * TT, n);
+        Px::ask(a.delta, p, (k - 1) * TT, n);
+        Px::ask(g.dy, p, (k - 1) * TT, n);
+        if (a.z.p) Px::ask(a.z, p, (k - 1) * TT, n);
+      }
+      constexpr int U = BackShared<S, QL>::U, FEW = BackShared<S, QL>::FEW, STEP = BackShared<S, QL>::STEP;
+      float* mid = sh.mid[warp];
+      // h in front of token t, a multiple of PART: a thread's own loads and stores, 16 bytes each
+      constexpr int PART = 2 * FEW;
+      auto place = [&](int t, int c) {
+        if constexpr (S > 4) return far_aside + (t / PART - 1) * (2 * S * THREADS) + c * (S * THREADS);
+        // token 16's lies in the first half of q, in the warp's own columns: by the time that half gets its own numbers it has been used
+        else return t == 16 ? &sh.q[c * 8 + lane / 4][warp * (CT / 4) + lane % 4 * 4] : sh.aside[t != 8][c][tid];
+      };
+      auto put_aside = [&](int t) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float* to = place(t, c);
+#pragma unroll
+          for (int i = 0; i < H; i += 2) *reinterpret_cast<ulonglong2*>(to + i / 2 * (4 * THREADS)) = make_ulonglong2(h[c][i], h[c][i + 1]);
+        }
+      };
+      auto take_aside = [&](int t) {
+        if (S > 4 && t == 0) { in_front(h); return; }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float* from = place(t, c);
+#pragma unroll
+          for (int i = 0; i < H; i += 2) {
+            const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(from + i / 2 * (4 * THREADS));
+            h[c][i] = u.x; h[c][i + 1] = u.y;
+          }
+        }
+      };
+      {
+        Token<H, true, true> next;
+        const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][q0], *p_c = &sh.c[0][q0];
+        float* p_y = &sh.y[own_row][own_ch];
+        f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[2][H];
+        next.get(p_dx, p_e, p_b, p_c);
+        decays<H>(dt, A, d_next);
+#pragma unroll 1
+        for (int t0 = 0; t0 < TT; t0 += U) {
+          float y[U][2];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (u == 0 && t0 > 0 && t0 % PART == 0) put_aside(t0);
+            const Token<H, true, true> now = next;
+            f32x2 d[2][H], hs[H], x[2], e[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
+            next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * NP, p_c + (u + 1) * NP);
+            dt = dt_next;
+            dt_next = ld2(p_dt + (u + 2) * CT);
+            decays<H>(dt, A, d_next);
+            splat2(now.x, x);
+            splat2(now.e, e);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              f32x2 yy;
+#pragma unroll
+              for (int i = 0; i < H; ++i) {
+                h[c][i] = f2_fma(d[c][i], h[c][i], f2_mul(x[c], now.B[i]));
+                hs[i] = c ? f2_fma(h[c][i], e[c], hs[i]) : f2_mul(h[c][i], e[c]);
+                yy = i ? f2_fma(h[c][i], now.C[i], yy) : f2_mul(h[c][i], now.C[i]);
+              }
+              y[u][c] = both(yy);
+            }
+            put_channels<S, QL>(mid + u * STEP, hs, lane);
+          }
+#pragma unroll
+          for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(y[u][0], y[u][1], y[u + 1][0], y[u + 1][1], lane);
+          sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
+          p_y += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * NP; p_c += U * NP;
+        }
+      }
+      take_aside(TT - PART);
+      __syncthreads();
+      auto parts_to = [&](float* out) {
+        const long long row = (long long)a.groups * NP;
+        out += (((long long)p.tile * a.batch + p.b) * a.len + k * TT) * row + p.g * NP + tid % NP;
+#pragma unroll
+        for (int j = 0; j < TT * NP / THREADS; ++j) {
+          const int i = tid + j * THREADS;
+          if (k * TT + i / NP < n)
+            out[i / NP * row] = ((&sh.part[0][0][0])[i] + (&sh.part[1][0][0])[i]) + ((&sh.part[2][0][0])[i] + (&sh.part[3][0][0])[i]);
+        }
+      };
+      parts_to(g.part_c);
+      f32x2 own[2][H], dA[2][H], cum = 0;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; i += 2) {
-          const ulonglong2 u = cl + c < p.valid ? __ldg(reinterpret_cast<const ulonglong2*>(saved + c * NP + 2 * i)) : make_ulonglong2(0, 0);
-          h[c][i] = u.x; h[c][i + 1] = u.y;
+        for (int i = 0; i < H; ++i) {
+          *reinterpret_cast<f32x2*>(sh.behind[c * H + i][tid]) = G[c][i];
+          own[c][i] = dA[c][i] = 0;
         }
-    };
-    f32x2 h[2][H];
-    in_front(h);
+      __syncthreads();
+      {
+        constexpr int LAST = (TT - U) * CT, LAST_N = (TT - U) * NP;
+        const float *p_dt = &sh.dt[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][q0] + LAST_N, *p_c = &sh.c[0][q0] + LAST_N;
+        const float* p_dx = &sh.dx[0][cl] + LAST;
+        float* to = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
+        constexpr int HALVES = PART > U ? 2 : 1;
 #pragma unroll 1
-    for (int part = 0; part < TT; part += Px::SPAN) {
-      x.fetch(a.x, p, k * TT + part, n);
-      delta.fetch(a.delta, p, k * TT + part, n);
-      dy.fetch(g.dy, p, k * TT + part, n);
-      if (a.z.p) z.fetch(a.z, p, k * TT + part, n);
-      float bias[E];
-      from_shared(sh.bias[0] + col, bias);
+        for (int t1 = TT - U; t1 >= 0; t1 -= HALVES * U)
 #pragma unroll
-      for (int i = 0; i < Px::P; ++i) {
-        const int t = part + row + i * Px::ROWS;
-        const bool in = k * TT + t < n;
-        float f[E], d[E], e[E];
-        Piece<T>::get(x.v[i], f);
-        Piece<T>::get(delta.v[i], d);
-        Piece<T>::get(dy.v[i], e);
-        if (a.z.p) {
-          float u[E];
-          Piece<T>::get(z.v[i], u);
+        for (int half = 0; half < HALVES; ++half) {
+          const int t0 = t1 - half * U;
 #pragma unroll
-          for (int j = 0; j < E; ++j) e[j] *= u[j] * sigmoid(u[j]);
-        }
+          for (int u0 = U - FEW; u0 >= 0; u0 -= FEW) {
+            f32x2 d[FEW][2][H], f[FEW][2][H];
+            float gb[2][2], q[2][2];
+            const bool second = PART > U ? half == 0 : u0 > 0;        // half of the part
+            if (second) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          d[j] = in ? step_of(d[j] + bias[j], a.softplus) : 0.f;
-          f[j] *= d[j];
-        }
-        to_shared(&sh.dt[t][col], d);
-        to_shared(&sh.dx[t][col], f);
-        to_shared(&sh.e[t][col], e);
-      }
-    }
-    fb.put(&sh.b[0][0]);
-    fc.put(&sh.c[0][0]);
-    __syncthreads();
-    const int own_row = (lane >> 1) & 1, own_ch = cl + (lane & 1);
-    if (k > first) {
-      Px::ask(a.x, p, (k - 1) * TT, n);
-      Px::ask(a.delta, p, (k - 1) * TT, n);
-      Px::ask(g.dy, p, (k - 1) * TT, n);
-      if (a.z.p) Px::ask(a.z, p, (k - 1) * TT, n);
-    }
-    constexpr int U = BackShared<S, QL>::U, FEW = BackShared<S, QL>::FEW, STEP = BackShared<S, QL>::STEP;
-    float* mid = sh.mid[warp];
-    // h in front of token t, a multiple of PART: a thread's own loads and stores, 16 bytes each
-    constexpr int PART = 2 * FEW;
-    auto place = [&](int t, int c) {
-      if constexpr (S > 4) return far_aside + (t / PART - 1) * (2 * S * THREADS) + c * (S * THREADS);
-      // token 16's lies in the first half of q, in the warp's own columns: by the time that half gets its own numbers it has been used
-      else return t == 16 ? &sh.q[c * 8 + lane / 4][warp * (CT / 4) + lane % 4 * 4] : sh.aside[t != 8][c][tid];
-    };
-    auto put_aside = [&](int t) {
+              for (int v = 0; v < FEW; ++v) {
+                const int u = u0 - FEW + v;
+                f32x2 x[2], B[H];
+                decays<H>(ld2(p_dt + u * CT), A, d[0]);
+                splat2(ld2(p_dx + u * CT), x);
+                ld_pairs<H>(p_b + u * NP, B);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float* to = place(t, c);
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < H; i += 2) *reinterpret_cast<ulonglong2*>(to + i / 2 * (4 * THREADS)) = make_ulonglong2(h[c][i], h[c][i + 1]);
-      }
-    };
-    auto take_aside = [&](int t) {
-      if (S > 4 && t == 0) { in_front(h); return; }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float* from = place(t, c);
-#pragma unroll
-        for (int i = 0; i < H; i += 2) {
-          const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(from + i / 2 * (4 * THREADS));
-          h[c][i] = u.x; h[c][i + 1] = u.y;
-        }
-      }
-    };
-    {
-      Token<H, true, true> next;
-      const float *p_dt = &sh.dt[0][cl], *p_dx = &sh.dx[0][cl], *p_e = &sh.e[0][cl], *p_b = &sh.b[0][q0], *p_c = &sh.c[0][q0];
-      float* p_y = &sh.y[own_row][own_ch];
-      f32x2 dt = ld2(p_dt), dt_next = ld2(p_dt + CT), d_next[2][H];
-      next.get(p_dx, p_e, p_b, p_c);
-      decays<H>(dt, A, d_next);
-#pragma unroll 1
-      for (int t0 = 0; t0 < TT; t0 += U) {
-        float y[U][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (u == 0 && t0 > 0 && t0 % PART == 0) put_aside(t0);
-          const Token<H, true, true> now = next;
-          f32x2 d[2][H], hs[H], x[2], e[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < H; ++i) d[c][i] = d_next[c][i];
-          next.get(p_dx + (u + 1) * CT, p_e + (u + 1) * CT, p_b + (u + 1) * NP, p_c + (u + 1) * NP);
-          dt = dt_next;
-          dt_next = ld2(p_dt + (u + 2) * CT);
-          decays<H>(dt, A, d_next);
-          splat2(now.x, x);
-          splat2(now.e, e);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            f32x2 yy;
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-              h[c][i] = f2_fma(d[c][i], h[c][i], f2_mul(x[c], now.B[i]));
-              hs[i] = c ? f2_fma(h[c][i], e[c], hs[i]) : f2_mul(h[c][i], e[c]);
-              yy = i ? f2_fma(h[c][i], now.C[i], yy) : f2_mul(h[c][i], now.C[i]);
+                  for (int i = 0; i < H; ++i) h[c][i] = f2_fma(d[0][c][i], h[c][i], f2_mul(x[c], B[i]));
+              }
             }
-            y[u][c] = both(yy);
-          }
-          put_channels<S, QL>(mid + u * STEP, hs, lane);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u += 2) p_y[u * CT] = sum_states<QL>(y[u][0], y[u][1], y[u + 1][0], y[u + 1][1], lane);
-        sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        p_y += U * CT; p_dt += U * CT; p_dx += U * CT; p_e += U * CT; p_b += U * NP; p_c += U * NP;
-      }
-    }
-    take_aside(TT - PART);
-    __syncthreads();
-    auto parts_to = [&](float* out) {
-      const long long row = (long long)a.groups * NP;
-      out += (((long long)p.tile * a.batch + p.b) * a.len + k * TT) * row + p.g * NP + tid % NP;
-#pragma unroll
-      for (int j = 0; j < TT * NP / THREADS; ++j) {
-        const int i = tid + j * THREADS;
-        if (k * TT + i / NP < n)
-          out[i / NP * row] = ((&sh.part[0][0][0])[i] + (&sh.part[1][0][0])[i]) + ((&sh.part[2][0][0])[i] + (&sh.part[3][0][0])[i]);
-      }
-    };
-    parts_to(g.part_c);
-    f32x2 own[2][H], dA[2][H], cum = 0;
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        *reinterpret_cast<f32x2*>(sh.behind[c * H + i][tid]) = G[c][i];
-        own[c][i] = dA[c][i] = 0;
-      }
-    __syncthreads();
-    {
-      constexpr int LAST = (TT - U) * CT, LAST_N = (TT - U) * NP;
-      const float *p_dt = &sh.dt[0][cl] + LAST, *p_e = &sh.e[0][cl] + LAST, *p_b = &sh.b[0][q0] + LAST_N, *p_c = &sh.c[0][q0] + LAST_N;
-      const float* p_dx = &sh.dx[0][cl] + LAST;
-      float* to = (own_row ? &sh.q[0][own_ch] : &sh.dx[0][own_ch]) + LAST;
-      constexpr int HALVES = PART > U ? 2 : 1;
-#pragma unroll 1
-      for (int t1 = TT - U; t1 >= 0; t1 -= HALVES * U)
-#pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        const int t0 = t1 - half * U;
-#pragma unroll
-        for (int u0 = U - FEW; u0 >= 0; u0 -= FEW) {
-          f32x2 d[FEW][2][H], f[FEW][2][H];
-          float gb[2][2], q[2][2];
-          const bool second = PART > U ? half == 0 : u0 > 0;        // half of the part
-          if (second) {
 #pragma unroll
             for (int v = 0; v < FEW; ++v) {
-              const int u = u0 - FEW + v;
+              const int u = u0 + v;
               f32x2 x[2], B[H];
-              decays<H>(ld2(p_dt + u * CT), A, d[0]);
+              decays<H>(ld2(p_dt + u * CT), A, d[v]);
               splat2(ld2(p_dx + u * CT), x);
               ld_pairs<H>(p_b + u * NP, B);
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < H; ++i) h[c][i] = f2_fma(d[0][c][i], h[c][i], f2_mul(x[c], B[i]));
+                for (int i = 0; i < H; ++i) {
+                  f[v][c][i] = f2_mul(d[v][c][i], h[c][i]);
+                  if (v < FEW - 1) h[c][i] = f2_fma(x[c], B[i], f[v][c][i]);
+                }
             }
-          }
+            if constexpr (S == 4) {
+              if (t0 == 24) {                                              // its states have been used
 #pragma unroll
-          for (int v = 0; v < FEW; ++v) {
-            const int u = u0 + v;
-            f32x2 x[2], B[H];
-            decays<H>(ld2(p_dt + u * CT), A, d[v]);
-            splat2(ld2(p_dx + u * CT), x);
-            ld_pairs<H>(p_b + u * NP, B);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < H; ++i) {
-                f[v][c][i] = f2_mul(d[v][c][i], h[c][i]);
-                if (v < FEW - 1) h[c][i] = f2_fma(x[c], B[i], f[v][c][i]);
+                for (int c = 0; c < 2; ++c) {
+                  if (cl + c < p.valid) copy_async<16>(sh.aside[1][c][tid], saved + c * NP);
+                  else *reinterpret_cast<float4*>(sh.aside[1][c][tid]) = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
               }
-          }
-          if constexpr (S == 4) {
-            if (t0 == 24) {                                              // its states have been used
+              if (t0 == 8) asm volatile("cp.async.wait_all;" ::: "memory");
+            }
+            if (t0 + u0 > 0) take_aside(t0 + u0 - (second ? FEW : PART));  // under way meanwhile
+#pragma unroll
+            for (int v = FEW - 1; v >= 0; --v) {
+              const int u = u0 + v;
+              Token<H, true, true> now;
+              now.get(p_dx + u * CT, p_e + u * CT, p_b + u * NP, p_c + u * NP);
+              f32x2 gs[H], x[2], e[2], dt[2];
+              const f32x2 steps = ld2(p_dt + u * CT);
+              cum = f2_add(cum, steps);
+              splat2(steps, dt);
+              splat2(now.x, x);
+              splat2(now.e, e);
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                if (cl + c < p.valid) copy_async<16>(sh.aside[1][c][tid], saved + c * NP);
-                else *reinterpret_cast<float4*>(sh.aside[1][c][tid]) = make_float4(0.f, 0.f, 0.f, 0.f);
+                f32x2 bb, qq;
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                  const f32x2 fed = f2_fma(e[c], now.C[i], G[c][i]), w = f2_mul(fed, f[v][c][i]);
+                  own[c][i] = f2_mul(d[v][c][i], f2_fma(e[c], now.C[i], own[c][i]));
+                  gs[i] = c ? f2_fma(fed, x[c], gs[i]) : f2_mul(fed, x[c]);
+                  bb = i ? f2_fma(fed, now.B[i], bb) : f2_mul(fed, now.B[i]);
+                  qq = i ? f2_fma(w, A[c][i], qq) : f2_mul(w, A[c][i]);
+                  dA[c][i] = f2_fma(dt[c], w, dA[c][i]);
+                  G[c][i] = f2_mul(d[v][c][i], fed);
+                }
+                gb[v % 2][c] = both(bb);
+                q[v % 2][c] = both(qq);
+              }
+              put_channels<S, QL>(mid + u * STEP, gs, lane);
+              if (v % 2 == 0) {
+                __syncwarp();                                              // all of the warp have read these tokens' s x
+#pragma unroll
+                for (int j = 0; j < 2; ++j) to[(u + j) * CT] = sum_states<QL>(gb[j][0], gb[j][1], q[j][0], q[j][1], lane);
               }
             }
-            if (t0 == 8) asm volatile("cp.async.wait_all;" ::: "memory");
           }
-          if (t0 + u0 > 0) take_aside(t0 + u0 - (second ? FEW : PART));  // under way meanwhile
-#pragma unroll
-          for (int v = FEW - 1; v >= 0; --v) {
-            const int u = u0 + v;
-            Token<H, true, true> now;
-            now.get(p_dx + u * CT, p_e + u * CT, p_b + u * NP, p_c + u * NP);
-            f32x2 gs[H], x[2], e[2], dt[2];
-            const f32x2 steps = ld2(p_dt + u * CT);
-            cum = f2_add(cum, steps);
-            splat2(steps, dt);
-            splat2(now.x, x);
-            splat2(now.e, e);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              f32x2 bb, qq;
-#pragma unroll
-              for (int i = 0; i < H; ++i) {
-                const f32x2 fed = f2_fma(e[c], now.C[i], G[c][i]), w = f2_mul(fed, f[v][c][i]);
-                own[c][i] = f2_mul(d[v][c][i], f2_fma(e[c], now.C[i], own[c][i]));
-                gs[i] = c ? f2_fma(fed, x[c], gs[i]) : f2_mul(fed, x[c]);
-                bb = i ? f2_fma(fed, now.B[i], bb) : f2_mul(fed, now.B[i]);
-                qq = i ? f2_fma(w, A[c][i], qq) : f2_mul(w, A[c][i]);
-                dA[c][i] = f2_fma(dt[c], w, dA[c][i]);
-                G[c][i] = f2_mul(d[v][c][i], fed);
-              }
-              gb[v % 2][c] = both(bb);
-              q[v % 2][c] = both(qq);
-            }
-            put_channels<S, QL>(mid + u * STEP, gs, lane);
-            if (v % 2 == 0) {
-              __syncwarp();                                              // all of the warp have read these tokens' s x
-#pragma unroll
-              for (int j = 0; j < 2; ++j) to[(u + j) * CT] = sum_states<QL>(gb[j][0], gb[j][1], q[j][0], q[j][1], lane);
-            }
-          }
+          sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
+          to -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
         }
-        sum_channels<S, QL>(mid, &sh.part[warp][t0][0], lane);
-        to -= U * CT; p_dt -= U * CT; p_dx -= U * CT; p_e -= U * CT; p_b -= U * NP; p_c -= U * NP;
+      }
+      // a tile's own sum first: 2048 tokens one by one lose half a digit
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (cl + c >= p.valid) continue;
+        float* to = g.part_a + (row_n + cl + c) * NP + q0;
+        if (k < used - 1) add_pairs<H>(to, dA[c]);
+        else st_pairs<H>(to, dA[c]);
+      }
+      // as in the forward pass: the carried gradient meets the tile's decays once
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < H; ++i) G[c][i] = ld2(sh.behind[c * H + i][tid]);
+      carry_pairs<H>(cum, A, G, own);
+      __syncthreads();
+      parts_to(g.part_b);
+#pragma unroll 1
+      for (int part = 0; part < TT; part += Px::SPAN) {
+        x.fetch(a.x, p, k * TT + part, n);      // again: they would fill 32 registers meanwhile
+        delta.fetch(a.delta, p, k * TT + part, n);
+        if (a.z.p) {
+          dy.fetch(g.dy, p, k * TT + part, n);
+          z.fetch(a.z, p, k * TT + part, n);
+        }
+        float bias[E], skip[E];
+        from_shared(sh.bias[0] + col, bias);
+        from_shared(sh.bias[1] + col, skip);
+#pragma unroll
+        for (int i = 0; i < Px::P; ++i) {
+          const int r = part + row + i * Px::ROWS, t = k * TT + r;
+          const bool in = t < n;
+          if (!in) {                         // for the sums
+            const float zero[E] = {};
+            to_shared(&sh.y[r][col], zero);
+            to_shared(&sh.q[r][col], zero);
+            if (t < a.len) {
+              store_piece<T>(dx + (long long)t * a.dim, zero, p.valid - col, g.vec);
+              store_piece<T>(dd + (long long)t * a.dim, zero, p.valid - col, g.vec);
+              if (g.dz) store_piece<T>(dz + (long long)t * a.dim, zero, p.valid - col, g.vec);
+            }
+            continue;
+          }
+          float u[E], e[E], gb[E], f[E], o[E];
+          Piece<T>::get(x.v[i], u);
+          from_shared(&sh.e[r][col], e);
+          if (g.dz) {
+            float zz[E], dout[E];
+            Piece<T>::get(z.v[i], zz);
+            Piece<T>::get(dy.v[i], dout);
+            from_shared(&sh.y[r][col], f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              const float s = sigmoid(zz[j]), yy = fmaf(skip[j], u[j], f[j]);
+              o[j] = dout[j] * yy * s * (1.f + zz[j] * (1.f - s));
+            }
+            store_piece<T>(dz + (long long)t * a.dim, o, p.valid - col, g.vec);
+          }
+          from_shared(&sh.dx[r][col], gb);
+          from_shared(&sh.dt[r][col], f);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            o[j] = fmaf(f[j], gb[j], skip[j] * e[j]);
+            e[j] *= u[j];
+          }
+          to_shared(&sh.y[r][col], e);
+          store_piece<T>(dx + (long long)t * a.dim, o, p.valid - col, g.vec);
+          from_shared(&sh.q[r][col], f);
+          float d[E];
+          Piece<T>::get(delta.v[i], d);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            o[j] = fmaf(gb[j], u[j], f[j] * LN2);          // a's unit was a factor of two
+            if (a.softplus) o[j] *= sigmoid(d[j] + bias[j]);
+          }
+          to_shared(&sh.q[r][col], o);
+          store_piece<T>(dd + (long long)t * a.dim, o, p.valid - col, g.vec);
+        }
+      }
+      __syncthreads();
+      if (tid < 2 * CT) {                  // a tile's own sums
+        const float* from = tid < CT ? &sh.y[0][tid] : &sh.q[0][tid - CT];
+        float v[4] = {};
+#pragma unroll
+        for (int r = 0; r < TT; r += 4)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += from[(r + j) * CT];
+        sum += (v[0] + v[1]) + (v[2] + v[3]);
       }
     }
-    // a tile's own sum first: 2048 tokens one by one lose half a digit
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       if (cl + c >= p.valid) continue;
-      float* to = g.part_a + (row_n + cl + c) * NP + q0;
-      if (k < used - 1) add_pairs<H>(to, dA[c]);
-      else st_pairs<H>(to, dA[c]);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        float w[2];
+        f2_unpack(G[c][i], w[0], w[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int s = q0 + 2 * i + j;
+          if (used <= first) g.part_a[(row_n + cl + c) * NP + s] = 0.f;
+          if (g.d_state_in && p.seg == 0 && s < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + c) * a.states + s] = w[j];
+        }
+      }
     }
-    // as in the forward pass: the carried gradient meets the tile's decays once
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int i = 0; i < H; ++i) G[c][i] = ld2(sh.behind[c * H + i][tid]);
-    carry_pairs<H>(cum, A, G, own);
+    if (tid < 2 * CT && tid % CT < p.valid) (tid < CT ? g.part_skip : g.part_bias)[row_n + tid % CT] = sum;
     __syncthreads();
-    parts_to(g.part_b);
-#pragma unroll 1
-    for (int part = 0; part < TT; part += Px::SPAN) {
-      x.fetch(a.x, p, k * TT + part, n);      // again: they would fill 32 registers meanwhile
-      delta.fetch(a.delta, p, k * TT + part, n);
-      if (a.z.p) {
-        dy.fetch(g.dy, p, k * TT + part, n);
-        z.fetch(a.z, p, k * TT + part, n);
-      }
-      float bias[E], skip[E];
-      from_shared(sh.bias[0] + col, bias);
-      from_shared(sh.bias[1] + col, skip);
-#pragma unroll
-      for (int i = 0; i < Px::P; ++i) {
-        const int r = part + row + i * Px::ROWS, t = k * TT + r;
-        const bool in = t < n;
-        if (!in) {                         // for the sums
-          const float zero[E] = {};
-          to_shared(&sh.y[r][col], zero);
-          to_shared(&sh.q[r][col], zero);
-          if (t < a.len) {
-            store_piece<T>(dx + (long long)t * a.dim, zero, p.valid - col, g.vec);
-            store_piece<T>(dd + (long long)t * a.dim, zero, p.valid - col, g.vec);
-            if (g.dz) store_piece<T>(dz + (long long)t * a.dim, zero, p.valid - col, g.vec);
-          }
-          continue;
-        }
-        float u[E], e[E], gb[E], f[E], o[E];
-        Piece<T>::get(x.v[i], u);
-        from_shared(&sh.e[r][col], e);
-        if (g.dz) {
-          float zz[E], dout[E];
-          Piece<T>::get(z.v[i], zz);
-          Piece<T>::get(dy.v[i], dout);
-          from_shared(&sh.y[r][col], f);
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float s = sigmoid(zz[j]), yy = fmaf(skip[j], u[j], f[j]);
-            o[j] = dout[j] * yy * s * (1.f + zz[j] * (1.f - s));
-          }
-          store_piece<T>(dz + (long long)t * a.dim, o, p.valid - col, g.vec);
-        }
-        from_shared(&sh.dx[r][col], gb);
-        from_shared(&sh.dt[r][col], f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          o[j] = fmaf(f[j], gb[j], skip[j] * e[j]);
-          e[j] *= u[j];
-        }
-        to_shared(&sh.y[r][col], e);
-        store_piece<T>(dx + (long long)t * a.dim, o, p.valid - col, g.vec);
-        from_shared(&sh.q[r][col], f);
-        float d[E];
-        Piece<T>::get(delta.v[i], d);
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          o[j] = fmaf(gb[j], u[j], f[j] * LN2);          // a's unit was a factor of two
-          if (a.softplus) o[j] *= sigmoid(d[j] + bias[j]);
-        }
-        to_shared(&sh.q[r][col], o);
-        store_piece<T>(dd + (long long)t * a.dim, o, p.valid - col, g.vec);
-      }
-    }
-    __syncthreads();
-    if (tid < 2 * CT) {                  // a tile's own sums
-      const float* from = tid < CT ? &sh.y[0][tid] : &sh.q[0][tid - CT];
-      float v[4] = {};
-#pragma unroll
-      for (int r = 0; r < TT; r += 4)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += from[(r + j) * CT];
-      sum += (v[0] + v[1]) + (v[2] + v[3]);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    if (cl + c >= p.valid) continue;
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      float w[2];
-      f2_unpack(G[c][i], w[0], w[1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int s = q0 + 2 * i + j;
-        if (used <= first) g.part_a[(row_n + cl + c) * NP + s] = 0.f;
-        if (g.d_state_in && p.seg == 0 && s < a.states) g.d_state_in[((long long)p.b * a.dim + p.ch0 + cl + c) * a.states + s] = w[j];
-      }
-    }
-  }
-  if (tid < 2 * CT && tid % CT < p.valid) (tid < CT ? g.part_skip : g.part_bias)[row_n + tid % CT] = sum;
-  __syncthreads();
   }
 }
 
